@@ -38,6 +38,36 @@ AUTO, GENERIC, TILE, DECODE, NARROW, TILE_F16, TILE_STREAMED, SHORT = 0, 1, 2, 3
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 
+_i64, _i32 = ctypes.c_int64, ctypes.c_int32
+
+
+class KVCache(ctypes.Structure):
+    """``ave_fp4_kv_cache``"""
+    _fields_ = [(n, _vp) for n in ("k", "k_scale", "v", "v_scale")] + [
+        (n, _i64) for n in ("k_page_stride", "k_scale_page_stride", "v_page_stride", "v_scale_page_stride")] + [
+        (n, _i32) for n in ("pages", "kv_heads", "page_size", "head_dim")]
+
+
+class Heads(ctypes.Structure):
+    """``ave_fp4_heads``"""
+    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64), ("heads", _i32), ("is_f32", _i32)]
+
+
+class NormRope(ctypes.Structure):
+    """``ave_fp4_norm_rope``"""
+    _fields_ = [(n, _vp) for n in ("q_weight", "k_weight", "cos", "sin", "positions")] + [
+        (n, _i32) for n in ("table_rows", "rotary_dim", "neighbours", "weight_is_f32")] + [("eps", ctypes.c_float)]
+
+
+class Attention(ctypes.Structure):
+    """``ave_fp4_attention``"""
+    _fields_ = [("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp), ("lse", _vp), ("page_table", _vp),
+                ("page_table_stride", _i64), ("seq_lens", _vp), ("cu_q", _vp), ("sinks", _vp)] + [
+        (n, _i32) for n in ("tokens", "batch", "heads", "table_pages", "max_q", "window", "causal")] + [("scale", ctypes.c_float)]
+
+
+_heads, _cache, _how, _attn = (ctypes.POINTER(c) for c in (Heads, KVCache, NormRope, Attention))
+
 #: symbol -> argtypes; every symbol ``include/ave_fp4.h`` and ``include/ave_fp4_debug.h`` declare
 SIGNATURES = {
     "ave_fp4_gemm_mxfp4": [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp],
@@ -91,6 +121,11 @@ SIGNATURES = {
     "ave_fp4_scales_to_blocked": [_vp, _int, _int, _vp, _vp],
     "ave_fp4_scales_from_blocked": [_vp, _int, _int, _vp, _vp],
     "ave_fp4_gemm_mxfp4_blocked_scales": [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp],
+    "ave_fp4_qk_norm_rope": [_heads, _heads, _int, _int, _how, _heads, _heads, _vp],
+    "ave_fp4_append_kv_mxfp4": [_heads, _heads, _int, _vp, _how, _cache, _heads, _heads, _vp],
+    "ave_fp4_gather_kv_mxfp4": [_cache, _vp, _int, _vp, _vp, _vp],
+    "ave_fp4_attention_mxfp4_workspace_bytes": [_attn, _cache],
+    "ave_fp4_attention_mxfp4": [_attn, _cache, _vp, ctypes.c_size_t, _vp],
     "ave_fp4_last_error": [],
     "ave_fp4_abi_version": [],
     "ave_fp4_debug_weights_from_hbm": [_vp, ctypes.c_size_t],
@@ -113,7 +148,8 @@ _RESTYPES = {"ave_fp4_last_error": ctypes.c_char_p, "ave_fp4_gemm_mxfp4_workspac
              "ave_fp4_gemm_mxfp4_planned_workspace_bytes": ctypes.c_size_t,
              "ave_fp4_gemm_mxfp4_swiglu_workspace_bytes": ctypes.c_size_t,
              "ave_fp4_gemm_nvfp4_workspace_bytes": ctypes.c_size_t,
-             "ave_fp4_moe_route_top2_workspace_bytes": ctypes.c_size_t}
+             "ave_fp4_moe_route_top2_workspace_bytes": ctypes.c_size_t,
+             "ave_fp4_attention_mxfp4_workspace_bytes": ctypes.c_size_t}
 
 
 def library_path() -> str:

@@ -10,6 +10,7 @@
 
 #include "../../include/ave_fp4.h"
 #include "../../include/ave_fp4_debug.h"
+#include "c_api_common.hpp"
 #include "kernels.hpp"
 #include "tile_map.hpp"
 
@@ -23,7 +24,9 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-int fail_inval(const char* fmt, ...) {
+}  // namespace
+
+int ave::fail_inval(const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -31,14 +34,20 @@ int fail_inval(const char* fmt, ...) {
   return AVE_FP4_EINVAL;
 }
 
-int finish(hipError_t e, const char* what) {
+int ave::finish(hipError_t e, const char* what) {
   if (e == hipSuccess) return 0;
   // same wording the reference uses for HIP failures (backends/amdgpu/driver.py:125-138)
   snprintf(g_err, sizeof(g_err), "ave-lang Error [HIP]: %s (%s)", hipGetErrorString(e), what);
   return (int)e;
 }
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+void ave::clear_error() { g_err[0] = 0; }
+
+using ave::aligned;
+using ave::fail_inval;
+using ave::finish;
+
+namespace {
 
 // Whether a GEMM's weights are likely to come from HBM rather than from the 256 MB last-level cache: a small model
 // of that cache's contents, kept per device -- the weight tensors of the latest shape-dispatched MXFP4 GEMMs, most

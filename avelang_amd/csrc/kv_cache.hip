@@ -1,0 +1,210 @@
+// What stands between the qkv projection and attention: norms of query and key heads, rotation by position, and the
+// quantiser that appends keys and values to a paged MXFP4 cache; and the way back from the cache to bf16.
+//
+// Norm:      n = (x * r) * w,  r = 1 / sqrt(sum(x^2) / D + eps)
+// Rotation:  a' = a cos - b sin,  b' = b cos + a sin   for the pairs (i, i + R/2) or (2i, 2i + 1), i < R/2
+// Quantiser: per 32 channels, as quantize_mx.hip.
+// Every product and sum is rounded by itself (no contraction) and the squares are added up neighbours first -- eight in a lane, then
+// lanes 1, 2, 4, ... apart -- so that codes behind a norm and a rotation are the same bits wherever they are computed.
+//
+// Bound by HBM for a prompt (each input read once, each output written once), by latency for a decode batch: one launch for
+// all roles of heads.
+#include "fp4_common.hpp"
+#include "kv_cache.hpp"
+
+#pragma clang fp contract(off)
+
+namespace ave {
+namespace {
+
+// Eight consecutive elements from any address of their type.
+template <typename T>
+__device__ inline void load8(const T* p, float (&v)[8]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    constexpr int V = (int)sizeof(T) / 2;
+    v4i raw[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) raw[q] = reinterpret_cast<const v4i*>(p)[q];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (sizeof(T) == 4) v[j] = __builtin_bit_cast(float, (int)raw[j / 4][j % 4]);
+      else v[j] = __builtin_bit_cast(float, j % 2 ? (unsigned)raw[0][j / 2] & 0xFFFF0000u : (unsigned)raw[0][j / 2] << 16);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)p[j];
+  }
+}
+
+__device__ inline void store8_bf16(uint16_t* p, const float (&v)[8]) {
+  const v4i w = {(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]), (int)pack_bf16x2(v[4], v[5]), (int)pack_bf16x2(v[6], v[7])};
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    *reinterpret_cast<v4i*>(p) = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = (uint16_t)((unsigned)w[j / 2] >> (16 * (j % 2)));
+  }
+}
+
+// D / 8 lanes share a head, eight channels each; a workgroup has 2048 / D heads of one token (blockIdx.x) under way and takes the
+// token's heads -- queries, keys, values -- gridDim.y such groups apart.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int all_heads, int page_shift) {
+  constexpr int L = D / 8;
+  const int token = blockIdx.x, lane = threadIdx.x % L, c0 = lane * 8;
+  const int half = p.how.rotary_dim / 2;
+  const bool turned = p.how.cos && c0 < 2 * half;
+  const bool upper = !p.how.neighbours && c0 >= half;      // this lane's channels are the second ones of their pairs
+  const int partner = p.how.neighbours ? c0 : (upper ? c0 - half : c0 + half);
+  float cs[8], sn[8];
+  if (turned) {
+    const int pos = p.how.positions[token];
+    if (pos >= 0 && pos < p.how.table_rows) {
+      const size_t row = (size_t)pos * half;
+      if (p.how.neighbours) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cs[j] = p.how.cos[row + c0 / 2 + j / 2], sn[j] = p.how.sin[row + c0 / 2 + j / 2];
+      } else {
+        load8(p.how.cos + row + (upper ? c0 - half : c0), cs);
+        load8(p.how.sin + row + (upper ? c0 - half : c0), sn);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cs[j] = sn[j] = __builtin_nanf("");
+    }
+  }
+  for (int h = blockIdx.y * (256 / L) + threadIdx.x / L; h < all_heads; h += gridDim.y * (256 / L)) {
+    const bool is_q = h < q_heads, is_v = p.v.data && h >= q_heads + p.k.heads;
+    const int head = is_q ? h : is_v ? h - q_heads - p.k.heads : h - q_heads;
+    const ave_fp4_heads& in = is_q ? p.q : is_v ? p.v : p.k;
+    const T* src = static_cast<const T*>(in.data) + token * in.token_stride + head * in.head_stride;
+    float x[8], y[8];
+    load8(src + c0, x);
+    if (!is_v) {
+      if (turned && !p.how.neighbours) load8(src + partner, y);
+      const void* weight = is_q ? p.how.q_weight : p.how.k_weight;
+      if (weight) {
+        float s[8], w[8], wy[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = x[j] * x[j];
+        float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+#pragma unroll
+        for (int m = 1; m < L; m *= 2) sum += __shfl_xor(sum, m, 64);
+        const float r = 1.0f / sqrtf(sum / (float)D + p.how.eps);
+        if (p.how.weight_is_f32) load8(static_cast<const float*>(weight) + c0, w);
+        else load8(static_cast<const __bf16*>(weight) + c0, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (x[j] * r) * w[j];
+        if (turned && !p.how.neighbours) {
+          if (p.how.weight_is_f32) load8(static_cast<const float*>(weight) + partner, wy);
+          else load8(static_cast<const __bf16*>(weight) + partner, wy);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = (y[j] * r) * wy[j];
+        }
+      }
+      if (turned) {
+        if (p.how.neighbours) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const float a = x[j], b = x[j + 1];
+            x[j] = a * cs[j] - b * sn[j];
+            x[j + 1] = b * cs[j] + a * sn[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = upper ? x[j] * cs[j] + y[j] * sn[j] : x[j] * cs[j] - y[j] * sn[j];
+        }
+      }
+    }
+    if (is_q || (!is_v && p.k_out.data)) {
+      const ave_fp4_heads& out = is_q ? p.q_out : p.k_out;
+      store8_bf16(static_cast<uint16_t*>(out.data) + token * out.token_stride + head * out.head_stride + c0, x);
+    } else {
+      const unsigned amax = lane_xor_max_bits(lane_xor_max_bits(abs_max_bits(x), 1), 2);   // four lanes share a block
+      const int byte = mx_scale_byte(amax);
+      const float scale = mx_scale_value(byte);
+      unsigned codes = 0;
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+      if (byte == 0xFF) codes = 0u;
+      const int slot = p.slots[token];
+      const int page = slot >> page_shift;
+      if (slot >= 0 && page < p.cache.pages) {
+        const size_t row = (size_t)head * p.cache.page_size + (slot & (p.cache.page_size - 1));   // within the page
+        uint8_t* c = (is_v ? p.cache.v + page * p.cache.v_page_stride : p.cache.k + page * p.cache.k_page_stride) + row * (D / 2);
+        uint8_t* f = (is_v ? p.cache.v_scale + page * p.cache.v_scale_page_stride : p.cache.k_scale + page * p.cache.k_scale_page_stride) + row * (D / 32);
+        reinterpret_cast<unsigned*>(c)[lane] = codes;
+        if (lane % 4 == 0) f[lane / 4] = (uint8_t)byte;
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_heads_as(const HeadArgs& p, hipStream_t s) {
+  const int q = p.q.data ? p.q.heads : 0, all = q + (p.k.data ? p.k.heads : 0) + (p.v.data ? p.v.heads : 0);
+  const int groups = (all + 2048 / D - 1) / (2048 / D);
+  if (p.tokens == 0 || all == 0) return hipSuccess;
+  // few tokens: a workgroup for every group of heads; many: one for every token, which loads its cosines once
+  const int y = p.tokens >= 1024 ? 1 : groups;
+  hipLaunchKernelGGL((heads_kernel<T, D>), dim3((unsigned)p.tokens, (unsigned)y), dim3(256), 0, s, p, q, all, log2_of(p.cache.page_size));
+  return hipGetLastError();
+}
+
+// A lane takes eight channels of one head of one token.
+template <int D>
+__global__ __launch_bounds__(256) void gather_kv_kernel(ave_fp4_kv_cache c, const int32_t* slots, size_t pieces, uint16_t* k, uint16_t* v,
+                                                        int page_shift) {
+  constexpr int L = D / 8;
+  const size_t per_token = (size_t)c.kv_heads * L;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < 2 * pieces; i += (size_t)gridDim.x * 256) {
+    const bool is_v = i >= pieces;
+    const size_t at = is_v ? i - pieces : i;
+    const size_t token = at / per_token;
+    const unsigned rest = (unsigned)(at - token * per_token), head = rest / L, lane = rest % L;
+    const int slot = slots[token], page = slot >> page_shift;
+    v4i out = {0, 0, 0, 0};
+    if (slot >= 0 && page < c.pages) {
+      const size_t row = (size_t)head * c.page_size + (slot & (c.page_size - 1));
+      const uint8_t* codes = (is_v ? c.v + page * c.v_page_stride : c.k + page * c.k_page_stride) + row * (D / 2);
+      const uint8_t* scales = (is_v ? c.v_scale + page * c.v_scale_page_stride : c.k_scale + page * c.k_scale_page_stride) + row * (D / 32);
+      const unsigned x = reinterpret_cast<const unsigned*>(codes)[lane];
+      const int byte = scales[lane / 4];
+      const float scale = byte == 0xFF ? __builtin_nanf("") : mx_scale_value(byte);
+      const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 1);
+      const v2f d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 3);
+      out = v4i{(int)pack_bf16x2(a[0] * scale, a[1] * scale), (int)pack_bf16x2(b[0] * scale, b[1] * scale),
+                (int)pack_bf16x2(d[0] * scale, d[1] * scale), (int)pack_bf16x2(e[0] * scale, e[1] * scale)};
+    }
+    reinterpret_cast<v4i*>(is_v ? v : k)[at] = out;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_heads(const HeadArgs& p, hipStream_t s) {
+  const bool f32 = p.q.data ? p.q.is_f32 : p.k.is_f32;
+  switch (p.head_dim) {
+    case 64: return f32 ? launch_heads_as<float, 64>(p, s) : launch_heads_as<__bf16, 64>(p, s);
+    case 128: return f32 ? launch_heads_as<float, 128>(p, s) : launch_heads_as<__bf16, 128>(p, s);
+    default: return f32 ? launch_heads_as<float, 256>(p, s) : launch_heads_as<__bf16, 256>(p, s);
+  }
+}
+
+hipError_t launch_gather_kv(const ave_fp4_kv_cache& c, const int32_t* slots, int tokens, uint16_t* k, uint16_t* v, hipStream_t s) {
+  const size_t pieces = (size_t)tokens * c.kv_heads * (c.head_dim / 8);
+  if (pieces == 0) return hipSuccess;
+  size_t grid = (2 * pieces + 255) / 256;
+  if (grid > 1u << 16) grid = 1u << 16;
+  const int shift = log2_of(c.page_size);
+#define AVE_GATHER(D) hipLaunchKernelGGL((gather_kv_kernel<D>), dim3((unsigned)grid), dim3(256), 0, s, c, slots, pieces, k, v, shift)
+  if (c.head_dim == 64) AVE_GATHER(64);
+  else if (c.head_dim == 128) AVE_GATHER(128);
+  else AVE_GATHER(256);
+#undef AVE_GATHER
+  return hipGetLastError();
+}
+
+}  // namespace ave

@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
+#include <cmath>
 
 #include "../../include/ave_fp4.h"
 
@@ -418,6 +419,213 @@ PyObject* gather_rows_mxfp4(PyObject* const* arg) {
   return ok ? pair_of(out, scale) : nullptr;
 }
 
+// ---- attention over an MXFP4 cache ------------------------------------------------------------------------------------------
+struct Cache {   // the tuple (k, k_scale, v, v_scale); sizes and alignment are checked by the library
+  ave_fp4_kv_cache c{};
+  c10::Device dev{c10::kCPU};
+  bool take(PyObject* o) {
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 4) return false;
+    const Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+      t[i] = tensor(PyTuple_GET_ITEM(o, i));
+      if (!t[i] || !is_byte(*t[i]) || t[i]->dim() != 4 || !t[i]->is_cuda()) return false;
+    }
+    dev = t[0]->device();
+    const int64_t pages = t[0]->size(0), heads = t[0]->size(1), page = t[0]->size(2), half = t[0]->size(3);
+    if (half != 32 && half != 64 && half != 128) return false;
+    if (!fits(pages) || !fits(heads) || !fits(page)) return false;
+    for (int i = 0; i < 4; ++i) {
+      const int64_t last = i % 2 ? half / 16 : half;
+      if (t[i]->device() != dev || t[i]->size(0) != pages || t[i]->size(1) != heads || t[i]->size(2) != page || t[i]->size(3) != last) return false;
+      if (t[i]->stride(3) != 1 || t[i]->stride(2) != last || t[i]->stride(1) != page * last) return false;
+    }
+    c = {ptr_as<uint8_t>(*t[0]), ptr_as<uint8_t>(*t[1]), ptr_as<uint8_t>(*t[2]), ptr_as<uint8_t>(*t[3]),
+         t[0]->stride(0), t[1]->stride(0), t[2]->stride(0), t[3]->stride(0), (int)pages, (int)heads, (int)page, (int)(2 * half)};
+    return true;
+  }
+};
+
+bool is_float(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
+
+struct Heads {   // [tokens, heads, head_dim] with consecutive channels; absent when None
+  ave_fp4_heads h{};
+  const Tensor* t = nullptr;
+  bool take(PyObject* o, c10::Device dev, int64_t tokens, int64_t head_dim) {
+    if (o == Py_None) return true;
+    t = tensor(o);
+    if (!t || !is_float(*t) || t->dim() != 3 || t->device() != dev || t->size(0) != tokens || t->size(2) != head_dim || t->stride(2) != 1 || !fits(t->size(1)))
+      return false;
+    h = {ptr(*t), t->stride(0), t->stride(1), (int32_t)t->size(1), t->scalar_type() == at::kFloat};
+    return true;
+  }
+  const ave_fp4_heads* get() const { return t ? &h : nullptr; }
+};
+
+// The bf16 output for `in` (None: a new tensor); false when a given one does not fit.
+struct HeadsOut {
+  Out out;
+  ave_fp4_heads h{};
+  bool have = false;
+  bool take(PyObject* o, const Heads& in, c10::Device dev) {
+    if (!in.t) return o == Py_None;
+    have = true;
+    if (o == Py_None) {
+      if (!out.take(o, in.t->sizes(), at::kBFloat16, dev)) return false;
+    } else {
+      Heads given;
+      if (!given.take(o, dev, in.t->size(0), in.t->size(2)) || given.h.is_f32 || given.h.heads != in.h.heads) return false;
+      out.t = *given.t;
+      out.given = o;
+    }
+    h = {ptr(out.t), out.t.stride(0), out.t.stride(1), in.h.heads, 0};
+    return true;
+  }
+  const ave_fp4_heads* get() const { return have ? &h : nullptr; }
+  PyObject* object() const {
+    if (have) return out.object();
+    Py_RETURN_NONE;
+  }
+};
+
+bool as_float(PyObject* o, float* v) {
+  if (!PyFloat_CheckExact(o)) return false;
+  *v = (float)PyFloat_AS_DOUBLE(o);
+  return true;
+}
+
+// cos, sin, positions, q_weight, k_weight, eps, neighbours
+bool take_how(PyObject* cos, PyObject* sin, PyObject* positions, PyObject* q_weight, PyObject* k_weight, PyObject* eps, PyObject* neighbours,
+              int64_t tokens, int64_t head_dim, c10::Device dev, ave_fp4_norm_rope* how) {
+  *how = {};
+  if (!as_float(eps, &how->eps) || !PyBool_Check(neighbours)) return false;
+  how->neighbours = neighbours == Py_True;
+  if (cos != Py_None || sin != Py_None) {
+    const Tensor *c = tensor(cos), *s = tensor(sin), *p = tensor(positions);
+    if (!c || !s || !p || c->scalar_type() != at::kFloat || s->scalar_type() != at::kFloat || c->dim() != 2) return false;
+    if (!fits(c->size(0)) || !fits(2 * c->size(1)) || !matrix(*c, dev, c->size(0), c->size(1)) || !matrix(*s, dev, c->size(0), c->size(1))) return false;
+    if (!vec(*p, dev, tokens, at::kInt)) return false;
+    how->cos = ptr_as<float>(*c), how->sin = ptr_as<float>(*s), how->positions = ptr_as<int32_t>(*p);
+    how->table_rows = (int32_t)c->size(0), how->rotary_dim = (int32_t)(2 * c->size(1));
+  }
+  const Tensor *qw = nullptr, *kw = nullptr;
+  if (q_weight != Py_None && (!(qw = tensor(q_weight)) || !is_float(*qw) || !vec(*qw, dev, head_dim, qw->scalar_type()))) return false;
+  if (k_weight != Py_None && (!(kw = tensor(k_weight)) || !is_float(*kw) || !vec(*kw, dev, head_dim, kw->scalar_type()))) return false;
+  if (qw && kw && qw->scalar_type() != kw->scalar_type()) return false;
+  how->q_weight = qw ? ptr(*qw) : nullptr, how->k_weight = kw ? ptr(*kw) : nullptr;
+  how->weight_is_f32 = (qw ? qw : kw) && (qw ? qw : kw)->scalar_type() == at::kFloat;
+  return true;
+}
+
+// q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, eps, neighbours
+PyObject* qk_norm_rope(PyObject* const* arg) {
+  const Tensor* x = tensor(arg[0] != Py_None ? arg[0] : arg[1]);
+  if (!x || x->dim() != 3 || !x->is_cuda() || !fits(x->size(0))) NOT_MINE;
+  const auto dev = x->device();
+  const int64_t t = x->size(0), d = x->size(2);
+  if (d != 64 && d != 128 && d != 256) NOT_MINE;
+  Heads q, k;
+  ave_fp4_norm_rope how;
+  if (!q.take(arg[0], dev, t, d) || !k.take(arg[1], dev, t, d) || (q.t && k.t && q.h.is_f32 != k.h.is_f32)) NOT_MINE;
+  if (!take_how(arg[2], arg[3], arg[4], arg[5], arg[6], arg[9], arg[10], t, d, dev, &how)) NOT_MINE;
+  HeadsOut qo, ko;
+  if (!qo.take(arg[7], q, dev) || !ko.take(arg[8], k, dev)) NOT_MINE;
+  if (!launch(dev, [&](void* s) { return ave_fp4_qk_norm_rope(q.get(), k.get(), (int)t, (int)d, &how, qo.get(), ko.get(), s); })) return nullptr;
+  PyObject* a = qo.object();
+  PyObject* b = a ? ko.object() : nullptr;
+  PyObject* r = b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return r;
+}
+
+// k, v, cache, slots, cos, sin, positions, k_weight, q, q_weight, q_out, eps, neighbours; returns (q_out,)
+PyObject* append_kv_mxfp4(PyObject* const* arg) {
+  Cache cache;
+  const Tensor* kt = tensor(arg[0]);
+  if (!cache.take(arg[2]) || !kt || kt->dim() != 3 || !fits(kt->size(0))) NOT_MINE;
+  const auto dev = cache.dev;
+  const int64_t t = kt->size(0), d = cache.c.head_dim;
+  Heads q, k, v;
+  if (!k.take(arg[0], dev, t, d) || !v.take(arg[1], dev, t, d) || !v.t || !q.take(arg[8], dev, t, d)) NOT_MINE;
+  if (k.h.heads != cache.c.kv_heads || v.h.heads != cache.c.kv_heads || v.h.is_f32 != k.h.is_f32 || (q.t && q.h.is_f32 != k.h.is_f32)) NOT_MINE;
+  const Tensor* slots = tensor(arg[3]);
+  ave_fp4_norm_rope how;
+  if (!slots || !vec(*slots, dev, t, at::kInt) || !take_how(arg[4], arg[5], arg[6], arg[9], arg[7], arg[11], arg[12], t, d, dev, &how)) NOT_MINE;
+  HeadsOut qo;
+  if (!qo.take(arg[10], q, dev)) NOT_MINE;
+  if (!launch(dev, [&](void* s) {
+        return ave_fp4_append_kv_mxfp4(k.get(), v.get(), (int)t, ptr_as<int32_t>(*slots), &how, &cache.c, q.get(), qo.get(), s);
+      }))
+    return nullptr;
+  PyObject* a = qo.object();
+  PyObject* r = a ? PyTuple_Pack(1, a) : nullptr;
+  Py_XDECREF(a);
+  return r;
+}
+
+// cache, slots, k_out, v_out
+PyObject* gather_kv_mxfp4(PyObject* const* arg) {
+  Cache cache;
+  const Tensor* slots = tensor(arg[1]);
+  if (!cache.take(arg[0]) || !slots || slots->dim() != 1 || !fits(slots->size(0)) || !vec(*slots, cache.dev, slots->size(0), at::kInt)) NOT_MINE;
+  const int64_t t = slots->size(0);
+  Out k, v;
+  if (!k.take(arg[2], {t, cache.c.kv_heads, cache.c.head_dim}, at::kBFloat16, cache.dev) ||
+      !v.take(arg[3], {t, cache.c.kv_heads, cache.c.head_dim}, at::kBFloat16, cache.dev))
+    NOT_MINE;
+  const bool ok = launch(cache.dev, [&](void* s) {
+    return ave_fp4_gather_kv_mxfp4(&cache.c, ptr_as<int32_t>(*slots), (int)t, ptr_as<uint16_t>(k.t), ptr_as<uint16_t>(v.t), s);
+  });
+  return ok ? pair_of(k, v) : nullptr;
+}
+
+// q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, causal
+PyObject* attention_mxfp4(PyObject* const* arg) {
+  Cache cache;
+  const Tensor *q = tensor(arg[0]), *table = tensor(arg[2]), *lens = tensor(arg[3]);
+  if (!cache.take(arg[1]) || !q || !table || !lens) NOT_MINE;
+  const auto dev = cache.dev;
+  const int64_t d = cache.c.head_dim;
+  if (q->scalar_type() != at::kBFloat16 || q->dim() != 3 || q->device() != dev || q->size(2) != d || q->stride(2) != 1 || !fits(q->size(0)) || !fits(q->size(1)))
+    NOT_MINE;
+  if (table->scalar_type() != at::kInt || table->dim() != 2 || table->device() != dev || (table->size(1) > 1 && table->stride(1) != 1) ||
+      !fits(table->size(0)) || !fits(table->size(1)))
+    NOT_MINE;
+  const int64_t t = q->size(0), heads = q->size(1), b = table->size(0);
+  if (!vec(*lens, dev, b, at::kInt)) NOT_MINE;
+  ave_fp4_attention a{};
+  a.q = ptr_as<uint16_t>(*q), a.q_token_stride = q->stride(0), a.q_head_stride = q->stride(1);
+  a.page_table = ptr_as<int32_t>(*table), a.page_table_stride = table->stride(0), a.seq_lens = ptr_as<int32_t>(*lens);
+  a.tokens = (int)t, a.batch = (int)b, a.heads = (int)heads, a.table_pages = (int)table->size(1);
+  if (arg[4] != Py_None) {
+    const Tensor* cu = tensor(arg[4]);
+    if (!cu || !vec(*cu, dev, b + 1, at::kInt)) NOT_MINE;
+    a.cu_q = ptr_as<int32_t>(*cu);
+  }
+  if (arg[10] != Py_None) {
+    const Tensor* sinks = tensor(arg[10]);
+    if (!sinks || !vec(*sinks, dev, heads, at::kFloat)) NOT_MINE;
+    a.sinks = ptr_as<float>(*sinks);
+  }
+  if (arg[6] != Py_None) {
+    const Tensor* lse = tensor(arg[6]);
+    if (!lse || lse->scalar_type() != at::kFloat || !matrix(*lse, dev, t, heads)) NOT_MINE;
+    a.lse = ptr_as<float>(*lse);
+  }
+  if (!as_int(arg[7], &a.max_q) || !as_int(arg[9], &a.window) || !PyBool_Check(arg[11])) NOT_MINE;
+  a.causal = arg[11] == Py_True;
+  if (arg[8] == Py_None) a.scale = d == 64 ? 0.125f : d == 256 ? 0.0625f : 0.08838834764831845f;
+  else if (!as_float(arg[8], &a.scale) || !std::isfinite(a.scale)) NOT_MINE;
+  Out out;
+  if (!out.take(arg[5], {t, heads, d}, at::kBFloat16, dev)) NOT_MINE;
+  a.out = ptr_as<uint16_t>(out.t);
+  const size_t bytes = on_device(dev, [&] { return ave_fp4_attention_mxfp4_workspace_bytes(&a, &cache.c); });
+  Tensor ws;
+  if (bytes) ws = empty({(int64_t)bytes}, at::kByte, dev);
+  const bool ok = launch(dev, [&](void* s) { return ave_fp4_attention_mxfp4(&a, &cache.c, bytes ? ptr(ws) : nullptr, bytes, s); });
+  return ok ? out.object() : nullptr;
+}
+
 // ---- the module -------------------------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int ARGS>
 PyObject* entry(PyObject*, PyObject* const* arg, Py_ssize_t n) {
@@ -445,6 +653,10 @@ PyMethodDef kMethods[] = {
     ENTRY(moe_route_top2, 5),
     ENTRY(moe_combine_top2, 5),
     ENTRY(gather_rows_mxfp4, 5),
+    ENTRY(qk_norm_rope, 11),
+    ENTRY(append_kv_mxfp4, 13),
+    ENTRY(gather_kv_mxfp4, 4),
+    ENTRY(attention_mxfp4, 12),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_calls", "the package's entry points on torch tensors, in C++", -1, kMethods, nullptr, nullptr, nullptr, nullptr};

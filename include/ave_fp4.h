@@ -370,6 +370,95 @@ int ave_fp4_scales_from_blocked(const uint8_t* blocked, int rows, int cols, uint
 int ave_fp4_gemm_mxfp4_blocked_scales(const uint8_t* A, const uint8_t* A_scale_blocked, const uint8_t* B,
                                       const uint8_t* B_scale_blocked, uint16_t* C, int M, int N, int K, void* hip_stream);
 
+/*
+ * ---- Between the qkv projection and the output projection: a paged key/value cache held in MXFP4 ----
+ *
+ * No counterpart in the reference, whose only library kernel is a GEMM; with these a decoder layer's attention runs on the
+ * library as its linear layers do.
+ *
+ * The cache of one layer is four device tensors: codes [pages, kv_heads, page_size, head_dim/2] (packed E2M1, low nibble =
+ * even channel) and scales [pages, kv_heads, page_size, head_dim/32] (E8M0) of the keys, and the same of the values.  A
+ * page may be followed by other data (the page strides, in bytes); inside a page all is contiguous.  head_dim is 64, 128
+ * or 256, page_size a power of two from 16 to 4096.  Codes 16-byte aligned with page strides that are multiples of 16,
+ * scales 4-byte aligned with multiples of 4.  A token's place is its slot: page * page_size + offset.
+ */
+typedef struct ave_fp4_kv_cache {
+  uint8_t *k, *k_scale, *v, *v_scale;
+  int64_t k_page_stride, k_scale_page_stride, v_page_stride, v_scale_page_stride; /* bytes */
+  int32_t pages, kv_heads, page_size, head_dim;
+} ave_fp4_kv_cache;
+
+/* Heads of a batch of tokens, [tokens, heads, head_dim] with consecutive channels; strides in elements, any alignment. */
+typedef struct ave_fp4_heads {
+  void* data; /* bf16, or fp32 where is_f32 (inputs only) */
+  int64_t token_stride, head_stride;
+  int32_t heads, is_f32;
+} ave_fp4_heads;
+
+/*
+ * What happens to query and key heads before they are stored.  Norm (weights set): n = (x * r) * w with
+ * r = 1 / sqrt(sum(x^2) / head_dim + eps).  Rotation (cos set) of the first rotary_dim channels (a multiple of 16):
+ * a' = a cos - b sin, b' = b cos + a sin for the pairs (i, i + rotary_dim/2), with `neighbours` (2i, 2i+1), cos and sin
+ * [table_rows, rotary_dim/2] fp32 at row positions[token]; a position outside the table gives NaN.  All of it in fp32,
+ * every product and sum rounded by itself and the squares added up neighbours first, so that the codes of normed and rotated
+ * keys have the same bits wherever they are computed; one rounding at the end (to bf16, or by the quantiser).
+ */
+typedef struct ave_fp4_norm_rope {
+  const void *q_weight, *k_weight; /* [head_dim], either may be null; bf16, or fp32 where weight_is_f32 */
+  const float *cos, *sin;          /* null: no rotation */
+  const int32_t* positions;        /* [tokens] */
+  int32_t table_rows, rotary_dim, neighbours, weight_is_f32;
+  float eps;
+} ave_fp4_norm_rope;
+
+/* Norm and rotation of query heads, key heads or both (a null pointer: none), bf16 out; an output may be its input. */
+int ave_fp4_qk_norm_rope(const ave_fp4_heads* q, const ave_fp4_heads* k, int tokens, int head_dim, const ave_fp4_norm_rope* how,
+                         const ave_fp4_heads* q_out, const ave_fp4_heads* k_out, void* hip_stream);
+
+/*
+ * Keys (normed and rotated as `how` says; null: as they are) and values of a batch of tokens into the cache at slots
+ * [tokens]: the quantiser of ave_fp4_quantize_mxfp4_* per 32 channels, from fp32.  A slot outside the cache stores nothing (padding);
+ * of two tokens with one slot either may stay.  With q the same launch norms and rotates the queries into q_out (bf16).
+ */
+int ave_fp4_append_kv_mxfp4(const ave_fp4_heads* k, const ave_fp4_heads* v, int tokens, const int32_t* slots, const ave_fp4_norm_rope* how,
+                            const ave_fp4_kv_cache* cache, const ave_fp4_heads* q, const ave_fp4_heads* q_out, void* hip_stream);
+
+/* Cached tokens back as bf16 [tokens, kv_heads, head_dim] (exact: E2M1 times a power of two; a scale byte 0xFF gives NaN); a slot
+ * outside the cache gives zeros. */
+int ave_fp4_gather_kv_mxfp4(const ave_fp4_kv_cache* cache, const int32_t* slots, int tokens, uint16_t* k, uint16_t* v, void* hip_stream);
+
+/*
+ * Attention of the new tokens of `batch` sequences over their cached keys and values (the new tokens' own among them).
+ * Sequence b holds seq_lens[b] tokens, token j in page page_table[b * page_table_stride + j / page_size]; its new tokens are rows
+ * cu_q[b] .. cu_q[b+1]-1 of q (cu_q null: one each, tokens == batch) and its last ones: row i of n stands at position
+ * p = seq_lens[b] - n + i.  It sees key j if j <= p (`causal`) and j > p - window (window > 0; causal only).  Query head h
+ * reads key head h / (heads / kv_heads).
+ *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink_h)),  s_j = scale * q . k_j      (sinks null: without the last term)
+ *   lse = log of the denominator (optional; natural logarithm, the sink included; -inf where it is zero)
+ * A row that sees no key gives zeros.  Scores, softmax and sums in fp32; queries enter the products with 19 bits and more below
+ * their row's largest one, probabilities as bf16.  A NaN or infinity in a query, or a NaN scale of a key or value it sees, gives NaN.
+ * Rows of q behind cu_q[batch] are left alone.  Device data is never trusted with addresses: lengths are cut to the page
+ * table's width, rows to q's, pages outside the cache are read as its nearest page.
+ * max_q: a bound on the new tokens of a sequence, by which the kernel is chosen (a wrong one costs time only).
+ * The workspace (16-byte aligned, no initialisation, garbage afterwards; calls that may overlap need their own) takes the
+ * partial results of sequences that several workgroups share; results do not depend on what it held.
+ */
+typedef struct ave_fp4_attention {
+  const uint16_t* q;
+  int64_t q_token_stride, q_head_stride; /* elements; consecutive channels, any alignment */
+  uint16_t* out;                         /* [tokens, heads, head_dim] contiguous, 4-byte aligned */
+  float* lse;                            /* [tokens, heads] or null */
+  const int32_t* page_table;
+  int64_t page_table_stride;             /* entries */
+  const int32_t *seq_lens, *cu_q;
+  const float* sinks;                    /* [heads] or null */
+  int32_t tokens, batch, heads, table_pages, max_q, window, causal;
+  float scale;
+} ave_fp4_attention;
+size_t ave_fp4_attention_mxfp4_workspace_bytes(const ave_fp4_attention* a, const ave_fp4_kv_cache* cache);
+int ave_fp4_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_kv_cache* cache, void* workspace, size_t workspace_bytes,
+                            void* hip_stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* ave_fp4_last_error(void);
 
