@@ -2,7 +2,8 @@
 //   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink)),  s_j = scale * q . k_j,  over the keys the row sees
 // One pass over the keys, 64 at a time, with the running maximum and sum of the softmax.
 #include "fp4_common.hpp"
-#include "kv_cache.hpp"
+#include "attn_common.hpp"
+#include "kernels.hpp"
 
 namespace ave {
 namespace {
@@ -116,9 +117,34 @@ __global__ __launch_bounds__(64) void attention_row_kernel(ave_fp4_attention a, 
 
 }  // namespace
 
-size_t attention_workspace_bytes(const ave_fp4_attention&, const ave_fp4_kv_cache&) { return 0; }
+namespace {
 
-hipError_t launch_attention(const ave_fp4_attention& a, const ave_fp4_kv_cache& c, void*, hipStream_t s) {
+AttnArgs args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
+  AttnArgs p{};
+  p.a = a, p.c = c;
+  p.group = a.heads / c.kv_heads;
+  p.page_shift = log2_of(c.page_size);
+  return p;
+}
+
+// Row tiles of 16 of the kernel for few rows; 0: another kernel
+int decode_row_tiles(const AttnArgs& p) {
+  const int64_t rows = (int64_t)(p.a.cu_q ? p.a.max_q : 1) * p.group;
+  const int most = p.c.head_dim == 256 ? 32 : 64;
+  return rows > most ? 0 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
+}
+
+}  // namespace
+
+size_t attention_workspace_bytes(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
+  const AttnArgs p = args_of(a, c);
+  if (const int tiles = decode_row_tiles(p)) return attn_decode_workspace(p, tiles);
+  return 0;
+}
+
+hipError_t launch_attention(const ave_fp4_attention& a, const ave_fp4_kv_cache& c, void* workspace, hipStream_t s) {
+  const AttnArgs args = args_of(a, c);
+  if (const int tiles = decode_row_tiles(args)) return launch_attn_decode(args, tiles, workspace, s);
   const dim3 grid((unsigned)a.tokens, (unsigned)a.heads);
   const int shift = log2_of(c.page_size);
 #define AVE_ROW(D) hipLaunchKernelGGL((attention_row_kernel<D>), grid, dim3(64), 0, s, a, c, shift)

@@ -1,0 +1,331 @@
+// What the kernels of attention over an MXFP4 cache share: how the work of a call is cut into equal parts on the device, where
+// partial results go, loads from the cache into LDS, and the queries' and probabilities' forms for the matrix cores.
+//
+// Work.  An item is a block of ROWS rows -- (new token, query head) pairs of one sequence and one key head, tokens first -- and has
+// as many units as there are TILE keys between the first and the last one that any of its rows sees (at least one).  Units are
+// numbered by sequence, key head, block, key; every workgroup takes the same number of consecutive ones, so that a long sequence
+// beside short ones, or the triangle of a prompt, costs no workgroup more than another.  Lengths are device memory: each workgroup adds the
+// units up for itself (one read of seq_lens and cu_q).  A part of an item that does not cover all of it goes to the workspace, and
+// a second launch joins the parts in order.
+#pragma once
+#include "fp4_common.hpp"
+#include "kv_cache.hpp"
+#include "tile_common.hpp"
+
+namespace ave {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
+constexpr float kNone = -3.0e38f;   // a score that is not there, below every one that is
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnArgs {
+  ave_fp4_attention a;
+  ave_fp4_kv_cache c;
+  int group;          // query heads per key head
+  int page_shift;
+  int whole;          // 1: items are not split; no workspace, no second launch
+  int min_units;      // of a workgroup, so that small calls are not cut into crumbs
+  int* meta;          // workspace: [workgroups][kMeta]
+  float* part_ml;     // [2 workgroups][ROWS][2]: maximum (base 2) and sum
+  float* part_o;      // [2 workgroups][ROWS][D]
+};
+
+// meta of a workgroup: first unit, first and last unit (exclusive) of the item that it starts in, that item's first row of q, its
+// valid rows, key head, first row; workgroups with work, units
+enum { kMetaU0, kMetaBegin, kMetaEnd, kMetaFirst, kMetaRows, kMetaHead, kMetaRow0, kMetaParts, kMetaUnits, kMeta = 12 };
+
+struct Sequence {
+  int first, n, len;   // first row of q, new tokens, keys
+};
+__device__ inline Sequence sequence(const AttnArgs& p, int b) {
+  Sequence s;
+  if (p.a.cu_q) {
+    s.first = p.a.cu_q[b];
+    s.first = s.first < 0 ? 0 : s.first > p.a.tokens ? p.a.tokens : s.first;
+    int end = p.a.cu_q[b + 1];
+    end = end < s.first ? s.first : end > p.a.tokens ? p.a.tokens : end;
+    s.n = end - s.first;
+  } else {
+    s.first = b, s.n = 1;
+  }
+  const int most = p.a.table_pages << p.page_shift;
+  s.len = p.a.seq_lens[b];
+  s.len = s.len < 0 ? 0 : s.len > most ? most : s.len;
+  return s;
+}
+
+// Keys that new token t of a sequence sees: [lo, hi)
+__device__ inline void visible(const AttnArgs& p, const Sequence& s, int t, int& lo, int& hi) {
+  const int pos = s.len - s.n + t;
+  hi = p.a.causal ? pos + 1 : s.len;
+  hi = hi < 0 ? 0 : hi;
+  lo = p.a.window > 0 && pos >= p.a.window ? pos - p.a.window + 1 : 0;
+}
+
+// A block of rows: units, and the first tile
+template <int ROWS, int TILE>
+__device__ inline int block_units(const AttnArgs& p, const Sequence& s, int row0, int& tile0) {
+  const int rows = s.n * p.group, last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
+  int lo, hi, other;
+  if (rows <= 0) {
+    tile0 = 0;
+    return 1;
+  }
+  visible(p, s, row0 / p.group, lo, other);
+  visible(p, s, last / p.group, other, hi);
+  tile0 = lo / TILE;
+  return hi > lo ? (hi + TILE - 1) / TILE - tile0 : 1;
+}
+template <int ROWS, int TILE>
+__device__ inline int sequence_units(const AttnArgs& p, const Sequence& s) {   // of one key head
+  int u = 0, tile0;
+  for (int row0 = 0; row0 < s.n * p.group; row0 += ROWS) u += block_units<ROWS, TILE>(p, s, row0, tile0);
+  return u;
+}
+
+__device__ inline unsigned wave_scan(unsigned v) {   // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const unsigned o = (unsigned)__shfl_up((int)v, d, 64);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// The part of a workgroup: units [u0, u1) of all `units`, cut into `parts` equal ones; sequence b holds u0, b_begin is its first unit.
+struct Part {
+  unsigned u0, u1, units, parts;
+  int b;
+  unsigned b_begin;
+};
+struct PartLds {
+  unsigned sums[16];
+  int b;
+  unsigned begin;
+};
+
+// First unit of part g (32 x 32 bits)
+__device__ inline unsigned part_start(unsigned units, unsigned parts, unsigned g) { return (unsigned)((uint64_t)units * g / parts); }
+
+template <int ROWS, int TILE, int THREADS>
+__device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgroups, PartLds& lds) {
+  constexpr int W = THREADS / 64;
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+  const auto units_of = [&](int b) -> unsigned { return b < p.a.batch ? (unsigned)(sequence_units<ROWS, TILE>(p, sequence(p, b)) * p.c.kv_heads) : 0u; };
+  const auto chunk_scan = [&](unsigned mine, unsigned& total) {   // inclusive prefix of the threads of the workgroup
+    unsigned in = wave_scan(mine);
+    __syncthreads();
+    if (lane == 63) lds.sums[wave] = in;
+    __syncthreads();
+    unsigned before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w == wave) before = total;
+      total += lds.sums[w];
+    }
+    return in + before;
+  };
+  unsigned mine = units_of(tid), total, all;
+  unsigned in = chunk_scan(mine, total);
+  all = total;
+  for (int b0 = THREADS; b0 < p.a.batch; b0 += THREADS) {   // (more sequences than threads: added up first, searched below)
+    unsigned t;
+    chunk_scan(units_of(b0 + tid), t);
+    all += t;
+  }
+  Part r;
+  r.units = all;
+  const unsigned want = (all + (unsigned)p.min_units - 1) / (unsigned)p.min_units;
+  r.parts = want < workgroups ? (want ? want : 1) : workgroups;
+  r.u0 = g < r.parts ? part_start(all, r.parts, g) : all;
+  r.u1 = g < r.parts ? part_start(all, r.parts, g + 1) : all;
+  r.b = 0, r.b_begin = 0;
+  if (r.u0 >= r.u1) return r;
+  unsigned base = 0;
+  for (int b0 = 0;;) {
+    if (r.u0 < base + total) {   // in this chunk of sequences
+      const unsigned begin = base + in - mine;
+      if (mine && begin <= r.u0 && r.u0 < begin + mine) lds.b = b0 + tid, lds.begin = begin;
+      break;
+    }
+    base += total;
+    b0 += THREADS;
+    mine = units_of(b0 + tid);
+    in = chunk_scan(mine, total);
+  }
+  __syncthreads();
+  r.b = __builtin_amdgcn_readfirstlane(lds.b);
+  r.b_begin = (unsigned)__builtin_amdgcn_readfirstlane((int)lds.begin);
+  return r;
+}
+
+// An item, and where the units of a walk stand in it
+struct Item {
+  Sequence s;
+  int head, row0, tile0;
+  unsigned begin, units;
+};
+// The item that holds unit u >= b_begin; moves b and b_begin on to its sequence.
+template <int ROWS, int TILE>
+__device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& b_begin) {
+  Item it;
+  unsigned per_head;
+  for (;;) {   // (u is below the number of all units; the bounds on b and row0 hold if lengths change under the call, too)
+    it.s = sequence(p, b);
+    per_head = (unsigned)sequence_units<ROWS, TILE>(p, it.s);
+    if (u < b_begin + per_head * (unsigned)p.c.kv_heads || b + 1 >= p.a.batch) break;
+    b_begin += per_head * (unsigned)p.c.kv_heads;
+    ++b;
+  }
+  it.head = per_head ? (int)((u - b_begin) / per_head) : 0;
+  it.head = it.head < p.c.kv_heads ? it.head : p.c.kv_heads - 1;
+  it.begin = b_begin + (unsigned)it.head * per_head;
+  for (it.row0 = 0;; it.row0 += ROWS) {
+    it.units = (unsigned)block_units<ROWS, TILE>(p, it.s, it.row0, it.tile0);
+    if (u < it.begin + it.units || it.row0 + ROWS >= it.s.n * p.group) break;
+    it.begin += it.units;
+  }
+  return it;
+}
+
+// ---- loads ---------------------------------------------------------------------------------------------------------------------
+// Lane l of the wave writes its 16 (4) bytes at LDS address lds + 16 l (4 l), straight from memory; counts on vmcnt.
+__device__ inline void to_lds16(const uint8_t* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
+}
+__device__ inline void to_lds4(const uint8_t* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
+}
+template <int N>
+__device__ inline void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;   // read through the scalar cache where the index is uniform
+
+// Page of tokens 16 i .. 16 i + 15 of a sequence; a valid one whatever the table holds (tokens behind the last key: the last key's)
+__device__ inline int page_at(const AttnArgs& p, ConstInts row, int token, int len) {
+  const int t = token < len ? token : len > 0 ? len - 1 : 0;
+  int page = p.a.table_pages > 0 ? row[t >> p.page_shift] : 0;
+  page = page < 0 ? 0 : page;
+  return page < p.c.pages ? page : p.c.pages - 1;
+}
+
+// Eight bf16 from any address
+__device__ inline v4i load8_bf16(const uint16_t* q) {
+  if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) return *reinterpret_cast<const v4i*>(q);
+  v4i r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (int)((unsigned)q[2 * i] | (unsigned)q[2 * i + 1] << 16);
+  return r;
+}
+__device__ inline float bf16_lo(int x) { return __builtin_bit_cast(float, (unsigned)x << 16); }
+__device__ inline float bf16_hi(int x) { return __builtin_bit_cast(float, (unsigned)x & 0xFFFF0000u); }
+
+// ---- queries: two 8-bit parts ------------------------------------------------------------------------------------------------------
+// The scaled MFMAs multiply E2M1 keys as they are with 8-bit queries.  A bf16 number has 8 significant bits, an E4M3 number 4:
+// q = 2^e hi + 2^(e-5) lo, hi the rounded q / 2^e and lo the rounded rest times 32, is exact down to 2^-19 of the row's largest element
+// (e puts that one into [2^7, 2^8)); two MFMAs take the time that one bf16 product of the same length would, and no key is converted.
+struct QueryScale {
+  float inv;      // 2^-e, negative for a negative softmax scale
+  int hi, lo;     // E8M0 bytes; 0xFF (NaN) for a row with an infinity or a NaN
+};
+__device__ inline QueryScale query_scale(unsigned amax_bits, bool negative) {
+  int f = (int)(amax_bits >> 23);
+  if (f == 0xFF) return {0.0f, 0xFF, 0xFF};
+  f = f < 13 ? 13 : f;   // e + 127 = f - 7
+  const float inv = __builtin_bit_cast(float, (unsigned)(261 - f) << 23);
+  return {negative ? -inv : inv, f - 7, f - 12};
+}
+__device__ inline void split_query(v4i x, float inv, int& h0, int& h1, int& l0, int& l1) {   // eight bf16 -> 2 x 4 bytes of each part
+  float v[8], r[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(x[i]) * inv, v[2 * i + 1] = bf16_hi(x[i]) * inv;
+  h0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  h0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], h0, true);
+  h1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+  h1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], h1, true);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int w = i < 2 ? h0 : h1;
+    const v2f b = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+    r[2 * i] = (v[2 * i] - b[0]) * 32.0f, r[2 * i + 1] = (v[2 * i + 1] - b[1]) * 32.0f;
+  }
+  l0 = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+  l0 = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], l0, true);
+  l1 = __builtin_amdgcn_cvt_pk_fp8_f32(r[4], r[5], 0, false);
+  l1 = __builtin_amdgcn_cvt_pk_fp8_f32(r[6], r[7], l1, true);
+}
+__device__ inline unsigned amax_bits8(v4i x, unsigned m) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned a = ((unsigned)x[i] << 16) & 0x7FFFFFFFu, b = (unsigned)x[i] & 0x7FFF0000u;
+    m = m > a ? m : a;
+    m = m > b ? m : b;
+  }
+  return m;
+}
+// NaN > infinity > numbers as bit patterns, so this is the row's largest magnitude or 0x7F8..... and more
+
+// Largest value of lanes l, l ^ 16, l ^ 32, l ^ 48 (XOR16) or l, l ^ 32
+__device__ inline float max_of_swapped(unsigned a, unsigned b) { return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)); }
+template <bool XOR16>
+__device__ inline float cross_max(float v) {   // (a vector's element is copied before __builtin_bit_cast, which reads element 0 of it otherwise)
+  unsigned a = __builtin_bit_cast(unsigned, v);
+  auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  v = max_of_swapped(r[0], r[1]);
+  if constexpr (XOR16) {
+    a = __builtin_bit_cast(unsigned, v);
+    r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    v = max_of_swapped(r[0], r[1]);
+  }
+  return v;
+}
+template <bool XOR16>
+__device__ inline float cross_sum(float v) {
+  v += __shfl_xor(v, 32, 64);
+  if constexpr (XOR16) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+// A row's place in the output: (token, query head)
+__device__ inline size_t row_index(const AttnArgs& p, int first, int head, int row) {
+  return (size_t)(first + row / p.group) * p.a.heads + head * p.group + row % p.group;
+}
+
+// Four channels of a finished row: o / l, with the sink's share of the sum; m in base 2 (-inf: the row saw nothing).
+__device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int channel, v4f o, float m, float l) {
+  const int head = (int)(row % (unsigned)p.a.heads);
+  const bool none = m == -INFINITY && l == l;   // (only NaN scores: the sum is NaN)
+  float total = l, top = m, fade = 1.0f;
+  if (p.a.sinks) {
+    const float sink = p.a.sinks[head] * kLog2e;
+    top = fmaxf(m, sink);
+    fade = none ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    total = l * fade + (sink == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sink - top));
+  }
+  const float f = none ? 0.0f : fade / total;
+  uint16_t* out = p.a.out + row * D + channel;
+  reinterpret_cast<unsigned*>(out)[0] = pack_bf16x2(o[0] * f, o[1] * f);
+  reinterpret_cast<unsigned*>(out)[1] = pack_bf16x2(o[2] * f, o[3] * f);
+  if (p.a.lse && channel == 0) p.a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* workspace, hipStream_t s);
+size_t attn_decode_workspace(const AttnArgs& p, int row_tiles);
+hipError_t launch_attn_combine(const AttnArgs& p, int rows, int workgroups, hipStream_t s);
+// meta, maxima and sums, partial results, in this order
+inline size_t attn_workspace(int rows, int head_dim, int workgroups) {
+  const size_t meta = ((size_t)workgroups * kMeta * 4 + 255) / 256 * 256;
+  return meta + (size_t)workgroups * 2 * rows * (2 + head_dim) * 4;
+}
+inline void place_workspace(AttnArgs& p, int rows, int workgroups, void* ws) {
+  p.meta = static_cast<int*>(ws);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + ((size_t)workgroups * kMeta * 4 + 255) / 256 * 256);
+  p.part_o = p.part_ml + (size_t)workgroups * 2 * rows * 2;
+}
+}  // namespace ave

@@ -1,0 +1,455 @@
+// Attention of few query rows over a paged MXFP4 cache: single tokens of a decode batch, a handful of tokens of a draft.
+//
+// Bound by HBM: a token's key and value are 34 bytes per 32 channels, read once.  A workgroup walks its share of the call's
+// units (64 keys, attn_common.hpp); its waves take the units of an item in turn, each through LDS stages of its own that are filled
+// straight from memory, and meet at the item's end only.
+//
+//   S^T = K Q^T   scaled MFMA 16x16x128, keys as they are (E2M1, E8M0), queries as two E4M3 parts.  Which token is row r of key
+//                 tile j is free: token 16 (r / 4) + 4 j + r % 4, so that lane group g = lane / 16 of the result holds the scores of
+//                 tokens 16 g .. 16 g + 15 for query row lane % 16.
+//   P             bf16 of exp(s - max), the running maximum shared by the four groups; sums per lane, in fp32, of what is not rounded
+//   O^T = V^T P^T bf16 MFMA 16x16x32: lane group g multiplies its own 16 tokens, so P stays in its registers.  A transposing LDS read
+//                 (4 bits) gives a lane 16 tokens' codes of one channel, two per conversion.  The E8M0 scales of the values differ from
+//                 token to token, the contracted axis: they go into P as integer additions to the bf16 exponent, one copy of P per
+//                 32 channels -- exact, saturating at zero.
+#include "attn_common.hpp"
+#include "kernels.hpp"
+
+namespace ave {
+namespace {
+
+template <int D>
+struct Shape {
+  static constexpr int kRow = D / 2, kBlocks = D / 32;                     // bytes of a token's codes and scales
+  static constexpr int kCodes = 64 * kRow, kScales = 64 * kBlocks;         // of a stage
+  static constexpr int kStage = 2 * kCodes + 2 * kScales;
+  static constexpr int kLoads = 2 * (kCodes / 1024) + (D == 64 ? 1 : 2 * kScales / 256);
+  // 16-byte pieces of a row are permuted in LDS so that the 16 lanes of a read touch different banks
+  __device__ static int key_swizzle(int t) { return D == 64 ? (t >> 4) & 1 : D == 128 ? (t >> 4) & 3 : ((t >> 1) & 1) | ((t >> 4) & 3) << 1; }
+  __device__ static int value_swizzle(int t) { return D == 64 ? (t >> 3) & 1 : D == 128 ? (t >> 2) & 3 : (t >> 1) & 7; }
+};
+
+__device__ inline unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+__device__ inline us2 as_us2(unsigned x) { return __builtin_bit_cast(us2, x); }
+__device__ inline unsigned as_u32(us2 x) { return __builtin_bit_cast(unsigned, x); }
+
+// Requests the 64 keys and values from token t0 on (a multiple of 64) of a sequence of len > 0 keys into the stage at `lds`.
+template <int D>
+__device__ inline void request_stage(const AttnArgs& p, ConstInts table, int len, int head, int t0, unsigned lds) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 63;
+  int page[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) page[i] = page_at(p, table, t0 + 16 * i, len);
+  const int mask = p.c.page_size - 1;
+  // codes: 1 KB an instruction
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint8_t* base = kv ? p.c.v : p.c.k;
+    const int64_t stride = kv ? p.c.v_page_stride : p.c.k_page_stride;
+#pragma unroll
+    for (int i = 0; i < S::kCodes / 1024; ++i) {
+      constexpr int kPieces = S::kRow / 16, kTokens = 1024 / S::kRow;   // pieces of a row, tokens of an instruction
+      const int t = i * kTokens + lane / kPieces;
+      const int piece = (lane % kPieces) ^ (kv ? S::value_swizzle(t) : S::key_swizzle(t));
+      const int pg = kTokens > 16 ? (lane < 32 ? page[(2 * i) & 3] : page[(2 * i + 1) & 3]) : page[i * kTokens / 16];
+      const uint8_t* src = base + pg * stride + ((size_t)head * p.c.page_size + ((t0 + t) & mask)) * S::kRow + piece * 16;
+      to_lds16(src, lds + kv * S::kCodes + i * 1024);
+    }
+  }
+  // scales: a lane's four bytes belong to the tokens of one group of 16
+  const auto scales = [&](int kv, int offset) {   // of the stage's kScales bytes
+    const int t = offset / S::kBlocks;
+    const int pg = t < 32 ? (t < 16 ? page[0] : page[1]) : (t < 48 ? page[2] : page[3]);
+    return (kv ? p.c.v_scale + pg * p.c.v_scale_page_stride : p.c.k_scale + pg * p.c.k_scale_page_stride) +
+           ((size_t)head * p.c.page_size + ((t0 + t) & mask)) * S::kBlocks + offset % S::kBlocks;
+  };
+  if constexpr (D == 64) {
+    to_lds4(scales(lane / 32, lane % 32 * 4), lds + 2 * S::kCodes);   // keys' scales by lanes 0-31, values' by 32-63
+  } else {
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int i = 0; i < S::kScales / 256; ++i)
+        to_lds4(scales(kv, i * 256 + lane * 4), lds + 2 * S::kCodes + kv * S::kScales + i * 256);
+  }
+}
+
+// The queries of a block of rows: 16 rows a tile, a tile's parts in the layout of the 16x16x128 MFMA (lane: column lane % 16; bytes 0-15 are
+// k = 16 g .., bytes 16-31 k = 64 + 16 g ..).  D = 64: one MFMA takes both parts, the second in the place of k >= 64.
+template <int D, int NT>
+struct Queries {
+  static constexpr int kSteps = D == 64 ? 1 : D / 128;
+  v8i hi[NT][kSteps], lo[NT][D == 64 ? 1 : kSteps];
+  int s_hi[NT], s_lo[NT];
+
+  __device__ inline void load(const AttnArgs& p, const Item& it, int rows) {
+    const int lane = threadIdx.x & 63, g = lane / 16;
+    const bool negative = p.a.scale < 0.0f;
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      const int row = it.row0 + ct * 16 + lane % 16;
+      const bool real = row < rows;
+      const uint16_t* q = p.a.q + (int64_t)(it.s.first + (real ? row / p.group : 0)) * p.a.q_token_stride +
+                          (int64_t)(it.head * p.group + (real ? row % p.group : 0)) * p.a.q_head_stride;
+      v4i x[D / 32];   // eight channels each: pairs of them at 16 g + 64 i
+      unsigned amax = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        x[i] = v4i{0, 0, 0, 0};
+        if (real) x[i] = load8_bf16(q + (i / 2) * 64 + g * 16 + (i % 2) * 8);
+        amax = amax_bits8(x[i], amax);
+      }
+      amax = lane_xor_max_bits(lane_xor_max_bits(amax, 16), 32);
+      const QueryScale s = query_scale(amax, negative);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        int h0, h1, l0, l1;
+        split_query(x[i], s.inv, h0, h1, l0, l1);
+        if (s.hi == 0xFF) h0 = h1 = l0 = l1 = 0;
+        if constexpr (D == 64) {
+          hi[ct][0][i * 2] = h0, hi[ct][0][i * 2 + 1] = h1, hi[ct][0][4 + i * 2] = l0, hi[ct][0][4 + i * 2 + 1] = l1;
+        } else {
+          hi[ct][i / 4][i % 4 * 2] = h0, hi[ct][i / 4][i % 4 * 2 + 1] = h1, lo[ct][i / 4][i % 4 * 2] = l0, lo[ct][i / 4][i % 4 * 2 + 1] = l1;
+        }
+      }
+      s_hi[ct] = D == 64 && g >= 2 ? s.lo : s.hi;
+      s_lo[ct] = s.lo;
+    }
+  }
+};
+
+template <int D, int NT, int NW, int NS>
+__global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p) {
+  using S = Shape<D>;
+  constexpr int ROWS = NT * 16, TILE = 64, C = D / 16;   // C: channel tiles of 16
+  constexpr int kPitch = D + 4;                          // floats of a row of a wave's result in LDS
+  constexpr int kRing = NW * NS * S::kStage, kJoin = NW * ROWS * kPitch * 4;
+  __shared__ __align__(16) unsigned char smem[kRing > kJoin ? kRing : kJoin];
+  __shared__ float join_ml[NW][ROWS][2];
+  __shared__ PartLds part_lds;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane / 16, col = lane % 16;
+  const Part part = take_part<ROWS, TILE, NW * 64>(p, blockIdx.x, gridDim.x, part_lds);
+  const unsigned ring = (unsigned)__builtin_amdgcn_readfirstlane(lds_address(smem)) + wave * NS * S::kStage;
+  const unsigned char* ring_ptr = smem + wave * NS * S::kStage;
+  const float c = fabsf(p.a.scale) * kLog2e;
+  int b = part.b;
+  unsigned b_begin = part.b_begin;
+  bool first_item = true;
+  if (!p.whole && threadIdx.x == 0 && part.u0 >= part.u1) {   // no work
+    int* m = p.meta + (size_t)blockIdx.x * kMeta;
+    m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
+    m[kMetaParts] = (int)part.parts, m[kMetaUnits] = (int)part.units;
+  }
+  for (unsigned u = part.u0; u < part.u1;) {
+    const Item it = item_of<ROWS, TILE>(p, u, b, b_begin);
+    const unsigned end = it.begin + it.units;
+    unsigned from = u, to = end < part.u1 ? end : part.u1;
+    if (!p.whole) {
+      if (first_item && threadIdx.x == 0) {
+        int* m = p.meta + (size_t)blockIdx.x * kMeta;
+        m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)end, m[kMetaFirst] = it.s.first;
+        m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
+        m[kMetaParts] = (int)part.parts, m[kMetaUnits] = (int)part.units;
+      }
+      u = to;
+    } else {   // the items that start in this part, as wholes
+      u = end;
+      if (it.begin < part.u0) {
+        first_item = false;
+        continue;
+      }
+      to = end;
+    }
+    const int rows = it.s.n * p.group;
+    const int tile0 = it.tile0 + (int)(from - it.begin), tiles = (int)(to - from);
+    const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
+
+    // what the rows see
+    int lo_row[NT], hi_row[NT], lo_max, hi_min, dummy;
+    {
+      const int last = it.row0 + ROWS < rows ? it.row0 + ROWS - 1 : rows - 1;
+      visible(p, it.s, it.row0 / p.group, dummy, hi_min);
+      visible(p, it.s, last / p.group, lo_max, dummy);
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        const int row = it.row0 + ct * 16 + col;
+        visible(p, it.s, (row < rows ? row : last) / p.group, lo_row[ct], hi_row[ct]);
+      }
+    }
+    const int mine = it.s.len > 0 && tiles > wave ? (tiles - wave + NW - 1) / NW : 0;   // tiles wave, wave + NW, ...
+    int requested = 0;
+    for (; requested < NS - 1 && requested < mine; ++requested)
+      request_stage<D>(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + requested * S::kStage);
+
+    Queries<D, NT> q;
+    q.load(p, it, rows);
+
+    v4f acc[NT][C];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      m[ct] = kNone, l[ct] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < C; ++i) acc[ct][i] = v4f{0, 0, 0, 0};
+    }
+
+    for (int i = 0; i < mine; ++i) {
+      const int t0 = (tile0 + wave + i * NW) * TILE;
+      if (requested < mine) {
+        request_stage<D>(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + (requested % NS) * S::kStage);
+        ++requested;
+        wait_loads<(NS - 1) * S::kLoads>();
+      } else {
+        const int behind = mine - 1 - i;   // stages requested behind this one: fewer than NS - 1
+        if (NS > 3 && behind >= 2) wait_loads<(NS > 3 ? 2 : 0) * S::kLoads>();
+        else if (NS > 2 && behind >= 1) wait_loads<(NS > 2 ? 1 : 0) * S::kLoads>();
+        else wait_loads<0>();
+      }
+      const unsigned char* st = ring_ptr + (i % NS) * S::kStage;
+      const unsigned char *keys = st, *values = st + S::kCodes, *ks = st + 2 * S::kCodes, *vs = ks + S::kScales;
+
+      // ---- scores
+      v4f s[NT][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = 16 * (col / 4) + 4 * j + col % 4;
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) s[ct][j] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int step = 0; step < Queries<D, NT>::kSteps; ++step) {
+          const int block = D == 64 ? g % 2 : step * 4 + g;
+          const v4i x = *reinterpret_cast<const v4i*>(keys + t * S::kRow + (block ^ S::key_swizzle(t)) * 16);
+          const int sk = ks[t * S::kBlocks + block];
+          const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+#pragma unroll
+          for (int ct = 0; ct < NT; ++ct) {
+            if constexpr (D != 64)
+              s[ct][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x8, q.lo[ct][step], s[ct][j], kFmtFp4, 0, 0, sk, 0, q.s_lo[ct]);
+            s[ct][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x8, q.hi[ct][step], s[ct][j], kFmtFp4, 0, 0, sk, 0, q.s_hi[ct]);
+          }
+        }
+      }
+
+      // ---- probabilities
+      const bool all_seen = t0 >= lo_max && t0 + TILE <= hi_min;
+      us2 prob[NT][8], bias[NT][8];   // pairs of tokens 16 g + 2 i, + 1; what is taken from their exponents
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        bool seen[16];
+        if (!all_seen) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const int key = t0 + 16 * g + 4 * j + t;
+              seen[4 * j + t] = key >= lo_row[ct] && key < hi_row[ct];
+              if (!seen[4 * j + t]) s[ct][j][t] = kNone;
+            }
+        }
+        float top = kNone;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fmaxf(s[ct][j][0], s[ct][j][1]), fmaxf(s[ct][j][2], s[ct][j][3])));
+        top = fmaxf(m[ct], cross_max<true>(top));
+        if (__any(top > m[ct])) {
+          const float fade = __builtin_amdgcn_exp2f((m[ct] - top) * c);
+          l[ct] *= fade;
+#pragma unroll
+          for (int k = 0; k < C; ++k) acc[ct][k] *= fade;
+          m[ct] = top;
+        }
+        const float shift = -m[ct] * c;
+        float pr[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j / 4][j % 4], c, shift));
+          if (!all_seen && !seen[j]) pr[j] = 0.0f;
+          l[ct] += pr[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          prob[ct][j] = as_us2(pack_bf16x2(pr[2 * j], pr[2 * j + 1]));
+          // 127 in the exponent's place, or more than everything for a probability of zero, which stays zero
+          const us2 zero = __builtin_elementwise_sub_sat(us2{1, 1}, prob[ct][j]);
+          bias[ct][j] = zero * us2{0xC07F, 0xC07F} + us2{0x3F80, 0x3F80};
+        }
+      }
+
+      // ---- values: a scale byte 0xFF (NaN) anywhere in the stage?  (also in what no key occupies: no row sees that)
+      bool nan = false;
+#pragma unroll
+      for (int k = 0; k < (S::kScales + 255) / 256; ++k) {
+        const int at = k * 256 + lane * 4;
+        const unsigned x = ~*reinterpret_cast<const unsigned*>(vs + (at < S::kScales ? at : 0));
+        nan = nan || ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
+      }
+      nan = __any(nan);
+#pragma unroll
+      for (int blk = 0; blk < S::kBlocks; ++blk) {
+        // P with the scales of this block of channels
+        v4i ps[NT][2];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          unsigned e2;   // the scale bytes of tokens 16 g + 2 k and + 1, in 16 bits each
+          if constexpr (D == 64) {
+            const unsigned w = reinterpret_cast<const unsigned*>(vs)[g * 8 + k];
+            e2 = __builtin_amdgcn_perm(w, w, blk ? 0x0c030c01u : 0x0c020c00u);
+          } else {
+            constexpr int kWords = S::kBlocks / 4;
+            const unsigned w0 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k) * kWords + blk / 4];
+            const unsigned w1 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k + 1) * kWords + blk / 4];
+            e2 = __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + 0x00010001u * (blk % 4));
+          }
+          const us2 e = as_us2(e2);
+#pragma unroll
+          for (int ct = 0; ct < NT; ++ct) {
+            us2 r = __builtin_elementwise_sub_sat(e * us2{128, 128} + prob[ct][k], bias[ct][k]);
+            if (nan) {   // NaN where the scale is one and the probability is not zero
+              const us2 is = __builtin_elementwise_sub_sat(e, us2{254, 254}) * __builtin_elementwise_min(prob[ct][k], us2{1, 1});
+              r = __builtin_elementwise_max(r, is * us2{0x7FC0, 0x7FC0});
+            }
+            ps[ct][k / 4][k % 4] = (int)as_u32(r);
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int ch = blk * 2 + half;
+          const int t = 16 * g + col;
+          const unsigned char* at = values + t * S::kRow + (blk ^ S::value_swizzle(t)) * 16 + half * 8;
+          const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) v2i*)at);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const unsigned x = (unsigned)w[k];
+            const v2bf a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, 1.0f, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, 1.0f, 1);
+            const v2bf a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, 1.0f, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, 1.0f, 3);
+            const v8bf a = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+#pragma unroll
+            for (int ct = 0; ct < NT; ++ct)
+              acc[ct][ch] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(v8bf, ps[ct][k]), acc[ct][ch], 0, 0, 0);
+          }
+        }
+      }
+    }
+
+    // ---- the waves' results joined
+    __syncthreads();   // (no load is under way any more: every wave has waited for its last one)
+    float* mine_o = reinterpret_cast<float*>(smem) + (size_t)wave * ROWS * kPitch;
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      const float sum = cross_sum<true>(l[ct]);
+      if (g == 0) {
+        join_ml[wave][ct * 16 + col][0] = m[ct] == kNone ? -INFINITY : m[ct] * c;
+        join_ml[wave][ct * 16 + col][1] = sum;
+      }
+#pragma unroll
+      for (int k = 0; k < C; ++k) *reinterpret_cast<v4f*>(mine_o + (ct * 16 + col) * kPitch + k * 16 + g * 4) = acc[ct][k];
+    }
+    __syncthreads();
+    const bool done = from == it.begin && to == end;
+    const int valid = rows - it.row0 < ROWS ? rows - it.row0 : ROWS;
+    const size_t slot = 2 * (size_t)blockIdx.x + (it.begin >= part.u0 ? 1 : 0);
+    for (int at = threadIdx.x; at < valid * (D / 4); at += NW * 64) {
+      const int row = at / (D / 4), ch = at % (D / 4) * 4;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, join_ml[w][row][0]);
+      v4f o = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = join_ml[w][row][0];
+        const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+        sum += join_ml[w][row][1] * f;
+        o += *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(smem) + ((size_t)w * ROWS + row) * kPitch + ch) * f;
+      }
+      if (done) {
+        finish_row(p, row_index(p, it.s.first, it.head, it.row0 + row), D, ch, o, top, sum);
+      } else {
+        *reinterpret_cast<v4f*>(p.part_o + (slot * ROWS + row) * D + ch) = o;
+        if (ch == 0) p.part_ml[(slot * ROWS + row) * 2] = top, p.part_ml[(slot * ROWS + row) * 2 + 1] = sum;
+      }
+    }
+    __syncthreads();   // before the next item's loads
+    first_item = false;
+  }
+}
+
+template <int D, int NT, int NW, int NS>
+hipError_t launch_form(AttnArgs p, void* ws, hipStream_t s) {
+  constexpr int ROWS = NT * 16;
+  const int workgroups = compute_units();
+  p.min_units = NW;
+  // items of at most two rounds of the waves stay whole: cutting them saves less than the second launch costs
+  p.whole = ((int64_t)p.a.table_pages << p.page_shift) <= 2 * NW * 64;
+  if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
+  hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS>), dim3((unsigned)workgroups), dim3(NW * 64), 0, s, p);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || p.whole) return e;
+  return launch_attn_combine(p, ROWS, workgroups, s);
+}
+
+}  // namespace
+
+size_t attn_decode_workspace(const AttnArgs& p, int row_tiles) { return attn_workspace(row_tiles * 16, p.c.head_dim, compute_units()); }
+
+hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s) {
+  switch (p.c.head_dim * 8 + row_tiles) {
+    case 64 * 8 + 1: return launch_form<64, 1, 8, 4>(p, ws, s);
+    case 64 * 8 + 2: return launch_form<64, 2, 8, 4>(p, ws, s);
+    case 64 * 8 + 4: return launch_form<64, 4, 4, 4>(p, ws, s);
+    case 128 * 8 + 1: return launch_form<128, 1, 8, 2>(p, ws, s);
+    case 128 * 8 + 2: return launch_form<128, 2, 8, 2>(p, ws, s);
+    case 128 * 8 + 4: return launch_form<128, 4, 4, 4>(p, ws, s);
+    case 256 * 8 + 1: return launch_form<256, 1, 4, 2>(p, ws, s);
+    default: return launch_form<256, 2, 4, 2>(p, ws, s);
+  }
+}
+
+// ---- parts of split items, joined -----------------------------------------------------------------------------------------------
+namespace {
+
+// blockIdx.x: a boundary between two workgroups of the first launch; the first boundary inside an item joins its parts.
+template <int D>
+__global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS) {
+  const int g = blockIdx.x + 1;
+  const int* m = p.meta + (size_t)g * kMeta;
+  const unsigned begin = (unsigned)m[kMetaBegin], end = (unsigned)m[kMetaEnd], u0 = (unsigned)m[kMetaU0];
+  if (begin >= u0 || (unsigned)m[kMetaU0 - kMeta] > begin) return;
+  const unsigned parts = (unsigned)m[kMetaParts], units = (unsigned)m[kMetaUnits];
+  int last = g;   // the last workgroup that starts inside the item
+  while (last + 1 < (int)parts && part_start(units, parts, (unsigned)last + 1) < end) ++last;
+  const int rows = m[kMetaRows], row0 = m[kMetaRow0];
+  const int valid = rows - row0 < ROWS ? rows - row0 : ROWS;
+  constexpr int kRowsAtOnce = 256 / (D / 4);
+  const int row = blockIdx.y * kRowsAtOnce + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
+  if (row >= valid) return;
+  const size_t before = 2 * (size_t)(g - 1) + 1;   // the part of the workgroup that the item starts in; then 2 g, 2 (g + 1), ...
+  const auto slot = [&](int i) { return i == 0 ? before : 2 * (size_t)(g + i - 1); };
+  const int n = last - g + 2;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_ml[(slot(i) * ROWS + row) * 2]);
+  v4f o = {0, 0, 0, 0};
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const size_t at = slot(i) * ROWS + row;
+    const float mw = p.part_ml[at * 2], f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+    sum += p.part_ml[at * 2 + 1] * f;
+    o += *reinterpret_cast<const v4f*>(p.part_o + at * D + ch) * f;
+  }
+  finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
+}
+
+}  // namespace
+
+hipError_t launch_attn_combine(const AttnArgs& p, int rows, int workgroups, hipStream_t s) {
+  const int at_once = 1024 / p.c.head_dim;
+  const dim3 grid((unsigned)workgroups - 1, (unsigned)((rows + at_once - 1) / at_once));
+  if (p.c.head_dim == 64) hipLaunchKernelGGL((attn_combine_kernel<64>), grid, dim3(256), 0, s, p, rows);
+  else if (p.c.head_dim == 128) hipLaunchKernelGGL((attn_combine_kernel<128>), grid, dim3(256), 0, s, p, rows);
+  else hipLaunchKernelGGL((attn_combine_kernel<256>), grid, dim3(256), 0, s, p, rows);
+  return hipGetLastError();
+}
+
+}  // namespace ave
