@@ -122,7 +122,7 @@ namespace {
 AttnArgs args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
   AttnArgs p{};
   p.a = a, p.c = c;
-  p.group = a.heads / c.kv_heads;
+  set_group(p, a.heads / c.kv_heads);
   p.page_shift = log2_of(c.page_size);
   return p;
 }

@@ -30,7 +30,18 @@ struct AttnArgs {
   int* meta;          // workspace: [workgroups][kMeta]
   float* part_ml;     // [2 workgroups][ROWS][2]: maximum (base 2) and sum
   float* part_o;      // [2 workgroups][ROWS][D]
+  unsigned group_mul, group_shift;   // division by `group` of numbers below 2^31: high word of the product, shifted (set_group)
+
+  __device__ inline int token_of(int row) const { return group == 1 ? row : (int)(__umulhi((unsigned)row, group_mul) >> group_shift); }
 };
+// 2^(31+s) / d rounded up with s = ceil(log2 d) has an error below 2^-31 of a quotient, so that n < 2^31 is divided exactly.
+inline void set_group(AttnArgs& p, int group) {
+  p.group = group;
+  int s = 0;
+  while ((1 << s) < group) ++s;
+  p.group_mul = group == 1 ? 0 : (unsigned)((((uint64_t)1 << (31 + s)) / (unsigned)group) + 1);
+  p.group_shift = group == 1 ? 0 : (unsigned)(s - 1);
+}
 
 // meta of a workgroup: first unit, first and last unit (exclusive) of the item that it starts in, that item's first row of q, its
 // valid rows, key head, first row; workgroups with work, units
@@ -73,8 +84,8 @@ __device__ inline int block_units(const AttnArgs& p, const Sequence& s, int row0
     tile0 = 0;
     return 1;
   }
-  visible(p, s, row0 / p.group, lo, other);
-  visible(p, s, last / p.group, other, hi);
+  visible(p, s, p.token_of(row0), lo, other);
+  visible(p, s, p.token_of(last), other, hi);
   tile0 = lo / TILE;
   return hi > lo ? (hi + TILE - 1) / TILE - tile0 : 1;
 }
@@ -99,12 +110,14 @@ __device__ inline unsigned wave_scan(unsigned v) {   // inclusive
 struct Part {
   unsigned u0, u1, units, parts;
   int b;
-  unsigned b_begin;
+  unsigned b_begin, per_head;
+  Sequence s;
 };
 struct PartLds {
   unsigned sums[16];
   int b;
-  unsigned begin;
+  unsigned begin, per_head;
+  Sequence s;
 };
 
 // First unit of part g (32 x 32 bits)
@@ -114,7 +127,13 @@ template <int ROWS, int TILE, int THREADS>
 __device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgroups, PartLds& lds) {
   constexpr int W = THREADS / 64;
   const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-  const auto units_of = [&](int b) -> unsigned { return b < p.a.batch ? (unsigned)(sequence_units<ROWS, TILE>(p, sequence(p, b)) * p.c.kv_heads) : 0u; };
+  Sequence s{};
+  const auto units_of = [&](int b) -> unsigned {   // of one key head
+    if (b >= p.a.batch) return 0u;
+    s = sequence(p, b);
+    return (unsigned)sequence_units<ROWS, TILE>(p, s);
+  };
+  const unsigned heads = (unsigned)p.c.kv_heads;
   const auto chunk_scan = [&](unsigned mine, unsigned& total) {   // inclusive prefix of the threads of the workgroup
     unsigned in = wave_scan(mine);
     __syncthreads();
@@ -130,11 +149,11 @@ __device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgro
     return in + before;
   };
   unsigned mine = units_of(tid), total, all;
-  unsigned in = chunk_scan(mine, total);
+  unsigned in = chunk_scan(mine * heads, total);
   all = total;
   for (int b0 = THREADS; b0 < p.a.batch; b0 += THREADS) {   // (more sequences than threads: added up first, searched below)
     unsigned t;
-    chunk_scan(units_of(b0 + tid), t);
+    chunk_scan(units_of(b0 + tid) * heads, t);
     all += t;
   }
   Part r;
@@ -145,21 +164,29 @@ __device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgro
   r.u1 = g < r.parts ? part_start(all, r.parts, g + 1) : all;
   r.b = 0, r.b_begin = 0;
   if (r.u0 >= r.u1) return r;
+  if (p.a.batch > THREADS) {   // from the first chunk again
+    mine = units_of(tid);
+    in = chunk_scan(mine * heads, total);
+  }
   unsigned base = 0;
   for (int b0 = 0;;) {
     if (r.u0 < base + total) {   // in this chunk of sequences
-      const unsigned begin = base + in - mine;
-      if (mine && begin <= r.u0 && r.u0 < begin + mine) lds.b = b0 + tid, lds.begin = begin;
+      const unsigned begin = base + in - mine * heads;
+      if (mine && begin <= r.u0 && r.u0 < begin + mine * heads) lds.b = b0 + tid, lds.begin = begin, lds.per_head = mine, lds.s = s;
       break;
     }
     base += total;
     b0 += THREADS;
     mine = units_of(b0 + tid);
-    in = chunk_scan(mine, total);
+    in = chunk_scan(mine * heads, total);
   }
   __syncthreads();
   r.b = __builtin_amdgcn_readfirstlane(lds.b);
   r.b_begin = (unsigned)__builtin_amdgcn_readfirstlane((int)lds.begin);
+  r.per_head = (unsigned)__builtin_amdgcn_readfirstlane((int)lds.per_head);
+  r.s.first = __builtin_amdgcn_readfirstlane(lds.s.first);
+  r.s.n = __builtin_amdgcn_readfirstlane(lds.s.n);
+  r.s.len = __builtin_amdgcn_readfirstlane(lds.s.len);
   return r;
 }
 
@@ -169,18 +196,18 @@ struct Item {
   int head, row0, tile0;
   unsigned begin, units;
 };
-// The item that holds unit u >= b_begin; moves b and b_begin on to its sequence.
+// The item that holds unit u >= b_begin; moves b, b_begin, the sequence s and its units of one head on to it.
 template <int ROWS, int TILE>
-__device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& b_begin) {
+__device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& b_begin, Sequence& s, unsigned& per_head) {
   Item it;
-  unsigned per_head;
-  for (;;) {   // (u is below the number of all units; the bounds on b and row0 hold if lengths change under the call, too)
-    it.s = sequence(p, b);
-    per_head = (unsigned)sequence_units<ROWS, TILE>(p, it.s);
-    if (u < b_begin + per_head * (unsigned)p.c.kv_heads || b + 1 >= p.a.batch) break;
+  // (u is below the number of all units; the bounds on b and row0 hold if lengths change under the call, too)
+  while (u >= b_begin + per_head * (unsigned)p.c.kv_heads && b + 1 < p.a.batch) {
     b_begin += per_head * (unsigned)p.c.kv_heads;
     ++b;
+    s = sequence(p, b);
+    per_head = (unsigned)sequence_units<ROWS, TILE>(p, s);
   }
+  it.s = s;
   it.head = per_head ? (int)((u - b_begin) / per_head) : 0;
   it.head = it.head < p.c.kv_heads ? it.head : p.c.kv_heads - 1;
   it.begin = b_begin + (unsigned)it.head * per_head;
@@ -196,6 +223,9 @@ __device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& 
 // Lane l of the wave writes its 16 (4) bytes at LDS address lds + 16 l (4 l), straight from memory; counts on vmcnt.
 __device__ inline void to_lds16(const uint8_t* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
+}
+__device__ inline void to_lds16(const uint8_t* base, unsigned offset, unsigned lds) {   // base is wave-uniform
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ inline void to_lds4(const uint8_t* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
@@ -225,6 +255,16 @@ __device__ inline v4i load8_bf16(const uint16_t* q) {
 }
 __device__ inline float bf16_lo(int x) { return __builtin_bit_cast(float, (unsigned)x << 16); }
 __device__ inline float bf16_hi(int x) { return __builtin_bit_cast(float, (unsigned)x & 0xFFFF0000u); }
+
+// Two 16-bit a * k + c, k a scalar pair
+__device__ inline unsigned pk_mad_u16(unsigned a, unsigned k, unsigned c) {
+  unsigned r;
+  asm("v_pk_mad_u16 %0, %1, %2, %3" : "=v"(r) : "v"(a), "s"(k), "v"(c));
+  return r;
+}
+__device__ inline us2 as_us2(unsigned x) { return __builtin_bit_cast(us2, x); }
+__device__ inline unsigned as_u32(us2 x) { return __builtin_bit_cast(unsigned, x); }
+__device__ inline unsigned pk_sub_sat(unsigned a, unsigned b) { return as_u32(__builtin_elementwise_sub_sat(as_us2(a), as_us2(b))); }
 
 // ---- queries: two 8-bit parts ------------------------------------------------------------------------------------------------------
 // The scaled MFMAs multiply E2M1 keys as they are with 8-bit queries.  A bf16 number has 8 significant bits, an E4M3 number 4:
@@ -294,7 +334,8 @@ __device__ inline float cross_sum(float v) {
 
 // A row's place in the output: (token, query head)
 __device__ inline size_t row_index(const AttnArgs& p, int first, int head, int row) {
-  return (size_t)(first + row / p.group) * p.a.heads + head * p.group + row % p.group;
+  const int t = p.token_of(row);
+  return (size_t)(first + t) * p.a.heads + head * p.group + (row - t * p.group);
 }
 
 // Four channels of a finished row: o / l, with the sink's share of the sum; m in base 2 (-inf: the row saw nothing).

@@ -32,50 +32,73 @@ struct Shape {
 __device__ inline unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
-__device__ inline us2 as_us2(unsigned x) { return __builtin_bit_cast(us2, x); }
-__device__ inline unsigned as_u32(us2 x) { return __builtin_bit_cast(unsigned, x); }
 
-// Requests the 64 keys and values from token t0 on (a multiple of 64) of a sequence of len > 0 keys into the stage at `lds`.
-template <int D>
-__device__ inline void request_stage(const AttnArgs& p, ConstInts table, int len, int head, int t0, unsigned lds) {
+// Requests for stages.  ONE_PAGE: pages of 64 tokens and more, so that a stage lies in one page and its addresses are a scalar base and
+// a lane's fixed offset (four groups of 16 tokens in pages of their own cost four times the scalar arithmetic).
+template <int D, bool ONE_PAGE>
+struct Request {
   using S = Shape<D>;
-  const int lane = threadIdx.x & 63;
-  int page[4];
+  static constexpr int kPieces = S::kRow / 16, kTokens = 1024 / S::kRow;   // pieces of a row, tokens of an instruction
+  static constexpr int kN = S::kCodes / 1024;
+  static constexpr int kGroups = ONE_PAGE ? 1 : 4, kGroupTokens = 64 / kGroups;
+  unsigned key[kN], value[kN];   // byte offsets of this lane's pieces within a group of tokens that lie in one page
+
+  __device__ inline Request() {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) page[i] = page_at(p, table, t0 + 16 * i, len);
-  const int mask = p.c.page_size - 1;
-  // codes: 1 KB an instruction
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const uint8_t* base = kv ? p.c.v : p.c.k;
-    const int64_t stride = kv ? p.c.v_page_stride : p.c.k_page_stride;
-#pragma unroll
-    for (int i = 0; i < S::kCodes / 1024; ++i) {
-      constexpr int kPieces = S::kRow / 16, kTokens = 1024 / S::kRow;   // pieces of a row, tokens of an instruction
+    for (int i = 0; i < kN; ++i) {
       const int t = i * kTokens + lane / kPieces;
-      const int piece = (lane % kPieces) ^ (kv ? S::value_swizzle(t) : S::key_swizzle(t));
-      const int pg = kTokens > 16 ? (lane < 32 ? page[(2 * i) & 3] : page[(2 * i + 1) & 3]) : page[i * kTokens / 16];
-      const uint8_t* src = base + pg * stride + ((size_t)head * p.c.page_size + ((t0 + t) & mask)) * S::kRow + piece * 16;
-      to_lds16(src, lds + kv * S::kCodes + i * 1024);
+      key[i] = t % kGroupTokens * S::kRow + ((lane % kPieces) ^ S::key_swizzle(t)) * 16;
+      value[i] = t % kGroupTokens * S::kRow + ((lane % kPieces) ^ S::value_swizzle(t)) * 16;
     }
   }
-  // scales: a lane's four bytes belong to the tokens of one group of 16
-  const auto scales = [&](int kv, int offset) {   // of the stage's kScales bytes
-    const int t = offset / S::kBlocks;
-    const int pg = t < 32 ? (t < 16 ? page[0] : page[1]) : (t < 48 ? page[2] : page[3]);
-    return (kv ? p.c.v_scale + pg * p.c.v_scale_page_stride : p.c.k_scale + pg * p.c.k_scale_page_stride) +
-           ((size_t)head * p.c.page_size + ((t0 + t) & mask)) * S::kBlocks + offset % S::kBlocks;
-  };
-  if constexpr (D == 64) {
-    to_lds4(scales(lane / 32, lane % 32 * 4), lds + 2 * S::kCodes);   // keys' scales by lanes 0-31, values' by 32-63
-  } else {
+
+  // The 64 keys and values from token t0 on (a multiple of 64) of a sequence of len > 0 keys into the stage at `lds`
+  __device__ inline void stage(const AttnArgs& p, ConstInts table, int len, int head, int t0, unsigned lds) const {
+    const int lane = threadIdx.x & 63;
+    int page[kGroups];
+    unsigned row[kGroups];   // within a page (all heads): below 2^30 / kRow
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv)
+    for (int i = 0; i < kGroups; ++i) {
+      page[i] = page_at(p, table, t0 + kGroupTokens * i, len);
+      row[i] = (unsigned)(head * p.c.page_size + ((t0 + kGroupTokens * i) & (p.c.page_size - 1)));
+    }
+    // codes: 1 KB an instruction
 #pragma unroll
-      for (int i = 0; i < S::kScales / 256; ++i)
-        to_lds4(scales(kv, i * 256 + lane * 4), lds + 2 * S::kCodes + kv * S::kScales + i * 256);
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint8_t* base[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        base[i] = (kv ? p.c.v + page[i] * p.c.v_page_stride : p.c.k + page[i] * p.c.k_page_stride) + row[i] * (unsigned)S::kRow;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const unsigned off = kv ? value[i] : key[i], at = lds + kv * S::kCodes + i * 1024;
+        if constexpr (ONE_PAGE) to_lds16(base[0], off, at);
+        else if constexpr (kTokens > 16) to_lds16((lane < 32 ? base[2 * i % kGroups] : base[(2 * i + 1) % kGroups]) + off, at);   // two groups
+        else to_lds16(base[i * kTokens / 16 % kGroups], off, at);
+      }
+    }
+    // scales: a lane's four bytes belong to the tokens of one group
+    const auto scales = [&](const uint8_t* from, int64_t stride, int offset) {   // of the stage's kScales bytes
+      const uint8_t* base[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) base[i] = from + page[i] * stride + row[i] * (unsigned)S::kBlocks;
+      if constexpr (ONE_PAGE) return base[0] + offset;
+      const int t = offset / S::kBlocks;
+      return (t < 32 ? (t < 16 ? base[0] : base[1 % kGroups]) : (t < 48 ? base[2 % kGroups] : base[3 % kGroups])) + offset % (16 * S::kBlocks);
+    };
+    if constexpr (D == 64) {   // keys' scales by lanes 0-31, values' by 32-63
+      const uint8_t *a = scales(p.c.k_scale, p.c.k_scale_page_stride, lane % 32 * 4), *b = scales(p.c.v_scale, p.c.v_scale_page_stride, lane % 32 * 4);
+      to_lds4(lane < 32 ? a : b, lds + 2 * S::kCodes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kScales / 256; ++i) {
+        to_lds4(scales(p.c.k_scale, p.c.k_scale_page_stride, i * 256 + lane * 4), lds + 2 * S::kCodes + i * 256);
+        to_lds4(scales(p.c.v_scale, p.c.v_scale_page_stride, i * 256 + lane * 4), lds + 2 * S::kCodes + S::kScales + i * 256);
+      }
+    }
   }
-}
+};
 
 // The queries of a block of rows: 16 rows a tile, a tile's parts in the layout of the 16x16x128 MFMA (lane: column lane % 16; bytes 0-15 are
 // k = 16 g .., bytes 16-31 k = 64 + 16 g ..).  D = 64: one MFMA takes both parts, the second in the place of k >= 64.
@@ -92,8 +115,8 @@ struct Queries {
     for (int ct = 0; ct < NT; ++ct) {
       const int row = it.row0 + ct * 16 + lane % 16;
       const bool real = row < rows;
-      const uint16_t* q = p.a.q + (int64_t)(it.s.first + (real ? row / p.group : 0)) * p.a.q_token_stride +
-                          (int64_t)(it.head * p.group + (real ? row % p.group : 0)) * p.a.q_head_stride;
+      const int t = real ? p.token_of(row) : 0;
+      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)(it.head * p.group + (real ? row - t * p.group : 0)) * p.a.q_head_stride;
       v4i x[D / 32];   // eight channels each: pairs of them at 16 g + 64 i
       unsigned amax = 0;
 #pragma unroll
@@ -121,7 +144,7 @@ struct Queries {
   }
 };
 
-template <int D, int NT, int NW, int NS>
+template <int D, int NT, int NW, int NS, bool ONE_PAGE>
 __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int ROWS = NT * 16, TILE = 64, C = D / 16;   // C: channel tiles of 16
@@ -135,8 +158,10 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
   const unsigned ring = (unsigned)__builtin_amdgcn_readfirstlane(lds_address(smem)) + wave * NS * S::kStage;
   const unsigned char* ring_ptr = smem + wave * NS * S::kStage;
   const float c = fabsf(p.a.scale) * kLog2e;
+  const Request<D, ONE_PAGE> request;
   int b = part.b;
-  unsigned b_begin = part.b_begin;
+  unsigned b_begin = part.b_begin, per_head = part.per_head;
+  Sequence seq = part.s;
   bool first_item = true;
   if (!p.whole && threadIdx.x == 0 && part.u0 >= part.u1) {   // no work
     int* m = p.meta + (size_t)blockIdx.x * kMeta;
@@ -144,7 +169,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
     m[kMetaParts] = (int)part.parts, m[kMetaUnits] = (int)part.units;
   }
   for (unsigned u = part.u0; u < part.u1;) {
-    const Item it = item_of<ROWS, TILE>(p, u, b, b_begin);
+    const Item it = item_of<ROWS, TILE>(p, u, b, b_begin, seq, per_head);
     const unsigned end = it.begin + it.units;
     unsigned from = u, to = end < part.u1 ? end : part.u1;
     if (!p.whole) {
@@ -171,18 +196,18 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
     int lo_row[NT], hi_row[NT], lo_max, hi_min, dummy;
     {
       const int last = it.row0 + ROWS < rows ? it.row0 + ROWS - 1 : rows - 1;
-      visible(p, it.s, it.row0 / p.group, dummy, hi_min);
-      visible(p, it.s, last / p.group, lo_max, dummy);
+      visible(p, it.s, p.token_of(it.row0), dummy, hi_min);
+      visible(p, it.s, p.token_of(last), lo_max, dummy);
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
         const int row = it.row0 + ct * 16 + col;
-        visible(p, it.s, (row < rows ? row : last) / p.group, lo_row[ct], hi_row[ct]);
+        visible(p, it.s, p.token_of(row < rows ? row : last), lo_row[ct], hi_row[ct]);
       }
     }
     const int mine = it.s.len > 0 && tiles > wave ? (tiles - wave + NW - 1) / NW : 0;   // tiles wave, wave + NW, ...
     int requested = 0;
     for (; requested < NS - 1 && requested < mine; ++requested)
-      request_stage<D>(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + requested * S::kStage);
+      request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + requested * S::kStage);
 
     Queries<D, NT> q;
     q.load(p, it, rows);
@@ -199,7 +224,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
     for (int i = 0; i < mine; ++i) {
       const int t0 = (tile0 + wave + i * NW) * TILE;
       if (requested < mine) {
-        request_stage<D>(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + (requested % NS) * S::kStage);
+        request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + (requested % NS) * S::kStage);
         ++requested;
         wait_loads<(NS - 1) * S::kLoads>();
       } else {
@@ -235,18 +260,16 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
 
       // ---- probabilities
       const bool all_seen = t0 >= lo_max && t0 + TILE <= hi_min;
-      us2 prob[NT][8], bias[NT][8];   // pairs of tokens 16 g + 2 i, + 1; what is taken from their exponents
+      unsigned prob[NT][8], bias[NT][8];   // pairs of tokens 16 g + 2 i, + 1; what is taken from their exponents
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
-        bool seen[16];
         if (!all_seen) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
               const int key = t0 + 16 * g + 4 * j + t;
-              seen[4 * j + t] = key >= lo_row[ct] && key < hi_row[ct];
-              if (!seen[4 * j + t]) s[ct][j][t] = kNone;
+              s[ct][j][t] = key >= lo_row[ct] && key < hi_row[ct] ? s[ct][j][t] : kNone;
             }
         }
         float top = kNone;
@@ -265,15 +288,14 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j / 4][j % 4], c, shift));
-          if (!all_seen && !seen[j]) pr[j] = 0.0f;
+          if (!all_seen) pr[j] = s[ct][j / 4][j % 4] == kNone ? 0.0f : pr[j];   // (where a row has seen nothing yet, or c is 0)
           l[ct] += pr[j];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          prob[ct][j] = as_us2(pack_bf16x2(pr[2 * j], pr[2 * j + 1]));
+          prob[ct][j] = pack_bf16x2(pr[2 * j], pr[2 * j + 1]);
           // 127 in the exponent's place, or more than everything for a probability of zero, which stays zero
-          const us2 zero = __builtin_elementwise_sub_sat(us2{1, 1}, prob[ct][j]);
-          bias[ct][j] = zero * us2{0xC07F, 0xC07F} + us2{0x3F80, 0x3F80};
+          bias[ct][j] = pk_mad_u16(pk_sub_sat(0x00010001u, prob[ct][j]), 0xC07FC07Fu, 0x3F803F80u);
         }
       }
 
@@ -286,31 +308,43 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
         nan = nan || ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
       }
       nan = __any(nan);
+      // the scale bytes of tokens 16 g + 2 k and + 1 for a block of channels, in 16 bits each
+      const auto scale_pair = [&](int blk, int k) -> unsigned {
+        if constexpr (D == 64) {
+          const unsigned w = reinterpret_cast<const unsigned*>(vs)[g * 8 + k];
+          return __builtin_amdgcn_perm(w, w, blk ? 0x0c030c01u : 0x0c020c00u);
+        } else {
+          constexpr int kWords = S::kBlocks / 4;
+          const unsigned w0 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k) * kWords + blk / 4];
+          const unsigned w1 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k + 1) * kWords + blk / 4];
+          return __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + 0x00010001u * (blk % 4));
+        }
+      };
+      if (nan) {   // a row to which a value with a NaN scale counts: its block of channels is NaN
+#pragma unroll
+        for (int blk = 0; blk < S::kBlocks; ++blk)
+#pragma unroll
+          for (int ct = 0; ct < NT; ++ct) {
+            unsigned hit = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              hit |= as_u32(as_us2(pk_sub_sat(scale_pair(blk, k), 0x00FE00FEu)) * __builtin_elementwise_min(as_us2(prob[ct][k]), us2{1, 1}));
+            const float poison = cross_max<true>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
+            acc[ct][2 * blk] += poison;
+            acc[ct][2 * blk + 1] += poison;
+          }
+      }
 #pragma unroll
       for (int blk = 0; blk < S::kBlocks; ++blk) {
         // P with the scales of this block of channels
         v4i ps[NT][2];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          unsigned e2;   // the scale bytes of tokens 16 g + 2 k and + 1, in 16 bits each
-          if constexpr (D == 64) {
-            const unsigned w = reinterpret_cast<const unsigned*>(vs)[g * 8 + k];
-            e2 = __builtin_amdgcn_perm(w, w, blk ? 0x0c030c01u : 0x0c020c00u);
-          } else {
-            constexpr int kWords = S::kBlocks / 4;
-            const unsigned w0 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k) * kWords + blk / 4];
-            const unsigned w1 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k + 1) * kWords + blk / 4];
-            e2 = __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + 0x00010001u * (blk % 4));
-          }
-          const us2 e = as_us2(e2);
+          const unsigned e = scale_pair(blk, k);
 #pragma unroll
           for (int ct = 0; ct < NT; ++ct) {
-            us2 r = __builtin_elementwise_sub_sat(e * us2{128, 128} + prob[ct][k], bias[ct][k]);
-            if (nan) {   // NaN where the scale is one and the probability is not zero
-              const us2 is = __builtin_elementwise_sub_sat(e, us2{254, 254}) * __builtin_elementwise_min(prob[ct][k], us2{1, 1});
-              r = __builtin_elementwise_max(r, is * us2{0x7FC0, 0x7FC0});
-            }
-            ps[ct][k / 4][k % 4] = (int)as_u32(r);
+            const unsigned r = pk_sub_sat(pk_mad_u16(e, 0x00800080u, prob[ct][k]), bias[ct][k]);
+            ps[ct][k / 4][k % 4] = (int)r;
           }
         }
 #pragma unroll
@@ -379,11 +413,13 @@ template <int D, int NT, int NW, int NS>
 hipError_t launch_form(AttnArgs p, void* ws, hipStream_t s) {
   constexpr int ROWS = NT * 16;
   const int workgroups = compute_units();
-  p.min_units = NW;
   // items of at most two rounds of the waves stay whole: cutting them saves less than the second launch costs
   p.whole = ((int64_t)p.a.table_pages << p.page_shift) <= 2 * NW * 64;
+  p.min_units = p.whole ? 1 : NW;
   if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
-  hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS>), dim3((unsigned)workgroups), dim3(NW * 64), 0, s, p);
+  const dim3 grid((unsigned)workgroups), block(NW * 64);
+  if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false>), grid, block, 0, s, p);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.whole) return e;
   return launch_attn_combine(p, ROWS, workgroups, s);
 }
