@@ -26,7 +26,7 @@ struct AttnArgs {
   int group;          // query heads per key head
   int page_shift;
   int whole;          // 1: items are not split; no workspace, no second launch
-  int min_units;      // of a workgroup, so that small calls are not cut into crumbs
+  int min_units_log2; // of a workgroup, so that small calls are not cut into crumbs
   int* meta;          // workspace: [workgroups][kMeta]
   float* part_ml;     // [2 workgroups][ROWS][2]: maximum (base 2) and sum
   float* part_o;      // [2 workgroups][ROWS][D]
@@ -43,9 +43,9 @@ inline void set_group(AttnArgs& p, int group) {
   p.group_shift = group == 1 ? 0 : (unsigned)(s - 1);
 }
 
-// meta of a workgroup: first unit, first and last unit (exclusive) of the item that it starts in, that item's first row of q, its
-// valid rows, key head, first row; workgroups with work, units
-enum { kMetaU0, kMetaBegin, kMetaEnd, kMetaFirst, kMetaRows, kMetaHead, kMetaRow0, kMetaParts, kMetaUnits, kMeta = 12 };
+// meta of a workgroup: its first unit, first and last unit (exclusive) of the item that it starts in, that item's first row of q, all
+// rows of its sequence, key head, first row of the block; a workgroup without work has nothing but first units beyond all units
+enum { kMetaU0, kMetaBegin, kMetaEnd, kMetaFirst, kMetaRows, kMetaHead, kMetaRow0, kMeta = 8 };
 
 struct Sequence {
   int first, n, len;   // first row of q, new tokens, keys
@@ -96,97 +96,72 @@ __device__ inline int sequence_units(const AttnArgs& p, const Sequence& s) {   /
   return u;
 }
 
-__device__ inline unsigned wave_scan(unsigned v) {   // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const unsigned o = (unsigned)__shfl_up((int)v, d, 64);
-    if (lane >= d) v += o;
-  }
+__device__ inline unsigned wave_scan(unsigned v) {   // inclusive prefix sums over the lanes
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // one, two, four, eight lanes to the right in a row of 16
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // a row's last lane to the next row
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
   return v;
 }
+__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
-// The part of a workgroup: units [u0, u1) of all `units`, cut into `parts` equal ones; sequence b holds u0, b_begin is its first unit.
+// The part of a workgroup: units [u0, u1) of all `units`, cut into `parts` equal ones; sequence b holds u0, b_begin is its first unit and
+// per_head the units of one of its key heads.  Every wave finds it by itself (no barrier): 64 sequences at a time, a lane each.
 struct Part {
   unsigned u0, u1, units, parts;
   int b;
   unsigned b_begin, per_head;
   Sequence s;
 };
-struct PartLds {
-  unsigned sums[16];
-  int b;
-  unsigned begin, per_head;
-  Sequence s;
-};
 
-// First unit of part g (32 x 32 bits)
-__device__ inline unsigned part_start(unsigned units, unsigned parts, unsigned g) { return (unsigned)((uint64_t)units * g / parts); }
+// First unit of part g: the first units % parts parts have one unit more
+__device__ inline unsigned part_start(unsigned each, unsigned more, unsigned g) { return g * each + (g < more ? g : more); }
 
-template <int ROWS, int TILE, int THREADS>
-__device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgroups, PartLds& lds) {
-  constexpr int W = THREADS / 64;
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-  Sequence s{};
-  const auto units_of = [&](int b) -> unsigned {   // of one key head
-    if (b >= p.a.batch) return 0u;
-    s = sequence(p, b);
-    return (unsigned)sequence_units<ROWS, TILE>(p, s);
-  };
+template <int ROWS, int TILE>
+__device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgroups) {
+  const int lane = threadIdx.x & 63;
   const unsigned heads = (unsigned)p.c.kv_heads;
-  const auto chunk_scan = [&](unsigned mine, unsigned& total) {   // inclusive prefix of the threads of the workgroup
-    unsigned in = wave_scan(mine);
-    __syncthreads();
-    if (lane == 63) lds.sums[wave] = in;
-    __syncthreads();
-    unsigned before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w == wave) before = total;
-      total += lds.sums[w];
-    }
-    return in + before;
+  const auto load = [&](int b) {
+    Sequence s{0, 0, 0};
+    if (b < p.a.batch) s = sequence(p, b);
+    return s;
   };
-  unsigned mine = units_of(tid), total, all;
-  unsigned in = chunk_scan(mine * heads, total);
-  all = total;
-  for (int b0 = THREADS; b0 < p.a.batch; b0 += THREADS) {   // (more sequences than threads: added up first, searched below)
-    unsigned t;
-    chunk_scan(units_of(b0 + tid) * heads, t);
-    all += t;
+  Part r{};
+  Sequence s = load(lane);
+  unsigned mine = (unsigned)sequence_units<ROWS, TILE>(p, s), in = wave_scan(mine * heads);
+  unsigned total = (unsigned)lane_value((int)in, 63);
+  r.units = total;
+  Sequence next = load(64 + lane);
+  for (int b0 = 64; b0 < p.a.batch; b0 += 64) {
+    const Sequence now = next;
+    next = load(b0 + 64 + lane);
+    r.units += (unsigned)lane_value((int)wave_scan((unsigned)sequence_units<ROWS, TILE>(p, now) * heads), 63);
   }
-  Part r;
-  r.units = all;
-  const unsigned want = (all + (unsigned)p.min_units - 1) / (unsigned)p.min_units;
+  const unsigned want = (r.units + (1u << p.min_units_log2) - 1) >> p.min_units_log2;
   r.parts = want < workgroups ? (want ? want : 1) : workgroups;
-  r.u0 = g < r.parts ? part_start(all, r.parts, g) : all;
-  r.u1 = g < r.parts ? part_start(all, r.parts, g + 1) : all;
-  r.b = 0, r.b_begin = 0;
+  const unsigned each = r.units / r.parts, more = r.units - each * r.parts;
+  r.u0 = g < r.parts ? part_start(each, more, g) : r.units;
+  r.u1 = g < r.parts ? part_start(each, more, g + 1) : r.units;
   if (r.u0 >= r.u1) return r;
-  if (p.a.batch > THREADS) {   // from the first chunk again
-    mine = units_of(tid);
-    in = chunk_scan(mine * heads, total);
-  }
   unsigned base = 0;
-  for (int b0 = 0;;) {
-    if (r.u0 < base + total) {   // in this chunk of sequences
-      const unsigned begin = base + in - mine * heads;
-      if (mine && begin <= r.u0 && r.u0 < begin + mine * heads) lds.b = b0 + tid, lds.begin = begin, lds.per_head = mine, lds.s = s;
-      break;
-    }
+  int b0 = 0;
+  while (r.u0 >= base + total && b0 + 64 < p.a.batch) {   // (u0 is below the number of units: found at the latest in the last 64)
     base += total;
-    b0 += THREADS;
-    mine = units_of(b0 + tid);
-    in = chunk_scan(mine * heads, total);
+    b0 += 64;
+    s = load(b0 + lane);
+    mine = (unsigned)sequence_units<ROWS, TILE>(p, s);
+    in = wave_scan(mine * heads);
+    total = (unsigned)lane_value((int)in, 63);
   }
-  __syncthreads();
-  r.b = __builtin_amdgcn_readfirstlane(lds.b);
-  r.b_begin = (unsigned)__builtin_amdgcn_readfirstlane((int)lds.begin);
-  r.per_head = (unsigned)__builtin_amdgcn_readfirstlane((int)lds.per_head);
-  r.s.first = __builtin_amdgcn_readfirstlane(lds.s.first);
-  r.s.n = __builtin_amdgcn_readfirstlane(lds.s.n);
-  r.s.len = __builtin_amdgcn_readfirstlane(lds.s.len);
+  const unsigned begin = base + in - mine * heads;
+  const uint64_t here = __ballot(begin <= r.u0 && r.u0 < begin + mine * heads);
+  const int at = here ? __ffsll((unsigned long long)here) - 1 : 0;
+  r.b = b0 + at;
+  r.b_begin = (unsigned)lane_value((int)begin, at);
+  r.per_head = (unsigned)lane_value((int)mine, at);
+  r.s = {lane_value(s.first, at), lane_value(s.n, at), lane_value(s.len, at)};
   return r;
 }
 
@@ -208,9 +183,9 @@ __device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& 
     per_head = (unsigned)sequence_units<ROWS, TILE>(p, s);
   }
   it.s = s;
-  it.head = per_head ? (int)((u - b_begin) / per_head) : 0;
-  it.head = it.head < p.c.kv_heads ? it.head : p.c.kv_heads - 1;
-  it.begin = b_begin + (unsigned)it.head * per_head;
+  it.head = 0;
+  it.begin = b_begin;
+  while (u >= it.begin + per_head && it.head + 1 < p.c.kv_heads) it.begin += per_head, ++it.head;
   for (it.row0 = 0;; it.row0 += ROWS) {
     it.units = (unsigned)block_units<ROWS, TILE>(p, it.s, it.row0, it.tile0);
     if (u < it.begin + it.units || it.row0 + ROWS >= it.s.n * p.group) break;
@@ -271,45 +246,45 @@ __device__ inline unsigned pk_sub_sat(unsigned a, unsigned b) { return as_u32(__
 // q = 2^e hi + 2^(e-5) lo, hi the rounded q / 2^e and lo the rounded rest times 32, is exact down to 2^-19 of the row's largest element
 // (e puts that one into [2^7, 2^8)); two MFMAs take the time that one bf16 product of the same length would, and no key is converted.
 struct QueryScale {
-  float inv;      // 2^-e, negative for a negative softmax scale
-  int hi, lo;     // E8M0 bytes; 0xFF (NaN) for a row with an infinity or a NaN
+  float hi, lo;             // 2^e, 2^(e-5)
+  int hi_byte, lo_byte;     // the same as E8M0; 0xFF (NaN) for a row with an infinity or a NaN
 };
-__device__ inline QueryScale query_scale(unsigned amax_bits, bool negative) {
-  int f = (int)(amax_bits >> 23);
-  if (f == 0xFF) return {0.0f, 0xFF, 0xFF};
+__device__ inline QueryScale query_scale(unsigned amax) {   // of bf16 bits
+  int f = (int)(amax >> 7);
+  const bool bad = f == 0xFF;
   f = f < 13 ? 13 : f;   // e + 127 = f - 7
-  const float inv = __builtin_bit_cast(float, (unsigned)(261 - f) << 23);
-  return {negative ? -inv : inv, f - 7, f - 12};
+  const float hi = __builtin_bit_cast(float, (unsigned)(f - 7) << 23), lo = __builtin_bit_cast(float, (unsigned)(f - 12) << 23);
+  return {hi, lo, bad ? 0xFF : f - 7, bad ? 0xFF : f - 12};
 }
-__device__ inline void split_query(v4i x, float inv, int& h0, int& h1, int& l0, int& l1) {   // eight bf16 -> 2 x 4 bytes of each part
-  float v[8], r[8];
+typedef short v2s __attribute__((ext_vector_type(2)));
+// Eight bf16 -> 2 x 4 bytes of each part (the conversions divide and multiply by their scale operand)
+__device__ inline void split_query(v4i x, const QueryScale& s, int (&hi)[2], int (&lo)[2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(x[i]) * inv, v[2 * i + 1] = bf16_hi(x[i]) * inv;
-  h0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-  h0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], h0, true);
-  h1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
-  h1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], h1, true);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int w = i < 2 ? h0 : h1;
-    const v2f b = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
-    r[2 * i] = (v[2 * i] - b[0]) * 32.0f, r[2 * i + 1] = (v[2 * i + 1] - b[1]) * 32.0f;
+  for (int i = 0; i < 2; ++i) {
+    const int x0 = x[2 * i], x1 = x[2 * i + 1];
+    v2s h = {0, 0}, l = {0, 0};
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(v2bf, x0), s.hi, false);
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(v2bf, x1), s.hi, true);
+    hi[i] = __builtin_bit_cast(int, h);
+    const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s.hi, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s.hi, true);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_lo(x0) - a[0], bf16_hi(x0) - a[1], s.lo, false);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_lo(x1) - b[0], bf16_hi(x1) - b[1], s.lo, true);
+    lo[i] = __builtin_bit_cast(int, l);
   }
-  l0 = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
-  l0 = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], l0, true);
-  l1 = __builtin_amdgcn_cvt_pk_fp8_f32(r[4], r[5], 0, false);
-  l1 = __builtin_amdgcn_cvt_pk_fp8_f32(r[6], r[7], l1, true);
 }
-__device__ inline unsigned amax_bits8(v4i x, unsigned m) {
+// Largest magnitudes of eight bf16 as bit patterns in the two halves of m (NaN > infinity > numbers)
+__device__ inline us2 amax_pairs(v4i x, us2 m) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned a = ((unsigned)x[i] << 16) & 0x7FFFFFFFu, b = (unsigned)x[i] & 0x7FFF0000u;
-    m = m > a ? m : a;
-    m = m > b ? m : b;
+    const unsigned w = (unsigned)x[i] & 0x7FFF7FFFu;
+    m = __builtin_elementwise_max(m, as_us2(w));
   }
   return m;
 }
-// NaN > infinity > numbers as bit patterns, so this is the row's largest magnitude or 0x7F8..... and more
+__device__ inline unsigned larger_half(us2 m) {
+  const unsigned a = m[0], b = m[1];
+  return a > b ? a : b;
+}
 
 // Largest value of lanes l, l ^ 16, l ^ 32, l ^ 48 (XOR16) or l, l ^ 32
 __device__ inline float max_of_swapped(unsigned a, unsigned b) { return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)); }
@@ -358,7 +333,8 @@ __device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int chan
 
 hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* workspace, hipStream_t s);
 size_t attn_decode_workspace(const AttnArgs& p, int row_tiles);
-hipError_t launch_attn_combine(const AttnArgs& p, int rows, int workgroups, hipStream_t s);
+// rows: of a block; rows_expected: of a sequence and key head
+hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s);
 // meta, maxima and sums, partial results, in this order
 inline size_t attn_workspace(int rows, int head_dim, int workgroups) {
   const size_t meta = ((size_t)workgroups * kMeta * 4 + 255) / 256 * 256;

@@ -33,6 +33,9 @@ __device__ inline unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
 
+// (values, not the elements of an array: a choice of elements would keep the array in memory)
+__device__ inline const uint8_t* pick(bool first, const uint8_t* a, const uint8_t* b) { return first ? a : b; }
+
 // Requests for stages.  ONE_PAGE: pages of 64 tokens and more, so that a stage lies in one page and its addresses are a scalar base and
 // a lane's fixed offset (four groups of 16 tokens in pages of their own cost four times the scalar arithmetic).
 template <int D, bool ONE_PAGE>
@@ -74,7 +77,7 @@ struct Request {
       for (int i = 0; i < kN; ++i) {
         const unsigned off = kv ? value[i] : key[i], at = lds + kv * S::kCodes + i * 1024;
         if constexpr (ONE_PAGE) to_lds16(base[0], off, at);
-        else if constexpr (kTokens > 16) to_lds16((lane < 32 ? base[2 * i % kGroups] : base[(2 * i + 1) % kGroups]) + off, at);   // two groups
+        else if constexpr (kTokens > 16) to_lds16(pick(lane < 32, base[2 * i % kGroups], base[(2 * i + 1) % kGroups]) + off, at);   // two groups
         else to_lds16(base[i * kTokens / 16 % kGroups], off, at);
       }
     }
@@ -85,7 +88,7 @@ struct Request {
       for (int i = 0; i < kGroups; ++i) base[i] = from + page[i] * stride + row[i] * (unsigned)S::kBlocks;
       if constexpr (ONE_PAGE) return base[0] + offset;
       const int t = offset / S::kBlocks;
-      return (t < 32 ? (t < 16 ? base[0] : base[1 % kGroups]) : (t < 48 ? base[2 % kGroups] : base[3 % kGroups])) + offset % (16 * S::kBlocks);
+      return pick(t < 32, pick(t < 16, base[0], base[1 % kGroups]), pick(t < 48, base[2 % kGroups], base[3 % kGroups])) + offset % (16 * S::kBlocks);
     };
     if constexpr (D == 64) {   // keys' scales by lanes 0-31, values' by 32-63
       const uint8_t *a = scales(p.c.k_scale, p.c.k_scale_page_stride, lane % 32 * 4), *b = scales(p.c.v_scale, p.c.v_scale_page_stride, lane % 32 * 4);
@@ -107,39 +110,44 @@ struct Queries {
   static constexpr int kSteps = D == 64 ? 1 : D / 128;
   v8i hi[NT][kSteps], lo[NT][D == 64 ? 1 : kSteps];
   int s_hi[NT], s_lo[NT];
+  v4i x[NT][D / 32];   // eight channels each: pairs of them at 16 g + 64 i
 
-  __device__ inline void load(const AttnArgs& p, const Item& it, int rows) {
+  __device__ inline void request(const AttnArgs& p, const Item& it, int rows) {
     const int lane = threadIdx.x & 63, g = lane / 16;
-    const bool negative = p.a.scale < 0.0f;
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
       const int row = it.row0 + ct * 16 + lane % 16;
       const bool real = row < rows;
       const int t = real ? p.token_of(row) : 0;
       const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)(it.head * p.group + (real ? row - t * p.group : 0)) * p.a.q_head_stride;
-      v4i x[D / 32];   // eight channels each: pairs of them at 16 g + 64 i
-      unsigned amax = 0;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        x[i] = v4i{0, 0, 0, 0};
-        if (real) x[i] = load8_bf16(q + (i / 2) * 64 + g * 16 + (i % 2) * 8);
-        amax = amax_bits8(x[i], amax);
+        x[ct][i] = v4i{0, 0, 0, 0};
+        if (real) x[ct][i] = load8_bf16(q + (i / 2) * 64 + g * 16 + (i % 2) * 8);
       }
-      amax = lane_xor_max_bits(lane_xor_max_bits(amax, 16), 32);
-      const QueryScale s = query_scale(amax, negative);
+    }
+  }
+  __device__ inline void convert(const AttnArgs& p) {
+    const int g = (threadIdx.x & 63) / 16;
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      us2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) m = amax_pairs(x[ct][i], m);
+      const QueryScale s = query_scale(lane_xor_max_bits(lane_xor_max_bits(larger_half(m), 16), 32));
+      const int sign = p.a.scale < 0.0f ? (int)0x80808080u : 0;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        int h0, h1, l0, l1;
-        split_query(x[i], s.inv, h0, h1, l0, l1);
-        if (s.hi == 0xFF) h0 = h1 = l0 = l1 = 0;
-        if constexpr (D == 64) {
-          hi[ct][0][i * 2] = h0, hi[ct][0][i * 2 + 1] = h1, hi[ct][0][4 + i * 2] = l0, hi[ct][0][4 + i * 2 + 1] = l1;
-        } else {
-          hi[ct][i / 4][i % 4 * 2] = h0, hi[ct][i / 4][i % 4 * 2 + 1] = h1, lo[ct][i / 4][i % 4 * 2] = l0, lo[ct][i / 4][i % 4 * 2 + 1] = l1;
+        int h[2], l[2];
+        split_query(x[ct][i], s, h, l);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (D == 64) hi[ct][0][i * 2 + k] = h[k] ^ sign, hi[ct][0][4 + i * 2 + k] = l[k] ^ sign;
+          else hi[ct][i / 4][i % 4 * 2 + k] = h[k] ^ sign, lo[ct][i / 4][i % 4 * 2 + k] = l[k] ^ sign;
         }
       }
-      s_hi[ct] = D == 64 && g >= 2 ? s.lo : s.hi;
-      s_lo[ct] = s.lo;
+      s_hi[ct] = D == 64 && g >= 2 ? s.lo_byte : s.hi_byte;
+      s_lo[ct] = s.lo_byte;
     }
   }
 };
@@ -152,9 +160,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
   constexpr int kRing = NW * NS * S::kStage, kJoin = NW * ROWS * kPitch * 4;
   __shared__ __align__(16) unsigned char smem[kRing > kJoin ? kRing : kJoin];
   __shared__ float join_ml[NW][ROWS][2];
-  __shared__ PartLds part_lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane / 16, col = lane % 16;
-  const Part part = take_part<ROWS, TILE, NW * 64>(p, blockIdx.x, gridDim.x, part_lds);
+  const Part part = take_part<ROWS, TILE>(p, blockIdx.x, gridDim.x);
   const unsigned ring = (unsigned)__builtin_amdgcn_readfirstlane(lds_address(smem)) + wave * NS * S::kStage;
   const unsigned char* ring_ptr = smem + wave * NS * S::kStage;
   const float c = fabsf(p.a.scale) * kLog2e;
@@ -166,7 +173,6 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
   if (!p.whole && threadIdx.x == 0 && part.u0 >= part.u1) {   // no work
     int* m = p.meta + (size_t)blockIdx.x * kMeta;
     m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
-    m[kMetaParts] = (int)part.parts, m[kMetaUnits] = (int)part.units;
   }
   for (unsigned u = part.u0; u < part.u1;) {
     const Item it = item_of<ROWS, TILE>(p, u, b, b_begin, seq, per_head);
@@ -177,7 +183,6 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
         int* m = p.meta + (size_t)blockIdx.x * kMeta;
         m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)end, m[kMetaFirst] = it.s.first;
         m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
-        m[kMetaParts] = (int)part.parts, m[kMetaUnits] = (int)part.units;
       }
       u = to;
     } else {   // the items that start in this part, as wholes
@@ -205,12 +210,13 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
       }
     }
     const int mine = it.s.len > 0 && tiles > wave ? (tiles - wave + NW - 1) / NW : 0;   // tiles wave, wave + NW, ...
+    Queries<D, NT> q;
+    q.request(p, it, rows);
     int requested = 0;
     for (; requested < NS - 1 && requested < mine; ++requested)
       request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + requested * S::kStage);
 
-    Queries<D, NT> q;
-    q.load(p, it, rows);
+    q.convert(p);
 
     v4f acc[NT][C];
     float m[NT], l[NT];
@@ -414,14 +420,15 @@ hipError_t launch_form(AttnArgs p, void* ws, hipStream_t s) {
   constexpr int ROWS = NT * 16;
   const int workgroups = compute_units();
   // items of at most two rounds of the waves stay whole: cutting them saves less than the second launch costs
-  p.whole = ((int64_t)p.a.table_pages << p.page_shift) <= 2 * NW * 64;
-  p.min_units = p.whole ? 1 : NW;
+  const int64_t in_table = (int64_t)p.a.table_pages << p.page_shift, in_window = p.a.window > 0 ? (int64_t)p.a.window + p.a.max_q : in_table;
+  p.whole = (in_window < in_table ? in_window : in_table) <= 2 * NW * 64;
+  p.min_units_log2 = p.whole ? 0 : log2_of(NW);
   if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
   const dim3 grid((unsigned)workgroups), block(NW * 64);
   if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false>), grid, block, 0, s, p);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.whole) return e;
-  return launch_attn_combine(p, ROWS, workgroups, s);
+  return launch_attn_combine(p, ROWS, p.a.cu_q ? p.a.max_q * p.group : p.group, workgroups, s);
 }
 
 }  // namespace
@@ -444,44 +451,58 @@ hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s
 // ---- parts of split items, joined -----------------------------------------------------------------------------------------------
 namespace {
 
-// blockIdx.x: a boundary between two workgroups of the first launch; the first boundary inside an item joins its parts.
+// blockIdx.x: a boundary between two workgroups of the first launch; the first boundary inside an item joins the item's parts, a row
+// (of every gridDim.y) per workgroup: 1024 / D groups of threads add up every so many parts and meet in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS) {
+  constexpr int T = D / 4, GROUPS = 256 / T;
+  __shared__ v4f sums[GROUPS][T];
+  __shared__ float ml[GROUPS][2];
   const int g = blockIdx.x + 1;
   const int* m = p.meta + (size_t)g * kMeta;
   const unsigned begin = (unsigned)m[kMetaBegin], end = (unsigned)m[kMetaEnd], u0 = (unsigned)m[kMetaU0];
   if (begin >= u0 || (unsigned)m[kMetaU0 - kMeta] > begin) return;
-  const unsigned parts = (unsigned)m[kMetaParts], units = (unsigned)m[kMetaUnits];
-  int last = g;   // the last workgroup that starts inside the item
-  while (last + 1 < (int)parts && part_start(units, parts, (unsigned)last + 1) < end) ++last;
-  const int rows = m[kMetaRows], row0 = m[kMetaRow0];
-  const int valid = rows - row0 < ROWS ? rows - row0 : ROWS;
-  constexpr int kRowsAtOnce = 256 / (D / 4);
-  const int row = blockIdx.y * kRowsAtOnce + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
-  if (row >= valid) return;
-  const size_t before = 2 * (size_t)(g - 1) + 1;   // the part of the workgroup that the item starts in; then 2 g, 2 (g + 1), ...
-  const auto slot = [&](int i) { return i == 0 ? before : 2 * (size_t)(g + i - 1); };
-  const int n = last - g + 2;
-  float top = -INFINITY;
+  const int rows = m[kMetaRows], row0 = m[kMetaRow0], valid = rows - row0 < ROWS ? rows - row0 : ROWS;
+  const int group = threadIdx.x / T, ch = threadIdx.x % T * 4, most = (int)gridDim.x + 1 - g;   // workgroups from g on
+  for (int row = blockIdx.y; row < valid; row += gridDim.y) {
+    float top = -INFINITY, sum = 0.0f;
+    v4f o = {0, 0, 0, 0};
+    // part 0: of the workgroup that the item starts in; part i: of workgroup g + i - 1, if that starts inside the item
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_ml[(slot(i) * ROWS + row) * 2]);
-  v4f o = {0, 0, 0, 0};
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const size_t at = slot(i) * ROWS + row;
-    const float mw = p.part_ml[at * 2], f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
-    sum += p.part_ml[at * 2 + 1] * f;
-    o += *reinterpret_cast<const v4f*>(p.part_o + at * D + ch) * f;
+    for (int i = group; i <= most; i += GROUPS) {
+      if (i > 0 && (unsigned)m[(i - 1) * kMeta + kMetaU0] >= end) break;
+      const size_t at = (i == 0 ? 2 * (size_t)(g - 1) + 1 : 2 * (size_t)(g + i - 1)) * ROWS + row;
+      const float mi = p.part_ml[at * 2], li = p.part_ml[at * 2 + 1];
+      const v4f oi = *reinterpret_cast<const v4f*>(p.part_o + at * D + ch);
+      const float t = fmaxf(top, mi), f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t), f1 = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - t);
+      sum = sum * f0 + li * f1;
+      o = o * f0 + oi * f1;
+      top = t;
+    }
+    sums[group][threadIdx.x % T] = o;
+    if (ch == 0) ml[group][0] = top, ml[group][1] = sum;
+    __syncthreads();
+    if (group == 0) {
+      top = -INFINITY, sum = 0.0f, o = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, ml[k][0]);
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) {
+        const float f = ml[k][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][0] - top);
+        sum += ml[k][1] * f;
+        o += sums[k][threadIdx.x] * f;
+      }
+      finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
+    }
+    __syncthreads();
   }
-  finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
 }
 
 }  // namespace
 
-hipError_t launch_attn_combine(const AttnArgs& p, int rows, int workgroups, hipStream_t s) {
-  const int at_once = 1024 / p.c.head_dim;
-  const dim3 grid((unsigned)workgroups - 1, (unsigned)((rows + at_once - 1) / at_once));
+hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s) {
+  if (workgroups < 2) return hipSuccess;
+  const dim3 grid((unsigned)workgroups - 1, (unsigned)(rows_expected < 1 ? 1 : rows_expected < rows ? rows_expected : rows));
   if (p.c.head_dim == 64) hipLaunchKernelGGL((attn_combine_kernel<64>), grid, dim3(256), 0, s, p, rows);
   else if (p.c.head_dim == 128) hipLaunchKernelGGL((attn_combine_kernel<128>), grid, dim3(256), 0, s, p, rows);
   else hipLaunchKernelGGL((attn_combine_kernel<256>), grid, dim3(256), 0, s, p, rows);
