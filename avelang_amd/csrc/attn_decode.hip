@@ -152,13 +152,24 @@ struct Queries {
   }
 };
 
+// LDS of a workgroup (stages, or the waves' results when they meet), and how many workgroups fit the 160 KB of a compute unit
+template <int D, int NT, int NW, int NS>
+constexpr int lds_bytes() {
+  constexpr int kRing = NW * NS * Shape<D>::kStage, kJoin = NW * NT * 16 * (D + 4) * 4;
+  return kRing > kJoin ? kRing : kJoin;
+}
+template <int D, int NT, int NW, int NS>
+constexpr int workgroups_per_cu() {
+  return lds_bytes<D, NT, NW, NS>() <= 78 * 1024 ? 2 : 1;
+}
+
 template <int D, int NT, int NW, int NS, bool ONE_PAGE>
-__global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p) {
+__global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW / 4)) void attn_decode_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int ROWS = NT * 16, TILE = 64, C = D / 16;   // C: channel tiles of 16
+  constexpr bool kEarly = NT == 1;            // registers for a whole stage beside the rest
   constexpr int kPitch = D + 4;                          // floats of a row of a wave's result in LDS
-  constexpr int kRing = NW * NS * S::kStage, kJoin = NW * ROWS * kPitch * 4;
-  __shared__ __align__(16) unsigned char smem[kRing > kJoin ? kRing : kJoin];
+  __shared__ __align__(16) unsigned char smem[lds_bytes<D, NT, NW, NS>()];
   __shared__ float join_ml[NW][ROWS][2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane / 16, col = lane % 16;
   const Part part = take_part<ROWS, TILE>(p, blockIdx.x, gridDim.x);
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
     Queries<D, NT> q;
     q.request(p, it, rows);
     int requested = 0;
-    for (; requested < NS - 1 && requested < mine; ++requested)
+    for (; requested < (kEarly ? NS : NS - 1) && requested < mine; ++requested)
       request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + requested * S::kStage);
 
     q.convert(p);
@@ -229,32 +240,68 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
 
     for (int i = 0; i < mine; ++i) {
       const int t0 = (tile0 + wave + i * NW) * TILE;
-      if (requested < mine) {
-        request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + (requested % NS) * S::kStage);
-        ++requested;
-        wait_loads<(NS - 1) * S::kLoads>();
-      } else {
-        const int behind = mine - 1 - i;   // stages requested behind this one: fewer than NS - 1
-        if (NS > 3 && behind >= 2) wait_loads<(NS > 3 ? 2 : 0) * S::kLoads>();
-        else if (NS > 2 && behind >= 1) wait_loads<(NS > 2 ? 1 : 0) * S::kLoads>();
-        else wait_loads<0>();
-      }
+      const auto request_next = [&] {
+        if (requested < mine) {
+          request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + (requested % NS) * S::kStage);
+          ++requested;
+        }
+      };
+      if constexpr (!kEarly) request_next();
+      const int behind = requested - 1 - i;   // stages requested behind this one: below NS
+      if (NS > 3 && behind >= 3) wait_loads<(NS > 3 ? 3 : 0) * S::kLoads>();
+      else if (NS > 2 && behind >= 2) wait_loads<(NS > 2 ? 2 : 0) * S::kLoads>();
+      else if (NS > 1 && behind >= 1) wait_loads<(NS > 1 ? 1 : 0) * S::kLoads>();
+      else wait_loads<0>();
       const unsigned char* st = ring_ptr + (i % NS) * S::kStage;
       const unsigned char *keys = st, *values = st + S::kCodes, *ks = st + 2 * S::kCodes, *vs = ks + S::kScales;
+
+      // ---- the stage out of LDS
+      constexpr int kSteps = Queries<D, NT>::kSteps, kScaleWords = S::kScales / 16, kCheck = (S::kScales + 255) / 256;
+      const auto read_key = [&](int j, int step, v4i& x, int& scale) {
+        const int t = 16 * (col / 4) + 4 * j + col % 4, block = D == 64 ? g % 2 : step * 4 + g;
+        x = *reinterpret_cast<const v4i*>(keys + t * S::kRow + (block ^ S::key_swizzle(t)) * 16);
+        scale = ks[t * S::kBlocks + block];
+      };
+      const auto read_value = [&](int ch) {
+        const int t = 16 * g + col;
+        const unsigned char* at = values + t * S::kRow + (ch / 2 ^ S::value_swizzle(t)) * 16 + ch % 2 * 8;
+        return __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) v2i*)at);
+      };
+      const auto read_scale = [&](int k) { return reinterpret_cast<const unsigned*>(vs)[g * kScaleWords + k]; };   // of this group's 16 tokens
+      v4i key[4][kSteps];
+      int key_scale[4][kSteps];
+      v2i value[C];
+      unsigned value_scale[kScaleWords], check[kCheck];
+#pragma unroll
+      for (int k = 0; k < kCheck; ++k) {   // each word of the stage once, over the lanes
+        const int at = k * 256 + lane * 4;
+        check[k] = *reinterpret_cast<const unsigned*>(vs + (at < S::kScales ? at : 0));
+      }
+      if constexpr (kEarly) {   // all of it into registers: the buffer is free for the stage after next
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int step = 0; step < kSteps; ++step) read_key(j, step, key[j][step], key_scale[j][step]);
+#pragma unroll
+        for (int ch = 0; ch < C; ++ch) value[ch] = read_value(ch);
+#pragma unroll
+        for (int k = 0; k < kScaleWords; ++k) value_scale[k] = read_scale(k);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        request_next();
+      }
 
       // ---- scores
       v4f s[NT][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int t = 16 * (col / 4) + 4 * j + col % 4;
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) s[ct][j] = v4f{0, 0, 0, 0};
 #pragma unroll
-        for (int step = 0; step < Queries<D, NT>::kSteps; ++step) {
-          const int block = D == 64 ? g % 2 : step * 4 + g;
-          const v4i x = *reinterpret_cast<const v4i*>(keys + t * S::kRow + (block ^ S::key_swizzle(t)) * 16);
-          const int sk = ks[t * S::kBlocks + block];
+        for (int step = 0; step < kSteps; ++step) {
+          if constexpr (!kEarly) read_key(j, step, key[j][step], key_scale[j][step]);
+          const v4i x = key[j][step];
           const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+          const int sk = key_scale[j][step];
 #pragma unroll
           for (int ct = 0; ct < NT; ++ct) {
             if constexpr (D != 64)
@@ -308,21 +355,20 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
       // ---- values: a scale byte 0xFF (NaN) anywhere in the stage?  (also in what no key occupies: no row sees that)
       bool nan = false;
 #pragma unroll
-      for (int k = 0; k < (S::kScales + 255) / 256; ++k) {
-        const int at = k * 256 + lane * 4;
-        const unsigned x = ~*reinterpret_cast<const unsigned*>(vs + (at < S::kScales ? at : 0));
+      for (int k = 0; k < kCheck; ++k) {
+        const unsigned x = ~check[k];
         nan = nan || ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
       }
       nan = __any(nan);
       // the scale bytes of tokens 16 g + 2 k and + 1 for a block of channels, in 16 bits each
       const auto scale_pair = [&](int blk, int k) -> unsigned {
         if constexpr (D == 64) {
-          const unsigned w = reinterpret_cast<const unsigned*>(vs)[g * 8 + k];
+          const unsigned w = kEarly ? value_scale[k] : read_scale(k);
           return __builtin_amdgcn_perm(w, w, blk ? 0x0c030c01u : 0x0c020c00u);
         } else {
           constexpr int kWords = S::kBlocks / 4;
-          const unsigned w0 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k) * kWords + blk / 4];
-          const unsigned w1 = reinterpret_cast<const unsigned*>(vs)[(g * 16 + 2 * k + 1) * kWords + blk / 4];
+          const int at = 2 * k * kWords + blk / 4;
+          const unsigned w0 = kEarly ? value_scale[at] : read_scale(at), w1 = kEarly ? value_scale[at + kWords] : read_scale(at + kWords);
           return __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + 0x00010001u * (blk % 4));
         }
       };
@@ -356,9 +402,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int ch = blk * 2 + half;
-          const int t = 16 * g + col;
-          const unsigned char* at = values + t * S::kRow + (blk ^ S::value_swizzle(t)) * 16 + half * 8;
-          const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) v2i*)at);
+          const v2i w = kEarly ? value[ch] : read_value(ch);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const unsigned x = (unsigned)w[k];
@@ -416,35 +460,42 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_decode_kernel(AttnArgs p
 }
 
 template <int D, int NT, int NW, int NS>
-hipError_t launch_form(AttnArgs p, void* ws, hipStream_t s) {
+hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
   constexpr int ROWS = NT * 16;
-  const int workgroups = compute_units();
-  // items of at most two rounds of the waves stay whole: cutting them saves less than the second launch costs
-  const int64_t in_table = (int64_t)p.a.table_pages << p.page_shift, in_window = p.a.window > 0 ? (int64_t)p.a.window + p.a.max_q : in_table;
-  p.whole = (in_window < in_table ? in_window : in_table) <= 2 * NW * 64;
+  const int workgroups = compute_units() * workgroups_per_cu<D, NT, NW, NS>();
+  p.whole = whole;
   p.min_units_log2 = p.whole ? 0 : log2_of(NW);
   if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
   const dim3 grid((unsigned)workgroups), block(NW * 64);
   if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false>), grid, block, 0, s, p);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.whole) return e;
-  return launch_attn_combine(p, ROWS, p.a.cu_q ? p.a.max_q * p.group : p.group, workgroups, s);
+  return launch_attn_combine(p, ROWS, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
+}
+
+// Items of at most 1024 keys stay whole: cutting them saves less than the second launch costs.
+bool keep_whole(const AttnArgs& p) {
+  const int64_t in_table = (int64_t)p.a.table_pages << p.page_shift, in_window = p.a.window > 0 ? (int64_t)p.a.window + p.a.max_q : in_table;
+  return (in_window < in_table ? in_window : in_table) <= 1024;
 }
 
 }  // namespace
 
-size_t attn_decode_workspace(const AttnArgs& p, int row_tiles) { return attn_workspace(row_tiles * 16, p.c.head_dim, compute_units()); }
+size_t attn_decode_workspace(const AttnArgs& p, int row_tiles) {
+  return keep_whole(p) ? 0 : attn_workspace(row_tiles * 16, p.c.head_dim, 2 * compute_units());
+}
 
 hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s) {
+  const bool whole = keep_whole(p);
   switch (p.c.head_dim * 8 + row_tiles) {
-    case 64 * 8 + 1: return launch_form<64, 1, 8, 4>(p, ws, s);
-    case 64 * 8 + 2: return launch_form<64, 2, 8, 4>(p, ws, s);
-    case 64 * 8 + 4: return launch_form<64, 4, 4, 4>(p, ws, s);
-    case 128 * 8 + 1: return launch_form<128, 1, 8, 2>(p, ws, s);
-    case 128 * 8 + 2: return launch_form<128, 2, 8, 2>(p, ws, s);
-    case 128 * 8 + 4: return launch_form<128, 4, 4, 4>(p, ws, s);
-    case 256 * 8 + 1: return launch_form<256, 1, 4, 2>(p, ws, s);
-    default: return launch_form<256, 2, 4, 2>(p, ws, s);
+    case 64 * 8 + 1: return whole ? launch_form<64, 1, 8, 4>(p, whole, ws, s) : launch_form<64, 1, 4, 4>(p, whole, ws, s);
+    case 64 * 8 + 2: return whole ? launch_form<64, 2, 8, 4>(p, whole, ws, s) : launch_form<64, 2, 4, 4>(p, whole, ws, s);
+    case 64 * 8 + 4: return launch_form<64, 4, 4, 4>(p, whole, ws, s);
+    case 128 * 8 + 1: return whole ? launch_form<128, 1, 8, 2>(p, whole, ws, s) : launch_form<128, 1, 4, 2>(p, whole, ws, s);
+    case 128 * 8 + 2: return whole ? launch_form<128, 2, 8, 2>(p, whole, ws, s) : launch_form<128, 2, 4, 2>(p, whole, ws, s);
+    case 128 * 8 + 4: return launch_form<128, 4, 4, 4>(p, whole, ws, s);
+    case 256 * 8 + 1: return launch_form<256, 1, 4, 2>(p, whole, ws, s);
+    default: return launch_form<256, 2, 4, 2>(p, whole, ws, s);
   }
 }
 
