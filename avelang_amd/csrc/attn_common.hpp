@@ -26,6 +26,7 @@ struct AttnArgs {
   int group;          // query heads per key head
   int page_shift;
   int whole;          // 1: items are not split; no workspace, no second launch
+  int few_long;       // few sequences of many blocks of rows each
   int min_units_log2; // of a workgroup, so that small calls are not cut into crumbs
   int* meta;          // workspace: [workgroups][kMeta]
   float* part_ml;     // [2 workgroups][ROWS][2]: maximum (base 2) and sum
@@ -50,19 +51,22 @@ enum { kMetaU0, kMetaBegin, kMetaEnd, kMetaFirst, kMetaRows, kMetaHead, kMetaRow
 struct Sequence {
   int first, n, len;   // first row of q, new tokens, keys
 };
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;   // read through the scalar cache where the index is uniform
+
 __device__ inline Sequence sequence(const AttnArgs& p, int b) {
+  const ConstInts cu = (ConstInts)p.a.cu_q, lens = (ConstInts)p.a.seq_lens;
   Sequence s;
   if (p.a.cu_q) {
-    s.first = p.a.cu_q[b];
+    s.first = cu[b];
     s.first = s.first < 0 ? 0 : s.first > p.a.tokens ? p.a.tokens : s.first;
-    int end = p.a.cu_q[b + 1];
+    int end = cu[b + 1];
     end = end < s.first ? s.first : end > p.a.tokens ? p.a.tokens : end;
     s.n = end - s.first;
   } else {
     s.first = b, s.n = 1;
   }
   const int most = p.a.table_pages << p.page_shift;
-  s.len = p.a.seq_lens[b];
+  s.len = lens[b];
   s.len = s.len < 0 ? 0 : s.len > most ? most : s.len;
   return s;
 }
@@ -96,6 +100,7 @@ __device__ inline int sequence_units(const AttnArgs& p, const Sequence& s) {   /
   return u;
 }
 
+__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ inline unsigned wave_scan(unsigned v) {   // inclusive prefix sums over the lanes
   v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // one, two, four, eight lanes to the right in a row of 16
   v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
@@ -105,7 +110,18 @@ __device__ inline unsigned wave_scan(unsigned v) {   // inclusive prefix sums ov
   v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
   return v;
 }
-__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// The same for a sequence of many blocks, which the lanes of a wave share
+template <int ROWS, int TILE>
+__device__ inline unsigned wave_sequence_units(const AttnArgs& p, const Sequence& s) {
+  unsigned u = 0;
+  int tile0;
+  const int rows = s.n * p.group, lane = threadIdx.x & 63;
+  for (int row0 = 0; row0 < rows; row0 += 64 * ROWS) {
+    const int mine = row0 + lane * ROWS;
+    u += (unsigned)lane_value((int)wave_scan(mine < rows ? (unsigned)block_units<ROWS, TILE>(p, s, mine, tile0) : 0u), 63);
+  }
+  return u;
+}
 
 // The part of a workgroup: units [u0, u1) of all `units`, cut into `parts` equal ones; sequence b holds u0, b_begin is its first unit and
 // per_head the units of one of its key heads.  Every wave finds it by itself (no barrier): 64 sequences at a time, a lane each.
@@ -119,8 +135,32 @@ struct Part {
 // First unit of part g: the first units % parts parts have one unit more
 __device__ inline unsigned part_start(unsigned each, unsigned more, unsigned g) { return g * each + (g < more ? g : more); }
 
-template <int ROWS, int TILE>
+__device__ inline void cut(const AttnArgs& p, Part& r, unsigned g, unsigned workgroups) {
+  const unsigned want = (r.units + (1u << p.min_units_log2) - 1) >> p.min_units_log2;
+  r.parts = want < workgroups ? (want ? want : 1) : workgroups;
+  const unsigned each = r.units / r.parts, more = r.units - each * r.parts;
+  r.u0 = g < r.parts ? part_start(each, more, g) : r.units;
+  r.u1 = g < r.parts ? part_start(each, more, g + 1) : r.units;
+}
+
+// LONG: sequences may have many blocks of rows; where p.few_long says so the wave takes one sequence after the other.
+template <int ROWS, int TILE, bool LONG = false>
 __device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgroups) {
+  if constexpr (LONG) {
+    if (p.few_long) {
+      Part r{};
+      const unsigned heads = (unsigned)p.c.kv_heads;
+      for (int b = 0; b < p.a.batch; ++b) r.units += heads * wave_sequence_units<ROWS, TILE>(p, sequence(p, b));
+      cut(p, r, g, workgroups);
+      for (r.b = 0; r.b < p.a.batch; ++r.b) {
+        r.s = sequence(p, r.b);
+        r.per_head = wave_sequence_units<ROWS, TILE>(p, r.s);
+        if (r.u0 < r.b_begin + heads * r.per_head) break;
+        r.b_begin += heads * r.per_head;
+      }
+      return r;
+    }
+  }
   const int lane = threadIdx.x & 63;
   const unsigned heads = (unsigned)p.c.kv_heads;
   const auto load = [&](int b) {
@@ -139,11 +179,7 @@ __device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgro
     next = load(b0 + 64 + lane);
     r.units += (unsigned)lane_value((int)wave_scan((unsigned)sequence_units<ROWS, TILE>(p, now) * heads), 63);
   }
-  const unsigned want = (r.units + (1u << p.min_units_log2) - 1) >> p.min_units_log2;
-  r.parts = want < workgroups ? (want ? want : 1) : workgroups;
-  const unsigned each = r.units / r.parts, more = r.units - each * r.parts;
-  r.u0 = g < r.parts ? part_start(each, more, g) : r.units;
-  r.u1 = g < r.parts ? part_start(each, more, g + 1) : r.units;
+  cut(p, r, g, workgroups);
   if (r.u0 >= r.u1) return r;
   unsigned base = 0;
   int b0 = 0;
@@ -172,20 +208,39 @@ struct Item {
   unsigned begin, units;
 };
 // The item that holds unit u >= b_begin; moves b, b_begin, the sequence s and its units of one head on to it.
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, bool LONG = false>
 __device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& b_begin, Sequence& s, unsigned& per_head) {
   Item it;
   // (u is below the number of all units; the bounds on b and row0 hold if lengths change under the call, too)
   while (u >= b_begin + per_head * (unsigned)p.c.kv_heads && b + 1 < p.a.batch) {
     b_begin += per_head * (unsigned)p.c.kv_heads;
-    ++b;
+    b = __builtin_amdgcn_readfirstlane(b + 1);
     s = sequence(p, b);
-    per_head = (unsigned)sequence_units<ROWS, TILE>(p, s);
+    per_head = LONG ? wave_sequence_units<ROWS, TILE>(p, s) : (unsigned)sequence_units<ROWS, TILE>(p, s);
   }
   it.s = s;
   it.head = 0;
   it.begin = b_begin;
   while (u >= it.begin + per_head && it.head + 1 < p.c.kv_heads) it.begin += per_head, ++it.head;
+  if constexpr (LONG) {   // 64 blocks at a time, a lane each
+    const int lane = threadIdx.x & 63, rows = s.n * p.group;
+    for (int row0 = 0;; row0 += 64 * ROWS) {
+      const int mine = row0 + lane * ROWS;
+      int tile0 = 0;
+      const unsigned units = mine < rows ? (unsigned)block_units<ROWS, TILE>(p, s, mine, tile0) : 0u, in = wave_scan(units);
+      const unsigned total = (unsigned)lane_value((int)in, 63);
+      if (u < it.begin + total || row0 + 64 * ROWS >= rows) {
+        const uint64_t here = __ballot(u < it.begin + in);
+        const int at = here ? __ffsll((unsigned long long)here) - 1 : 0;
+        it.row0 = row0 + at * ROWS;
+        it.units = (unsigned)lane_value((int)units, at);
+        it.tile0 = lane_value(tile0, at);
+        it.begin += (unsigned)lane_value((int)(in - units), at);
+        return it;
+      }
+      it.begin += total;
+    }
+  }
   for (it.row0 = 0;; it.row0 += ROWS) {
     it.units = (unsigned)block_units<ROWS, TILE>(p, it.s, it.row0, it.tile0);
     if (u < it.begin + it.units || it.row0 + ROWS >= it.s.n * p.group) break;
@@ -210,7 +265,11 @@ __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-typedef const __attribute__((address_space(4))) int32_t* ConstInts;   // read through the scalar cache where the index is uniform
+__device__ inline unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+// A barrier that orders LDS and leaves loads to LDS under way
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Page of tokens 16 i .. 16 i + 15 of a sequence; a valid one whatever the table holds (tokens behind the last key: the last key's)
 __device__ inline int page_at(const AttnArgs& p, ConstInts row, int token, int len) {
@@ -313,24 +372,34 @@ __device__ inline size_t row_index(const AttnArgs& p, int first, int head, int r
   return (size_t)(first + t) * p.a.heads + head * p.group + (row - t * p.group);
 }
 
-// Four channels of a finished row: o / l, with the sink's share of the sum; m in base 2 (-inf: the row saw nothing).
-__device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int channel, v4f o, float m, float l) {
-  const int head = (int)(row % (unsigned)p.a.heads);
+// What the sums of a finished row are multiplied with, and its lse; m in base 2 (-inf: the row saw nothing).
+struct RowEnd {
+  float factor, lse;
+};
+__device__ inline RowEnd row_end(const AttnArgs& p, int query_head, float m, float l) {
   const bool none = m == -INFINITY && l == l;   // (only NaN scores: the sum is NaN)
   float total = l, top = m, fade = 1.0f;
   if (p.a.sinks) {
-    const float sink = p.a.sinks[head] * kLog2e;
+    const float sink = p.a.sinks[query_head] * kLog2e;
     top = fmaxf(m, sink);
     fade = none ? 0.0f : __builtin_amdgcn_exp2f(m - top);
     total = l * fade + (sink == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sink - top));
   }
-  const float f = none ? 0.0f : fade / total;
-  uint16_t* out = p.a.out + row * D + channel;
-  reinterpret_cast<unsigned*>(out)[0] = pack_bf16x2(o[0] * f, o[1] * f);
-  reinterpret_cast<unsigned*>(out)[1] = pack_bf16x2(o[2] * f, o[3] * f);
-  if (p.a.lse && channel == 0) p.a.lse[row] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+  return {none ? 0.0f : fade / total, (top + __builtin_amdgcn_logf(total)) * kLn2};
+}
+__device__ inline void store4_bf16(uint16_t* out, v4f o) {
+  reinterpret_cast<unsigned*>(out)[0] = pack_bf16x2(o[0], o[1]);
+  reinterpret_cast<unsigned*>(out)[1] = pack_bf16x2(o[2], o[3]);
+}
+// Four channels of a finished row
+__device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int channel, v4f o, float m, float l) {
+  const RowEnd e = row_end(p, (int)(row % (unsigned)p.a.heads), m, l);
+  store4_bf16(p.a.out + row * D + channel, o * e.factor);
+  if (p.a.lse && channel == 0) p.a.lse[row] = e.lse;
 }
 
+hipError_t launch_attn_prompt(AttnArgs p, void* workspace, hipStream_t s);
+size_t attn_prompt_workspace(const AttnArgs& p);
 hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* workspace, hipStream_t s);
 size_t attn_decode_workspace(const AttnArgs& p, int row_tiles);
 // rows: of a block; rows_expected: of a sequence and key head

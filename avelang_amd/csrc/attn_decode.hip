@@ -29,9 +29,6 @@ struct Shape {
   __device__ static int value_swizzle(int t) { return D == 64 ? (t >> 3) & 1 : D == 128 ? (t >> 2) & 3 : (t >> 1) & 7; }
 };
 
-__device__ inline unsigned lds_address(const void* p) {
-  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
-}
 
 // (values, not the elements of an array: a choice of elements would keep the array in memory)
 __device__ inline const uint8_t* pick(bool first, const uint8_t* a, const uint8_t* b) { return first ? a : b; }
@@ -352,12 +349,12 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
         }
       }
 
-      // ---- values: a scale byte 0xFF (NaN) anywhere in the stage?  (also in what no key occupies: no row sees that)
+      // ---- values: a scale byte from 253 on (NaN) anywhere in the stage?  (also in what no key occupies: no row sees that)
       bool nan = false;
 #pragma unroll
       for (int k = 0; k < kCheck; ++k) {
         const unsigned x = ~check[k];
-        nan = nan || ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
+        nan = nan || ((x - 0x03030303u) & ~x & 0x80808080u) != 0;
       }
       nan = __any(nan);
       // the scale bytes of tokens 16 g + 2 k and + 1 for a block of channels, in 16 bits each
@@ -380,7 +377,7 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
             unsigned hit = 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              hit |= as_u32(as_us2(pk_sub_sat(scale_pair(blk, k), 0x00FE00FEu)) * __builtin_elementwise_min(as_us2(prob[ct][k]), us2{1, 1}));
+              hit |= as_u32(as_us2(pk_sub_sat(scale_pair(blk, k), 0x00FC00FCu)) * __builtin_elementwise_min(as_us2(prob[ct][k]), us2{1, 1}));
             const float poison = cross_max<true>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
             acc[ct][2 * blk] += poison;
             acc[ct][2 * blk + 1] += poison;

@@ -1,0 +1,344 @@
+// Attention of many query rows over a paged MXFP4 cache: prompts and chunks of prompts.
+//
+// Bound by the matrix cores and by the exponentials beside them.  A workgroup takes blocks of 128 rows -- (token, query head) pairs of one
+// key head, 32 a wave -- through 64 keys at a time (attn_common.hpp cuts the triangle of a prompt into equal parts):
+//
+//   S^T = K Q^T   scaled MFMA 32x32x64, keys as they are (E2M1 codes and E8M0 scales straight from memory into LDS), queries as two E4M3
+//                 parts.  Row 8 i + 4 h + t of a tile of 32 keys is key 16 h + 4 i + t, so that lane half h = lane / 32 of the result holds
+//                 keys 16 h .. 16 h + 15 of the tile for query row lane % 32.
+//   O^T = V^T P^T bf16 MFMA 32x32x16: P goes from the result's registers into the operand as it is, rounded to bf16.  Values are converted once
+//                 a workgroup, codes times their scales (exact), and lie in LDS as bf16 rows that transposing reads hand out by columns.
+//
+// The next 64 keys and values are requested before the present ones are multiplied; two workgroups a compute unit.
+#include "attn_common.hpp"
+#include "kernels.hpp"
+
+namespace ave {
+namespace {
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 64, kWaves = 4, kRows = 32 * kWaves;
+
+template <int D>
+struct Shape {
+  static constexpr int kRow = D / 2, kBlocks = D / 32, kSteps = D / 64, C = D / 32;
+  static constexpr int kKeys = kTile * kRow, kScales = kTile * kBlocks, kValues = kTile * D * 2;
+  static constexpr int kBuffer = kKeys + kScales + kValues;
+  static constexpr int kThreadBytes = kTile * kRow / (kWaves * 64);   // of values' codes: 8, 16 or 32, within one or two blocks of a token
+  // LDS positions.  Keys: 16-byte pieces permuted so that the 16 lanes of a read touch different banks.  Values: a row's 64-byte segments, and
+  // the pieces of a segment, permuted by the token for the transposing reads (four tokens, 64 bytes each) and the writes.
+  __device__ static int key_swizzle(int t) {
+    return D == 64 ? (t >> 4) & 1 : D == 128 ? ((t >> 2) & 1) | ((t >> 4) & 1) << 1 : ((t >> 1) & 1) | ((t >> 2) & 1) << 1 | ((t >> 4) & 1) << 2;
+  }
+  __device__ static int value_swizzle(int t) { return D == 64 ? 5 * ((t >> 1) & 1) : 5 * (t & 3); }
+};
+
+// Values' codes of one thread for one tile, and their scale bytes
+template <int D>
+struct Values {
+  static constexpr int kWords = Shape<D>::kThreadBytes / 4, kScaleBytes = D == 256 ? 2 : 1;
+  unsigned code[kWords];
+  int scale[kScaleBytes];
+};
+
+template <int D>
+__global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p) {
+  using S = Shape<D>;
+  constexpr int C = S::C;
+  __shared__ __align__(16) unsigned char smem[2 * S::kBuffer];
+  __shared__ uint64_t nan_in[2][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
+  // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
+  const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+  const Part part = take_part<kRows, kTile, true>(p, g, gridDim.x);
+  const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
+  const float c = fabsf(p.a.scale) * kLog2e;
+  int b = part.b;
+  unsigned b_begin = part.b_begin, per_head = part.per_head;
+  Sequence seq = part.s;
+  if (!p.whole && tid == 0 && part.u0 >= part.u1) {   // no work
+    int* m = p.meta + (size_t)g * kMeta;
+    m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
+  }
+  bool first_item = true;
+  for (unsigned u = part.u0; u < part.u1;) {
+    const Item it = item_of<kRows, kTile, true>(p, u, b, b_begin, seq, per_head);
+    const unsigned end = it.begin + it.units, from = u, to = end < part.u1 ? end : part.u1;
+    u = to;
+    if (first_item && tid == 0) {
+      int* m = p.meta + (size_t)g * kMeta;
+      m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)end, m[kMetaFirst] = it.s.first;
+      m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
+    }
+    first_item = false;
+    const int rows = it.s.n * p.group, tile0 = it.tile0 + (int)(from - it.begin);
+    const int tiles = it.s.len > 0 ? (int)(to - from) : 0;
+    const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
+
+    // what this wave's rows see: [lo_row, hi_row) of a lane's row, [lo_max, hi_min) of all, [lo_min, hi_max) of any
+    const int row0 = it.row0 + 32 * wave;
+    const bool active = row0 < rows;
+    int lo_row, hi_row, lo_max, hi_min, lo_min, hi_max;
+    {
+      const int last = row0 + 32 < rows ? row0 + 31 : rows - 1, row = row0 + col < rows ? row0 + col : last;
+      visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
+      visible(p, it.s, p.token_of(last), lo_max, hi_max);
+      visible(p, it.s, p.token_of(row), lo_row, hi_row);
+    }
+
+    // ---- queries: lane (column col): bytes 0-15 of a step are k = 16 h .., bytes 16-31 k = 32 + 16 h ..
+    v8i q_hi[S::kSteps], q_lo[S::kSteps];
+    int s_hi, s_lo;
+    {
+      const bool real = row0 + col < rows;
+      const int t = real ? p.token_of(row0 + col) : 0;
+      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)(it.head * p.group + (real ? row0 + col - t * p.group : 0)) * p.a.q_head_stride;
+      v4i x[S::kSteps][4];
+      us2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[i][k] = v4i{0, 0, 0, 0};
+          if (real) x[i][k] = load8_bf16(q + 64 * i + 32 * (k / 2) + 16 * h + 8 * (k % 2));
+          m = amax_pairs(x[i][k], m);
+        }
+      const QueryScale s = query_scale(lane_xor_max_bits(larger_half(m), 32));
+      const int sign = p.a.scale < 0.0f ? (int)0x80808080u : 0;
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          int hi[2], lo[2];
+          split_query(x[i][k], s, hi, lo);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) q_hi[i][2 * k + e] = hi[e] ^ sign, q_lo[i][2 * k + e] = lo[e] ^ sign;
+        }
+      s_hi = s.hi_byte, s_lo = s.lo_byte;
+    }
+
+    // ---- a tile's requests: keys and their scales to LDS, values to registers; a wave takes 16 tokens, which lie in one page
+    Values<D> next;
+    const auto request_tile = [&](int t0, int buffer) {
+      const int t = t0 + 16 * wave, pg = page_at(p, table, t, it.s.len);
+      const unsigned row = (unsigned)(it.head * p.c.page_size + (t & (p.c.page_size - 1)));
+      const uint8_t* key = p.c.k + (int64_t)pg * p.c.k_page_stride + row * (unsigned)S::kRow;
+      const unsigned at = lds + buffer * S::kBuffer;
+      constexpr int kPieces = S::kRow / 16;
+#pragma unroll
+      for (int i = 0; i < (16 * S::kRow + 1023) / 1024; ++i) {
+        const int token = i * (64 / kPieces) + lane / kPieces;
+        const unsigned off = token * S::kRow + ((lane % kPieces) ^ S::key_swizzle(16 * wave + token)) * 16;
+        if (D > 64 || lane < 32) to_lds16(key, off, at + wave * (16 * S::kRow) + i * 1024);
+      }
+      const uint8_t* key_scale = p.c.k_scale + (int64_t)pg * p.c.k_scale_page_stride + row * (unsigned)S::kBlocks;
+      if (lane < 4 * S::kBlocks) to_lds4(key_scale + lane * 4, at + S::kKeys + wave * (16 * S::kBlocks));
+      const uint8_t* value = p.c.v + (int64_t)pg * p.c.v_page_stride + row * (unsigned)S::kRow + lane * S::kThreadBytes;
+#pragma unroll
+      for (int k = 0; k < Values<D>::kWords; k += 2) {
+        const v2i x = *reinterpret_cast<const v2i*>(value + 4 * k);
+        next.code[k] = (unsigned)x[0], next.code[k + 1] = (unsigned)x[1];
+      }
+      const uint8_t* value_scale = p.c.v_scale + (int64_t)pg * p.c.v_scale_page_stride + row * (unsigned)S::kBlocks + lane / 4 * S::kBlocks;
+#pragma unroll
+      for (int k = 0; k < Values<D>::kScaleBytes; ++k) next.scale[k] = value_scale[D == 64 ? lane % 4 / 2 : D == 128 ? lane % 4 : 2 * (lane % 4) + k];
+    };
+    const auto store_values = [&](int t0, int buffer) {
+      const int token = 16 * wave + lane / 4, quarter = lane % 4;
+      unsigned char* at = smem + buffer * S::kBuffer + S::kKeys + S::kScales + token * (2 * D);
+      const bool there = t0 + token < it.s.len;   // what no key occupies is zero
+#pragma unroll
+      for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
+        constexpr int kOfScale = Values<D>::kWords / Values<D>::kScaleBytes;
+        const bool bad = there && next.scale[k] >= 253, none = bad || !there;
+#pragma unroll
+        for (int w = 0; w < kOfScale; ++w) next.code[k * kOfScale + w] = none ? 0 : next.code[k * kOfScale + w];
+        next.scale[k] = none ? 127 : next.scale[k];
+        const uint64_t lanes = __ballot(bad);
+        if (lane == 0) nan_in[buffer][k][wave] = lanes;
+      }
+#pragma unroll
+      for (int w = 0; w < Values<D>::kWords; ++w) {   // eight channels, one 16-byte piece
+        const float f = __builtin_bit_cast(float, (unsigned)next.scale[D == 256 ? w / 4 : 0] << 23);
+        const unsigned x = next.code[w];
+        const v2bf a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 1);
+        const v2bf a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 3);
+        const v8bf v = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+        const int piece = quarter * Values<D>::kWords + w;
+        *reinterpret_cast<v8bf*>(at + (piece ^ S::value_swizzle(token)) * 16) = v;
+      }
+    };
+
+    v16f acc[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) acc[i] = v16f{};
+    float m = kNone, l = 0.0f;
+
+    if (tiles > 0) {
+      request_tile(tile0 * kTile, 0);
+      store_values(tile0 * kTile, 0);
+      wait_loads<0>();
+    }
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      const int t0 = (tile0 + i) * kTile;
+      if (i + 1 < tiles) request_tile(t0 + kTile, (i + 1) & 1);
+      if (active && t0 < hi_max && t0 + kTile > lo_min) {
+        const unsigned char* keys = smem + (i & 1) * S::kBuffer;
+        const unsigned char *ks = keys + S::kKeys, *values = ks + S::kScales;
+        // ---- scores
+        v16f s[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int t = 32 * j + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);   // row 8 i + 4 h' + t' is key 16 h' + 4 i + t'
+          unsigned sk[(S::kBlocks + 3) / 4];
+          if constexpr (D == 64) {
+            sk[0] = *reinterpret_cast<const uint16_t*>(ks + t * 2) >> (8 * h);
+          } else {
+#pragma unroll
+            for (int k = 0; k < S::kBlocks / 4; ++k) sk[k] = reinterpret_cast<const unsigned*>(ks)[t * (S::kBlocks / 4) + k] >> (8 * h);
+          }
+          s[j] = v16f{};
+#pragma unroll
+          for (int step = 0; step < S::kSteps; ++step) {
+            const v4i x = *reinterpret_cast<const v4i*>(keys + t * S::kRow + ((2 * step + h) ^ S::key_swizzle(t)) * 16);
+            const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+            if (step % 2 == 0) {
+              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[step], s[j], kFmtFp4, 0, 0, (int)sk[step / 2], 0, s_lo);
+              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[step], s[j], kFmtFp4, 0, 0, (int)sk[step / 2], 0, s_hi);
+            } else {
+              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[step], s[j], kFmtFp4, 0, 2, (int)sk[step / 2], 0, s_lo);
+              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[step], s[j], kFmtFp4, 0, 2, (int)sk[step / 2], 0, s_hi);
+            }
+          }
+        }
+        // ---- probabilities
+        const bool all_seen = t0 >= lo_max && t0 + kTile <= hi_min;
+        if (!all_seen) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+              const int key = t0 + 32 * j + 16 * h + t;
+              s[j][t] = key >= lo_row && key < hi_row ? s[j][t] : kNone;
+            }
+        }
+        float top = kNone;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < 16; t += 2) top = fmaxf(top, fmaxf(s[j][t], s[j][t + 1]));
+        top = fmaxf(m, cross_max<false>(top));
+        if (__any(top > m)) {
+          const float fade = __builtin_amdgcn_exp2f((m - top) * c);
+          l *= fade;
+#pragma unroll
+          for (int k = 0; k < C; ++k) acc[k] *= fade;
+          m = top;
+        }
+        const float shift = -m * c;
+        unsigned prob[2][8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < 16; t += 2) {
+            float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t + 1], c, shift));
+            if (!all_seen) {   // (where a row has seen nothing yet, or c is 0)
+              a = s[j][t] == kNone ? 0.0f : a;
+              d = s[j][t + 1] == kNone ? 0.0f : d;
+            }
+            l += a + d;
+            prob[j][t / 2] = pack_bf16x2(a, d);
+          }
+        // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
+        uint64_t nan = 0;
+#pragma unroll
+        for (int k = 0; k < Values<D>::kScaleBytes; ++k)
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) nan |= nan_in[i & 1][k][w];
+        if (__builtin_amdgcn_readfirstlane((int)(nan | nan >> 32))) {
+          uint64_t some[2] = {0, 0};   // four bits for each of this lane's keys, set where its probability is not zero
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int t = 0; t < 16; ++t) some[j] |= (prob[j][t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
+#pragma unroll
+          for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
+            const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
+            const uint64_t hits = (nan_in[i & 1][D == 256 ? k % 2 : 0][h] & some[0]) | (nan_in[i & 1][D == 256 ? k % 2 : 0][2 + h] & some[1]);
+            const bool hit = (hits & (0x1111111111111111ull << quarter)) != 0;
+            acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
+          }
+        }
+        // ---- values
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const v4i w = {(int)prob[j][4 * half], (int)prob[j][4 * half + 1], (int)prob[j][4 * half + 2], (int)prob[j][4 * half + 3]};
+            const v8bf pb = __builtin_bit_cast(v8bf, w);
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+              const int r = lane % 16 / 4;   // token within four
+              const int piece = 4 * k + 2 * ((lane / 16) & 1) + (lane % 4) / 2;
+              const unsigned char* at = values + (32 * j + 16 * h + 8 * half + r) * (2 * D) + (piece ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
+              const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)at);
+              const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at + 4 * 2 * D));
+              typedef short v8s __attribute__((ext_vector_type(8)));
+              const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+              acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), pb, acc[k], 0, 0, 0);
+            }
+          }
+      }
+      if (i + 1 < tiles) store_values(t0 + kTile, (i + 1) & 1);
+      wait_loads<0>();
+      __syncthreads();
+    }
+
+    // ---- results: lane (column col) has channels 32 k + 8 i + 4 h .. + 3 of its row
+    if (active) {
+      const float sum = cross_sum<false>(l), m2 = m == kNone ? -INFINITY : m * c;
+      const bool done = from == it.begin && to == end;
+      const int row = row0 + col;
+      if (row < rows) {
+        const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + 32 * wave + col;
+        const size_t place = row_index(p, it.s.first, it.head, row);
+        const RowEnd e = row_end(p, it.head * p.group + (row - p.token_of(row) * p.group), m2, sum);
+        if (done && p.a.lse && h == 0) p.a.lse[place] = e.lse;
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const v4f o = {acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]};
+            const int ch = 32 * k + 8 * i + 4 * h;
+            if (done) store4_bf16(p.a.out + place * D + ch, o * e.factor);
+            else *reinterpret_cast<v4f*>(p.part_o + at * D + ch) = o;
+          }
+        if (!done && h == 0) p.part_ml[at * 2] = m2, p.part_ml[at * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+int workgroups_of() { return 2 * compute_units(); }
+
+}  // namespace
+
+size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p.c.head_dim, workgroups_of()); }
+
+hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
+  const int workgroups = workgroups_of();
+  p.whole = 0;
+  p.min_units_log2 = 2;
+  p.few_long = p.a.batch <= 16;
+  place_workspace(p, kRows, workgroups, ws);
+  const dim3 grid((unsigned)workgroups), block(kWaves * 64);
+  if (p.c.head_dim == 64) hipLaunchKernelGGL((attn_prompt_kernel<64>), grid, block, 0, s, p);
+  else if (p.c.head_dim == 128) hipLaunchKernelGGL((attn_prompt_kernel<128>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attn_prompt_kernel<256>), grid, block, 0, s, p);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  return launch_attn_combine(p, kRows, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
+}
+
+}  // namespace ave

@@ -436,7 +436,8 @@ int ave_fp4_gather_kv_mxfp4(const ave_fp4_kv_cache* cache, const int32_t* slots,
  *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink_h)),  s_j = scale * q . k_j      (sinks null: without the last term)
  *   lse = log of the denominator (optional; natural logarithm, the sink included; -inf where it is zero)
  * A row that sees no key gives zeros.  Scores, softmax and sums in fp32; queries enter the products with 19 bits and more below
- * their row's largest one, probabilities as bf16.  A NaN or infinity in a query, or a NaN scale of a key or value it sees, gives NaN.
+ * their row's largest one, probabilities as bf16.  A NaN or infinity in a query, or a NaN scale (0xFF) of a key it sees, gives NaN; so does,
+ * in its 32 channels, a scale of a value it sees from 253 on (beyond what bf16 holds; the quantiser writes 252 at most).
  * Rows of q behind cu_q[batch] are left alone.  Device data is never trusted with addresses: lengths are cut to the page
  * table's width, rows to q's, pages outside the cache are read as its nearest page.
  * max_q: a bound on the new tokens of a sequence, by which the kernel is chosen (a wrong one costs time only).
