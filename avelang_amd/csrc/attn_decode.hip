@@ -499,11 +499,12 @@ hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s
 // ---- parts of split items, joined -----------------------------------------------------------------------------------------------
 namespace {
 
-// blockIdx.x: a boundary between two workgroups of the first launch; the first boundary inside an item joins the item's parts, a row
-// (of every gridDim.y) per workgroup: 1024 / D groups of threads add up every so many parts and meet in LDS.
-template <int D>
+// blockIdx.x: a boundary between two workgroups of the first launch; the first boundary inside an item joins the item's parts.  A thread
+// takes four channels of a row.  GROUPS > 1 (few rows of many parts): the threads of a row are GROUPS groups that take every so many parts and
+// meet in LDS; GROUPS = 1 (prompts: many rows of two or three parts): 1024 / D rows at once.
+template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS) {
-  constexpr int T = D / 4, GROUPS = 256 / T;
+  constexpr int T = D / 4, R = 256 / T / GROUPS;
   __shared__ v4f sums[GROUPS][T];
   __shared__ float ml[GROUPS][2];
   const int g = blockIdx.x + 1;
@@ -511,49 +512,65 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS)
   const unsigned begin = (unsigned)m[kMetaBegin], end = (unsigned)m[kMetaEnd], u0 = (unsigned)m[kMetaU0];
   if (begin >= u0 || (unsigned)m[kMetaU0 - kMeta] > begin) return;
   const int rows = m[kMetaRows], row0 = m[kMetaRow0], valid = rows - row0 < ROWS ? rows - row0 : ROWS;
-  const int group = threadIdx.x / T, ch = threadIdx.x % T * 4, most = (int)gridDim.x + 1 - g;   // workgroups from g on
-  for (int row = blockIdx.y; row < valid; row += gridDim.y) {
+  const int group = GROUPS > 1 ? threadIdx.x / T : 0, ch = threadIdx.x % T * 4, most = (int)gridDim.x + 1 - g;   // workgroups from g on
+  for (int first = blockIdx.y * R; first < valid; first += gridDim.y * R) {
+    const int row = first + (GROUPS > 1 ? 0 : threadIdx.x / T);
     float top = -INFINITY, sum = 0.0f;
     v4f o = {0, 0, 0, 0};
     // part 0: of the workgroup that the item starts in; part i: of workgroup g + i - 1, if that starts inside the item
+    if (row < valid) {
 #pragma unroll 4
-    for (int i = group; i <= most; i += GROUPS) {
-      if (i > 0 && (unsigned)m[(i - 1) * kMeta + kMetaU0] >= end) break;
-      const size_t at = (i == 0 ? 2 * (size_t)(g - 1) + 1 : 2 * (size_t)(g + i - 1)) * ROWS + row;
-      const float mi = p.part_ml[at * 2], li = p.part_ml[at * 2 + 1];
-      const v4f oi = *reinterpret_cast<const v4f*>(p.part_o + at * D + ch);
-      const float t = fmaxf(top, mi), f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t), f1 = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - t);
-      sum = sum * f0 + li * f1;
-      o = o * f0 + oi * f1;
-      top = t;
-    }
-    sums[group][threadIdx.x % T] = o;
-    if (ch == 0) ml[group][0] = top, ml[group][1] = sum;
-    __syncthreads();
-    if (group == 0) {
-      top = -INFINITY, sum = 0.0f, o = v4f{0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, ml[k][0]);
-#pragma unroll
-      for (int k = 0; k < GROUPS; ++k) {
-        const float f = ml[k][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][0] - top);
-        sum += ml[k][1] * f;
-        o += sums[k][threadIdx.x] * f;
+      for (int i = group; i <= most; i += GROUPS) {
+        if (i > 0 && (unsigned)m[(i - 1) * kMeta + kMetaU0] >= end) break;
+        const size_t at = (i == 0 ? 2 * (size_t)(g - 1) + 1 : 2 * (size_t)(g + i - 1)) * ROWS + row;
+        const float mi = p.part_ml[at * 2], li = p.part_ml[at * 2 + 1];
+        const v4f oi = *reinterpret_cast<const v4f*>(p.part_o + at * D + ch);
+        const float t = fmaxf(top, mi), f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t), f1 = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - t);
+        sum = sum * f0 + li * f1;
+        o = o * f0 + oi * f1;
+        top = t;
       }
+    }
+    if constexpr (GROUPS > 1) {
+      sums[group][threadIdx.x % T] = o;
+      if (ch == 0) ml[group][0] = top, ml[group][1] = sum;
+      __syncthreads();
+      if (group == 0) {
+        top = -INFINITY, sum = 0.0f, o = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, ml[k][0]);
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+          const float f = ml[k][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][0] - top);
+          sum += ml[k][1] * f;
+          o += sums[k][threadIdx.x] * f;
+        }
+        finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
+      }
+      __syncthreads();
+    } else if (row < valid) {
       finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
     }
-    __syncthreads();
   }
+}
+
+template <int D>
+void launch_combine_of(const AttnArgs& p, int rows, int64_t expected, int workgroups, hipStream_t s) {
+  const unsigned x = (unsigned)workgroups - 1, at_once = 1024 / D;
+  if (rows <= 64)
+    hipLaunchKernelGGL((attn_combine_kernel<D, 1024 / D>), dim3(x, (unsigned)expected), dim3(256), 0, s, p, rows);
+  else
+    hipLaunchKernelGGL((attn_combine_kernel<D, 1>), dim3(x, ((unsigned)expected + at_once - 1) / at_once), dim3(256), 0, s, p, rows);
 }
 
 }  // namespace
 
 hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s) {
   if (workgroups < 2) return hipSuccess;
-  const dim3 grid((unsigned)workgroups - 1, (unsigned)(rows_expected < 1 ? 1 : rows_expected < rows ? rows_expected : rows));
-  if (p.c.head_dim == 64) hipLaunchKernelGGL((attn_combine_kernel<64>), grid, dim3(256), 0, s, p, rows);
-  else if (p.c.head_dim == 128) hipLaunchKernelGGL((attn_combine_kernel<128>), grid, dim3(256), 0, s, p, rows);
-  else hipLaunchKernelGGL((attn_combine_kernel<256>), grid, dim3(256), 0, s, p, rows);
+  const int64_t expected = rows_expected < 1 ? 1 : rows_expected < rows ? rows_expected : rows;
+  if (p.c.head_dim == 64) launch_combine_of<64>(p, rows, expected, workgroups, s);
+  else if (p.c.head_dim == 128) launch_combine_of<128>(p, rows, expected, workgroups, s);
+  else launch_combine_of<256>(p, rows, expected, workgroups, s);
   return hipGetLastError();
 }
 
