@@ -17,7 +17,10 @@ namespace ave {
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
-constexpr float kNone = -3.0e38f;   // a score that is not there, below every one that is
+// A score that is not there: below every one that is, and exp2(kNone c - m c) is zero for every maximum m that is a score, and for m = 0,
+// because c is 1e-30 at least (a softmax scale of zero is taken as 1e-30, which leaves scores without effect just the same).
+constexpr float kNone = -3.0e38f;
+__device__ inline float softmax_scale(float scale) { return fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f); }   // base 2
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
@@ -290,6 +293,12 @@ __device__ inline v4i load8_bf16(const uint16_t* q) {
 __device__ inline float bf16_lo(int x) { return __builtin_bit_cast(float, (unsigned)x << 16); }
 __device__ inline float bf16_hi(int x) { return __builtin_bit_cast(float, (unsigned)x & 0xFFFF0000u); }
 
+// max3 as it is: fmaxf makes the compiler pass every operand through another maximum first (signalling NaN).  A NaN loses to a number.
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 // Two 16-bit a * k + c, k a scalar pair
 __device__ inline unsigned pk_mad_u16(unsigned a, unsigned k, unsigned c) {
   unsigned r;

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
   const Part part = take_part<ROWS, TILE>(p, blockIdx.x, gridDim.x);
   const unsigned ring = (unsigned)__builtin_amdgcn_readfirstlane(lds_address(smem)) + wave * NS * S::kStage;
   const unsigned char* ring_ptr = smem + wave * NS * S::kStage;
-  const float c = fabsf(p.a.scale) * kLog2e;
+  const float c = softmax_scale(p.a.scale);
   const Request<D, ONE_PAGE> request;
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
         }
         float top = kNone;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fmaxf(s[ct][j][0], s[ct][j][1]), fmaxf(s[ct][j][2], s[ct][j][3])));
+        for (int j = 0; j < 4; ++j) top = max3(max3(top, s[ct][j][0], s[ct][j][1]), s[ct][j][2], s[ct][j][3]);
         top = fmaxf(m[ct], cross_max<true>(top));
         if (__any(top > m[ct])) {
           const float fade = __builtin_amdgcn_exp2f((m[ct] - top) * c);
@@ -333,12 +333,11 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
           for (int k = 0; k < C; ++k) acc[ct][k] *= fade;
           m[ct] = top;
         }
-        const float shift = -m[ct] * c;
+        const float shift = m[ct] == kNone ? 0.0f : -m[ct] * c;
         float pr[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j / 4][j % 4], c, shift));
-          if (!all_seen) pr[j] = s[ct][j / 4][j % 4] == kNone ? 0.0f : pr[j];   // (where a row has seen nothing yet, or c is 0)
           l[ct] += pr[j];
         }
 #pragma unroll

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
   const Part part = take_part<kRows, kTile, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
-  const float c = fabsf(p.a.scale) * kLog2e;
+  const float c = softmax_scale(p.a.scale), slack = 8.0f / c;
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
@@ -228,27 +228,27 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int t = 0; t < 16; t += 2) top = fmaxf(top, fmaxf(s[j][t], s[j][t + 1]));
-        top = fmaxf(m, cross_max<false>(top));
-        if (__any(top > m)) {
+          for (int t = 0; t < 16; t += 2) top = max3(top, s[j][t], s[j][t + 1]);
+        top = cross_max<false>(top);
+        // What is subtracted from the scores follows the maximum only where that runs ahead by more than 2^8: probabilities up to 256
+        // have the same relative error, and most tiles go without touching the sums.
+        if (__any(top > m + slack)) {
+          top = fmaxf(m, top);
           const float fade = __builtin_amdgcn_exp2f((m - top) * c);
           l *= fade;
 #pragma unroll
           for (int k = 0; k < C; ++k) acc[k] *= fade;
           m = top;
         }
-        const float shift = -m * c;
+        const float shift = m == kNone ? 0.0f : -m * c;
         unsigned prob[2][8];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int t = 0; t < 16; t += 2) {
-            float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t + 1], c, shift));
-            if (!all_seen) {   // (where a row has seen nothing yet, or c is 0)
-              a = s[j][t] == kNone ? 0.0f : a;
-              d = s[j][t + 1] == kNone ? 0.0f : d;
-            }
-            l += a + d;
+            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t + 1], c, shift));
+            l += a;
+            l += d;
             prob[j][t / 2] = pack_bf16x2(a, d);
           }
         // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
