@@ -18,13 +18,14 @@ namespace {
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64, kWaves = 4, kRows = 32 * kWaves;
+constexpr float kNoMax = -1.0e30f;   // a maximum of nothing
+constexpr int kTile = 64, kWaves = 4, kRows = 32 * kWaves, kBuffers = 3;
 
 template <int D>
 struct Shape {
   static constexpr int kRow = D / 2, kBlocks = D / 32, kSteps = D / 64, C = D / 32;
   static constexpr int kKeys = kTile * kRow, kScales = kTile * kBlocks, kValues = kTile * D * 2;
-  static constexpr int kBuffer = kKeys + kScales + kValues;
+  static constexpr int kBuffer = kKeys + kScales, kLds = kBuffers * (kBuffer + kValues);   // keys' buffers, then values'
   static constexpr int kThreadBytes = kTile * kRow / (kWaves * 64);   // of values' codes: 8, 16 or 32, within one or two blocks of a token
   // LDS positions.  Keys: 16-byte pieces permuted so that the 16 lanes of a read touch different banks.  Values: a row's 64-byte segments, and
   // the pieces of a segment, permuted by the token for the transposing reads (four tokens, 64 bytes each) and the writes.
@@ -42,18 +43,30 @@ struct Values {
   int scale[kScaleBytes];
 };
 
+template <int N>
+struct Index {
+  static constexpr int value = N;
+};
+template <int N, int I = 0, typename F>
+__device__ inline void unrolled(F&& f) {   // f(Index<0>), ..., f(Index<N - 1>)
+  if constexpr (I < N) {
+    f(Index<I>{});
+    unrolled<N, I + 1>(f);
+  }
+}
+
 template <int D>
 __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int C = S::C;
-  __shared__ __align__(16) unsigned char smem[2 * S::kBuffer];
-  __shared__ uint64_t nan_in[2][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
+  __shared__ __align__(16) unsigned char smem[S::kLds];
+  __shared__ uint64_t nan_in[kBuffers][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
   const Part part = take_part<kRows, kTile, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
-  const float c = softmax_scale(p.a.scale), slack = 8.0f / c;
+  const float c = softmax_scale(p.a.scale);
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
@@ -76,14 +89,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
     const int tiles = it.s.len > 0 ? (int)(to - from) : 0;
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
-    // what this wave's rows see: [lo_row, hi_row) of a lane's row, [lo_max, hi_min) of all, [lo_min, hi_max) of any
+    // what this wave's rows see: [lo_row, hi_row) of a lane's row, [lo_max, hi_min) of all
     const int row0 = it.row0 + 32 * wave;
     const bool active = row0 < rows;
-    int lo_row, hi_row, lo_max, hi_min, lo_min, hi_max;
+    int lo_row, hi_row, lo_max, hi_min, dummy;
     {
       const int last = row0 + 32 < rows ? row0 + 31 : rows - 1, row = row0 + col < rows ? row0 + col : last;
-      visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
-      visible(p, it.s, p.token_of(last), lo_max, hi_max);
+      visible(p, it.s, p.token_of(active ? row0 : 0), dummy, hi_min);
+      visible(p, it.s, p.token_of(last), lo_max, dummy);
       visible(p, it.s, p.token_of(row), lo_row, hi_row);
     }
 
@@ -120,8 +133,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
 
     // ---- a tile's requests: keys and their scales to LDS, values to registers; a wave takes 16 tokens, which lie in one page
     Values<D> next;
-    const auto request_tile = [&](int t0, int buffer) {
-      const int t = t0 + 16 * wave, pg = page_at(p, table, t, it.s.len);
+    const auto request_keys = [&](int tile, int buffer) {
+      const int t = tile * kTile + 16 * wave, pg = page_at(p, table, t, it.s.len);
       const unsigned row = (unsigned)(it.head * p.c.page_size + (t & (p.c.page_size - 1)));
       const uint8_t* key = p.c.k + (int64_t)pg * p.c.k_page_stride + row * (unsigned)S::kRow;
       const unsigned at = lds + buffer * S::kBuffer;
@@ -134,6 +147,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
       }
       const uint8_t* key_scale = p.c.k_scale + (int64_t)pg * p.c.k_scale_page_stride + row * (unsigned)S::kBlocks;
       if (lane < 4 * S::kBlocks) to_lds4(key_scale + lane * 4, at + S::kKeys + wave * (16 * S::kBlocks));
+    };
+    const auto request_values = [&](int tile) {
+      const int t = tile * kTile + 16 * wave, pg = page_at(p, table, t, it.s.len);
+      const unsigned row = (unsigned)(it.head * p.c.page_size + (t & (p.c.page_size - 1)));
       const uint8_t* value = p.c.v + (int64_t)pg * p.c.v_page_stride + row * (unsigned)S::kRow + lane * S::kThreadBytes;
 #pragma unroll
       for (int k = 0; k < Values<D>::kWords; k += 2) {
@@ -144,9 +161,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
 #pragma unroll
       for (int k = 0; k < Values<D>::kScaleBytes; ++k) next.scale[k] = value_scale[D == 64 ? lane % 4 / 2 : D == 128 ? lane % 4 : 2 * (lane % 4) + k];
     };
-    const auto store_values = [&](int t0, int buffer) {
-      const int token = 16 * wave + lane / 4, quarter = lane % 4;
-      unsigned char* at = smem + buffer * S::kBuffer + S::kKeys + S::kScales + token * (2 * D);
+    const auto store_values = [&](int tile, int buffer) {
+      const int t0 = tile * kTile, token = 16 * wave + lane / 4, quarter = lane % 4;
+      unsigned char* at = smem + kBuffers * S::kBuffer + buffer * S::kValues + token * (2 * D);
       const bool there = t0 + token < it.s.len;   // what no key occupies is zero
 #pragma unroll
       for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
@@ -173,132 +190,184 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
     v16f acc[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) acc[i] = v16f{};
-    float m = kNone, l = 0.0f;
+    float m = kNoMax, l = 0.0f;   // base 2, whole numbers: a step of the maximum is a power of two
+
+    // 32 keys at a time (n) go through three steps: scores, probabilities, values.  Scores of n + 1 and values of n - 1 are independent of
+    // the probabilities of n, so the matrix cores work on the former under the exponentials of the latter.  Before the first step there
+    // are probabilities of zero, and behind the last one scores that nobody reads.
+    v16f score[2];
+    unsigned prob[2][8];
+    struct KeyFragments {
+      v4i code[S::kSteps];
+      unsigned scale[(S::kBlocks + 3) / 4];
+    };
+    const auto read_keys = [&](int buffer, int j, KeyFragments& f) {   // half j of the tile in a buffer
+      const unsigned char* keys = smem + buffer * S::kBuffer;
+      const unsigned char* ks = keys + S::kKeys;
+      const int t = 32 * j + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);   // row 8 i + 4 h' + t' is key 16 h' + 4 i + t'
+      if constexpr (D == 64) {
+        f.scale[0] = *reinterpret_cast<const uint16_t*>(ks + t * 2) >> (8 * h);
+      } else {
+#pragma unroll
+        for (int k = 0; k < S::kBlocks / 4; ++k) f.scale[k] = reinterpret_cast<const unsigned*>(ks)[t * (S::kBlocks / 4) + k] >> (8 * h);
+      }
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k) f.code[k] = *reinterpret_cast<const v4i*>(keys + t * S::kRow + ((2 * k + h) ^ S::key_swizzle(t)) * 16);
+    };
+    const auto score_mfma = [&](const KeyFragments& f, auto index, v16f& s) {   // 64 channels of keys with one part of the queries
+      constexpr int k = decltype(index)::value / 2;
+      const v4i x = f.code[k];
+      const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+      constexpr int kByte = k % 2 == 0 ? 0 : 2;
+      if constexpr (decltype(index)::value % 2 == 0) s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], k == 0 ? v16f{} : s, kFmtFp4, 0, kByte, (int)f.scale[k / 2], 0, s_lo);
+      else s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, kByte, (int)f.scale[k / 2], 0, s_hi);
+    };
+    const auto scores = [&](int buffer, int j, v16f& s) {
+      KeyFragments f;
+      read_keys(buffer, j, f);
+      unrolled<2 * S::kSteps>([&](auto index) { score_mfma(f, index, s); });
+    };
+    // Masks the scores of n and sees to the maximum.  What is subtracted from the scores follows the maximum only where that runs ahead by
+    // more than 2^8 (probabilities up to 256 have the same relative error, and most steps go without touching the sums); `waiting` are the
+    // probabilities of n - 1, whose values are not added yet.
+    const auto prepare = [&](int n, v16f& s, unsigned (&waiting)[8]) {
+      const int key0 = n * 32;
+      if (key0 < lo_max || key0 + 32 > hi_min) {
+        const int from = lo_row - key0 - 16 * h;
+        const unsigned many = (unsigned)(hi_row > lo_row ? hi_row - lo_row : 0);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
+      }
+      float top = max3(s[0], s[1], s[2]);
+#pragma unroll
+      for (int t = 3; t < 15; t += 2) top = max3(top, s[t], s[t + 1]);
+      top = cross_max<false>(max3(top, s[15], s[15]));
+      const float top2 = top > 0.5f * kNone ? top * c : kNoMax;
+      if (__any(top2 > m + 8.0f)) {
+        const float to_m = fmaxf(m, __builtin_ceilf(top2)), fade = __builtin_amdgcn_exp2f(m - to_m);
+        l *= fade;
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc[k] *= fade;
+        const unsigned down = (unsigned)fminf(to_m - m, 255.0f) * 0x00800080u;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) waiting[t] = pk_sub_sat(waiting[t], down);
+        m = to_m;
+      }
+    };
+    const auto probability_pair = [&](const v16f& s, float shift, int t, unsigned (&out)[8]) {
+      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t + 1], c, shift));
+      l += a;
+      l += d;
+      out[t] = pack_bf16x2(a, d);
+    };
+    const auto read_values = [&](int buffer, int j, int half, int k) {
+      typedef short v8s __attribute__((ext_vector_type(8)));
+      const int r = lane % 16 / 4;   // token within four
+      const int piece = 4 * k + 2 * ((lane / 16) & 1) + (lane % 4) / 2;
+      const unsigned char* at = smem + kBuffers * S::kBuffer + buffer * S::kValues + (32 * j + 16 * h + 8 * half + r) * (2 * D) +
+                                (piece ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)at);
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at + 4 * 2 * D));
+      return __builtin_bit_cast(v8bf, v8s{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    };
+    const auto of_half = [&](const unsigned (&w)[8], int half) {
+      return __builtin_bit_cast(v8bf, v4i{(int)w[4 * half], (int)w[4 * half + 1], (int)w[4 * half + 2], (int)w[4 * half + 3]});
+    };
+    const auto values = [&](int buffer, int j, const unsigned (&w)[8]) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_values(buffer, j, half, k), of_half(w, half), acc[k], 0, 0, 0);
+    };
+    // All three steps at once, for half j of the present tile: after every MFMA its share of the exponentials
+    const auto step = [&](int next_keys, int last_values, int j, const v16f& s, v16f& next_s, unsigned (&out)[8], const unsigned (&waiting)[8]) {
+      constexpr int kQk = 2 * S::kSteps, kMfma = kQk + 2 * C, kAhead = C < 4 ? C : 4;   // value fragments that wait in registers
+      const float shift = m == kNoMax ? 0.0f : -m;
+      KeyFragments f;
+      read_keys(next_keys, j ^ 1, f);
+      v8bf v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) v[k] = read_values(last_values, j ^ 1, 0, k);
+      unrolled<kMfma>([&](auto index) {
+        constexpr int n = decltype(index)::value, half = n >= kMfma / 2, in_half = n - half * (kMfma / 2);
+        if constexpr (in_half < kQk / 2) {
+          score_mfma(f, Index<in_half + half * (kQk / 2)>{}, next_s);
+        } else {
+          constexpr int k = in_half - kQk / 2, at = half * C + k;
+          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[at % kAhead], of_half(waiting, half), acc[k], 0, 0, 0);
+          if constexpr (at + kAhead < 2 * C) v[at % kAhead] = read_values(last_values, j ^ 1, (at + kAhead) / C, (at + kAhead) % C);
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          if (t * kMfma / 8 == n) probability_pair(s, shift, t, out);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    // Values with a NaN scale, zeros in LDS: NaN for the rows to which they count
+    const auto poison = [&](int buffer, int j, const unsigned (&w)[8]) {
+      uint64_t nan = 0;
+#pragma unroll
+      for (int k = 0; k < Values<D>::kScaleBytes; ++k) nan |= nan_in[buffer][k][2 * j] | nan_in[buffer][k][2 * j + 1];
+      if (__builtin_amdgcn_readfirstlane((int)(nan | nan >> 32))) {
+        uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
+#pragma unroll
+        for (int t = 0; t < 16; ++t) some |= (w[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
+#pragma unroll
+        for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
+          const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
+          const bool hit = (nan_in[buffer][D == 256 ? k % 2 : 0][2 * j + h] & some & (0x1111111111111111ull << quarter)) != 0;
+          acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
+        }
+      }
+    };
 
     if (tiles > 0) {
-      request_tile(tile0 * kTile, 0);
-      store_values(tile0 * kTile, 0);
+      request_keys(tile0, 0);
+      request_values(tile0);
+      if (tiles > 1) request_keys(tile0 + 1, 1);
+      store_values(tile0, 0);
       wait_loads<0>();
     }
     __syncthreads();
+    if (active && tiles > 0) scores(0, 0, score[0]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) prob[1][k] = 0;
+    int buffer = 0, last = 0, next_buffer = 1, free_buffer = 2;   // of this tile, the one before (the first has none: its own), the next two
     for (int i = 0; i < tiles; ++i) {
-      const int t0 = (tile0 + i) * kTile;
-      if (i + 1 < tiles) request_tile(t0 + kTile, (i + 1) & 1);
-      if (active && t0 < hi_max && t0 + kTile > lo_min) {
-        const unsigned char* keys = smem + (i & 1) * S::kBuffer;
-        const unsigned char *ks = keys + S::kKeys, *values = ks + S::kScales;
-        // ---- scores
-        v16f s[2];
+      const int tile = tile0 + i;
+      if (i + 1 < tiles) request_values(tile + 1);
+      if (i + 2 < tiles) request_keys(tile + 2, free_buffer);
+      if (active) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int t = 32 * j + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);   // row 8 i + 4 h' + t' is key 16 h' + 4 i + t'
-          unsigned sk[(S::kBlocks + 3) / 4];
-          if constexpr (D == 64) {
-            sk[0] = *reinterpret_cast<const uint16_t*>(ks + t * 2) >> (8 * h);
-          } else {
+          prepare(2 * tile + j, score[j], prob[j ^ 1]);
+          poison(j ? buffer : last, j ? 0 : 1, prob[j ^ 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          step(j ? next_buffer : buffer, j ? buffer : last, j, score[j], score[j ^ 1], prob[j], prob[j ^ 1]);
+          // here and not where they are used
 #pragma unroll
-            for (int k = 0; k < S::kBlocks / 4; ++k) sk[k] = reinterpret_cast<const unsigned*>(ks)[t * (S::kBlocks / 4) + k] >> (8 * h);
-          }
-          s[j] = v16f{};
-#pragma unroll
-          for (int step = 0; step < S::kSteps; ++step) {
-            const v4i x = *reinterpret_cast<const v4i*>(keys + t * S::kRow + ((2 * step + h) ^ S::key_swizzle(t)) * 16);
-            const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-            if (step % 2 == 0) {
-              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[step], s[j], kFmtFp4, 0, 0, (int)sk[step / 2], 0, s_lo);
-              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[step], s[j], kFmtFp4, 0, 0, (int)sk[step / 2], 0, s_hi);
-            } else {
-              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[step], s[j], kFmtFp4, 0, 2, (int)sk[step / 2], 0, s_lo);
-              s[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[step], s[j], kFmtFp4, 0, 2, (int)sk[step / 2], 0, s_hi);
-            }
-          }
+          for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(prob[j][k]));
+          asm volatile("" : "+v"(l));
+          __builtin_amdgcn_sched_barrier(0);
         }
-        // ---- probabilities
-        const bool all_seen = t0 >= lo_max && t0 + kTile <= hi_min;
-        if (!all_seen) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int t = 0; t < 16; ++t) {
-              const int key = t0 + 32 * j + 16 * h + t;
-              s[j][t] = key >= lo_row && key < hi_row ? s[j][t] : kNone;
-            }
-        }
-        float top = kNone;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int t = 0; t < 16; t += 2) top = max3(top, s[j][t], s[j][t + 1]);
-        top = cross_max<false>(top);
-        // What is subtracted from the scores follows the maximum only where that runs ahead by more than 2^8: probabilities up to 256
-        // have the same relative error, and most tiles go without touching the sums.
-        if (__any(top > m + slack)) {
-          top = fmaxf(m, top);
-          const float fade = __builtin_amdgcn_exp2f((m - top) * c);
-          l *= fade;
-#pragma unroll
-          for (int k = 0; k < C; ++k) acc[k] *= fade;
-          m = top;
-        }
-        const float shift = m == kNone ? 0.0f : -m * c;
-        unsigned prob[2][8];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int t = 0; t < 16; t += 2) {
-            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][t + 1], c, shift));
-            l += a;
-            l += d;
-            prob[j][t / 2] = pack_bf16x2(a, d);
-          }
-        // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
-        uint64_t nan = 0;
-#pragma unroll
-        for (int k = 0; k < Values<D>::kScaleBytes; ++k)
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) nan |= nan_in[i & 1][k][w];
-        if (__builtin_amdgcn_readfirstlane((int)(nan | nan >> 32))) {
-          uint64_t some[2] = {0, 0};   // four bits for each of this lane's keys, set where its probability is not zero
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int t = 0; t < 16; ++t) some[j] |= (prob[j][t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
-#pragma unroll
-          for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
-            const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
-            const uint64_t hits = (nan_in[i & 1][D == 256 ? k % 2 : 0][h] & some[0]) | (nan_in[i & 1][D == 256 ? k % 2 : 0][2 + h] & some[1]);
-            const bool hit = (hits & (0x1111111111111111ull << quarter)) != 0;
-            acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
-          }
-        }
-        // ---- values
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const v4i w = {(int)prob[j][4 * half], (int)prob[j][4 * half + 1], (int)prob[j][4 * half + 2], (int)prob[j][4 * half + 3]};
-            const v8bf pb = __builtin_bit_cast(v8bf, w);
-#pragma unroll
-            for (int k = 0; k < C; ++k) {
-              const int r = lane % 16 / 4;   // token within four
-              const int piece = 4 * k + 2 * ((lane / 16) & 1) + (lane % 4) / 2;
-              const unsigned char* at = values + (32 * j + 16 * h + 8 * half + r) * (2 * D) + (piece ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
-              const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)at);
-              const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at + 4 * 2 * D));
-              typedef short v8s __attribute__((ext_vector_type(8)));
-              const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-              acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), pb, acc[k], 0, 0, 0);
-            }
-          }
       }
-      if (i + 1 < tiles) store_values(t0 + kTile, (i + 1) & 1);
+      if (i + 1 < tiles) store_values(tile + 1, next_buffer);
       wait_loads<0>();
       __syncthreads();
+      last = buffer;
+      buffer = next_buffer;
+      next_buffer = free_buffer;
+      free_buffer = last;
     }
+    if (active && tiles > 0) {   // the last step's values
+      poison(last, 1, prob[1]);
+      values(last, 1, prob[1]);
+    }
+    __syncthreads();
 
     // ---- results: lane (column col) has channels 32 k + 8 i + 4 h .. + 3 of its row
     if (active) {
-      const float sum = cross_sum<false>(l), m2 = m == kNone ? -INFINITY : m * c;
+      const float sum = cross_sum<false>(l), m2 = m == kNoMax ? -INFINITY : m;
       const bool done = from == it.begin && to == end;
       const int row = row0 + col;
       if (row < rows) {
