@@ -8,6 +8,7 @@ AttnArgs args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
   AttnArgs p{};
   p.a = a, p.c = c;
   set_group(p, a.heads / c.kv_heads);
+  p.q_aligned = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
   p.page_shift = log2_of(c.page_size);
   return p;
 }

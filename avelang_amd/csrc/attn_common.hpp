@@ -29,6 +29,7 @@ struct AttnArgs {
   int group;          // query heads per key head
   int page_shift;
   int whole;          // 1: items are not split; no workspace, no second launch
+  int q_aligned;      // every row of q starts at a multiple of 16 bytes
   int few_long;       // few sequences of many blocks of rows each
   int min_units_log2; // of a workgroup, so that small calls are not cut into crumbs
   int* meta;          // workspace: [workgroups][kMeta]
@@ -257,11 +258,18 @@ __device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& 
 __device__ inline void to_lds16(const uint8_t* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
 }
+__device__ inline const uint8_t* uniform_pointer(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const uint8_t*>((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)v) | (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
 __device__ inline void to_lds16(const uint8_t* base, unsigned offset, unsigned lds) {   // base is wave-uniform
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ inline void to_lds4(const uint8_t* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
+}
+__device__ inline void to_lds4(const uint8_t* base, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
 }
 template <int N>
 __device__ inline void wait_loads() {
@@ -282,9 +290,9 @@ __device__ inline int page_at(const AttnArgs& p, ConstInts row, int token, int l
   return page < p.c.pages ? page : p.c.pages - 1;
 }
 
-// Eight bf16 from any address
-__device__ inline v4i load8_bf16(const uint16_t* q) {
-  if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) return *reinterpret_cast<const v4i*>(q);
+// Eight bf16, from any address where `aligned` is not set
+__device__ inline v4i load8_bf16(const uint16_t* q, bool aligned) {
+  if (aligned) return *reinterpret_cast<const v4i*>(q);
   v4i r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = (int)((unsigned)q[2 * i] | (unsigned)q[2 * i + 1] << 16);
@@ -294,10 +302,25 @@ __device__ inline float bf16_lo(int x) { return __builtin_bit_cast(float, (unsig
 __device__ inline float bf16_hi(int x) { return __builtin_bit_cast(float, (unsigned)x & 0xFFFF0000u); }
 
 // max3 as it is: fmaxf makes the compiler pass every operand through another maximum first (signalling NaN).  A NaN loses to a number.
-__device__ inline float max3(float a, float b, float c) {
+// The compiler does not see inside, so it does not wait for a matrix instruction whose result is an operand: `after` must come from an
+// ordinary instruction on that result, for which it has waited.
+__device__ inline float max3(float a, float b, float c, float after) {
   float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c), "v"(after));
   return r;
+}
+// Largest of the sixteen results of one matrix instruction, from `first` to `last`, and of `other`
+template <int first, int last>
+__device__ inline float largest_of(const v16f& s, float other) {
+  static_assert((last - first) % 2 == 1 && last > first + 2, "");
+  const float after = fmaxf(s[first], s[first + 1]);
+  float top = max3(after, s[first + 2], s[first + 3], after), two = other;
+#pragma unroll
+  for (int t = first + 4; t < last; t += 4) {
+    two = max3(two, s[t], s[t + 1], after);
+    if (t + 2 < last) top = max3(top, s[t + 2], s[t + 3], after);
+  }
+  return fmaxf(top, two);
 }
 // Two 16-bit a * k + c, k a scalar pair
 __device__ inline unsigned pk_mad_u16(unsigned a, unsigned k, unsigned c) {
@@ -385,15 +408,11 @@ __device__ inline size_t row_index(const AttnArgs& p, int first, int head, int r
 struct RowEnd {
   float factor, lse;
 };
-__device__ inline RowEnd row_end(const AttnArgs& p, int query_head, float m, float l) {
+__device__ inline float sink_of(const AttnArgs& p, int query_head) { return p.a.sinks ? p.a.sinks[query_head] * kLog2e : -INFINITY; }
+__device__ inline RowEnd row_end(float sink, float m, float l) {   // sink in base 2
   const bool none = m == -INFINITY && l == l;   // (only NaN scores: the sum is NaN)
-  float total = l, top = m, fade = 1.0f;
-  if (p.a.sinks) {
-    const float sink = p.a.sinks[query_head] * kLog2e;
-    top = fmaxf(m, sink);
-    fade = none ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    total = l * fade + (sink == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sink - top));
-  }
+  const float top = fmaxf(m, sink), fade = none ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+  const float total = (none ? 0.0f : l * fade) + (sink == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sink - top));
   return {none ? 0.0f : fade / total, (top + __builtin_amdgcn_logf(total)) * kLn2};
 }
 __device__ inline void store4_bf16(uint16_t* out, v4f o) {
@@ -402,7 +421,7 @@ __device__ inline void store4_bf16(uint16_t* out, v4f o) {
 }
 // Four channels of a finished row
 __device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int channel, v4f o, float m, float l) {
-  const RowEnd e = row_end(p, (int)(row % (unsigned)p.a.heads), m, l);
+  const RowEnd e = row_end(sink_of(p, (int)(row % (unsigned)p.a.heads)), m, l);
   store4_bf16(p.a.out + row * D + channel, o * e.factor);
   if (p.a.lse && channel == 0) p.a.lse[row] = e.lse;
 }

@@ -120,7 +120,7 @@ struct Queries {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         x[ct][i] = v4i{0, 0, 0, 0};
-        if (real) x[ct][i] = load8_bf16(q + (i / 2) * 64 + g * 16 + (i % 2) * 8);
+        if (real) x[ct][i] = load8_bf16(q + (i / 2) * 64 + g * 16 + (i % 2) * 8, p.q_aligned);
       }
     }
   }
@@ -324,7 +324,10 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
         }
         float top = kNone;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = max3(max3(top, s[ct][j][0], s[ct][j][1]), s[ct][j][2], s[ct][j][3]);
+        for (int j = 0; j < 4; ++j) {
+          const float two = fmaxf(s[ct][j][0], s[ct][j][1]);
+          top = fmaxf(top, max3(two, s[ct][j][2], s[ct][j][3], two));
+        }
         top = fmaxf(m[ct], cross_max<true>(top));
         if (__any(top > m[ct])) {
           const float fade = __builtin_amdgcn_exp2f((m[ct] - top) * c);

@@ -55,7 +55,8 @@ __device__ inline void unrolled(F&& f) {   // f(Index<0>), ..., f(Index<N - 1>)
   }
 }
 
-template <int D>
+// SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset.
+template <int D, bool SMALL>
 __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int C = S::C;
@@ -75,8 +76,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
     m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
   }
   bool first_item = true;
+  Item it{};
   for (unsigned u = part.u0; u < part.u1;) {
-    const Item it = item_of<kRows, kTile, true>(p, u, b, b_begin, seq, per_head);
+    if (!first_item && it.row0 + kRows < it.s.n * p.group) {   // the next block of the same key head
+      it.row0 += kRows;
+      it.begin = u;
+      it.units = (unsigned)block_units<kRows, kTile>(p, it.s, it.row0, it.tile0);
+    } else {
+      it = item_of<kRows, kTile, true>(p, u, b, b_begin, seq, per_head);
+    }
     const unsigned end = it.begin + it.units, from = u, to = end < part.u1 ? end : part.u1;
     u = to;
     if (first_item && tid == 0) {
@@ -98,15 +106,94 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
       visible(p, it.s, p.token_of(active ? row0 : 0), dummy, hi_min);
       visible(p, it.s, p.token_of(last), lo_max, dummy);
       visible(p, it.s, p.token_of(row), lo_row, hi_row);
+      lo_max = __builtin_amdgcn_readfirstlane(lo_max), hi_min = __builtin_amdgcn_readfirstlane(hi_min);
     }
 
+    // ---- a tile's requests: keys and their scales to LDS, values to registers; a wave takes 16 tokens, which lie in one page
+    Values<D> next;
+    const auto page_of = [&](int tile) { return page_at(p, table, tile * kTile + 16 * wave, it.s.len); };
+    // A tensor's base and offset for this wave's tokens of a tile, `bytes` a token and head
+    const auto place = [&](const uint8_t* tensor, int64_t stride, int pg, int tile, unsigned bytes, const uint8_t*& base) -> unsigned {
+      const int t = tile * kTile + 16 * wave;
+      const unsigned in_page = (unsigned)(it.head * p.c.page_size + (t & (p.c.page_size - 1))) * bytes;
+      if constexpr (SMALL) {
+        base = tensor;
+        return (unsigned)pg * (unsigned)stride + in_page;
+      } else {
+        base = uniform_pointer(tensor + (int64_t)pg * stride + in_page);
+        return 0;
+      }
+    };
+    unsigned key_offset[(16 * S::kRow + 1023) / 1024];   // of this lane within its wave's 16 tokens
+#pragma unroll
+    for (int i = 0; i < (16 * S::kRow + 1023) / 1024; ++i) {
+      constexpr int kPieces = S::kRow / 16;
+      const int token = i * (64 / kPieces) + lane / kPieces;
+      key_offset[i] = token * S::kRow + ((lane % kPieces) ^ S::key_swizzle(16 * wave + token)) * 16;
+    }
+    const auto request_keys = [&](int tile, int pg, int buffer) {
+      const unsigned at = lds + buffer * S::kBuffer;
+      const uint8_t* base;
+      unsigned off = place(p.c.k, p.c.k_page_stride, pg, tile, S::kRow, base);
+#pragma unroll
+      for (int i = 0; i < (16 * S::kRow + 1023) / 1024; ++i)
+        if (D > 64 || lane < 32) to_lds16(base, off + key_offset[i], at + wave * (16 * S::kRow) + i * 1024);
+      off = place(p.c.k_scale, p.c.k_scale_page_stride, pg, tile, S::kBlocks, base);
+      if (lane < 4 * S::kBlocks) to_lds4(base, off + lane * 4, at + S::kKeys + wave * (16 * S::kBlocks));
+    };
+    const auto request_values = [&](int tile, int pg) {
+      const uint8_t* base;
+      unsigned off = place(p.c.v, p.c.v_page_stride, pg, tile, S::kRow, base) + lane * S::kThreadBytes;
+#pragma unroll
+      for (int k = 0; k < Values<D>::kWords; k += 2) {
+        const v2i x = *reinterpret_cast<const v2i*>(base + (off + 4 * k));
+        next.code[k] = (unsigned)x[0], next.code[k + 1] = (unsigned)x[1];
+      }
+      off = place(p.c.v_scale, p.c.v_scale_page_stride, pg, tile, S::kBlocks, base) + lane / 4 * S::kBlocks;
+#pragma unroll
+      for (int k = 0; k < Values<D>::kScaleBytes; ++k) next.scale[k] = base[off + (D == 64 ? lane % 4 / 2 : D == 128 ? lane % 4 : 2 * (lane % 4) + k)];
+    };
+    const auto prepare_values = [&](int tile, int buffer) {   // what no key occupies, and what has a NaN scale, is zero
+      const bool there = tile * kTile + 16 * wave + lane / 4 < it.s.len;
+#pragma unroll
+      for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
+        constexpr int kOfScale = Values<D>::kWords / Values<D>::kScaleBytes;
+        const bool bad = there && next.scale[k] >= 253, none = bad || !there;
+#pragma unroll
+        for (int w = 0; w < kOfScale; ++w) next.code[k * kOfScale + w] = none ? 0 : next.code[k * kOfScale + w];
+        next.scale[k] = none ? 127 : next.scale[k];
+        const uint64_t lanes = __ballot(bad);
+        if (lane == 0) nan_in[buffer][k][wave] = lanes;
+      }
+    };
+    const auto store_value_word = [&](int buffer, int w) {   // eight channels, one 16-byte piece
+      const int token = 16 * wave + lane / 4;
+      unsigned char* at = smem + kBuffers * S::kBuffer + buffer * S::kValues + token * (2 * D);
+      const float f = __builtin_bit_cast(float, (unsigned)next.scale[D == 256 ? w / 4 : 0] << 23);
+      const unsigned x = next.code[w];
+      const v2bf a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 1);
+      const v2bf a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 3);
+      const v8bf v = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+      const int piece = lane % 4 * Values<D>::kWords + w;
+      *reinterpret_cast<v8bf*>(at + (piece ^ S::value_swizzle(token)) * 16) = v;
+    };
+
+    // ---- the first requests, then the queries, whose way is as long
+    int page[3] = {page_of(tile0), page_of(tile0 + 1), page_of(tile0 + 2)};   // of the present tile, the next, the one after
+    if (tiles > 0) {
+      request_keys(tile0, page[0], 0);
+      request_values(tile0, page[0]);
+      if (tiles > 1) request_keys(tile0 + 1, page[1], 1);
+    }
     // ---- queries: lane (column col): bytes 0-15 of a step are k = 16 h .., bytes 16-31 k = 32 + 16 h ..
     v8i q_hi[S::kSteps], q_lo[S::kSteps];
     int s_hi, s_lo;
+    float sink;
     {
       const bool real = row0 + col < rows;
-      const int t = real ? p.token_of(row0 + col) : 0;
-      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)(it.head * p.group + (real ? row0 + col - t * p.group : 0)) * p.a.q_head_stride;
+      const int t = real ? p.token_of(row0 + col) : 0, query_head = it.head * p.group + (real ? row0 + col - t * p.group : 0);
+      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)query_head * p.a.q_head_stride;
+      sink = sink_of(p, query_head);
       v4i x[S::kSteps][4];
       us2 m = {0, 0};
 #pragma unroll
@@ -114,7 +201,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           x[i][k] = v4i{0, 0, 0, 0};
-          if (real) x[i][k] = load8_bf16(q + 64 * i + 32 * (k / 2) + 16 * h + 8 * (k % 2));
+          if (real) x[i][k] = load8_bf16(q + 64 * i + 32 * (k / 2) + 16 * h + 8 * (k % 2), p.q_aligned);
           m = amax_pairs(x[i][k], m);
         }
       const QueryScale s = query_scale(lane_xor_max_bits(larger_half(m), 32));
@@ -130,62 +217,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
         }
       s_hi = s.hi_byte, s_lo = s.lo_byte;
     }
-
-    // ---- a tile's requests: keys and their scales to LDS, values to registers; a wave takes 16 tokens, which lie in one page
-    Values<D> next;
-    const auto request_keys = [&](int tile, int buffer) {
-      const int t = tile * kTile + 16 * wave, pg = page_at(p, table, t, it.s.len);
-      const unsigned row = (unsigned)(it.head * p.c.page_size + (t & (p.c.page_size - 1)));
-      const uint8_t* key = p.c.k + (int64_t)pg * p.c.k_page_stride + row * (unsigned)S::kRow;
-      const unsigned at = lds + buffer * S::kBuffer;
-      constexpr int kPieces = S::kRow / 16;
-#pragma unroll
-      for (int i = 0; i < (16 * S::kRow + 1023) / 1024; ++i) {
-        const int token = i * (64 / kPieces) + lane / kPieces;
-        const unsigned off = token * S::kRow + ((lane % kPieces) ^ S::key_swizzle(16 * wave + token)) * 16;
-        if (D > 64 || lane < 32) to_lds16(key, off, at + wave * (16 * S::kRow) + i * 1024);
-      }
-      const uint8_t* key_scale = p.c.k_scale + (int64_t)pg * p.c.k_scale_page_stride + row * (unsigned)S::kBlocks;
-      if (lane < 4 * S::kBlocks) to_lds4(key_scale + lane * 4, at + S::kKeys + wave * (16 * S::kBlocks));
-    };
-    const auto request_values = [&](int tile) {
-      const int t = tile * kTile + 16 * wave, pg = page_at(p, table, t, it.s.len);
-      const unsigned row = (unsigned)(it.head * p.c.page_size + (t & (p.c.page_size - 1)));
-      const uint8_t* value = p.c.v + (int64_t)pg * p.c.v_page_stride + row * (unsigned)S::kRow + lane * S::kThreadBytes;
-#pragma unroll
-      for (int k = 0; k < Values<D>::kWords; k += 2) {
-        const v2i x = *reinterpret_cast<const v2i*>(value + 4 * k);
-        next.code[k] = (unsigned)x[0], next.code[k + 1] = (unsigned)x[1];
-      }
-      const uint8_t* value_scale = p.c.v_scale + (int64_t)pg * p.c.v_scale_page_stride + row * (unsigned)S::kBlocks + lane / 4 * S::kBlocks;
-#pragma unroll
-      for (int k = 0; k < Values<D>::kScaleBytes; ++k) next.scale[k] = value_scale[D == 64 ? lane % 4 / 2 : D == 128 ? lane % 4 : 2 * (lane % 4) + k];
-    };
-    const auto store_values = [&](int tile, int buffer) {
-      const int t0 = tile * kTile, token = 16 * wave + lane / 4, quarter = lane % 4;
-      unsigned char* at = smem + kBuffers * S::kBuffer + buffer * S::kValues + token * (2 * D);
-      const bool there = t0 + token < it.s.len;   // what no key occupies is zero
-#pragma unroll
-      for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
-        constexpr int kOfScale = Values<D>::kWords / Values<D>::kScaleBytes;
-        const bool bad = there && next.scale[k] >= 253, none = bad || !there;
-#pragma unroll
-        for (int w = 0; w < kOfScale; ++w) next.code[k * kOfScale + w] = none ? 0 : next.code[k * kOfScale + w];
-        next.scale[k] = none ? 127 : next.scale[k];
-        const uint64_t lanes = __ballot(bad);
-        if (lane == 0) nan_in[buffer][k][wave] = lanes;
-      }
-#pragma unroll
-      for (int w = 0; w < Values<D>::kWords; ++w) {   // eight channels, one 16-byte piece
-        const float f = __builtin_bit_cast(float, (unsigned)next.scale[D == 256 ? w / 4 : 0] << 23);
-        const unsigned x = next.code[w];
-        const v2bf a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 1);
-        const v2bf a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 3);
-        const v8bf v = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
-        const int piece = quarter * Values<D>::kWords + w;
-        *reinterpret_cast<v8bf*>(at + (piece ^ S::value_swizzle(token)) * 16) = v;
-      }
-    };
 
     v16f acc[C];
 #pragma unroll
@@ -230,18 +261,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
     // Masks the scores of n and sees to the maximum.  What is subtracted from the scores follows the maximum only where that runs ahead by
     // more than 2^8 (probabilities up to 256 have the same relative error, and most steps go without touching the sums); `waiting` are the
     // probabilities of n - 1, whose values are not added yet.
-    const auto prepare = [&](int n, v16f& s, unsigned (&waiting)[8]) {
+    const auto prepare = [&](int n, v16f& s, float top, unsigned (&waiting)[8]) {   // top: of all scores
       const int key0 = n * 32;
       if (key0 < lo_max || key0 + 32 > hi_min) {
         const int from = lo_row - key0 - 16 * h;
         const unsigned many = (unsigned)(hi_row > lo_row ? hi_row - lo_row : 0);
 #pragma unroll
         for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
+        top = cross_max<false>(largest_of<0, 15>(s, kNone));
       }
-      float top = max3(s[0], s[1], s[2]);
-#pragma unroll
-      for (int t = 3; t < 15; t += 2) top = max3(top, s[t], s[t + 1]);
-      top = cross_max<false>(max3(top, s[15], s[15]));
       const float top2 = top > 0.5f * kNone ? top * c : kNoMax;
       if (__any(top2 > m + 8.0f)) {
         const float to_m = fmaxf(m, __builtin_ceilf(top2)), fade = __builtin_amdgcn_exp2f(m - to_m);
@@ -279,8 +307,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
 #pragma unroll
         for (int k = 0; k < C; ++k) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_values(buffer, j, half, k), of_half(w, half), acc[k], 0, 0, 0);
     };
-    // All three steps at once, for half j of the present tile: after every MFMA its share of the exponentials
-    const auto step = [&](int next_keys, int last_values, int j, const v16f& s, v16f& next_s, unsigned (&out)[8], const unsigned (&waiting)[8]) {
+    // All three steps at once, for half j of the present tile: after every MFMA its share of the exponentials, in the second half also of the
+    // next tile's values on their way to LDS (behind the last tile: whatever the registers hold, to where nobody reads)
+    const auto step = [&](int next_keys, int last_values, auto which, const v16f& s, v16f& next_s, unsigned (&out)[8], const unsigned (&waiting)[8], float& next_top, int store_to) {
+      constexpr int j = decltype(which)::value;
       constexpr int kQk = 2 * S::kSteps, kMfma = kQk + 2 * C, kAhead = C < 4 ? C : 4;   // value fragments that wait in registers
       const float shift = m == kNoMax ? 0.0f : -m;
       KeyFragments f;
@@ -288,79 +318,104 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
       v8bf v[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) v[k] = read_values(last_values, j ^ 1, 0, k);
-      unrolled<kMfma>([&](auto index) {
-        constexpr int n = decltype(index)::value, half = n >= kMfma / 2, in_half = n - half * (kMfma / 2);
-        if constexpr (in_half < kQk / 2) {
-          score_mfma(f, Index<in_half + half * (kQk / 2)>{}, next_s);
+      float top[2];
+      unrolled<kMfma>([&](auto index) {   // two of the scores', two of the values', and so on; the rest of the values'
+        constexpr int n = decltype(index)::value;
+        if constexpr (n < 2 * kQk && n % 4 < 2) {
+          score_mfma(f, Index<n / 4 * 2 + n % 4>{}, next_s);
         } else {
-          constexpr int k = in_half - kQk / 2, at = half * C + k;
-          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[at % kAhead], of_half(waiting, half), acc[k], 0, 0, 0);
+          constexpr int at = n < 2 * kQk ? n / 4 * 2 + n % 4 - 2 : n - kQk, k = at % C;
+          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[at % kAhead], of_half(waiting, at / C), acc[k], 0, 0, 0);
           if constexpr (at + kAhead < 2 * C) v[at % kAhead] = read_values(last_values, j ^ 1, (at + kAhead) / C, (at + kAhead) % C);
         }
+        if constexpr (n == kMfma - 3) top[0] = largest_of<0, 7>(next_s, kNone);
+        if constexpr (n == kMfma - 2) top[1] = largest_of<8, 15>(next_s, top[0]);
+        if constexpr (n == kMfma - 1) next_top = cross_max<false>(top[1]);
 #pragma unroll
         for (int t = 0; t < 8; ++t)
           if (t * kMfma / 8 == n) probability_pair(s, shift, t, out);
+        if constexpr (j == 1) {
+#pragma unroll
+          for (int w = 0; w < Values<D>::kWords; ++w)
+            if ((2 * w + 1) * kMfma / (2 * Values<D>::kWords) + 1 == n) store_value_word(store_to, w);
+        }
         __builtin_amdgcn_sched_barrier(0);
       });
     };
     // Values with a NaN scale, zeros in LDS: NaN for the rows to which they count
     const auto poison = [&](int buffer, int j, const unsigned (&w)[8]) {
-      uint64_t nan = 0;
+      uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
 #pragma unroll
-      for (int k = 0; k < Values<D>::kScaleBytes; ++k) nan |= nan_in[buffer][k][2 * j] | nan_in[buffer][k][2 * j + 1];
-      if (__builtin_amdgcn_readfirstlane((int)(nan | nan >> 32))) {
-        uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
+      for (int t = 0; t < 16; ++t) some |= (w[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) some |= (w[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
-#pragma unroll
-        for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
-          const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
-          const bool hit = (nan_in[buffer][D == 256 ? k % 2 : 0][2 * j + h] & some & (0x1111111111111111ull << quarter)) != 0;
-          acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
-        }
+      for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
+        const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
+        const bool hit = (nan_in[buffer][D == 256 ? k % 2 : 0][2 * j + h] & some & (0x1111111111111111ull << quarter)) != 0;
+        acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
       }
     };
 
     if (tiles > 0) {
-      request_keys(tile0, 0);
-      request_values(tile0);
-      if (tiles > 1) request_keys(tile0 + 1, 1);
-      store_values(tile0, 0);
+      prepare_values(tile0, 0);
+#pragma unroll
+      for (int w = 0; w < Values<D>::kWords; ++w) store_value_word(0, w);
       wait_loads<0>();
     }
     __syncthreads();
-    if (active && tiles > 0) scores(0, 0, score[0]);
+    float top = kNone;   // of the scores that come next
+    if (active && tiles > 0) {
+      scores(0, 0, score[0]);
+      top = cross_max<false>(largest_of<0, 15>(score[0], kNone));
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) prob[1][k] = 0;
     int buffer = 0, last = 0, next_buffer = 1, free_buffer = 2;   // of this tile, the one before (the first has none: its own), the next two
+    bool nan_last = false;
     for (int i = 0; i < tiles; ++i) {
       const int tile = tile0 + i;
-      if (i + 1 < tiles) request_values(tile + 1);
-      if (i + 2 < tiles) request_keys(tile + 2, free_buffer);
-      if (active) {
+      if (i + 1 < tiles) request_values(tile + 1, page[1]);
+      if (i + 2 < tiles) request_keys(tile + 2, page[2], free_buffer);
+      page[1] = page[2];
+      page[2] = page_of(tile + 3);
+      uint64_t nan = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          prepare(2 * tile + j, score[j], prob[j ^ 1]);
-          poison(j ? buffer : last, j ? 0 : 1, prob[j ^ 1]);
+      for (int k = 0; k < Values<D>::kScaleBytes; ++k)
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) nan |= nan_in[buffer][k][w];
+      bool nan_now = false;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (active) {
+          prepare(2 * tile + j, score[j], top, prob[j ^ 1]);
+          if (j) nan_now = __builtin_amdgcn_readfirstlane((int)(nan | nan >> 32)) != 0;
+          if (j ? nan_now : nan_last) poison(j ? buffer : last, j ? 0 : 1, prob[j ^ 1]);
+        }
+        if (j && i + 1 < tiles) prepare_values(tile + 1, next_buffer);
+        if (active) {
           __builtin_amdgcn_sched_barrier(0);
-          step(j ? next_buffer : buffer, j ? buffer : last, j, score[j], score[j ^ 1], prob[j], prob[j ^ 1]);
+          if (j) step(next_buffer, buffer, Index<1>{}, score[1], score[0], prob[1], prob[0], top, next_buffer);
+          else step(buffer, last, Index<0>{}, score[0], score[1], prob[0], prob[1], top, 0);
           // here and not where they are used
 #pragma unroll
           for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(prob[j][k]));
-          asm volatile("" : "+v"(l));
+          asm volatile("" : "+v"(l), "+v"(top));
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (i + 1 < tiles) store_values(tile + 1, next_buffer);
+      if (!active) {
+#pragma unroll
+        for (int w = 0; w < Values<D>::kWords; ++w) store_value_word(next_buffer, w);
+      }
       wait_loads<0>();
       __syncthreads();
+      nan_last = nan_now;
       last = buffer;
       buffer = next_buffer;
       next_buffer = free_buffer;
       free_buffer = last;
     }
     if (active && tiles > 0) {   // the last step's values
-      poison(last, 1, prob[1]);
+      if (nan_last) poison(last, 1, prob[1]);
       values(last, 1, prob[1]);
     }
     __syncthreads();
@@ -373,7 +428,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
       if (row < rows) {
         const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + 32 * wave + col;
         const size_t place = row_index(p, it.s.first, it.head, row);
-        const RowEnd e = row_end(p, it.head * p.group + (row - p.token_of(row) * p.group), m2, sum);
+        const RowEnd e = row_end(sink, m2, sum);
         if (done && p.a.lse && h == 0) p.a.lse[place] = e.lse;
 #pragma unroll
         for (int k = 0; k < C; ++k)
@@ -403,9 +458,20 @@ hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   p.few_long = p.a.batch <= 16;
   place_workspace(p, kRows, workgroups, ws);
   const dim3 grid((unsigned)workgroups), block(kWaves * 64);
-  if (p.c.head_dim == 64) hipLaunchKernelGGL((attn_prompt_kernel<64>), grid, block, 0, s, p);
-  else if (p.c.head_dim == 128) hipLaunchKernelGGL((attn_prompt_kernel<128>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((attn_prompt_kernel<256>), grid, block, 0, s, p);
+  const int64_t last = p.c.pages - 1, page = (int64_t)p.c.kv_heads * p.c.page_size * p.c.head_dim / 2;   // bytes of codes; of scales a 16th
+  const auto small = [&](int64_t stride, int64_t bytes) { return last * stride + bytes <= (int64_t)1 << 32; };
+  const bool all = small(p.c.k_page_stride, page) && small(p.c.v_page_stride, page) && small(p.c.k_scale_page_stride, page / 16) && small(p.c.v_scale_page_stride, page / 16);
+#define AVE_PROMPT(D)                                                                                  \
+  if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true>), grid, block, 0, s, p);                    \
+  else hipLaunchKernelGGL((attn_prompt_kernel<D, false>), grid, block, 0, s, p)
+  if (p.c.head_dim == 64) {
+    AVE_PROMPT(64);
+  } else if (p.c.head_dim == 128) {
+    AVE_PROMPT(128);
+  } else {
+    AVE_PROMPT(256);
+  }
+#undef AVE_PROMPT
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   return launch_attn_combine(p, kRows, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
 }
