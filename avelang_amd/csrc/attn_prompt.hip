@@ -19,7 +19,7 @@ namespace {
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr float kNoMax = -1.0e30f;   // a maximum of nothing
-constexpr int kTile = 64, kWaves = 4, kRows = 32 * kWaves, kBuffers = 3;
+constexpr int kTile = 64, kWaves = 4, kRows = 32 * kWaves, kBuffers = 2;
 
 template <int D>
 struct Shape {
@@ -47,17 +47,25 @@ template <int N>
 struct Index {
   static constexpr int value = N;
 };
-template <int N, int I = 0, typename F>
-__device__ inline void unrolled(F&& f) {   // f(Index<0>), ..., f(Index<N - 1>)
-  if constexpr (I < N) {
-    f(Index<I>{});
-    unrolled<N, I + 1>(f);
-  }
+
+typedef __attribute__((address_space(3))) v4i LdsInt4;
+typedef __attribute__((address_space(3))) unsigned LdsInt;
+typedef __attribute__((address_space(3))) uint16_t LdsShort;
+typedef __attribute__((address_space(3))) v4s LdsShort4;
+template <typename T>
+__device__ inline T* lds_at(unsigned address) {
+  return (T*)(uintptr_t)address;
+}
+
+// Waves of a SIMD, each of another workgroup: by registers
+template <int D>
+constexpr int waves_per_simd() {
+  return D == 64 ? 4 : D == 128 ? 3 : 1;
 }
 
 // SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset.
 template <int D, bool SMALL>
-__global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p) {
+__global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int C = S::C;
   __shared__ __align__(16) unsigned char smem[S::kLds];
@@ -68,6 +76,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
   const Part part = take_part<kRows, kTile, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
   const float c = softmax_scale(p.a.scale);
+  // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
+  // key's scales, and by 32 channels the values
+  unsigned key_at[S::kSteps], value_at[C], scale_at;
+  {
+    const int t = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), r = lane % 16 / 4;   // r: token within four
+#pragma unroll
+    for (int k = 0; k < S::kSteps; ++k) {
+      key_at[k] = lds + t * S::kRow + ((2 * k + h) ^ S::key_swizzle(t)) * 16;
+      asm volatile("" : "+v"(key_at[k]));
+    }
+    scale_at = lds + S::kKeys + t * S::kBlocks;
+    asm volatile("" : "+v"(scale_at));
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int piece = 4 * k + 2 * ((lane / 16) & 1) + (lane % 4) / 2;
+      value_at[k] = lds + kBuffers * S::kBuffer + (16 * h + r) * (2 * D) + (piece ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
+      asm volatile("" : "+v"(value_at[k]));
+    }
+  }
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
@@ -100,11 +127,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
     // what this wave's rows see: [lo_row, hi_row) of a lane's row, [lo_max, hi_min) of all
     const int row0 = it.row0 + 32 * wave;
     const bool active = row0 < rows;
-    int lo_row, hi_row, lo_max, hi_min, dummy;
+    int lo_row, hi_row, lo_max, hi_min, lo_min, hi_max;
     {
       const int last = row0 + 32 < rows ? row0 + 31 : rows - 1, row = row0 + col < rows ? row0 + col : last;
-      visible(p, it.s, p.token_of(active ? row0 : 0), dummy, hi_min);
-      visible(p, it.s, p.token_of(last), lo_max, dummy);
+      visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
+      visible(p, it.s, p.token_of(last), lo_max, hi_max);
       visible(p, it.s, p.token_of(row), lo_row, hi_row);
       lo_max = __builtin_amdgcn_readfirstlane(lo_max), hi_min = __builtin_amdgcn_readfirstlane(hi_min);
     }
@@ -179,11 +206,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
     };
 
     // ---- the first requests, then the queries, whose way is as long
-    int page[3] = {page_of(tile0), page_of(tile0 + 1), page_of(tile0 + 2)};   // of the present tile, the next, the one after
+    int page[2] = {page_of(tile0), page_of(tile0 + 1)};   // of the first tile, the next
     if (tiles > 0) {
       request_keys(tile0, page[0], 0);
       request_values(tile0, page[0]);
-      if (tiles > 1) request_keys(tile0 + 1, page[1], 1);
     }
     // ---- queries: lane (column col): bytes 0-15 of a step are k = 16 h .., bytes 16-31 k = 32 + 16 h ..
     v8i q_hi[S::kSteps], q_lo[S::kSteps];
@@ -220,205 +246,125 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
 
     v16f acc[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) acc[i] = v16f{};
-    float m = kNoMax, l = 0.0f;   // base 2, whole numbers: a step of the maximum is a power of two
+    for (int k = 0; k < C; ++k) acc[k] = v16f{};
+    float m = kNoMax, l = 0.0f;   // m: base 2
 
-    // 32 keys at a time (n) go through three steps: scores, probabilities, values.  Scores of n + 1 and values of n - 1 are independent of
-    // the probabilities of n, so the matrix cores work on the former under the exponentials of the latter.  Before the first step there
-    // are probabilities of zero, and behind the last one scores that nobody reads.
-    v16f score[2];
-    unsigned prob[2][8];
-    struct KeyFragments {
-      v4i code[S::kSteps];
-      unsigned scale[(S::kBlocks + 3) / 4];
-    };
-    const auto read_keys = [&](int buffer, int j, KeyFragments& f) {   // half j of the tile in a buffer
-      const unsigned char* keys = smem + buffer * S::kBuffer;
-      const unsigned char* ks = keys + S::kKeys;
-      const int t = 32 * j + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);   // row 8 i + 4 h' + t' is key 16 h' + 4 i + t'
-      if constexpr (D == 64) {
-        f.scale[0] = *reinterpret_cast<const uint16_t*>(ks + t * 2) >> (8 * h);
-      } else {
+    // 32 keys, half j of the tile in a buffer
+    const auto multiply = [&](int tile, int buffer, auto which) {
+      constexpr int j = decltype(which)::value;
+      const int key0 = tile * kTile + 32 * j;
+      // ---- scores
+      v16f s = {};
+      {
+        unsigned scale[(S::kBlocks + 3) / 4];
+        const unsigned ks = scale_at + buffer * S::kBuffer + 32 * j * S::kBlocks;
+        if constexpr (D == 64) {
+          scale[0] = *lds_at<const LdsShort>(ks) >> (8 * h);
+        } else {
 #pragma unroll
-        for (int k = 0; k < S::kBlocks / 4; ++k) f.scale[k] = reinterpret_cast<const unsigned*>(ks)[t * (S::kBlocks / 4) + k] >> (8 * h);
+          for (int k = 0; k < S::kBlocks / 4; ++k) scale[k] = lds_at<const LdsInt>(ks)[k] >> (8 * h);
+        }
+#pragma unroll
+        for (int k = 0; k < S::kSteps; ++k) {
+          const v4i x = *lds_at<const LdsInt4>(key_at[k] + buffer * S::kBuffer + 32 * j * S::kRow);
+          const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+          if (k % 2 == 0) {
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 0, s_lo);
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 0, s_hi);
+          } else {
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 0, s_lo);
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 0, s_hi);
+          }
+        }
       }
-#pragma unroll
-      for (int k = 0; k < S::kSteps; ++k) f.code[k] = *reinterpret_cast<const v4i*>(keys + t * S::kRow + ((2 * k + h) ^ S::key_swizzle(t)) * 16);
-    };
-    const auto score_mfma = [&](const KeyFragments& f, auto index, v16f& s) {   // 64 channels of keys with one part of the queries
-      constexpr int k = decltype(index)::value / 2;
-      const v4i x = f.code[k];
-      const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-      constexpr int kByte = k % 2 == 0 ? 0 : 2;
-      if constexpr (decltype(index)::value % 2 == 0) s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], k == 0 ? v16f{} : s, kFmtFp4, 0, kByte, (int)f.scale[k / 2], 0, s_lo);
-      else s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, kByte, (int)f.scale[k / 2], 0, s_hi);
-    };
-    const auto scores = [&](int buffer, int j, v16f& s) {
-      KeyFragments f;
-      read_keys(buffer, j, f);
-      unrolled<2 * S::kSteps>([&](auto index) { score_mfma(f, index, s); });
-    };
-    // Masks the scores of n and sees to the maximum.  What is subtracted from the scores follows the maximum only where that runs ahead by
-    // more than 2^8 (probabilities up to 256 have the same relative error, and most steps go without touching the sums); `waiting` are the
-    // probabilities of n - 1, whose values are not added yet.
-    const auto prepare = [&](int n, v16f& s, float top, unsigned (&waiting)[8]) {   // top: of all scores
-      const int key0 = n * 32;
       if (key0 < lo_max || key0 + 32 > hi_min) {
         const int from = lo_row - key0 - 16 * h;
         const unsigned many = (unsigned)(hi_row > lo_row ? hi_row - lo_row : 0);
 #pragma unroll
         for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
-        top = cross_max<false>(largest_of<0, 15>(s, kNone));
       }
-      const float top2 = top > 0.5f * kNone ? top * c : kNoMax;
-      if (__any(top2 > m + 8.0f)) {
-        const float to_m = fmaxf(m, __builtin_ceilf(top2)), fade = __builtin_amdgcn_exp2f(m - to_m);
+      // ---- probabilities.  Any reference will do that keeps them in range, so the scores' maximum is looked for only where a row has none yet
+      // or a lane's sixteen come to more than 2^8: probabilities up to there have the same relative error, and most steps go without.
+      unsigned prob[8];
+      float sum;
+      const auto probabilities = [&] {
+        const float shift = m == kNoMax ? 0.0f : -m;
+        sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t + 1], c, shift));
+          sum += a;
+          sum += d;
+          prob[t] = pack_bf16x2(a, d);
+        }
+      };
+      probabilities();
+      if (const bool over = m == kNoMax || !(sum <= 256.0f); __any(over)) {   // a row by itself: what others hold leaves it as it is
+        const float top = cross_max<false>(largest_of<0, 15>(s, kNone)), to_row = fmaxf(m, top > 0.5f * kNone ? top * c : kNoMax);
+        const float to = cross_max<false>(over ? 1.0f : 0.0f) != 0.0f ? to_row : m, fade = __builtin_amdgcn_exp2f(m - to);
         l *= fade;
 #pragma unroll
         for (int k = 0; k < C; ++k) acc[k] *= fade;
-        const unsigned down = (unsigned)fminf(to_m - m, 255.0f) * 0x00800080u;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) waiting[t] = pk_sub_sat(waiting[t], down);
-        m = to_m;
+        m = to;
+        probabilities();
       }
-    };
-    const auto probability_pair = [&](const v16f& s, float shift, int t, unsigned (&out)[8]) {
-      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t + 1], c, shift));
-      l += a;
-      l += d;
-      out[t] = pack_bf16x2(a, d);
-    };
-    const auto read_values = [&](int buffer, int j, int half, int k) {
-      typedef short v8s __attribute__((ext_vector_type(8)));
-      const int r = lane % 16 / 4;   // token within four
-      const int piece = 4 * k + 2 * ((lane / 16) & 1) + (lane % 4) / 2;
-      const unsigned char* at = smem + kBuffers * S::kBuffer + buffer * S::kValues + (32 * j + 16 * h + 8 * half + r) * (2 * D) +
-                                (piece ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)at);
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at + 4 * 2 * D));
-      return __builtin_bit_cast(v8bf, v8s{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-    };
-    const auto of_half = [&](const unsigned (&w)[8], int half) {
-      return __builtin_bit_cast(v8bf, v4i{(int)w[4 * half], (int)w[4 * half + 1], (int)w[4 * half + 2], (int)w[4 * half + 3]});
-    };
-    const auto values = [&](int buffer, int j, const unsigned (&w)[8]) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int k = 0; k < C; ++k) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_values(buffer, j, half, k), of_half(w, half), acc[k], 0, 0, 0);
-    };
-    // All three steps at once, for half j of the present tile: after every MFMA its share of the exponentials, in the second half also of the
-    // next tile's values on their way to LDS (behind the last tile: whatever the registers hold, to where nobody reads)
-    const auto step = [&](int next_keys, int last_values, auto which, const v16f& s, v16f& next_s, unsigned (&out)[8], const unsigned (&waiting)[8], float& next_top, int store_to) {
-      constexpr int j = decltype(which)::value;
-      constexpr int kQk = 2 * S::kSteps, kMfma = kQk + 2 * C, kAhead = C < 4 ? C : 4;   // value fragments that wait in registers
-      const float shift = m == kNoMax ? 0.0f : -m;
-      KeyFragments f;
-      read_keys(next_keys, j ^ 1, f);
-      v8bf v[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) v[k] = read_values(last_values, j ^ 1, 0, k);
-      float top[2];
-      unrolled<kMfma>([&](auto index) {   // two of the scores', two of the values', and so on; the rest of the values'
-        constexpr int n = decltype(index)::value;
-        if constexpr (n < 2 * kQk && n % 4 < 2) {
-          score_mfma(f, Index<n / 4 * 2 + n % 4>{}, next_s);
-        } else {
-          constexpr int at = n < 2 * kQk ? n / 4 * 2 + n % 4 - 2 : n - kQk, k = at % C;
-          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[at % kAhead], of_half(waiting, at / C), acc[k], 0, 0, 0);
-          if constexpr (at + kAhead < 2 * C) v[at % kAhead] = read_values(last_values, j ^ 1, (at + kAhead) / C, (at + kAhead) % C);
-        }
-        if constexpr (n == kMfma - 3) top[0] = largest_of<0, 7>(next_s, kNone);
-        if constexpr (n == kMfma - 2) top[1] = largest_of<8, 15>(next_s, top[0]);
-        if constexpr (n == kMfma - 1) next_top = cross_max<false>(top[1]);
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          if (t * kMfma / 8 == n) probability_pair(s, shift, t, out);
-        if constexpr (j == 1) {
-#pragma unroll
-          for (int w = 0; w < Values<D>::kWords; ++w)
-            if ((2 * w + 1) * kMfma / (2 * Values<D>::kWords) + 1 == n) store_value_word(store_to, w);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      });
-    };
-    // Values with a NaN scale, zeros in LDS: NaN for the rows to which they count
-    const auto poison = [&](int buffer, int j, const unsigned (&w)[8]) {
-      uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
-#pragma unroll
-      for (int t = 0; t < 16; ++t) some |= (w[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
-#pragma unroll
-      for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
-        const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
-        const bool hit = (nan_in[buffer][D == 256 ? k % 2 : 0][2 * j + h] & some & (0x1111111111111111ull << quarter)) != 0;
-        acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
-      }
-    };
-
-    if (tiles > 0) {
-      prepare_values(tile0, 0);
-#pragma unroll
-      for (int w = 0; w < Values<D>::kWords; ++w) store_value_word(0, w);
-      wait_loads<0>();
-    }
-    __syncthreads();
-    float top = kNone;   // of the scores that come next
-    if (active && tiles > 0) {
-      scores(0, 0, score[0]);
-      top = cross_max<false>(largest_of<0, 15>(score[0], kNone));
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) prob[1][k] = 0;
-    int buffer = 0, last = 0, next_buffer = 1, free_buffer = 2;   // of this tile, the one before (the first has none: its own), the next two
-    bool nan_last = false;
-    for (int i = 0; i < tiles; ++i) {
-      const int tile = tile0 + i;
-      if (i + 1 < tiles) request_values(tile + 1, page[1]);
-      if (i + 2 < tiles) request_keys(tile + 2, page[2], free_buffer);
-      page[1] = page[2];
-      page[2] = page_of(tile + 3);
+      l += sum;
+      // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
       uint64_t nan = 0;
 #pragma unroll
       for (int k = 0; k < Values<D>::kScaleBytes; ++k)
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) nan |= nan_in[buffer][k][w];
-      bool nan_now = false;
+      if (__builtin_amdgcn_readfirstlane((int)(nan | nan >> 32))) {
+        uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (active) {
-          prepare(2 * tile + j, score[j], top, prob[j ^ 1]);
-          if (j) nan_now = __builtin_amdgcn_readfirstlane((int)(nan | nan >> 32)) != 0;
-          if (j ? nan_now : nan_last) poison(j ? buffer : last, j ? 0 : 1, prob[j ^ 1]);
-        }
-        if (j && i + 1 < tiles) prepare_values(tile + 1, next_buffer);
-        if (active) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (j) step(next_buffer, buffer, Index<1>{}, score[1], score[0], prob[1], prob[0], top, next_buffer);
-          else step(buffer, last, Index<0>{}, score[0], score[1], prob[0], prob[1], top, 0);
-          // here and not where they are used
+        for (int t = 0; t < 16; ++t) some |= (prob[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(prob[j][k]));
-          asm volatile("" : "+v"(l), "+v"(top));
-          __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
+          const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
+          const bool hit = (nan_in[buffer][D == 256 ? k % 2 : 0][2 * j + h] & some & (0x1111111111111111ull << quarter)) != 0;
+          acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
         }
       }
-      if (!active) {
+      // ---- values
 #pragma unroll
-        for (int w = 0; w < Values<D>::kWords; ++w) store_value_word(next_buffer, w);
+      for (int half = 0; half < 2; ++half) {
+        const v4i w = {(int)prob[4 * half], (int)prob[4 * half + 1], (int)prob[4 * half + 2], (int)prob[4 * half + 3]};
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+          typedef short v8s __attribute__((ext_vector_type(8)));
+          const unsigned at = value_at[k] + buffer * S::kValues + (32 * j + 8 * half) * (2 * D);
+          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at));
+          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at + 4 * 2 * D));
+          const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), __builtin_bit_cast(v8bf, w), acc[k], 0, 0, 0);
+        }
       }
+    };
+    const auto store_values = [&](int tile, int buffer) {
+      prepare_values(tile, buffer);
+#pragma unroll
+      for (int w = 0; w < Values<D>::kWords; ++w) store_value_word(buffer, w);
+    };
+
+    if (tiles > 0) store_values(tile0, 0);
+    wait_loads<0>();
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      const int tile = tile0 + i, buffer = i & 1;
+      if (i + 1 < tiles) {
+        request_values(tile + 1, page[1]);
+        request_keys(tile + 1, page[1], buffer ^ 1);
+        page[1] = page_of(tile + 2);
+      }
+      if (active && tile * kTile < hi_max && tile * kTile + kTile > lo_min) {
+        multiply(tile, buffer, Index<0>{});
+        multiply(tile, buffer, Index<1>{});
+      }
+      if (i + 1 < tiles) store_values(tile + 1, buffer ^ 1);
       wait_loads<0>();
       __syncthreads();
-      nan_last = nan_now;
-      last = buffer;
-      buffer = next_buffer;
-      next_buffer = free_buffer;
-      free_buffer = last;
     }
-    if (active && tiles > 0) {   // the last step's values
-      if (nan_last) poison(last, 1, prob[1]);
-      values(last, 1, prob[1]);
-    }
-    __syncthreads();
 
     // ---- results: lane (column col) has channels 32 k + 8 i + 4 h .. + 3 of its row
     if (active) {
@@ -445,33 +391,33 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_prompt_kernel(AttnArgs p)
   }
 }
 
-int workgroups_of() { return 2 * compute_units(); }
+int workgroups_of(const AttnArgs& p) {
+  const int d = p.c.head_dim;
+  return compute_units() * (d == 64 ? waves_per_simd<64>() : d == 128 ? waves_per_simd<128>() : waves_per_simd<256>());
+}
+template <int D>
+void launch(const AttnArgs& p, int workgroups, hipStream_t s) {
+  const dim3 grid((unsigned)workgroups), block(kWaves * 64);
+  const int64_t last = p.c.pages - 1, page = (int64_t)p.c.kv_heads * p.c.page_size * D / 2;   // bytes of codes; of scales a 16th
+  const auto small = [&](int64_t stride, int64_t bytes) { return last * stride + bytes <= (int64_t)1 << 32; };
+  const bool all = small(p.c.k_page_stride, page) && small(p.c.v_page_stride, page) && small(p.c.k_scale_page_stride, page / 16) && small(p.c.v_scale_page_stride, page / 16);
+  if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attn_prompt_kernel<D, false>), grid, block, 0, s, p);
+}
 
 }  // namespace
 
-size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p.c.head_dim, workgroups_of()); }
+size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p.c.head_dim, workgroups_of(p)); }
 
 hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
-  const int workgroups = workgroups_of();
+  const int workgroups = workgroups_of(p);
   p.whole = 0;
   p.min_units_log2 = 2;
   p.few_long = p.a.batch <= 16;
   place_workspace(p, kRows, workgroups, ws);
-  const dim3 grid((unsigned)workgroups), block(kWaves * 64);
-  const int64_t last = p.c.pages - 1, page = (int64_t)p.c.kv_heads * p.c.page_size * p.c.head_dim / 2;   // bytes of codes; of scales a 16th
-  const auto small = [&](int64_t stride, int64_t bytes) { return last * stride + bytes <= (int64_t)1 << 32; };
-  const bool all = small(p.c.k_page_stride, page) && small(p.c.v_page_stride, page) && small(p.c.k_scale_page_stride, page / 16) && small(p.c.v_scale_page_stride, page / 16);
-#define AVE_PROMPT(D)                                                                                  \
-  if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true>), grid, block, 0, s, p);                    \
-  else hipLaunchKernelGGL((attn_prompt_kernel<D, false>), grid, block, 0, s, p)
-  if (p.c.head_dim == 64) {
-    AVE_PROMPT(64);
-  } else if (p.c.head_dim == 128) {
-    AVE_PROMPT(128);
-  } else {
-    AVE_PROMPT(256);
-  }
-#undef AVE_PROMPT
+  if (p.c.head_dim == 64) launch<64>(p, workgroups, s);
+  else if (p.c.head_dim == 128) launch<128>(p, workgroups, s);
+  else launch<256>(p, workgroups, s);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   return launch_attn_combine(p, kRows, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
 }
