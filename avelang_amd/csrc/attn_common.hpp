@@ -282,13 +282,20 @@ __device__ inline unsigned lds_address(const void* p) {
 // A barrier that orders LDS and leaves loads to LDS under way
 __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Page of tokens 16 i .. 16 i + 15 of a sequence; a valid one whatever the table holds (tokens behind the last key: the last key's)
-__device__ inline int page_at(const AttnArgs& p, ConstInts row, int token, int len) {
+// Page of tokens 16 i .. 16 i + 15 of a sequence (tokens behind the last key: the last key's): what the table holds, and a valid one of that
+__device__ inline int page_entry(const AttnArgs& p, ConstInts row, int token, int len) {
   const int t = token < len ? token : len > 0 ? len - 1 : 0;
-  int page = p.a.table_pages > 0 ? row[t >> p.page_shift] : 0;
-  page = page < 0 ? 0 : page;
+  return p.a.table_pages > 0 ? row[t >> p.page_shift] : 0;
+}
+__device__ inline int page_of(const AttnArgs& p, int entry) {
+  const int page = entry < 0 ? 0 : entry;
   return page < p.c.pages ? page : p.c.pages - 1;
 }
+__device__ inline int page_at(const AttnArgs& p, ConstInts row, int token, int len) { return page_of(p, page_entry(p, row, token, len)); }
+
+// A value that all lanes hold, in a scalar register
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 
 // Eight bf16, from any address where `aligned` is not set
 __device__ inline v4i load8_bf16(const uint16_t* q, bool aligned) {

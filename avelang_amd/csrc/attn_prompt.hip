@@ -39,8 +39,10 @@ struct Shape {
 template <int D>
 struct Values {
   static constexpr int kWords = Shape<D>::kThreadBytes / 4, kScaleBytes = D == 256 ? 2 : 1;
-  unsigned code[kWords];
-  int scale[kScaleBytes];
+  unsigned code[kWords], scales;   // scales: the four bytes that hold them
+  // where those lie behind the wave's first token, and from which bit this lane's own
+  __device__ static unsigned scales_at(int lane) { return D == 64 ? lane / 8 * 4 : D == 128 ? lane / 4 * 4 : lane / 2 * 4; }
+  __device__ static int shift(int lane) { return D == 64 ? 8 * (lane / 2 % 4) : D == 128 ? 8 * (lane % 4) : 16 * (lane % 2); }
 };
 
 template <int N>
@@ -52,6 +54,7 @@ typedef __attribute__((address_space(3))) v4i LdsInt4;
 typedef __attribute__((address_space(3))) unsigned LdsInt;
 typedef __attribute__((address_space(3))) uint16_t LdsShort;
 typedef __attribute__((address_space(3))) v4s LdsShort4;
+typedef __attribute__((address_space(3))) v8bf Lds8Bf16;
 template <typename T>
 __device__ inline T* lds_at(unsigned address) {
   return (T*)(uintptr_t)address;
@@ -68,32 +71,25 @@ template <int D, bool SMALL>
 __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int C = S::C;
-  __shared__ __align__(16) unsigned char smem[S::kLds];
+  __shared__ __align__(512) unsigned char smem[S::kLds];
   __shared__ uint64_t nan_in[kBuffers][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
+  __shared__ __align__(16) int nan_any[kBuffers][kWaves];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
   const Part part = take_part<kRows, kTile, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
-  const float c = softmax_scale(p.a.scale);
+  const float c = uniform(softmax_scale(p.a.scale));
   // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
   // key's scales, and by 32 channels the values
-  unsigned key_at[S::kSteps], value_at[C], scale_at;
+  // (k steps of 64 or 32 channels on they differ by an exclusive or alone)
+  unsigned key_at, value_at, scale_at;
   {
     const int t = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), r = lane % 16 / 4;   // r: token within four
-#pragma unroll
-    for (int k = 0; k < S::kSteps; ++k) {
-      key_at[k] = lds + t * S::kRow + ((2 * k + h) ^ S::key_swizzle(t)) * 16;
-      asm volatile("" : "+v"(key_at[k]));
-    }
+    key_at = lds + t * S::kRow + (h ^ S::key_swizzle(t)) * 16;
     scale_at = lds + S::kKeys + t * S::kBlocks;
-    asm volatile("" : "+v"(scale_at));
-#pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int piece = 4 * k + 2 * ((lane / 16) & 1) + (lane % 4) / 2;
-      value_at[k] = lds + kBuffers * S::kBuffer + (16 * h + r) * (2 * D) + (piece ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
-      asm volatile("" : "+v"(value_at[k]));
-    }
+    value_at = lds + kBuffers * S::kBuffer + (16 * h + r) * (2 * D) + ((2 * ((lane / 16) & 1) + (lane % 4) / 2) ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
+    asm volatile("" : "+v"(key_at), "+v"(value_at), "+v"(scale_at));
   }
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
@@ -124,21 +120,17 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     const int tiles = it.s.len > 0 ? (int)(to - from) : 0;
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
-    // what this wave's rows see: [lo_row, hi_row) of a lane's row, [lo_max, hi_min) of all
-    const int row0 = it.row0 + 32 * wave;
-    const bool active = row0 < rows;
-    int lo_row, hi_row, lo_max, hi_min, lo_min, hi_max;
-    {
-      const int last = row0 + 32 < rows ? row0 + 31 : rows - 1, row = row0 + col < rows ? row0 + col : last;
-      visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
-      visible(p, it.s, p.token_of(last), lo_max, hi_max);
-      visible(p, it.s, p.token_of(row), lo_row, hi_row);
-      lo_max = __builtin_amdgcn_readfirstlane(lo_max), hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-    }
+    // what this wave's rows see: [lo_max, hi_min) all of them, [lo_min, hi_max) any
+    const int row0 = uniform(it.row0 + 32 * wave), row = row0 + col;
+    const bool active = row0 < uniform(rows);
+    int lo_max, hi_min, lo_min, hi_max;
+    visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
+    visible(p, it.s, p.token_of(row0 + 32 < rows ? row0 + 31 : rows - 1), lo_max, hi_max);
+    lo_max = uniform(lo_max), hi_min = uniform(hi_min), lo_min = uniform(lo_min), hi_max = uniform(hi_max);
 
     // ---- a tile's requests: keys and their scales to LDS, values to registers; a wave takes 16 tokens, which lie in one page
     Values<D> next;
-    const auto page_of = [&](int tile) { return page_at(p, table, tile * kTile + 16 * wave, it.s.len); };
+    const auto entry_of = [&](int tile) { return page_entry(p, table, tile * kTile + 16 * wave, it.s.len); };   // one tile ahead of its use: nobody waits
     // A tensor's base and offset for this wave's tokens of a tile, `bytes` a token and head
     const auto place = [&](const uint8_t* tensor, int64_t stride, int pg, int tile, unsigned bytes, const uint8_t*& base) -> unsigned {
       const int t = tile * kTile + 16 * wave;
@@ -176,50 +168,48 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         const v2i x = *reinterpret_cast<const v2i*>(base + (off + 4 * k));
         next.code[k] = (unsigned)x[0], next.code[k + 1] = (unsigned)x[1];
       }
-      off = place(p.c.v_scale, p.c.v_scale_page_stride, pg, tile, S::kBlocks, base) + lane / 4 * S::kBlocks;
-#pragma unroll
-      for (int k = 0; k < Values<D>::kScaleBytes; ++k) next.scale[k] = base[off + (D == 64 ? lane % 4 / 2 : D == 128 ? lane % 4 : 2 * (lane % 4) + k)];
+      off = place(p.c.v_scale, p.c.v_scale_page_stride, pg, tile, S::kBlocks, base) + Values<D>::scales_at(lane);
+      next.scales = *reinterpret_cast<const unsigned*>(base + off);
     };
-    const auto prepare_values = [&](int tile, int buffer) {   // what no key occupies, and what has a NaN scale, is zero
-      const bool there = tile * kTile + 16 * wave + lane / 4 < it.s.len;
+    const auto store_values = [&](int tile, int buffer) {   // what no key occupies, and what has a NaN scale, is zero
+      const int token = 16 * wave + lane / 4;
+      const bool there = tile * kTile + token < it.s.len;
+      const unsigned at = lds + kBuffers * S::kBuffer + buffer * S::kValues + token * (2 * D) + ((lane % 4 * Values<D>::kWords) ^ S::value_swizzle(token)) * 16;
+      uint64_t any = 0;
 #pragma unroll
       for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
         constexpr int kOfScale = Values<D>::kWords / Values<D>::kScaleBytes;
-        const bool bad = there && next.scale[k] >= 253, none = bad || !there;
+        const unsigned scale = next.scales >> (Values<D>::shift(lane) + 8 * k) & 255;
+        const bool bad = there && scale >= 253, none = bad || !there;
+        const float f = __builtin_bit_cast(float, none ? 0x3F800000u : scale << 23);
 #pragma unroll
-        for (int w = 0; w < kOfScale; ++w) next.code[k * kOfScale + w] = none ? 0 : next.code[k * kOfScale + w];
-        next.scale[k] = none ? 127 : next.scale[k];
+        for (int w = k * kOfScale; w < (k + 1) * kOfScale; ++w) {   // eight channels, one 16-byte piece
+          const unsigned x = none ? 0 : next.code[w];
+          const v2bf a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 1);
+          const v2bf a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 3);
+          *lds_at<Lds8Bf16>(at ^ 16 * w) = v8bf{a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+        }
         const uint64_t lanes = __ballot(bad);
+        any |= lanes;
         if (lane == 0) nan_in[buffer][k][wave] = lanes;
       }
-    };
-    const auto store_value_word = [&](int buffer, int w) {   // eight channels, one 16-byte piece
-      const int token = 16 * wave + lane / 4;
-      unsigned char* at = smem + kBuffers * S::kBuffer + buffer * S::kValues + token * (2 * D);
-      const float f = __builtin_bit_cast(float, (unsigned)next.scale[D == 256 ? w / 4 : 0] << 23);
-      const unsigned x = next.code[w];
-      const v2bf a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 1);
-      const v2bf a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 3);
-      const v8bf v = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
-      const int piece = lane % 4 * Values<D>::kWords + w;
-      *reinterpret_cast<v8bf*>(at + (piece ^ S::value_swizzle(token)) * 16) = v;
+      if (lane == 0) nan_any[buffer][wave] = any != 0;
     };
 
     // ---- the first requests, then the queries, whose way is as long
-    int page[2] = {page_of(tile0), page_of(tile0 + 1)};   // of the first tile, the next
+    int entry = entry_of(tile0 + 1);
     if (tiles > 0) {
-      request_keys(tile0, page[0], 0);
-      request_values(tile0, page[0]);
+      const int page = page_of(p, entry_of(tile0));
+      request_keys(tile0, page, 0);
+      request_values(tile0, page);
     }
     // ---- queries: lane (column col): bytes 0-15 of a step are k = 16 h .., bytes 16-31 k = 32 + 16 h ..
     v8i q_hi[S::kSteps], q_lo[S::kSteps];
-    int s_hi, s_lo;
-    float sink;
+    int q_scale;   // of the first part; of the second in the next byte
     {
-      const bool real = row0 + col < rows;
-      const int t = real ? p.token_of(row0 + col) : 0, query_head = it.head * p.group + (real ? row0 + col - t * p.group : 0);
+      const bool real = row < rows;
+      const int t = real ? p.token_of(row) : 0, query_head = it.head * p.group + (real ? row - t * p.group : 0);
       const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)query_head * p.a.q_head_stride;
-      sink = sink_of(p, query_head);
       v4i x[S::kSteps][4];
       us2 m = {0, 0};
 #pragma unroll
@@ -241,7 +231,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
 #pragma unroll
           for (int e = 0; e < 2; ++e) q_hi[i][2 * k + e] = hi[e] ^ sign, q_lo[i][2 * k + e] = lo[e] ^ sign;
         }
-      s_hi = s.hi_byte, s_lo = s.lo_byte;
+      q_scale = s.hi_byte | s.lo_byte << 8;
     }
 
     v16f acc[C];
@@ -250,7 +240,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     float m = kNoMax, l = 0.0f;   // m: base 2
 
     // 32 keys, half j of the tile in a buffer
-    const auto multiply = [&](int tile, int buffer, auto which) {
+    const auto multiply = [&](int tile, int buffer, auto which, int& nan) {
       constexpr int j = decltype(which)::value;
       const int key0 = tile * kTile + 32 * j;
       // ---- scores
@@ -266,20 +256,27 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         }
 #pragma unroll
         for (int k = 0; k < S::kSteps; ++k) {
-          const v4i x = *lds_at<const LdsInt4>(key_at[k] + buffer * S::kBuffer + 32 * j * S::kRow);
+          const v4i x = *lds_at<const LdsInt4>((key_at ^ 32 * k) + buffer * S::kBuffer + 32 * j * S::kRow);
           const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
           if (k % 2 == 0) {
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 0, s_lo);
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 0, s_hi);
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 1, q_scale);
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 0, q_scale);
           } else {
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 0, s_lo);
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 0, s_hi);
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 1, q_scale);
+            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 0, q_scale);
           }
         }
       }
+      if constexpr (j == 0) {
+        const v4i any = *reinterpret_cast<const v4i*>(nan_any[buffer]);
+        nan = uniform(any[0] | any[1] | any[2] | any[3]);
+      }
       if (key0 < lo_max || key0 + 32 > hi_min) {
-        const int from = lo_row - key0 - 16 * h;
-        const unsigned many = (unsigned)(hi_row > lo_row ? hi_row - lo_row : 0);
+        int mine = row, lo, hi;
+        asm volatile("" : "+v"(mine));   // here and not in a register
+        visible(p, it.s, p.token_of(mine), lo, hi);   // (a row behind the last: whatever)
+        const int from = lo - key0 - 16 * h;
+        const unsigned many = (unsigned)(hi > lo ? hi - lo : 0);
 #pragma unroll
         for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
       }
@@ -310,12 +307,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       }
       l += sum;
       // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
-      uint64_t nan = 0;
-#pragma unroll
-      for (int k = 0; k < Values<D>::kScaleBytes; ++k)
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) nan |= nan_in[buffer][k][w];
-      if (__builtin_amdgcn_readfirstlane((int)(nan | nan >> 32))) {
+      if (nan) {
         uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
 #pragma unroll
         for (int t = 0; t < 16; ++t) some |= (prob[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
@@ -333,7 +325,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
 #pragma unroll
         for (int k = 0; k < C; ++k) {
           typedef short v8s __attribute__((ext_vector_type(8)));
-          const unsigned at = value_at[k] + buffer * S::kValues + (32 * j + 8 * half) * (2 * D);
+          const unsigned at = (value_at ^ 64 * k) + buffer * S::kValues + (32 * j + 8 * half) * (2 * D);
           const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at));
           const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at + 4 * 2 * D));
           const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -341,25 +333,21 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         }
       }
     };
-    const auto store_values = [&](int tile, int buffer) {
-      prepare_values(tile, buffer);
-#pragma unroll
-      for (int w = 0; w < Values<D>::kWords; ++w) store_value_word(buffer, w);
-    };
-
     if (tiles > 0) store_values(tile0, 0);
     wait_loads<0>();
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       const int tile = tile0 + i, buffer = i & 1;
       if (i + 1 < tiles) {
-        request_values(tile + 1, page[1]);
-        request_keys(tile + 1, page[1], buffer ^ 1);
-        page[1] = page_of(tile + 2);
+        const int page = page_of(p, entry);
+        request_values(tile + 1, page);
+        request_keys(tile + 1, page, buffer ^ 1);
+        entry = entry_of(tile + 2);
       }
       if (active && tile * kTile < hi_max && tile * kTile + kTile > lo_min) {
-        multiply(tile, buffer, Index<0>{});
-        multiply(tile, buffer, Index<1>{});
+        int nan = 0;
+        multiply(tile, buffer, Index<0>{}, nan);
+        multiply(tile, buffer, Index<1>{}, nan);
       }
       if (i + 1 < tiles) store_values(tile + 1, buffer ^ 1);
       wait_loads<0>();
@@ -370,11 +358,10 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     if (active) {
       const float sum = cross_sum<false>(l), m2 = m == kNoMax ? -INFINITY : m;
       const bool done = from == it.begin && to == end;
-      const int row = row0 + col;
       if (row < rows) {
         const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + 32 * wave + col;
         const size_t place = row_index(p, it.s.first, it.head, row);
-        const RowEnd e = row_end(sink, m2, sum);
+        const RowEnd e = row_end(sink_of(p, it.head * p.group + (row - p.token_of(row) * p.group)), m2, sum);
         if (done && p.a.lse && h == 0) p.a.lse[place] = e.lse;
 #pragma unroll
         for (int k = 0; k < C; ++k)
