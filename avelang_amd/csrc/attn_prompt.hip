@@ -98,6 +98,9 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     int* m = p.meta + (size_t)g * kMeta;
     m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
   }
+  // Among waves that could issue, the oldest goes first, and with equal parts the workgroups that a compute unit got last would end long
+  // after the others.  Each takes its turn before the rest, a tile at a time.
+  int turn = blockIdx.x * waves_per_simd<D>() / gridDim.x;
   bool first_item = true;
   Item it{};
   for (unsigned u = part.u0; u < part.u1;) {
@@ -338,6 +341,11 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       const int tile = tile0 + i, buffer = i & 1;
+      if constexpr (waves_per_simd<D>() > 1) {
+        if (turn == 0) __builtin_amdgcn_s_setprio(1);
+        else if (turn == 1) __builtin_amdgcn_s_setprio(0);
+        turn = turn + 1 < waves_per_simd<D>() ? turn + 1 : 0;
+      }
       if (i + 1 < tiles) {
         const int page = page_of(p, entry);
         request_values(tile + 1, page);
