@@ -31,6 +31,7 @@ struct AttnArgs {
   int whole;          // 1: items are not split; no workspace, no second launch
   int q_aligned;      // every row of q starts at a multiple of 16 bytes
   int few_long;       // few sequences of many blocks of rows each
+  int item_units;     // that the start and the end of an item count for beside its tiles
   int min_units_log2; // of a workgroup, so that small calls are not cut into crumbs
   int* meta;          // workspace: [workgroups][kMeta]
   float* part_ml;     // [2 workgroups][ROWS][2]: maximum (base 2) and sum
@@ -83,19 +84,19 @@ __device__ inline void visible(const AttnArgs& p, const Sequence& s, int t, int&
   lo = p.a.window > 0 && pos >= p.a.window ? pos - p.a.window + 1 : 0;
 }
 
-// A block of rows: units, and the first tile
+// A block of rows: units (those for its start come before its tiles), and the first tile
 template <int ROWS, int TILE>
 __device__ inline int block_units(const AttnArgs& p, const Sequence& s, int row0, int& tile0) {
   const int rows = s.n * p.group, last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
   int lo, hi, other;
   if (rows <= 0) {
     tile0 = 0;
-    return 1;
+    return 1 + p.item_units;
   }
   visible(p, s, p.token_of(row0), lo, other);
   visible(p, s, p.token_of(last), other, hi);
   tile0 = lo / TILE;
-  return hi > lo ? (hi + TILE - 1) / TILE - tile0 : 1;
+  return (hi > lo ? (hi + TILE - 1) / TILE - tile0 : 1) + p.item_units;
 }
 template <int ROWS, int TILE>
 __device__ inline int sequence_units(const AttnArgs& p, const Sequence& s) {   // of one key head

@@ -463,6 +463,7 @@ hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
   constexpr int ROWS = NT * 16;
   const int workgroups = compute_units() * workgroups_per_cu<D, NT, NW, NS>();
   p.whole = whole;
+  p.item_units = 0;
   p.min_units_log2 = p.whole ? 0 : log2_of(NW);
   if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
   const dim3 grid((unsigned)workgroups), block(NW * 64);

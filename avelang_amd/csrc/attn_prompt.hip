@@ -100,7 +100,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   }
   // Among waves that could issue, the oldest goes first, and with equal parts the workgroups that a compute unit got last would end long
   // after the others.  Each takes its turn before the rest, a tile at a time.
-  int turn = blockIdx.x * waves_per_simd<D>() / gridDim.x;
+  const int late = blockIdx.x * waves_per_simd<D>() / gridDim.x;
+  int turn = 0;
   bool first_item = true;
   Item it{};
   for (unsigned u = part.u0; u < part.u1;) {
@@ -119,8 +120,10 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
     }
     first_item = false;
-    const int rows = it.s.n * p.group, tile0 = it.tile0 + (int)(from - it.begin);
-    const int tiles = it.s.len > 0 ? (int)(to - from) : 0;
+    const unsigned start = it.begin + p.item_units;   // unit of the item's first tile
+    const unsigned first = from > start ? from : start;
+    const int rows = it.s.n * p.group, tile0 = it.tile0 + (int)(first - start);
+    const int tiles = it.s.len > 0 && to > first ? (int)(to - first) : 0;
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
     // what this wave's rows see: [lo_max, hi_min) all of them, [lo_min, hi_max) any
@@ -342,8 +345,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     for (int i = 0; i < tiles; ++i) {
       const int tile = tile0 + i, buffer = i & 1;
       if constexpr (waves_per_simd<D>() > 1) {
-        if (turn == 0) __builtin_amdgcn_s_setprio(1);
-        else if (turn == 1) __builtin_amdgcn_s_setprio(0);
+        if (turn < late) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
         turn = turn + 1 < waves_per_simd<D>() ? turn + 1 : 0;
       }
       if (i + 1 < tiles) {
@@ -407,6 +410,7 @@ size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p
 hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   const int workgroups = workgroups_of(p);
   p.whole = 0;
+  p.item_units = 2;
   p.min_units_log2 = 2;
   p.few_long = p.a.batch <= 16;
   place_workspace(p, kRows, workgroups, ws);
