@@ -82,15 +82,15 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   const float c = uniform(softmax_scale(p.a.scale));
   // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
   // key's scales, and by 32 channels the values
-  // (k steps of 64 or 32 channels on they differ by an exclusive or alone)
-  unsigned key_at, value_at, scale_at;
-  {
+  // (k steps of 64 or 32 channels on they differ by an exclusive or alone).  They wait in LDS, as registers are short.
+  __shared__ __align__(16) v4i places[64];
+  if (tid < 64) {
     const int t = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), r = lane % 16 / 4;   // r: token within four
-    key_at = lds + t * S::kRow + (h ^ S::key_swizzle(t)) * 16;
-    scale_at = lds + S::kKeys + t * S::kBlocks;
-    value_at = lds + kBuffers * S::kBuffer + (16 * h + r) * (2 * D) + ((2 * ((lane / 16) & 1) + (lane % 4) / 2) ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
-    asm volatile("" : "+v"(key_at), "+v"(value_at), "+v"(scale_at));
+    const unsigned key_at = lds + t * S::kRow + (h ^ S::key_swizzle(t)) * 16, scale_at = lds + S::kKeys + t * S::kBlocks;
+    const unsigned value_at = lds + kBuffers * S::kBuffer + (16 * h + r) * (2 * D) + ((2 * ((lane / 16) & 1) + (lane % 4) / 2) ^ S::value_swizzle(r)) * 16 + (lane & 1) * 8;
+    places[lane] = v4i{(int)key_at, (int)scale_at, (int)value_at, 8 * h};
   }
+  __syncthreads();
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
@@ -245,73 +245,90 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     for (int k = 0; k < C; ++k) acc[k] = v16f{};
     float m = kNoMax, l = 0.0f;   // m: base 2
 
-    // 32 keys, half j of the tile in a buffer
-    const auto multiply = [&](int tile, int buffer, auto which, int& nan) {
+    // ---- 32 keys, half j of a tile.  What the matrix instructions take out of LDS is read ahead of them, by hand: the compiler, short of
+    // registers, waits for each piece.
+    constexpr int kAhead = 3;   // fragments of values on their way
+    struct Keys {
+      v4i code[S::kSteps];
+      unsigned scale[(S::kBlocks + 3) / 4];
+    };
+    const auto read_keys = [&](int buffer, int j, const v4i& at_lane, Keys& f) {
+      const unsigned at = at_lane[0] + buffer * S::kBuffer, ks = at_lane[1] + buffer * S::kBuffer + 32 * j * S::kBlocks;
+      if constexpr (D == 64) {
+        f.scale[0] = *lds_at<const LdsShort>(ks);
+      } else {
+#pragma unroll
+        for (int k = 0; k < S::kBlocks / 4; ++k) f.scale[k] = lds_at<const LdsInt>(ks)[k];
+      }
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k) f.code[k] = *lds_at<const LdsInt4>((at ^ 32 * k) + 32 * j * S::kRow);
+    };
+    const auto scores = [&](const Keys& f, int shift) {
+      v16f s = {};
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k) {
+        const v4i x = f.code[k];
+        const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+        const int scale = (int)(f.scale[k / 2] >> shift);
+        if (k % 2 == 0) {
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 0, scale, 1, q_scale);
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 0, scale, 0, q_scale);
+        } else {
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 2, scale, 1, q_scale);
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 2, scale, 0, q_scale);
+        }
+      }
+      return s;
+    };
+    const auto read_values = [&](unsigned at, int j, int n) {   // 16 of the 32 keys (n / C), 32 channels (n % C)
+      typedef short v8s __attribute__((ext_vector_type(8)));
+      at = (at ^ 64 * (n % C)) + (32 * j + 8 * (n / C)) * (2 * D);
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at + 4 * 2 * D));
+      return __builtin_bit_cast(v8bf, v8s{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    };
+    // Probabilities from scores.  Any reference will do that keeps them in range, so the scores' maximum is looked for only where a lane's
+    // sixteen come to more than 2^8 (the first ones that a row sees: to infinity): up to there they have the same relative error, and most
+    // steps go without.
+    const auto probabilities = [&](int tile, auto which, v16f& s, unsigned (&prob)[8]) {
       constexpr int j = decltype(which)::value;
       const int key0 = tile * kTile + 32 * j;
-      // ---- scores
-      v16f s = {};
-      {
-        unsigned scale[(S::kBlocks + 3) / 4];
-        const unsigned ks = scale_at + buffer * S::kBuffer + 32 * j * S::kBlocks;
-        if constexpr (D == 64) {
-          scale[0] = *lds_at<const LdsShort>(ks) >> (8 * h);
-        } else {
-#pragma unroll
-          for (int k = 0; k < S::kBlocks / 4; ++k) scale[k] = lds_at<const LdsInt>(ks)[k] >> (8 * h);
-        }
-#pragma unroll
-        for (int k = 0; k < S::kSteps; ++k) {
-          const v4i x = *lds_at<const LdsInt4>((key_at ^ 32 * k) + buffer * S::kBuffer + 32 * j * S::kRow);
-          const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-          if (k % 2 == 0) {
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 1, q_scale);
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 0, (int)scale[k / 2], 0, q_scale);
-          } else {
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 1, q_scale);
-            s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 2, (int)scale[k / 2], 0, q_scale);
-          }
-        }
-      }
-      if constexpr (j == 0) {
-        const v4i any = *reinterpret_cast<const v4i*>(nan_any[buffer]);
-        nan = uniform(any[0] | any[1] | any[2] | any[3]);
-      }
       if (key0 < lo_max || key0 + 32 > hi_min) {
-        int mine = row, lo, hi;
-        asm volatile("" : "+v"(mine));   // here and not in a register
-        visible(p, it.s, p.token_of(mine), lo, hi);   // (a row behind the last: whatever)
-        const int from = lo - key0 - 16 * h;
+        int here = lane, lo, hi;
+        asm volatile("" : "+v"(here));   // here, and not in registers all the time
+        visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);   // (a row behind the last: whatever)
+        const int from = lo - key0 - here / 32 * 16;
         const unsigned many = (unsigned)(hi > lo ? hi - lo : 0);
 #pragma unroll
         for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
       }
-      // ---- probabilities.  Any reference will do that keeps them in range, so the scores' maximum is looked for only where a row has none yet
-      // or a lane's sixteen come to more than 2^8: probabilities up to there have the same relative error, and most steps go without.
-      unsigned prob[8];
       float sum;
-      const auto probabilities = [&] {
-        const float shift = m == kNoMax ? 0.0f : -m;
+      const auto exponentials = [&](float reference) {
         sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t], c, shift)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t + 1], c, shift));
+          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t], c, -reference)), d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * t + 1], c, -reference));
           sum += a;
           sum += d;
           prob[t] = pack_bf16x2(a, d);
+          asm volatile("" : "+v"(prob[t]));   // here, not where it is used
         }
       };
-      probabilities();
-      if (const bool over = m == kNoMax || !(sum <= 256.0f); __any(over)) {   // a row by itself: what others hold leaves it as it is
+      exponentials(m);
+      if (const bool over = !(sum <= 256.0f); __any(over)) {   // a row by itself: what others hold leaves it as it is
         const float top = cross_max<false>(largest_of<0, 15>(s, kNone)), to_row = fmaxf(m, top > 0.5f * kNone ? top * c : kNoMax);
         const float to = cross_max<false>(over ? 1.0f : 0.0f) != 0.0f ? to_row : m, fade = __builtin_amdgcn_exp2f(m - to);
         l *= fade;
 #pragma unroll
         for (int k = 0; k < C; ++k) acc[k] *= fade;
         m = to;
-        probabilities();
+        exponentials(m == kNoMax ? 0.0f : m);
       }
       l += sum;
+    };
+    const auto add_values = [&](int buffer, auto which, const unsigned (&prob)[8], int nan, const v4i& place, v8bf (&v)[kAhead], Keys& keys) {
+      const unsigned at = place[2] + buffer * S::kValues;
+      constexpr int j = decltype(which)::value;
       // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
       if (nan) {
         uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
@@ -320,30 +337,45 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
 #pragma unroll
         for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
           const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
-          const bool hit = (nan_in[buffer][D == 256 ? k % 2 : 0][2 * j + h] & some & (0x1111111111111111ull << quarter)) != 0;
+          const uint64_t* lanes = nan_in[buffer][D == 256 ? k % 2 : 0] + 2 * j;
+          const bool hit = ((lane < 32 ? lanes[0] : lanes[1]) & some & (0x1111111111111111ull << quarter)) != 0;
           acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
         }
       }
-      // ---- values
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const v4i w = {(int)prob[4 * half], (int)prob[4 * half + 1], (int)prob[4 * half + 2], (int)prob[4 * half + 3]};
-#pragma unroll
-        for (int k = 0; k < C; ++k) {
-          typedef short v8s __attribute__((ext_vector_type(8)));
-          const unsigned at = (value_at ^ 64 * k) + buffer * S::kValues + (32 * j + 8 * half) * (2 * D);
-          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at));
-          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<LdsShort4>(at + 4 * 2 * D));
-          const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), __builtin_bit_cast(v8bf, w), acc[k], 0, 0, 0);
-        }
+      for (int n = 0; n < 2 * C; ++n) {
+        const v4i w = {(int)prob[4 * (n / C)], (int)prob[4 * (n / C) + 1], (int)prob[4 * (n / C) + 2], (int)prob[4 * (n / C) + 3]};
+        acc[n % C] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % kAhead], __builtin_bit_cast(v8bf, w), acc[n % C], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (n + kAhead < 2 * C) v[n % kAhead] = read_values(at, j, n + kAhead);
+        if (j == 0 && n + kAhead == 2 * C) read_keys(buffer, 1, place, keys);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
+    const auto half_tile = [&](int tile, int buffer, auto which, int& nan, const v4i& place, Keys& keys) {
+      constexpr int j = decltype(which)::value;
+      v8bf v[kAhead];
+      unsigned prob[8];
+      if constexpr (j == 0) read_keys(buffer, 0, place, keys);
+      v4i any;
+      if constexpr (j == 0) any = *reinterpret_cast<const v4i*>(nan_any[buffer]);
+      v16f s = scores(keys, place[3]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) v[n] = read_values(place[2] + buffer * S::kValues, j, n);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (j == 0) nan = uniform(any[0] | any[1] | any[2] | any[3]);
+      probabilities(tile, which, s, prob);
+      add_values(buffer, which, prob, nan, place, v, keys);
+    };
+
     if (tiles > 0) store_values(tile0, 0);
     wait_loads<0>();
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       const int tile = tile0 + i, buffer = i & 1;
+      const v4i place = places[lane];
       if constexpr (waves_per_simd<D>() > 1) {
         if (turn < late) __builtin_amdgcn_s_setprio(1);
         else __builtin_amdgcn_s_setprio(0);
@@ -357,8 +389,9 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       }
       if (active && tile * kTile < hi_max && tile * kTile + kTile > lo_min) {
         int nan = 0;
-        multiply(tile, buffer, Index<0>{}, nan);
-        multiply(tile, buffer, Index<1>{}, nan);
+        Keys keys;
+        half_tile(tile, buffer, Index<0>{}, nan, place, keys);
+        half_tile(tile, buffer, Index<1>{}, nan, place, keys);
       }
       if (i + 1 < tiles) store_values(tile + 1, buffer ^ 1);
       wait_loads<0>();
