@@ -17,22 +17,33 @@
 namespace ave {
 namespace {
 
-// Eight consecutive elements from any address of their type.
+// Eight consecutive elements, as they are: from any address of their type unless ALIGNED says 16 bytes
 template <typename T>
-__device__ inline void load8(const T* p, float (&v)[8]) {
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    constexpr int V = (int)sizeof(T) / 2;
-    v4i raw[V];
+struct Eight {
+  v4i raw[sizeof(T) / 2];
+};
+template <bool ALIGNED, typename T>
+__device__ inline Eight<T> load8(const T* p) {
+  Eight<T> r;
+  if (ALIGNED || (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) raw[q] = reinterpret_cast<const v4i*>(p)[q];
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q) r.raw[q] = reinterpret_cast<const v4i*>(p)[q];
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (sizeof(T) == 4) v[j] = __builtin_bit_cast(float, (int)raw[j / 4][j % 4]);
-      else v[j] = __builtin_bit_cast(float, j % 2 ? (unsigned)raw[0][j / 2] & 0xFFFF0000u : (unsigned)raw[0][j / 2] << 16);
-    }
+    for (int j = 0; j < 8; ++j) r.raw[j / 4][j % 4] = reinterpret_cast<const int*>(p)[j];
   } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)p[j];
+    for (int j = 0; j < 4; ++j) r.raw[0][j] = (int)((unsigned)h[2 * j] | (unsigned)h[2 * j + 1] << 16);
+  }
+  return r;
+}
+template <typename T>
+__device__ inline void unpack(const Eight<T>& r, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (sizeof(T) == 4) v[j] = __builtin_bit_cast(float, (int)r.raw[j / 4][j % 4]);
+    else v[j] = __builtin_bit_cast(float, j % 2 ? (unsigned)r.raw[0][j / 2] & 0xFFFF0000u : (unsigned)r.raw[0][j / 2] << 16);
   }
 }
 
@@ -46,16 +57,33 @@ __device__ inline void store8_bf16(uint16_t* p, const float (&v)[8]) {
   }
 }
 
-// D / 8 lanes share a head, eight channels each; a workgroup has 2048 / D heads of one token (blockIdx.x) under way and takes the
-// token's heads -- queries, keys, values -- gridDim.y such groups apart.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int all_heads, int page_shift) {
+// D / 8 lanes share a head, eight channels each; a workgroup has 2048 / D heads of one token side by side, and `each` (at most kEach) such
+// groups -- queries, then keys, then values -- under way at once: what bounds a prompt is how many bytes are.  Neighbouring tokens go to
+// one XCD, whose L2 puts their pieces of a cache line together.
+constexpr int kEach = 4;
+
+template <typename T, int D, bool ALIGNED>
+__global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int all_heads, int each, int page_shift) {
   constexpr int L = D / 8;
-  const int token = blockIdx.x, lane = threadIdx.x % L, c0 = lane * 8;
+  const int token = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8, lane = threadIdx.x % L, c0 = lane * 8;
+  if (token >= p.tokens) return;
+  const int h0 = blockIdx.y * each * (256 / L) + threadIdx.x / L;
+  Eight<T> raw[kEach];
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int h = h0 + u * (256 / L);
+    if (u >= each || h >= all_heads) continue;
+    const bool is_q = h < q_heads, is_v = p.v.data && h >= q_heads + p.k.heads;
+    const int head = is_q ? h : is_v ? h - q_heads - p.k.heads : h - q_heads;
+    const void* data = is_q ? p.q.data : is_v ? p.v.data : p.k.data;
+    const int64_t token_stride = is_q ? p.q.token_stride : is_v ? p.v.token_stride : p.k.token_stride;
+    const int64_t head_stride = is_q ? p.q.head_stride : is_v ? p.v.head_stride : p.k.head_stride;
+    raw[u] = load8<ALIGNED>(static_cast<const T*>(data) + token * token_stride + head * head_stride + c0);
+  }
   const int half = p.how.rotary_dim / 2;
   const bool turned = p.how.cos && c0 < 2 * half;
   const bool upper = !p.how.neighbours && c0 >= half;      // this lane's channels are the second ones of their pairs
-  const int partner = p.how.neighbours ? c0 : (upper ? c0 - half : c0 + half);
+  const int partner = (threadIdx.x & 63) + (upper ? -half / 8 : half / 8);   // the lane that has the others
   float cs[8], sn[8];
   if (turned) {
     const int pos = p.how.positions[token];
@@ -65,42 +93,37 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int
 #pragma unroll
         for (int j = 0; j < 8; ++j) cs[j] = p.how.cos[row + c0 / 2 + j / 2], sn[j] = p.how.sin[row + c0 / 2 + j / 2];
       } else {
-        load8(p.how.cos + row + (upper ? c0 - half : c0), cs);
-        load8(p.how.sin + row + (upper ? c0 - half : c0), sn);
+        unpack(load8<false>(p.how.cos + row + (upper ? c0 - half : c0)), cs);
+        unpack(load8<false>(p.how.sin + row + (upper ? c0 - half : c0)), sn);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) cs[j] = sn[j] = __builtin_nanf("");
     }
   }
-  for (int h = blockIdx.y * (256 / L) + threadIdx.x / L; h < all_heads; h += gridDim.y * (256 / L)) {
+  const int slot = p.slots ? p.slots[token] : -1, page = slot >> page_shift;
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int h = h0 + u * (256 / L);
+    if (u >= each || h >= all_heads) continue;
     const bool is_q = h < q_heads, is_v = p.v.data && h >= q_heads + p.k.heads;
     const int head = is_q ? h : is_v ? h - q_heads - p.k.heads : h - q_heads;
-    const ave_fp4_heads& in = is_q ? p.q : is_v ? p.v : p.k;
-    const T* src = static_cast<const T*>(in.data) + token * in.token_stride + head * in.head_stride;
-    float x[8], y[8];
-    load8(src + c0, x);
+    float x[8];
+    unpack(raw[u], x);
     if (!is_v) {
-      if (turned && !p.how.neighbours) load8(src + partner, y);
       const void* weight = is_q ? p.how.q_weight : p.how.k_weight;
       if (weight) {
-        float s[8], w[8], wy[8];
+        float s[8], w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[j] = x[j] * x[j];
         float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 #pragma unroll
         for (int m = 1; m < L; m *= 2) sum += __shfl_xor(sum, m, 64);
         const float r = 1.0f / sqrtf(sum / (float)D + p.how.eps);
-        if (p.how.weight_is_f32) load8(static_cast<const float*>(weight) + c0, w);
-        else load8(static_cast<const __bf16*>(weight) + c0, w);
+        if (p.how.weight_is_f32) unpack(load8<false>(static_cast<const float*>(weight) + c0), w);
+        else unpack(load8<false>(static_cast<const __bf16*>(weight) + c0), w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = (x[j] * r) * w[j];
-        if (turned && !p.how.neighbours) {
-          if (p.how.weight_is_f32) load8(static_cast<const float*>(weight) + partner, wy);
-          else load8(static_cast<const __bf16*>(weight) + partner, wy);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = (y[j] * r) * wy[j];
-        }
       }
       if (turned) {
         if (p.how.neighbours) {
@@ -112,13 +135,17 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = upper ? x[j] * cs[j] + y[j] * sn[j] : x[j] * cs[j] - y[j] * sn[j];
+          for (int j = 0; j < 8; ++j) {
+            const float y = __shfl(x[j], partner, 64);
+            x[j] = upper ? x[j] * cs[j] + y * sn[j] : x[j] * cs[j] - y * sn[j];
+          }
         }
       }
     }
     if (is_q || (!is_v && p.k_out.data)) {
-      const ave_fp4_heads& out = is_q ? p.q_out : p.k_out;
-      store8_bf16(static_cast<uint16_t*>(out.data) + token * out.token_stride + head * out.head_stride + c0, x);
+      void* data = is_q ? p.q_out.data : p.k_out.data;
+      const int64_t token_stride = is_q ? p.q_out.token_stride : p.k_out.token_stride, head_stride = is_q ? p.q_out.head_stride : p.k_out.head_stride;
+      store8_bf16(static_cast<uint16_t*>(data) + token * token_stride + head * head_stride + c0, x);
     } else {
       const unsigned amax = lane_xor_max_bits(lane_xor_max_bits(abs_max_bits(x), 1), 2);   // four lanes share a block
       const int byte = mx_scale_byte(amax);
@@ -129,8 +156,6 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int
       codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
       codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
       if (byte == 0xFF) codes = 0u;
-      const int slot = p.slots[token];
-      const int page = slot >> page_shift;
       if (slot >= 0 && page < p.cache.pages) {
         const size_t row = (size_t)head * p.cache.page_size + (slot & (p.cache.page_size - 1));   // within the page
         uint8_t* c = (is_v ? p.cache.v + page * p.cache.v_page_stride : p.cache.k + page * p.cache.k_page_stride) + row * (D / 2);
@@ -147,9 +172,15 @@ hipError_t launch_heads_as(const HeadArgs& p, hipStream_t s) {
   const int q = p.q.data ? p.q.heads : 0, all = q + (p.k.data ? p.k.heads : 0) + (p.v.data ? p.v.heads : 0);
   const int groups = (all + 2048 / D - 1) / (2048 / D);
   if (p.tokens == 0 || all == 0) return hipSuccess;
-  // few tokens: a workgroup for every group of heads; many: one for every token, which loads its cosines once
-  const int y = p.tokens >= 1024 ? 1 : groups;
-  hipLaunchKernelGGL((heads_kernel<T, D>), dim3((unsigned)p.tokens, (unsigned)y), dim3(256), 0, s, p, q, all, log2_of(p.cache.page_size));
+  // few tokens: a workgroup for every group of heads; many: the fewest, which load their cosines once
+  const int want = (groups + kEach - 1) / kEach, each = p.tokens >= 1024 ? (groups + want - 1) / want : 1;
+  const auto wide = [](const ave_fp4_heads& h) {
+    return !h.data || ((reinterpret_cast<uintptr_t>(h.data) & 15) == 0 && h.token_stride * (int64_t)sizeof(T) % 16 == 0 && h.head_stride * (int64_t)sizeof(T) % 16 == 0);
+  };
+  const dim3 grid((unsigned)((p.tokens + 7) / 8 * 8), (unsigned)((groups + each - 1) / each));
+  const int shift = log2_of(p.cache.page_size);
+  if (wide(p.q) && wide(p.k) && wide(p.v)) hipLaunchKernelGGL((heads_kernel<T, D, true>), grid, dim3(256), 0, s, p, q, all, each, shift);
+  else hipLaunchKernelGGL((heads_kernel<T, D, false>), grid, dim3(256), 0, s, p, q, all, each, shift);
   return hipGetLastError();
 }
 
