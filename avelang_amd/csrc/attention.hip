@@ -13,10 +13,13 @@ AttnArgs args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
   return p;
 }
 
-// Row tiles of 16 of the kernel for few rows; 0: the kernel for prompts
+// Row tiles of 16 of the kernel for few rows; 0: the kernel for prompts.  Up to 32 rows the former is ahead (64 sequences of 4096 keys,
+// 8 new tokens, 32 query heads on 8 of 128: 87 us to 117), from 33 the latter (64 query heads: 310 to 166), but for single tokens on
+// one key head of 128 channels (48 query heads, 16 sequences of 16384 keys: 47 to 56 us, one of 131072: 67 to 106).
 int decode_row_tiles(const AttnArgs& p) {
-  const int64_t rows = (int64_t)(p.a.cu_q ? p.a.max_q : 1) * p.group;
-  const int most = p.c.head_dim == 256 ? 32 : 64;
+  const int new_tokens = p.a.cu_q ? p.a.max_q : 1;
+  const int64_t rows = (int64_t)new_tokens * p.group;
+  const int most = p.c.head_dim == 128 && new_tokens == 1 ? 64 : 32;
   return rows > most ? 0 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
 }
 

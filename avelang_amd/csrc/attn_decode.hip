@@ -490,7 +490,6 @@ hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s
   switch (p.c.head_dim * 8 + row_tiles) {
     case 64 * 8 + 1: return whole ? launch_form<64, 1, 8, 4>(p, whole, ws, s) : launch_form<64, 1, 4, 4>(p, whole, ws, s);
     case 64 * 8 + 2: return whole ? launch_form<64, 2, 8, 4>(p, whole, ws, s) : launch_form<64, 2, 4, 4>(p, whole, ws, s);
-    case 64 * 8 + 4: return launch_form<64, 4, 4, 4>(p, whole, ws, s);
     case 128 * 8 + 1: return whole ? launch_form<128, 1, 8, 2>(p, whole, ws, s) : launch_form<128, 1, 4, 2>(p, whole, ws, s);
     case 128 * 8 + 2: return whole ? launch_form<128, 2, 8, 2>(p, whole, ws, s) : launch_form<128, 2, 4, 2>(p, whole, ws, s);
     case 128 * 8 + 4: return launch_form<128, 4, 4, 4>(p, whole, ws, s);
@@ -559,18 +558,19 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS)
 
 template <int D>
 void launch_combine_of(const AttnArgs& p, int rows, int64_t expected, int workgroups, hipStream_t s) {
-  const unsigned x = (unsigned)workgroups - 1, at_once = 1024 / D;
-  if (rows <= 64)
-    hipLaunchKernelGGL((attn_combine_kernel<D, 1024 / D>), dim3(x, (unsigned)expected), dim3(256), 0, s, p, rows);
+  const unsigned x = (unsigned)workgroups - 1, at_once = 1024 / D, of_block = (unsigned)(expected < rows ? expected : rows);
+  const int64_t items = (int64_t)p.a.batch * p.c.kv_heads * ((expected + rows - 1) / rows);   // as far as the host knows
+  if (of_block <= 32 || workgroups >= 8 * items)
+    hipLaunchKernelGGL((attn_combine_kernel<D, 1024 / D>), dim3(x, of_block < 32 ? of_block : 32), dim3(256), 0, s, p, rows);
   else
-    hipLaunchKernelGGL((attn_combine_kernel<D, 1>), dim3(x, ((unsigned)expected + at_once - 1) / at_once), dim3(256), 0, s, p, rows);
+    hipLaunchKernelGGL((attn_combine_kernel<D, 1>), dim3(x, (of_block + at_once - 1) / at_once), dim3(256), 0, s, p, rows);
 }
 
 }  // namespace
 
 hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s) {
   if (workgroups < 2) return hipSuccess;
-  const int64_t expected = rows_expected < 1 ? 1 : rows_expected < rows ? rows_expected : rows;
+  const int64_t expected = rows_expected < 1 ? 1 : rows_expected;
   if (p.c.head_dim == 64) launch_combine_of<64>(p, rows, expected, workgroups, s);
   else if (p.c.head_dim == 128) launch_combine_of<128>(p, rows, expected, workgroups, s);
   else launch_combine_of<256>(p, rows, expected, workgroups, s);
