@@ -25,7 +25,9 @@ template <int D>
 struct Shape {
   static constexpr int kRow = D / 2, kBlocks = D / 32, kSteps = D / 64, C = D / 32;
   static constexpr int kKeys = kTile * kRow, kScales = kTile * kBlocks, kValues = kTile * D * 2;
-  static constexpr int kBuffer = kKeys + kScales, kLds = kBuffers * (kBuffer + kValues);   // keys' buffers, then values'
+  static constexpr int kFar = D == 256 ? 2 : 0;
+  static constexpr int kValueBuffers = D == 256 ? 1 : kBuffers;   // (two workgroups a compute unit)
+  static constexpr int kBuffer = kKeys + kScales, kLds = kBuffers * kBuffer + kValueBuffers * kValues;   // keys' buffers, then values'
   static constexpr int kThreadBytes = kTile * kRow / (kWaves * 64);   // of values' codes: 8, 16 or 32, within one or two blocks of a token
   // LDS positions.  Keys: 16-byte pieces permuted so that the 16 lanes of a read touch different banks.  Values: a row's 64-byte segments, and
   // the pieces of a segment, permuted by the token for the transposing reads (four tokens, 64 bytes each) and the writes.
@@ -63,7 +65,7 @@ __device__ inline T* lds_at(unsigned address) {
 // Waves of a SIMD, each of another workgroup: by registers
 template <int D>
 constexpr int waves_per_simd() {
-  return D == 64 ? 4 : D == 128 ? 3 : 1;
+  return D == 64 ? 4 : D == 128 ? 3 : 2;
 }
 
 // SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset.
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
   // key's scales, and by 32 channels the values
   // (k steps of 64 or 32 channels on they differ by an exclusive or alone).  They wait in LDS, as registers are short.
-  __shared__ __align__(16) v4i places[64];
+  __shared__ __align__(16) v4i places[64], far_q[2 * S::kFar + 1][S::kFar ? kWaves * 64 : 1];
   if (tid < 64) {
     const int t = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), r = lane % 16 / 4;   // r: token within four
     const unsigned key_at = lds + t * S::kRow + (h ^ S::key_swizzle(t)) * 16, scale_at = lds + S::kKeys + t * S::kBlocks;
@@ -180,7 +182,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     const auto store_values = [&](int tile, int buffer) {   // what no key occupies, and what has a NaN scale, is zero
       const int token = 16 * wave + lane / 4;
       const bool there = tile * kTile + token < it.s.len;
-      const unsigned at = lds + kBuffers * S::kBuffer + buffer * S::kValues + token * (2 * D) + ((lane % 4 * Values<D>::kWords) ^ S::value_swizzle(token)) * 16;
+      const unsigned at = lds + kBuffers * S::kBuffer + buffer % S::kValueBuffers * S::kValues + token * (2 * D) + ((lane % 4 * Values<D>::kWords) ^ S::value_swizzle(token)) * 16;
       uint64_t any = 0;
 #pragma unroll
       for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       request_values(tile0, page);
     }
     // ---- queries: lane (column col): bytes 0-15 of a step are k = 16 h .., bytes 16-31 k = 32 + 16 h ..
-    v8i q_hi[S::kSteps], q_lo[S::kSteps];
+    v8i q_hi[S::kSteps], q_lo[S::kSteps];   // (of q_lo the first kFar steps lie in LDS instead, as registers are short)
     int q_scale;   // of the first part; of the second in the next byte
     {
       const bool real = row < rows;
@@ -237,6 +239,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
 #pragma unroll
           for (int e = 0; e < 2; ++e) q_hi[i][2 * k + e] = hi[e] ^ sign, q_lo[i][2 * k + e] = lo[e] ^ sign;
         }
+#pragma unroll
+      for (int i = 0; i < S::kFar; ++i) far_q[2 * i][tid] = q_lo[i].lo, far_q[2 * i + 1][tid] = q_lo[i].hi;
       q_scale = s.hi_byte | s.lo_byte << 8;
     }
 
@@ -270,11 +274,13 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         const v4i x = f.code[k];
         const v8i x8 = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
         const int scale = (int)(f.scale[k / 2] >> shift);
+        v8i low = q_lo[k];
+        if (k < S::kFar) low.lo = far_q[2 * k][tid], low.hi = far_q[2 * k + 1][tid];
         if (k % 2 == 0) {
-          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 0, scale, 1, q_scale);
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, low, s, kFmtFp4, 0, 0, scale, 1, q_scale);
           s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 0, scale, 0, q_scale);
         } else {
-          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_lo[k], s, kFmtFp4, 0, 2, scale, 1, q_scale);
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, low, s, kFmtFp4, 0, 2, scale, 1, q_scale);
           s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, q_hi[k], s, kFmtFp4, 0, 2, scale, 0, q_scale);
         }
       }
@@ -327,7 +333,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       l += sum;
     };
     const auto add_values = [&](int buffer, auto which, const unsigned (&prob)[8], int nan, const v4i& place, v8bf (&v)[kAhead], Keys& keys) {
-      const unsigned at = place[2] + buffer * S::kValues;
+      const unsigned at = place[2] + buffer % S::kValueBuffers * S::kValues;
       constexpr int j = decltype(which)::value;
       // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
       if (nan) {
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       v16f s = scores(keys, place[3]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) v[n] = read_values(place[2] + buffer * S::kValues, j, n);
+      for (int n = 0; n < kAhead; ++n) v[n] = read_values(place[2] + buffer % S::kValueBuffers * S::kValues, j, n);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (j == 0) nan = uniform(any[0] | any[1] | any[2] | any[3]);
       probabilities(tile, which, s, prob);
@@ -393,6 +399,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         half_tile(tile, buffer, Index<0>{}, nan, place, keys);
         half_tile(tile, buffer, Index<1>{}, nan, place, keys);
       }
+      if constexpr (S::kValueBuffers == 1) __syncthreads();
       if (i + 1 < tiles) store_values(tile + 1, buffer ^ 1);
       wait_loads<0>();
       __syncthreads();
