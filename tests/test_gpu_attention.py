@@ -304,3 +304,64 @@ def test_nothing_to_do(gpu):
     assert ave.attention_mxfp4(q, cache, i(3, 1), i(3), i(4), max_q=2).shape == (0, 4, 64)
     q = torch.ones(2, 4, 64, dtype=torch.bfloat16, device=gpu)
     assert ave.attention_mxfp4(q, cache, i(2, 0), i(2) + 5).eq(0).all()      # a table without pages: no keys
+
+
+@pytest.mark.parametrize("heads", ["gqa64", "gqa128"])
+@pytest.mark.parametrize("count", [17, 65, 150])
+def test_many_sequences(gpu, heads, count):
+    """More sequences than a wave has lanes, empty ones among them; single tokens, then several each."""
+    rng = np.random.default_rng(count)
+    keys = rng.integers(0, 90, count)
+    keys[[0, count // 2, count - 1]] = 0, 89, 1
+    _check(gpu, A.Batch([(1, int(k)) for k in keys], *HEADS[heads], 16, seed=20))
+    _check(gpu, A.Batch([(int(rng.integers(0, 20)), int(k)) for k in keys], *HEADS[heads], 16, seed=21))
+
+
+@pytest.mark.parametrize("heads", ["gqa64", "gqa128", "gqa256"])
+@pytest.mark.parametrize("rows", [[(1, 2500)], [(9, 2500), (1, 10)], [(40, 2500)]], ids=str)
+def test_maxima_that_climb(gpu, heads, rows):
+    """Keys that grow towards the sequence's end: what is subtracted from the scores has to follow, again and again."""
+    hq, hkv, d = HEADS[heads]
+    batch = A.Batch(rows, hq, hkv, d, 32, seed=22)
+    for b, (_, keys) in enumerate(rows):
+        for j in range(keys):
+            page, at = batch.place(b, j)
+            up = j // 250
+            batch.cache[1][page, :, at] += up
+            batch.k[b][j] *= 2.0 ** up
+    _check(gpu, batch, scale=d ** -0.5 / 16)
+
+
+@pytest.mark.parametrize("heads", ["gqa64", "gqa128", "gqa256"])
+def test_few_blocks_of_many_parts(gpu, heads):
+    """One block of rows over a long cache: its keys are shared by many workgroups; one row, a few, more than a block."""
+    for new in (1, 6, 40):
+        _check(gpu, A.Batch([(new, 6000)], *HEADS[heads], 256, seed=23 + new))
+    batch = A.Batch([(33, 3001)], *HEADS[heads], 64, seed=24)
+    _check(gpu, batch, window=2200, sinks=batch.sinks)
+
+
+def test_prompts_beyond_32_bit_offsets(gpu):
+    batch = A.Batch([(60, 170), (1, 20)], 4, 2, 128, 64, seed=25, spare=0)
+    t, out = _check(gpu, batch)
+    gap = (1 << 31) + 4096
+    buf = torch.zeros((t["cache"][0].shape[0] - 1) * gap + (1 << 20), dtype=torch.uint8, device=gpu)
+    cache, at = [], 0
+    for c in t["cache"]:
+        view = buf[at:].as_strided(tuple(c.shape), (gap, *c.stride()[1:]))
+        view.copy_(c)
+        cache.append(view)
+        at += c[0].numel()
+    got = ave.attention_mxfp4(t["q"], tuple(cache), t["page_table"], t["seq_lens"], t["cu_q"], max_q=60)
+    assert torch.equal(got, out)
+
+
+def test_untrusted_prompts_stay_inside_the_cache(gpu):
+    """The same as for single tokens: lengths, pages and row ranges that do not fit; the sequence that does is untouched."""
+    batch = A.Batch([(40, 90), (50, 60), (20, 40)], 4, 2, 64, 16, seed=26)
+    t, out = _check(gpu, batch)
+    lens, table = t["seq_lens"].clone(), t["page_table"].clone()
+    lens[0], lens[2] = 2 ** 31 - 1, -5
+    table[0, 2], table[0, 3] = -1, 2 ** 31 - 1
+    got = ave.attention_mxfp4(t["q"], t["cache"], table, lens, t["cu_q"], max_q=50)
+    assert torch.equal(got[40:90], out[40:90]) and got[90:].eq(0).all()
