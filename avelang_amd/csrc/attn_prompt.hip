@@ -397,7 +397,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         int nan = 0;
         Keys keys;
         half_tile(tile, buffer, Index<0>{}, nan, place, keys);
-        half_tile(tile, buffer, Index<1>{}, nan, place, keys);
+        if (tile * kTile + 32 < hi_max) half_tile(tile, buffer, Index<1>{}, nan, place, keys);
       }
       if constexpr (S::kValueBuffers == 1) __syncthreads();
       if (i + 1 < tiles) store_values(tile + 1, buffer ^ 1);
