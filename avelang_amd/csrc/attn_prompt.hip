@@ -450,7 +450,7 @@ size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p
 hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   const int workgroups = workgroups_of(p);
   p.whole = 0;
-  p.item_units = 2;
+  p.item_units = p.c.head_dim == 64 ? 2 : 3;
   p.min_units_log2 = 2;
   p.few_long = p.a.batch <= 16;
   place_workspace(p, kRows, workgroups, ws);
