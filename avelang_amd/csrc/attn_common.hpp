@@ -283,11 +283,8 @@ __device__ inline unsigned lds_address(const void* p) {
 // A barrier that orders LDS and leaves loads to LDS under way
 __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Page of tokens 16 i .. 16 i + 15 of a sequence (tokens behind the last key: the last key's): what the table holds, and a valid one of that
-__device__ inline int page_entry(const AttnArgs& p, ConstInts row, int token, int len) {
-  const int t = token < len ? token : len > 0 ? len - 1 : 0;
-  return p.a.table_pages > 0 ? row[t >> p.page_shift] : 0;
-}
+// Page of tokens 16 i .. 16 i + 15 of a sequence of len > 0 keys (behind the last: the last one's): what the table holds, and a valid one of that
+__device__ inline int page_entry(const AttnArgs& p, ConstInts row, int token, int len) { return row[(token < len ? token : len - 1) >> p.page_shift]; }
 __device__ inline int page_of(const AttnArgs& p, int entry) {
   const int page = entry < 0 ? 0 : entry;
   return page < p.c.pages ? page : p.c.pages - 1;

@@ -93,6 +93,11 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     places[lane] = v4i{(int)key_at, (int)scale_at, (int)value_at, 8 * h};
   }
   __syncthreads();
+  const auto lane_here = [&] {   // for what is derived from the lane where it is used, and not kept in registers all the time
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
@@ -129,7 +134,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
     // what this wave's rows see: [lo_max, hi_min) all of them, [lo_min, hi_max) any
-    const int row0 = uniform(it.row0 + 32 * wave), row = row0 + col;
+    const int row0 = uniform(it.row0 + 32 * wave);
     const bool active = row0 < uniform(rows);
     int lo_max, hi_min, lo_min, hi_max;
     visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
@@ -180,14 +185,14 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       next.scales = *reinterpret_cast<const unsigned*>(base + off);
     };
     const auto store_values = [&](int tile, int buffer) {   // what no key occupies, and what has a NaN scale, is zero
-      const int token = 16 * wave + lane / 4;
+      const int here = lane_here(), token = 16 * wave + here / 4;
       const bool there = tile * kTile + token < it.s.len;
-      const unsigned at = lds + kBuffers * S::kBuffer + buffer % S::kValueBuffers * S::kValues + token * (2 * D) + ((lane % 4 * Values<D>::kWords) ^ S::value_swizzle(token)) * 16;
+      const unsigned at = lds + kBuffers * S::kBuffer + buffer % S::kValueBuffers * S::kValues + token * (2 * D) + ((here % 4 * Values<D>::kWords) ^ S::value_swizzle(token)) * 16;
       uint64_t any = 0;
 #pragma unroll
       for (int k = 0; k < Values<D>::kScaleBytes; ++k) {
         constexpr int kOfScale = Values<D>::kWords / Values<D>::kScaleBytes;
-        const unsigned scale = next.scales >> (Values<D>::shift(lane) + 8 * k) & 255;
+        const unsigned scale = next.scales >> (Values<D>::shift(here) + 8 * k) & 255;
         const bool bad = there && scale >= 253, none = bad || !there;
         const float f = __builtin_bit_cast(float, none ? 0x3F800000u : scale << 23);
 #pragma unroll
@@ -204,30 +209,44 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       if (lane == 0) nan_any[buffer][wave] = any != 0;
     };
 
-    // ---- the first requests, then the queries, whose way is as long
-    int entry = entry_of(tile0 + 1);
-    if (tiles > 0) {
-      const int page = page_of(p, entry_of(tile0));
-      request_keys(tile0, page, 0);
-      request_values(tile0, page);
-    }
-    // ---- queries: lane (column col): bytes 0-15 of a step are k = 16 h .., bytes 16-31 k = 32 + 16 h ..
+    // ---- the queries' loads, then the first requests.  Queries: lane (column lane % 32): bytes 0-15 of a step are k = 16 h .., bytes 16-31
+    // k = 32 + 16 h ..
+    int entry = tiles > 0 ? entry_of(tile0 + 1) : 0;
     v8i q_hi[S::kSteps], q_lo[S::kSteps];   // (of q_lo the first kFar steps lie in LDS instead, as registers are short)
     int q_scale;   // of the first part; of the second in the next byte
     {
+      const int first_entry = tiles > 0 ? entry_of(tile0) : 0, here = lane_here(), row = row0 + here % 32;
       const bool real = row < rows;
       const int t = real ? p.token_of(row) : 0, query_head = it.head * p.group + (real ? row - t * p.group : 0);
-      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)query_head * p.a.q_head_stride;
+      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)query_head * p.a.q_head_stride + here / 32 * 16;
       v4i x[S::kSteps][4];
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[i][k] = v4i{0, 0, 0, 0};
+      if (real) {
+        if (p.q_aligned) {
+#pragma unroll
+          for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[i][k] = load8_bf16(q + 64 * i + 32 * (k / 2) + 8 * (k % 2), true);
+        } else {
+#pragma unroll
+          for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[i][k] = load8_bf16(q + 64 * i + 32 * (k / 2) + 8 * (k % 2), false);
+        }
+      }
+      if (tiles > 0) {
+        const int page = page_of(p, first_entry);
+        request_keys(tile0, page, 0);
+        request_values(tile0, page);
+      }
       us2 m = {0, 0};
 #pragma unroll
       for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[i][k] = v4i{0, 0, 0, 0};
-          if (real) x[i][k] = load8_bf16(q + 64 * i + 32 * (k / 2) + 16 * h + 8 * (k % 2), p.q_aligned);
-          m = amax_pairs(x[i][k], m);
-        }
+        for (int k = 0; k < 4; ++k) m = amax_pairs(x[i][k], m);
       const QueryScale s = query_scale(lane_xor_max_bits(larger_half(m), 32));
       const int sign = p.a.scale < 0.0f ? (int)0x80808080u : 0;
 #pragma unroll
@@ -300,8 +319,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       constexpr int j = decltype(which)::value;
       const int key0 = tile * kTile + 32 * j;
       if (key0 < lo_max || key0 + 32 > hi_min) {
-        int here = lane, lo, hi;
-        asm volatile("" : "+v"(here));   // here, and not in registers all the time
+        const int here = lane_here();
+        int lo, hi;
         visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);   // (a row behind the last: whatever)
         const int from = lo - key0 - here / 32 * 16;
         const unsigned many = (unsigned)(hi > lo ? hi - lo : 0);
@@ -405,25 +424,32 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       __syncthreads();
     }
 
-    // ---- results: lane (column col) has channels 32 k + 8 i + 4 h .. + 3 of its row
+    // ---- results: lane (column lane % 32) has channels 32 k + 8 i + 4 (lane / 32) .. + 3 of its row
     if (active) {
       const float sum = cross_sum<false>(l), m2 = m == kNoMax ? -INFINITY : m;
       const bool done = from == it.begin && to == end;
+      const int here = lane_here(), row = row0 + here % 32, ch0 = here / 32 * 4;
       if (row < rows) {
-        const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + 32 * wave + col;
-        const size_t place = row_index(p, it.s.first, it.head, row);
-        const RowEnd e = row_end(sink_of(p, it.head * p.group + (row - p.token_of(row) * p.group)), m2, sum);
-        if (done && p.a.lse && h == 0) p.a.lse[place] = e.lse;
+        if (done) {
+          const size_t place = row_index(p, it.s.first, it.head, row);
+          const RowEnd e = row_end(sink_of(p, it.head * p.group + (row - p.token_of(row) * p.group)), m2, sum);
+          if (p.a.lse && ch0 == 0) p.a.lse[place] = e.lse;
+          uint16_t* out = p.a.out + place * D + ch0;
 #pragma unroll
-        for (int k = 0; k < C; ++k)
+          for (int k = 0; k < C; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const v4f o = {acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]};
-            const int ch = 32 * k + 8 * i + 4 * h;
-            if (done) store4_bf16(p.a.out + place * D + ch, o * e.factor);
-            else *reinterpret_cast<v4f*>(p.part_o + at * D + ch) = o;
-          }
-        if (!done && h == 0) p.part_ml[at * 2] = m2, p.part_ml[at * 2 + 1] = sum;
+            for (int i = 0; i < 4; ++i)
+              store4_bf16(out + 32 * k + 8 * i, v4f{acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]} * e.factor);
+        } else {
+          const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + (row - it.row0);
+          float* out = p.part_o + at * D + ch0;
+#pragma unroll
+          for (int k = 0; k < C; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<v4f*>(out + 32 * k + 8 * i) = v4f{acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]};
+          if (ch0 == 0) p.part_ml[at * 2] = m2, p.part_ml[at * 2 + 1] = sum;
+        }
       }
     }
   }
@@ -452,7 +478,7 @@ hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   p.whole = 0;
   p.item_units = p.c.head_dim == 64 ? 2 : 3;
   p.min_units_log2 = 2;
-  p.few_long = p.a.batch <= 16;
+  p.few_long = p.a.batch <= 8;
   place_workspace(p, kRows, workgroups, ws);
   if (p.c.head_dim == 64) launch<64>(p, workgroups, s);
   else if (p.c.head_dim == 128) launch<128>(p, workgroups, s);
