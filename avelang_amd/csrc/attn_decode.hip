@@ -473,20 +473,25 @@ hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
   return launch_attn_combine(p, ROWS, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
 }
 
-// Items of at most 1024 keys stay whole: cutting them saves less than the second launch costs.
-bool keep_whole(const AttnArgs& p) {
+// Short items stay whole: one launch, no partial results.  Cut in parts they cost a second launch and 128 bytes of partial results for each
+// row and 32 channels; whole they keep one workgroup each busy, which matters where there are few of them.  32 query heads on 8 of 128, one
+// sequence: single tokens 500 keys 9.6 us whole, 11.3 cut, 1500 keys 13.2 and 11.3; 8 tokens 13.7 and 16.8, 20.7 and 16.6; of 256 channels 500
+// keys 23.1 and 22.0.  16 sequences, 8 tokens, 1500 keys: 22.5 and 28.9, of 64 channels 17.5 and 28.9, of 256 45.0 and 39.8; 64 sequences of
+// 1500, single tokens: 30.9 and 27.3.  The bound on an item's keys is what the page table or the window can hold.
+bool keep_whole(const AttnArgs& p, int row_tiles) {
   const int64_t in_table = (int64_t)p.a.table_pages << p.page_shift, in_window = p.a.window > 0 ? (int64_t)p.a.window + p.a.max_q : in_table;
-  return (in_window < in_table ? in_window : in_table) <= 1024;
+  const bool many = 2 * (int64_t)p.a.batch * p.c.kv_heads >= compute_units() && (row_tiles > 1 || p.c.head_dim == 64);
+  return (in_window < in_table ? in_window : in_table) <= (p.c.head_dim == 256 ? 512 : 1024) * (many ? 2 : 1);
 }
 
 }  // namespace
 
 size_t attn_decode_workspace(const AttnArgs& p, int row_tiles) {
-  return keep_whole(p) ? 0 : attn_workspace(row_tiles * 16, p.c.head_dim, 2 * compute_units());
+  return keep_whole(p, row_tiles) ? 0 : attn_workspace(row_tiles * 16, p.c.head_dim, 2 * compute_units());
 }
 
 hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s) {
-  const bool whole = keep_whole(p);
+  const bool whole = keep_whole(p, row_tiles);
   switch (p.c.head_dim * 8 + row_tiles) {
     case 64 * 8 + 1: return whole ? launch_form<64, 1, 8, 4>(p, whole, ws, s) : launch_form<64, 1, 4, 4>(p, whole, ws, s);
     case 64 * 8 + 2: return whole ? launch_form<64, 2, 8, 4>(p, whole, ws, s) : launch_form<64, 2, 4, 4>(p, whole, ws, s);

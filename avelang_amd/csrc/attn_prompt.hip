@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
 
     // ---- 32 keys, half j of a tile.  What the matrix instructions take out of LDS is read ahead of them, by hand: the compiler, short of
     // registers, waits for each piece.
-    constexpr int kAhead = D == 64 ? 2 : 3;   // fragments of values on their way
+    constexpr int kAhead = 3;   // fragments of values on their way
     struct Keys {
       v4i code[S::kSteps];
       unsigned scale[(S::kBlocks + 3) / 4];
