@@ -9,7 +9,19 @@
 //   O^T = V^T P^T bf16 MFMA 32x32x16: P goes from the result's registers into the operand as it is, rounded to bf16.  Values are converted once
 //                 a workgroup, codes times their scales (exact), and lie in LDS as bf16 rows that transposing reads hand out by columns.
 //
-// The next 64 keys and values are requested before the present ones are multiplied; two workgroups a compute unit.
+// What a wave does for 64 keys: 8 scaled and 16 bf16 MFMAs at 128 channels (about 1090 cycles), and beside them 32 each of fma, exponential
+// and addition a lane, 16 conversions of P, a quarter of a tile's values converted, requests and addresses (about 950).  Scores, exponentials and
+// values come one after the other; three waves a SIMD (four at 64 channels, two at 256), each of another workgroup and at another point, put
+// the ones under the others.  That measured faster than two waves with the three interleaved by hand (677 us against 642, 8192 tokens, 32 heads on
+// 8 of 128) and than 64 rows a wave in 512 registers (1354: one wave issues an instruction in five cycles).  What then counted:
+//   - nobody waits between the requests for the next tile and the products (scales unpacked and table entries checked where they are used, lane
+//     constants in LDS instead of spilled: 642 -> 609);
+//   - equal ends: workgroups of a compute unit take turns in going first, and an item's start and end count as tiles (609 -> 537);
+//   - LDS reads ahead of the products (four long sequences: 348 -> 332); half tiles that nobody sees skipped (533 -> 515).
+// 8192 tokens, 32 heads on 8 of 128: 488 us, 1.13 PFLOP/s of 4 D flop a score (the matrix cores also multiply the queries' second part, half as much
+// again); 4 sequences of up to 16000 keys, 600 new tokens, 40 heads on 8: 320 us,
+// 1.10 PFLOP/s; six prompts of about 1000 tokens, 64 heads on 8 of 64: 87 us, where an
+// item of 128 rows has but 8 tiles for its start and end, and half the work is exponentials.
 #include "attn_common.hpp"
 #include "kernels.hpp"
 
@@ -62,13 +74,14 @@ __device__ inline T* lds_at(unsigned address) {
   return (T*)(uintptr_t)address;
 }
 
-// Waves of a SIMD, each of another workgroup: by registers
+// Waves of a SIMD, each of another workgroup: by registers (a wave's sums are D / 2 of them, its queries D / 4)
 template <int D>
 constexpr int waves_per_simd() {
   return D == 64 ? 4 : D == 128 ? 3 : 2;
 }
 
-// SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset.
+// SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 133 us, with 64-bit
+// bases for every tile 141).
 template <int D, bool SMALL>
 __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
@@ -105,8 +118,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     int* m = p.meta + (size_t)g * kMeta;
     m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
   }
-  // Among waves that could issue, the oldest goes first, and with equal parts the workgroups that a compute unit got last would end long
-  // after the others.  Each takes its turn before the rest, a tile at a time.
+  // Among waves that could issue, the oldest goes first, so that of equal parts the workgroups that a compute unit got last would end
+  // long after the others (452 us the first, 677 the last).  The later a workgroup came, the more of its tiles it takes at a higher priority.
   const int late = blockIdx.x * waves_per_simd<D>() / gridDim.x;
   int turn = 0;
   bool first_item = true;
@@ -476,9 +489,9 @@ size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p
 hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   const int workgroups = workgroups_of(p);
   p.whole = 0;
-  p.item_units = p.c.head_dim == 64 ? 2 : 3;
+  p.item_units = p.c.head_dim == 64 ? 2 : 3;   // (8192 tokens, 128 channels: with 1 674 us, 2 647, 3 and 4 633; prompts of 400, 64 channels: 2 80, 4 83)
   p.min_units_log2 = 2;
-  p.few_long = p.a.batch <= 8;
+  p.few_long = p.a.batch <= 8;   // (6 prompts of 1000: 135 us so, 142 otherwise; 16 of 500: 112 and 106)
   place_workspace(p, kRows, workgroups, ws);
   if (p.c.head_dim == 64) launch<64>(p, workgroups, s);
   else if (p.c.head_dim == 128) launch<128>(p, workgroups, s);
