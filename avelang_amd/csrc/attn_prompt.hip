@@ -328,7 +328,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     // Probabilities from scores.  Any reference will do that keeps them in range, so the scores' maximum is looked for only where a lane's
     // sixteen come to more than 2^8 (the first ones that a row sees: to infinity): up to there they have the same relative error, and most
     // steps go without.
-    const auto probabilities = [&](int tile, auto which, v16f& s, unsigned (&prob)[8]) {
+    const auto probabilities = [&](int tile, auto which, bool first, v16f& s, unsigned (&prob)[8]) {   // first: of the item
       constexpr int j = decltype(which)::value;
       const int key0 = tile * kTile + 32 * j;
       if (key0 < lo_max || key0 + 32 > hi_min) {
@@ -352,8 +352,12 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
           asm volatile("" : "+v"(prob[t]));   // here, not where it is used
         }
       };
-      exponentials(m);
-      if (const bool over = !(sum <= 256.0f); __any(over)) {   // a row by itself: what others hold leaves it as it is
+      bool over = true;
+      if (!first) {
+        exponentials(m);
+        over = !(sum <= 256.0f);
+      }
+      if (__any(over)) {   // a row by itself: what others hold leaves it as it is
         const float top = cross_max<false>(largest_of<0, 15>(s, kNone)), to_row = fmaxf(m, top > 0.5f * kNone ? top * c : kNoMax);
         const float to = cross_max<false>(over ? 1.0f : 0.0f) != 0.0f ? to_row : m, fade = __builtin_amdgcn_exp2f(m - to);
         l *= fade;
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    const auto half_tile = [&](int tile, int buffer, auto which, int& nan, const v4i& place, Keys& keys) {
+    const auto half_tile = [&](int tile, int buffer, auto which, bool first, int& nan, const v4i& place, Keys& keys) {
       constexpr int j = decltype(which)::value;
       v8bf v[kAhead];
       unsigned prob[8];
@@ -404,7 +408,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       for (int n = 0; n < kAhead; ++n) v[n] = read_values(place[2] + buffer % S::kValueBuffers * S::kValues, j, n);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (j == 0) nan = uniform(any[0] | any[1] | any[2] | any[3]);
-      probabilities(tile, which, s, prob);
+      probabilities(tile, which, first, s, prob);
       add_values(buffer, which, prob, nan, place, v, keys);
     };
 
@@ -428,8 +432,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       if (active && tile * kTile < hi_max && tile * kTile + kTile > lo_min) {
         int nan = 0;
         Keys keys;
-        half_tile(tile, buffer, Index<0>{}, nan, place, keys);
-        if (tile * kTile + 32 < hi_max) half_tile(tile, buffer, Index<1>{}, nan, place, keys);
+        half_tile(tile, buffer, Index<0>{}, i == 0, nan, place, keys);
+        if (tile * kTile + 32 < hi_max) half_tile(tile, buffer, Index<1>{}, false, nan, place, keys);
       }
       if constexpr (S::kValueBuffers == 1) __syncthreads();
       if (i + 1 < tiles) store_values(tile + 1, buffer ^ 1);

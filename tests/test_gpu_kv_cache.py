@@ -204,3 +204,28 @@ def test_no_tokens(gpu):
     assert ave.append_kv_mxfp4(none, none, cache, slots, q=none).shape == (0, 2, 64)
     assert ave.gather_kv_mxfp4(cache, slots)[0].shape == (0, 2, 64)
     assert ave.qk_norm_rope(none, none)[1].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,d,rot", [(70, 9, 128, 96), (131, 3, 64, 64), (20, 3, 256, 256), (33, 8, 256, 32)])
+def test_many_heads_of_many_tokens(gpu, hq, hkv, d, rot, dtype):
+    """Several groups of heads in a workgroup, the last one not full; a token count that no eight divides; then from an odd address."""
+    t = 1029
+    dev, q, k, v = _case(gpu, t, hq, hkv, d, rot, True, False, dtype, seed=d + hq)
+    slots = torch.randperm(1040, generator=torch.Generator().manual_seed(1))[:t].int().to(gpu)
+    args = (dev["cos"], dev["sin"], dev["positions"], dev["k_weight"])
+    caches = []
+    for shift in (0, 1):
+        wide = torch.zeros(t * (hq + 2 * hkv) * d + 8, dtype=dtype, device=gpu)
+        x = wide[shift:shift + t * (hq + 2 * hkv) * d].view(t, hq + 2 * hkv, d)
+        x.copy_(torch.cat([dev["q"], dev["k"], dev["v"]], 1))
+        cache = ave.kv_cache_mxfp4(65, hkv, 16, d, gpu)
+        q_out = ave.append_kv_mxfp4(x[:, hq:hq + hkv], x[:, hq + hkv:], cache, slots, *args, q=x[:, :hq], q_weight=dev["q_weight"], eps=A.EPS)
+        assert np.array_equal(_bits(q_out), orc.f32_to_bf16_bits(q))
+        caches.append(cache)
+    assert all(torch.equal(a, b) for a, b in zip(*caches))
+    at = slots.cpu().numpy()
+    for i, x in enumerate((k, v)):
+        codes, scale = orc.quantize_mxfp4(x.reshape(t * hkv, d))
+        assert np.array_equal(caches[0][2 * i].cpu().numpy()[at // 16, :, at % 16], codes.reshape(t, hkv, -1))
+        assert np.array_equal(caches[0][2 * i + 1].cpu().numpy()[at // 16, :, at % 16], scale.reshape(t, hkv, -1))
