@@ -66,9 +66,11 @@ struct Index {
 
 typedef __attribute__((address_space(3))) v4i LdsInt4;
 typedef __attribute__((address_space(3))) unsigned LdsInt;
+typedef __attribute__((address_space(3))) v2i LdsInt2;
 typedef __attribute__((address_space(3))) uint16_t LdsShort;
 typedef __attribute__((address_space(3))) v4s LdsShort4;
 typedef __attribute__((address_space(3))) v8bf Lds8Bf16;
+typedef int Loose4 __attribute__((ext_vector_type(4), aligned(4)));   // (results are aligned to 4 bytes)
 template <typename T>
 __device__ inline T* lds_at(unsigned address) {
   return (T*)(uintptr_t)address;
@@ -442,33 +444,49 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     }
 
     // ---- results: lane (column lane % 32) has channels 32 k + 8 i + 4 (lane / 32) .. + 3 of its row
+    const bool done = from == it.begin && to == end;
     if (active) {
       const float sum = cross_sum<false>(l), m2 = m == kNoMax ? -INFINITY : m;
-      const bool done = from == it.begin && to == end;
       const int here = lane_here(), row = row0 + here % 32, ch0 = here / 32 * 4;
-      if (row < rows) {
-        if (done) {
-          const size_t place = row_index(p, it.s.first, it.head, row);
+      const bool real = row < rows;
+      if (done) {   // by way of LDS, whose values nobody needs any more, so that whole rows are stored (16 bytes a row at a time: 6000 cycles an item)
+        float factor = 0.0f;
+        if (real) {
           const RowEnd e = row_end(sink_of(p, it.head * p.group + (row - p.token_of(row) * p.group)), m2, sum);
-          if (p.a.lse && ch0 == 0) p.a.lse[place] = e.lse;
-          uint16_t* out = p.a.out + place * D + ch0;
-#pragma unroll
-          for (int k = 0; k < C; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              store4_bf16(out + 32 * k + 8 * i, v4f{acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]} * e.factor);
-        } else {
-          const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + (row - it.row0);
-          float* out = p.part_o + at * D + ch0;
-#pragma unroll
-          for (int k = 0; k < C; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<v4f*>(out + 32 * k + 8 * i) = v4f{acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]};
-          if (ch0 == 0) p.part_ml[at * 2] = m2, p.part_ml[at * 2 + 1] = sum;
+          if (p.a.lse && ch0 == 0) p.a.lse[row_index(p, it.s.first, it.head, row)] = e.lse;
+          factor = e.factor;
         }
+        constexpr int kWide = D < 128 ? D : 128, kPieces = kWide / 8, kAtOnce = 64 / kPieces;   // channels at a time, 16-byte pieces of them, rows of a store
+        const unsigned own = lds + kBuffers * S::kBuffer + wave * (32 * 2 * kWide);
+#pragma unroll
+        for (int wide = 0; wide < D / kWide; ++wide) {
+#pragma unroll
+          for (int k = 0; k < kWide / 32; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const v16f& a = acc[wide * (kWide / 32) + k];
+              *lds_at<LdsInt2>(own + here % 32 * (2 * kWide) + ((4 * k + i) ^ (here % kPieces)) * 16 + ch0 * 2) =
+                  v2i{(int)pack_bf16x2(a[4 * i] * factor, a[4 * i + 1] * factor), (int)pack_bf16x2(a[4 * i + 2] * factor, a[4 * i + 3] * factor)};
+            }
+#pragma unroll
+          for (int n = 0; n < 32 / kAtOnce; ++n) {
+            const int r = n * kAtOnce + here / kPieces;
+            const v4i x = *lds_at<const LdsInt4>(own + r * (2 * kWide) + ((here % kPieces) ^ (r % kPieces)) * 16);
+            if (row0 + r < rows) *reinterpret_cast<Loose4*>(p.a.out + row_index(p, it.s.first, it.head, row0 + r) * D + wide * kWide + here % kPieces * 8) = x;
+          }
+        }
+      } else if (real) {
+        const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + (row - it.row0);
+        float* out = p.part_o + at * D + ch0;
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<v4f*>(out + 32 * k + 8 * i) = v4f{acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]};
+        if (ch0 == 0) p.part_ml[at * 2] = m2, p.part_ml[at * 2 + 1] = sum;
       }
     }
+    if (done) __syncthreads();   // before the next item's values
   }
 }
 
