@@ -82,6 +82,34 @@ constexpr int waves_per_simd() {
   return D == 64 ? 4 : D == 128 ? 3 : 2;
 }
 
+// Whole items in falling order, for calls of up to 64 sequences.  Level k has the k-th last block of each sequence and key head that has so many;
+// items are numbered level by level (by sequence, then head, within one), so that causal ones, which have fewer keys the earlier their rows
+// stand, come largest first.  `all` is a table of the sequences in LDS, {first, n, len, blocks}; every lane of the wave takes part.
+__device__ inline unsigned items_below(const v4i* all, unsigned level, unsigned heads) {   // of levels below
+  const unsigned blocks = (unsigned)all[threadIdx.x & 63][3];
+  return heads * (unsigned)lane_value((int)wave_scan(blocks < level ? blocks : level), 63);
+}
+template <int ROWS>
+__device__ inline Item ranked_item(const AttnArgs& p, const v4i* all, unsigned rank, int& b) {   // rank: below the number of items
+  const unsigned heads = (unsigned)p.c.kv_heads;
+  unsigned level = 0, step = 1;   // the level: the last one with at most `rank` items below it
+  while (items_below(all, level + step, heads) <= rank) level += step, step *= 2;
+  for (; step > 0; step /= 2)
+    if (items_below(all, level + step, heads) <= rank) level += step;
+  const unsigned rest = rank - items_below(all, level, heads), index = rest / heads;
+  const v4i mine = all[threadIdx.x & 63];
+  const uint64_t have = __ballot((unsigned)mine[3] > level);
+  const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(have >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)have, 0u));
+  const uint64_t found = __ballot((unsigned)mine[3] > level && before == index);
+  b = uniform(found ? __ffsll((unsigned long long)found) - 1 : 0);
+  Item it{};
+  it.s = {lane_value(mine[0], b), lane_value(mine[1], b), lane_value(mine[2], b)};
+  it.head = uniform((int)(rest - index * heads));
+  it.row0 = uniform((lane_value(mine[3], b) - 1 - (int)level) * ROWS);
+  it.units = (unsigned)uniform(block_units<ROWS, kTile>(p, it.s, it.row0, it.tile0));
+  return it;
+}
+
 // SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 133 us, with 64-bit
 // bases for every tile 141).
 template <int D, bool SMALL>
@@ -92,9 +120,29 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   __shared__ uint64_t nan_in[kBuffers][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
   __shared__ __align__(16) int nan_any[kBuffers][kWaves];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
+  // Equal parts, or whole items: then workgroup g takes item g of the first gridDim.x, in the next the one as far from the end, and so on to and
+  // fro.  The largest of the last round is what that may leave some workgroups waiting; up to kWholeUnits of it are less than what partial
+  // results cost (64 prompts of 200 tokens: 114 us in parts).
+  constexpr unsigned kWholeUnits = 8;
+  __shared__ __align__(16) v4i sequences[64];
+  unsigned items = 0, rounds = 0;
+  bool by_items = false;
+  if (p.a.batch <= 64) {
+    if (tid < 64) {
+      Sequence s{0, 0, 0};
+      if (tid < p.a.batch) s = sequence(p, tid);
+      sequences[tid] = v4i{s.first, s.n, s.len, (s.n * p.group + kRows - 1) / kRows};
+    }
+    __syncthreads();
+    items = items_below(sequences, 0x7FFFFFFFu, (unsigned)p.c.kv_heads);
+    rounds = (items + gridDim.x - 1) / gridDim.x;
+    int any;
+    by_items = rounds == 0 || ranked_item<kRows>(p, sequences, (rounds - 1) * gridDim.x, any).units <= kWholeUnits;
+  }
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
-  const Part part = take_part<kRows, kTile, true>(p, g, gridDim.x);
+  Part part{};
+  if (!by_items) part = take_part<kRows, kTile, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
   const float c = uniform(softmax_scale(p.a.scale));
   // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
@@ -126,22 +174,32 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   int turn = 0;
   bool first_item = true;
   Item it{};
-  for (unsigned u = part.u0; u < part.u1;) {
-    if (!first_item && it.row0 + kRows < it.s.n * p.group) {   // the next block of the same key head
-      it.row0 += kRows;
-      it.begin = u;
-      it.units = (unsigned)block_units<kRows, kTile>(p, it.s, it.row0, it.tile0);
+  unsigned u = part.u0;
+  for (unsigned round = 0; by_items ? round < rounds : u < part.u1; ++round) {
+    unsigned from = 0, to;
+    if (by_items) {
+      const unsigned rank = round * gridDim.x + (round % 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      if (rank >= items) break;
+      it = ranked_item<kRows>(p, sequences, rank, b);
+      to = it.units;
     } else {
-      it = item_of<kRows, kTile, true>(p, u, b, b_begin, seq, per_head);
+      if (!first_item && it.row0 + kRows < it.s.n * p.group) {   // the next block of the same key head
+        it.row0 += kRows;
+        it.begin = u;
+        it.units = (unsigned)block_units<kRows, kTile>(p, it.s, it.row0, it.tile0);
+      } else {
+        it = item_of<kRows, kTile, true>(p, u, b, b_begin, seq, per_head);
+      }
+      from = u, to = it.begin + it.units < part.u1 ? it.begin + it.units : part.u1;
+      u = to;
+      if (first_item && tid == 0) {
+        int* m = p.meta + (size_t)g * kMeta;
+        m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)(it.begin + it.units), m[kMetaFirst] = it.s.first;
+        m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
+      }
+      first_item = false;
     }
-    const unsigned end = it.begin + it.units, from = u, to = end < part.u1 ? end : part.u1;
-    u = to;
-    if (first_item && tid == 0) {
-      int* m = p.meta + (size_t)g * kMeta;
-      m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)end, m[kMetaFirst] = it.s.first;
-      m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
-    }
-    first_item = false;
+    const unsigned end = it.begin + it.units;
     const unsigned start = it.begin + p.item_units;   // unit of the item's first tile
     const unsigned first = from > start ? from : start;
     const int rows = it.s.n * p.group, tile0 = it.tile0 + (int)(first - start);
