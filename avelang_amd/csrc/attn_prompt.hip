@@ -120,10 +120,10 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   __shared__ uint64_t nan_in[kBuffers][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
   __shared__ __align__(16) int nan_any[kBuffers][kWaves];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
-  // Equal parts, or whole items: then workgroup g takes item g of the first gridDim.x, in the next the one as far from the end, and so on to and
-  // fro.  The largest of the last round is what that may leave some workgroups waiting; up to kWholeUnits of it are less than what partial
-  // results cost (64 prompts of 200 tokens: 114 us in parts).
-  constexpr unsigned kWholeUnits = 8;
+  // Equal parts, or whole items: then a workgroup takes one of the first gridDim.x, in the next round the one as far from the end, and so on to
+  // and fro.  What that may cost is the largest item of the last round (`most` units, the smallest `least`), less a workgroup's share of that round;
+  // up to 24 units it is below the cost of partial results, their launch and the items' second starts (six prompts of 1000 tokens, 64 channels: 71 us,
+  // in parts 88; 4 of 2000, 256 channels 173 and 222; one of 8192, 128 channels, 22 units: 591 and 624).
   __shared__ __align__(16) v4i sequences[64];
   unsigned items = 0, rounds = 0;
   bool by_items = false;
@@ -136,8 +136,14 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     __syncthreads();
     items = items_below(sequences, 0x7FFFFFFFu, (unsigned)p.c.kv_heads);
     rounds = (items + gridDim.x - 1) / gridDim.x;
-    int any;
-    by_items = rounds == 0 || ranked_item<kRows>(p, sequences, (rounds - 1) * gridDim.x, any).units <= kWholeUnits;
+    if (rounds == 0) {
+      by_items = true;
+    } else {
+      int any;
+      const uint64_t all = gridDim.x, last = items - (rounds - 1) * gridDim.x;
+      const uint64_t most = ranked_item<kRows>(p, sequences, (rounds - 1) * gridDim.x, any).units;
+      by_items = most <= 8 || 2 * all * most <= 48 * all + last * (most + ranked_item<kRows>(p, sequences, items - 1, any).units);
+    }
   }
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
