@@ -1,7 +1,7 @@
 // Attention of many query rows over a paged MXFP4 cache: prompts and chunks of prompts.
 //
 // Bound by the matrix cores and by the exponentials beside them.  A workgroup takes blocks of 128 rows -- (token, query head) pairs of one
-// key head, 32 a wave -- through 64 keys at a time (attn_common.hpp cuts the triangle of a prompt into equal parts):
+// key head, 32 a wave -- through 64 keys at a time, in equal parts of the call (attn_common.hpp) or as whole blocks, largest first:
 //
 //   S^T = K Q^T   scaled MFMA 32x32x64, keys as they are (E2M1 codes and E8M0 scales straight from memory into LDS), queries as two E4M3
 //                 parts.  Row 8 i + 4 h + t of a tile of 32 keys is key 16 h + 4 i + t, so that lane half h = lane / 32 of the result holds
@@ -18,10 +18,11 @@
 //     constants in LDS instead of spilled: 642 -> 609);
 //   - equal ends: workgroups of a compute unit take turns in going first, and an item's start and end count as tiles (609 -> 537);
 //   - LDS reads ahead of the products (four long sequences: 348 -> 332); half tiles that nobody sees skipped (533 -> 515).
-// 8192 tokens, 32 heads on 8 of 128: 488 us, 1.13 PFLOP/s of 4 D flop a score (the matrix cores also multiply the queries' second part, half as much
-// again); 4 sequences of up to 16000 keys, 600 new tokens, 40 heads on 8: 320 us,
-// 1.10 PFLOP/s; six prompts of about 1000 tokens, 64 heads on 8 of 64: 87 us, where an
-// item of 128 rows has but 8 tiles for its start and end, and half the work is exponentials.
+//   - whole items instead of parts where that leaves little waiting (503 -> 480; six prompts of about 1000 tokens 88 -> 72).
+// (Cards differ by some per cent; a figure and the one it is compared with are of one card.)
+// 8192 tokens, 32 heads on 8 of 128: 459 us, 1.20 PFLOP/s of 4 D flop a score (the matrix cores also multiply the queries' second part, half as much
+// again); 4 sequences of up to 16000 keys, 600 new tokens, 40 heads on 8: 325 us, 1.09 PFLOP/s; six prompts of about 1000 tokens, 64 heads on 8 of 64:
+// 67 us, where an item of 128 rows has but 8 tiles for its start and end, and half the work is exponentials.
 #include "attn_common.hpp"
 #include "kernels.hpp"
 
