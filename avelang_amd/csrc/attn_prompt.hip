@@ -83,30 +83,48 @@ constexpr int waves_per_simd() {
   return D == 64 ? 4 : D == 128 ? 3 : 2;
 }
 
-// Whole items in falling order, for calls of up to 64 sequences.  Level k has the k-th last block of each sequence and key head that has so many;
+// Whole items in falling order, for calls of up to kSequences.  Level k has the k-th last block of each sequence and key head that has so many;
 // items are numbered level by level (by sequence, then head, within one), so that causal ones, which have fewer keys the earlier their rows
 // stand, come largest first.  `all` is a table of the sequences in LDS, {first, n, len, blocks}; every lane of the wave takes part.
-__device__ inline unsigned items_below(const v4i* all, unsigned level, unsigned heads) {   // of levels below
-  const unsigned blocks = (unsigned)all[threadIdx.x & 63][3];
-  return heads * (unsigned)lane_value((int)wave_scan(blocks < level ? blocks : level), 63);
+constexpr int kSequences = kWaves * 64;
+__device__ inline unsigned items_below(const AttnArgs& p, const v4i* all, unsigned level) {   // of levels below
+  const auto of_lane = [&](int b0) {
+    const unsigned blocks = (unsigned)all[b0 + (threadIdx.x & 63)][3];
+    return blocks < level ? blocks : level;
+  };
+  unsigned mine = of_lane(0);
+  if (p.a.batch > 64)
+    for (int b0 = 64; b0 < kSequences; b0 += 64) mine += of_lane(b0);   // (nothing behind the last sequence)
+  return (unsigned)p.c.kv_heads * (unsigned)lane_value((int)wave_scan(mine), 63);
 }
 template <int ROWS>
 __device__ inline Item ranked_item(const AttnArgs& p, const v4i* all, unsigned rank, int& b) {   // rank: below the number of items
   const unsigned heads = (unsigned)p.c.kv_heads;
   unsigned level = 0, step = 1;   // the level: the last one with at most `rank` items below it
-  while (items_below(all, level + step, heads) <= rank) level += step, step *= 2;
+  while (items_below(p, all, level + step) <= rank) level += step, step *= 2;
   for (; step > 0; step /= 2)
-    if (items_below(all, level + step, heads) <= rank) level += step;
-  const unsigned rest = rank - items_below(all, level, heads), index = rest / heads;
-  const v4i mine = all[threadIdx.x & 63];
-  const uint64_t have = __ballot((unsigned)mine[3] > level);
+    if (items_below(p, all, level + step) <= rank) level += step;
+  const unsigned rest = rank - items_below(p, all, level);
+  unsigned index = rest / heads;   // among the sequences that have so many blocks
+  const unsigned head = rest - index * heads;
+  int b0 = 0;
+  v4i mine = all[threadIdx.x & 63];
+  uint64_t have = __ballot((unsigned)mine[3] > level);
+  if (p.a.batch > 64)
+    while (index >= (unsigned)__popcll(have) && b0 + 64 < kSequences) {
+      index -= (unsigned)__popcll(have);
+      b0 += 64;
+      mine = all[b0 + (threadIdx.x & 63)];
+      have = __ballot((unsigned)mine[3] > level);
+    }
   const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(have >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)have, 0u));
   const uint64_t found = __ballot((unsigned)mine[3] > level && before == index);
-  b = uniform(found ? __ffsll((unsigned long long)found) - 1 : 0);
+  const int at = uniform(found ? __ffsll((unsigned long long)found) - 1 : 0);
+  b = b0 + at;
   Item it{};
-  it.s = {lane_value(mine[0], b), lane_value(mine[1], b), lane_value(mine[2], b)};
-  it.head = uniform((int)(rest - index * heads));
-  it.row0 = uniform((lane_value(mine[3], b) - 1 - (int)level) * ROWS);
+  it.s = {lane_value(mine[0], at), lane_value(mine[1], at), lane_value(mine[2], at)};
+  it.head = uniform((int)head);
+  it.row0 = uniform((lane_value(mine[3], at) - 1 - (int)level) * ROWS);
   it.units = (unsigned)uniform(block_units<ROWS, kTile>(p, it.s, it.row0, it.tile0));
   return it;
 }
@@ -122,20 +140,18 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   __shared__ __align__(16) int nan_any[kBuffers][kWaves];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
   // Equal parts, or whole items: then a workgroup takes one of the first gridDim.x, in the next round the one as far from the end, and so on to
-  // and fro.  What that may cost is the largest item of the last round (`most` units, the smallest `least`), less a workgroup's share of that round;
+  // and fro.  What that may cost is the largest item of the last round (`most` units), less a workgroup's share of that round;
   // up to 24 units it is below the cost of partial results, their launch and the items' second starts (six prompts of 1000 tokens, 64 channels: 71 us,
-  // in parts 88; 4 of 2000, 256 channels 173 and 222; one of 8192, 128 channels, 22 units: 591 and 624).
-  __shared__ __align__(16) v4i sequences[64];
+  // in parts 88; 4 of 2000, 256 channels 173 and 222; one of 8192, 128 channels, 22 units: 591 and 624; 150 of 100 89 and 108).
+  __shared__ __align__(16) v4i sequences[kSequences];
   unsigned items = 0, rounds = 0;
   bool by_items = false;
-  if (p.a.batch <= 64) {
-    if (tid < 64) {
-      Sequence s{0, 0, 0};
-      if (tid < p.a.batch) s = sequence(p, tid);
-      sequences[tid] = v4i{s.first, s.n, s.len, (s.n * p.group + kRows - 1) / kRows};
-    }
+  if (p.a.batch <= kSequences) {
+    Sequence s{0, 0, 0};
+    if (tid < p.a.batch) s = sequence(p, tid);
+    sequences[tid] = v4i{s.first, s.n, s.len, (s.n * p.group + kRows - 1) / kRows};
     __syncthreads();
-    items = items_below(sequences, 0x7FFFFFFFu, (unsigned)p.c.kv_heads);
+    items = items_below(p, sequences, 0x7FFFFFFFu);
     rounds = (items + gridDim.x - 1) / gridDim.x;
     if (rounds == 0) {
       by_items = true;
