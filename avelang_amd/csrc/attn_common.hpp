@@ -280,8 +280,6 @@ __device__ inline void wait_loads() {
 __device__ inline unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
-// A barrier that orders LDS and leaves loads to LDS under way
-__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Page of tokens 16 i .. 16 i + 15 of a sequence of len > 0 keys (behind the last: the last one's): what the table holds, and a valid one of that
 __device__ inline int page_entry(const AttnArgs& p, ConstInts row, int token, int len) { return row[(token < len ? token : len - 1) >> p.page_shift]; }

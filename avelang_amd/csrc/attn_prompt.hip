@@ -6,8 +6,9 @@
 //   S^T = K Q^T   scaled MFMA 32x32x64, keys as they are (E2M1 codes and E8M0 scales straight from memory into LDS), queries as two E4M3
 //                 parts.  Row 8 i + 4 h + t of a tile of 32 keys is key 16 h + 4 i + t, so that lane half h = lane / 32 of the result holds
 //                 keys 16 h .. 16 h + 15 of the tile for query row lane % 32.
-//   O^T = V^T P^T bf16 MFMA 32x32x16: P goes from the result's registers into the operand as it is, rounded to bf16.  Values are converted once
-//                 a workgroup, codes times their scales (exact), and lie in LDS as bf16 rows that transposing reads hand out by columns.
+//   O^T = V^T P^T bf16 MFMA 32x32x16: P goes from the result's registers into the operand as it is, rounded to bf16 (for the reason in
+//                 attn_decode.hip).  Values are converted once a workgroup, codes times their scales (exact), and lie in LDS as bf16 rows that
+//                 transposing reads hand out by columns.
 //
 // What a wave does for 64 keys: 8 scaled and 16 bf16 MFMAs at 128 channels (about 1090 cycles), and beside them 32 each of fma, exponential
 // and addition a lane, 16 conversions of P, a quarter of a tile's values converted, requests and addresses (about 950).  Scores, exponentials and
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   int b = part.b;
   unsigned b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
-  if (!p.whole && tid == 0 && part.u0 >= part.u1) {   // no work
+  if (tid == 0 && part.u0 >= part.u1) {   // no part, nothing to join
     int* m = p.meta + (size_t)g * kMeta;
     m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
   }
