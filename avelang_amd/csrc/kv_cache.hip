@@ -8,8 +8,8 @@
 // lanes 1, 2, 4, ... apart -- so that codes behind a norm and a rotation are the same bits wherever they are computed.
 //
 // Bound by HBM for a prompt (each input read once, each output written once), by latency for a decode batch: one launch for
-// all roles of heads.  8192 tokens, 32 query and 8 key heads of 128, norm and rotation: 46 us, 3.8 TB/s; the append of 64 + 8 + 8 heads of 64:
-// 34 us, 4.7 TB/s (a large copy reaches 5.2); the way back 4.3 TB/s.  64 tokens of 32 + 8 + 8 heads of 128: 3.8 us in a graph.
+// all roles of heads.  8192 tokens, 32 query and 8 key heads of 128, norm and rotation: 41 us, 4.2 TB/s; the append of 64 + 8 + 8 heads of 64:
+// 31 us, 5.1 TB/s (a large copy reaches 5.2); the way back 4.3 TB/s.  64 tokens of 32 + 8 + 8 heads of 128: 3.8 us in a graph.
 #include "fp4_common.hpp"
 #include "kv_cache.hpp"
 
@@ -28,7 +28,7 @@ __device__ inline Eight<T> load8(const T* p) {
   Eight<T> r;
   if (ALIGNED || (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
-    for (int q = 0; q < (int)sizeof(T) / 2; ++q) r.raw[q] = reinterpret_cast<const v4i*>(p)[q];
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q) r.raw[q] = ALIGNED ? __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p) + q) : reinterpret_cast<const v4i*>(p)[q];
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) r.raw[j / 4][j % 4] = reinterpret_cast<const int*>(p)[j];
@@ -48,10 +48,11 @@ __device__ inline void unpack(const Eight<T>& r, float (&v)[8]) {
   }
 }
 
-__device__ inline void store8_bf16(uint16_t* p, const float (&v)[8]) {
+__device__ inline void store8_bf16(uint16_t* p, const float (&v)[8], bool stream) {
   const v4i w = {(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]), (int)pack_bf16x2(v[4], v[5]), (int)pack_bf16x2(v[6], v[7])};
   if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    *reinterpret_cast<v4i*>(p) = w;
+    if (stream) __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(p));
+    else *reinterpret_cast<v4i*>(p) = w;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = (uint16_t)((unsigned)w[j / 2] >> (16 * (j % 2)));
@@ -61,7 +62,7 @@ __device__ inline void store8_bf16(uint16_t* p, const float (&v)[8]) {
 // D / 8 lanes share a head, eight channels each; a workgroup has 2048 / D heads of one token side by side, and `each` (at most kEach) such
 // groups -- queries, then keys, then values -- under way at once: what bounds a prompt is how many bytes are.  Neighbouring tokens go to
 // one XCD, whose L2 puts their pieces of a cache line together.  A pair's other half comes from the lane that has it.  (One group after the other,
-// the other half loaded again, tokens dealt out to the XCDs: 69 and 52 us where it is 44 and 34 now.)
+// the other half loaded again, tokens dealt out to the XCDs: 69 and 52 us where this came to 44 and 34.)
 constexpr int kEach = 4;
 
 template <typename T, int D, bool ALIGNED>
@@ -82,6 +83,9 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int
     const int64_t head_stride = is_q ? p.q.head_stride : is_v ? p.v.head_stride : p.k.head_stride;
     raw[u] = load8<ALIGNED>(static_cast<const T*>(data) + token * token_stride + head * head_stride + c0);
   }
+  // inputs are read once, outputs of prompts are larger than the caches on the way (8192 tokens: 45.7 us without the hints, 41.3 with; the append
+  // and the way back 43.8 and 38.8)
+  const bool stream = gridDim.x >= 1024;
   const int half = p.how.rotary_dim / 2;
   const bool turned = p.how.cos && c0 < 2 * half;
   const bool upper = !p.how.neighbours && c0 >= half;      // this lane's channels are the second ones of their pairs
@@ -147,7 +151,7 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int
     if (is_q || (!is_v && p.k_out.data)) {
       void* data = is_q ? p.q_out.data : p.k_out.data;
       const int64_t token_stride = is_q ? p.q_out.token_stride : p.k_out.token_stride, head_stride = is_q ? p.q_out.head_stride : p.k_out.head_stride;
-      store8_bf16(static_cast<uint16_t*>(data) + token * token_stride + head * head_stride + c0, x);
+      store8_bf16(static_cast<uint16_t*>(data) + token * token_stride + head * head_stride + c0, x, stream);
     } else {
       const unsigned amax = lane_xor_max_bits(lane_xor_max_bits(abs_max_bits(x), 1), 2);   // four lanes share a block
       const int byte = mx_scale_byte(amax);
