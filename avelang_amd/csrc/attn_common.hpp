@@ -263,8 +263,10 @@ __device__ inline const uint8_t* uniform_pointer(const uint8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
   return reinterpret_cast<const uint8_t*>((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)v) | (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
 }
+template <bool ONCE = false>   // ONCE: nobody else will want it (non-temporal)
 __device__ inline void to_lds16(const uint8_t* base, unsigned offset, unsigned lds) {   // base is wave-uniform
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
+  if constexpr (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ inline void to_lds4(const uint8_t* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");

@@ -82,9 +82,9 @@ struct Request {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         const unsigned off = kv ? value[i] : key[i], at = lds + kv * S::kCodes + i * 1024;
-        if constexpr (ONE_PAGE) to_lds16(base[0], off, at);
+        if constexpr (ONE_PAGE) to_lds16<true>(base[0], off, at);
         else if constexpr (kTokens > 16) to_lds16(pick(lane < 32, base[2 * i % kGroups], base[(2 * i + 1) % kGroups]) + off, at);   // two groups
-        else to_lds16(base[i * kTokens / 16 % kGroups], off, at);
+        else to_lds16<true>(base[i * kTokens / 16 % kGroups], off, at);
       }
     }
     // scales: a lane's four bytes belong to the tokens of one group
