@@ -16,10 +16,11 @@
 // P is rounded to bf16 because the values' codes reach the matrix cores as bf16 without loss and the result is bf16 anyway: 2^-9 of a
 // probability, averaged over the keys.  Scores, maxima, sums and results are fp32.
 //
-// 32 heads on 8 of 128: 64 sequences of 2048 to 4096 keys 54 us (4.0 TB/s; of 16384 keys each 5.8, of 256 channels 5.7, of 64 4.9), one of 131072 39.5 us.
-// Non-temporal hints on what nobody else reads are 4 of them (58.5 and 43 us without, 16384 keys 215 and 199).  About 15 us are no traffic: the launches (5 each), and the way from the lengths by the table to the first keys.  For up to
-// 16 rows four waves with two stages each, two workgroups a compute unit, read ahead best (eight waves, one workgroup: 63 and 45 us); items
-// that stay whole get eight waves, which halve their way.
+// 32 heads on 8 of 128: 64 sequences of 2048 to 4096 keys 54 us (4.0 TB/s; of 16384 keys each 5.8, of 256 channels 5.7, of 64 4.9), one of
+// 131072 39.5 us.  Non-temporal hints on what nobody else reads are 4 of them (58.5 and 43 us without, 16384 keys 215 and 199).  About 15 us are
+// no traffic: the launches (5 each), and the way from the lengths by the table to the first keys.  For up to 16 rows four waves with two stages
+// each, two workgroups a compute unit, read ahead best (eight waves, one workgroup: 63 and 45 us); items that stay whole get eight waves, which
+// halve their way.
 #include "attn_common.hpp"
 #include "kernels.hpp"
 
