@@ -6,8 +6,9 @@
 // numbered by sequence, key head, block, key; every workgroup takes the same number of consecutive ones, so that a long sequence
 // beside short ones, or the triangle of a prompt, costs no workgroup more than another.  Lengths are device memory: each workgroup adds the
 // units up for itself (one read of seq_lens and cu_q).  A part of an item that does not cover all of it goes to the workspace, and
-// a second launch joins the parts in order.
+// a second launch joins the parts in order.  (The arithmetic: attn_units.hpp.)
 #pragma once
+#include "attn_units.hpp"
 #include "fp4_common.hpp"
 #include "kv_cache.hpp"
 #include "tile_common.hpp"
@@ -23,39 +24,6 @@ constexpr float kNone = -3.0e38f;
 __device__ inline float softmax_scale(float scale) { return fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f); }   // base 2
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-struct AttnArgs {
-  ave_fp4_attention a;
-  ave_fp4_kv_cache c;
-  int group;          // query heads per key head
-  int page_shift;
-  int whole;          // 1: items are not split; no workspace, no second launch
-  int q_aligned;      // every row of q starts at a multiple of 16 bytes
-  int few_long;       // few sequences of many blocks of rows each
-  int item_units;     // that the start and the end of an item count for beside its tiles
-  int min_units_log2; // of a workgroup, so that small calls are not cut into crumbs
-  int* meta;          // workspace: [workgroups][kMeta]
-  float* part_ml;     // [2 workgroups][ROWS][2]: maximum (base 2) and sum
-  float* part_o;      // [2 workgroups][ROWS][D]
-  unsigned group_mul, group_shift;   // division by `group` of numbers below 2^31: high word of the product, shifted (set_group)
-
-  __device__ inline int token_of(int row) const { return group == 1 ? row : (int)(__umulhi((unsigned)row, group_mul) >> group_shift); }
-};
-// 2^(31+s) / d rounded up with s = ceil(log2 d) has an error below 2^-31 of a quotient, so that n < 2^31 is divided exactly.
-inline void set_group(AttnArgs& p, int group) {
-  p.group = group;
-  int s = 0;
-  while ((1 << s) < group) ++s;
-  p.group_mul = group == 1 ? 0 : (unsigned)((((uint64_t)1 << (31 + s)) / (unsigned)group) + 1);
-  p.group_shift = group == 1 ? 0 : (unsigned)(s - 1);
-}
-
-// meta of a workgroup: its first unit, first and last unit (exclusive) of the item that it starts in, that item's first row of q, all
-// rows of its sequence, key head, first row of the block; a workgroup without work has nothing but first units beyond all units
-enum { kMetaU0, kMetaBegin, kMetaEnd, kMetaFirst, kMetaRows, kMetaHead, kMetaRow0, kMeta = 8 };
-
-struct Sequence {
-  int first, n, len;   // first row of q, new tokens, keys
-};
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;   // read through the scalar cache where the index is uniform
 
 __device__ inline Sequence sequence(const AttnArgs& p, int b) {
@@ -76,35 +44,6 @@ __device__ inline Sequence sequence(const AttnArgs& p, int b) {
   return s;
 }
 
-// Keys that new token t of a sequence sees: [lo, hi)
-__device__ inline void visible(const AttnArgs& p, const Sequence& s, int t, int& lo, int& hi) {
-  const int pos = s.len - s.n + t;
-  hi = p.a.causal ? pos + 1 : s.len;
-  hi = hi < 0 ? 0 : hi;
-  lo = p.a.window > 0 && pos >= p.a.window ? pos - p.a.window + 1 : 0;
-}
-
-// A block of rows: units (those for its start come before its tiles), and the first tile
-template <int ROWS, int TILE>
-__device__ inline int block_units(const AttnArgs& p, const Sequence& s, int row0, int& tile0) {
-  const int rows = s.n * p.group, last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
-  int lo, hi, other;
-  if (rows <= 0) {
-    tile0 = 0;
-    return 1 + p.item_units;
-  }
-  visible(p, s, p.token_of(row0), lo, other);
-  visible(p, s, p.token_of(last), other, hi);
-  tile0 = lo / TILE;
-  return (hi > lo ? (hi + TILE - 1) / TILE - tile0 : 1) + p.item_units;
-}
-template <int ROWS, int TILE>
-__device__ inline int sequence_units(const AttnArgs& p, const Sequence& s) {   // of one key head
-  int u = 0, tile0;
-  for (int row0 = 0; row0 < s.n * p.group; row0 += ROWS) u += block_units<ROWS, TILE>(p, s, row0, tile0);
-  return u;
-}
-
 __device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ inline unsigned wave_scan(unsigned v) {   // inclusive prefix sums over the lanes
   v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // one, two, four, eight lanes to the right in a row of 16
@@ -115,52 +54,40 @@ __device__ inline unsigned wave_scan(unsigned v) {   // inclusive prefix sums ov
   v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
   return v;
 }
-// The same for a sequence of many blocks, which the lanes of a wave share
-template <int ROWS, int TILE>
-__device__ inline unsigned wave_sequence_units(const AttnArgs& p, const Sequence& s) {
-  unsigned u = 0;
+__device__ inline unsigned lane_value(unsigned v, int lane) { return (unsigned)lane_value((int)v, lane); }
+__device__ inline Units lane_value(Units v, int lane) {
+  return (Units)(unsigned)lane_value((int)(unsigned)v, lane) | (Units)(unsigned)lane_value((int)(unsigned)(v >> 32), lane) << 32;
+}
+__device__ inline Units wave_scan(Units v) {   // of numbers whose sum is below 2^58: 26 bits and the rest, so that neither sum overflows
+  return wave_scan((unsigned)v & 0x3FFFFFFu) + ((Units)wave_scan((unsigned)(v >> 26)) << 26);
+}
+// Units of one key head of a sequence of many blocks, which the lanes of a wave share
+template <int ROWS, int TILE, typename U>
+__device__ inline U wave_sequence_units(const AttnArgs& p, const Sequence& s) {
+  U u = 0;
   int tile0;
   const int rows = s.n * p.group, lane = threadIdx.x & 63;
   for (int row0 = 0; row0 < rows; row0 += 64 * ROWS) {
     const int mine = row0 + lane * ROWS;
-    u += (unsigned)lane_value((int)wave_scan(mine < rows ? (unsigned)block_units<ROWS, TILE>(p, s, mine, tile0) : 0u), 63);
+    u += lane_value(wave_scan(mine < rows ? (unsigned)block_units<ROWS, TILE>(p, s, mine, tile0) : 0u), 63);
   }
   return u;
 }
 
-// The part of a workgroup: units [u0, u1) of all `units`, cut into `parts` equal ones; sequence b holds u0, b_begin is its first unit and
-// per_head the units of one of its key heads.  Every wave finds it by itself (no barrier): 64 sequences at a time, a lane each.
-struct Part {
-  unsigned u0, u1, units, parts;
-  int b;
-  unsigned b_begin, per_head;
-  Sequence s;
-};
-
-// First unit of part g: the first units % parts parts have one unit more
-__device__ inline unsigned part_start(unsigned each, unsigned more, unsigned g) { return g * each + (g < more ? g : more); }
-
-__device__ inline void cut(const AttnArgs& p, Part& r, unsigned g, unsigned workgroups) {
-  const unsigned want = (r.units + (1u << p.min_units_log2) - 1) >> p.min_units_log2;
-  r.parts = want < workgroups ? (want ? want : 1) : workgroups;
-  const unsigned each = r.units / r.parts, more = r.units - each * r.parts;
-  r.u0 = g < r.parts ? part_start(each, more, g) : r.units;
-  r.u1 = g < r.parts ? part_start(each, more, g + 1) : r.units;
-}
-
+// The part of workgroup g.  Every wave finds it by itself (no barrier): 64 sequences at a time, a lane each.
 // LONG: sequences may have many blocks of rows; where p.few_long says so the wave takes one sequence after the other.
-template <int ROWS, int TILE, bool LONG = false>
-__device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgroups) {
+template <int ROWS, int TILE, typename U, bool LONG = false>
+__device__ inline Part<U> take_part(const AttnArgs& p, unsigned g, unsigned workgroups) {
   if constexpr (LONG) {
     if (p.few_long) {
-      Part r{};
+      Part<U> r{};
       const unsigned heads = (unsigned)p.c.kv_heads;
-      for (int b = 0; b < p.a.batch; ++b) r.units += heads * wave_sequence_units<ROWS, TILE>(p, sequence(p, b));
+      for (int b = 0; b < p.a.batch; ++b) r.units += heads * wave_sequence_units<ROWS, TILE, U>(p, sequence(p, b));
       cut(p, r, g, workgroups);
-      for (r.b = 0; r.b < p.a.batch; ++r.b) {
+      for (r.b = 0;; ++r.b) {   // (the last one if lengths change under the call)
         r.s = sequence(p, r.b);
-        r.per_head = wave_sequence_units<ROWS, TILE>(p, r.s);
-        if (r.u0 < r.b_begin + heads * r.per_head) break;
+        r.per_head = wave_sequence_units<ROWS, TILE, U>(p, r.s);
+        if (r.u0 < r.b_begin + heads * r.per_head || r.b + 1 >= p.a.batch) break;
         r.b_begin += heads * r.per_head;
       }
       return r;
@@ -173,55 +100,57 @@ __device__ inline Part take_part(const AttnArgs& p, unsigned g, unsigned workgro
     if (b < p.a.batch) s = sequence(p, b);
     return s;
   };
-  Part r{};
+  Part<U> r{};
   Sequence s = load(lane);
-  unsigned mine = (unsigned)sequence_units<ROWS, TILE>(p, s), in = wave_scan(mine * heads);
-  unsigned total = (unsigned)lane_value((int)in, 63);
+  U mine = sequence_units<ROWS, TILE, U>(p, s), in = wave_scan(mine * heads), total = lane_value(in, 63);
   r.units = total;
   Sequence next = load(64 + lane);
   for (int b0 = 64; b0 < p.a.batch; b0 += 64) {
     const Sequence now = next;
     next = load(b0 + 64 + lane);
-    r.units += (unsigned)lane_value((int)wave_scan((unsigned)sequence_units<ROWS, TILE>(p, now) * heads), 63);
+    r.units += lane_value(wave_scan(sequence_units<ROWS, TILE, U>(p, now) * heads), 63);
   }
   cut(p, r, g, workgroups);
   if (r.u0 >= r.u1) return r;
-  unsigned base = 0;
+  U base = 0;
   int b0 = 0;
   while (r.u0 >= base + total && b0 + 64 < p.a.batch) {   // (u0 is below the number of units: found at the latest in the last 64)
     base += total;
     b0 += 64;
     s = load(b0 + lane);
-    mine = (unsigned)sequence_units<ROWS, TILE>(p, s);
+    mine = sequence_units<ROWS, TILE, U>(p, s);
     in = wave_scan(mine * heads);
-    total = (unsigned)lane_value((int)in, 63);
+    total = lane_value(in, 63);
   }
-  const unsigned begin = base + in - mine * heads;
+  const U begin = base + in - mine * heads;
   const uint64_t here = __ballot(begin <= r.u0 && r.u0 < begin + mine * heads);
   const int at = here ? __ffsll((unsigned long long)here) - 1 : 0;
   r.b = b0 + at;
-  r.b_begin = (unsigned)lane_value((int)begin, at);
-  r.per_head = (unsigned)lane_value((int)mine, at);
+  r.b_begin = lane_value(begin, at);
+  r.per_head = lane_value(mine, at);
   r.s = {lane_value(s.first, at), lane_value(s.n, at), lane_value(s.len, at)};
   return r;
 }
 
 // An item, and where the units of a walk stand in it
+template <typename U>
 struct Item {
   Sequence s;
   int head, row0, tile0;
-  unsigned begin, units;
+  unsigned units;
+  U begin;
 };
-// The item that holds unit u >= b_begin; moves b, b_begin, the sequence s and its units of one head on to it.
-template <int ROWS, int TILE, bool LONG = false>
-__device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& b_begin, Sequence& s, unsigned& per_head) {
-  Item it;
+// The item that holds unit u >= b_begin; moves b, b_begin, the sequence s and its units of one head on to it.  (Where lengths change under the call
+// it may end before u, and never begins behind it.)
+template <int ROWS, int TILE, typename U, bool LONG = false>
+__device__ inline Item<U> item_of(const AttnArgs& p, U u, int& b, U& b_begin, Sequence& s, U& per_head) {
+  Item<U> it;
   // (u is below the number of all units; the bounds on b and row0 hold if lengths change under the call, too)
   while (u >= b_begin + per_head * (unsigned)p.c.kv_heads && b + 1 < p.a.batch) {
     b_begin += per_head * (unsigned)p.c.kv_heads;
     b = __builtin_amdgcn_readfirstlane(b + 1);
     s = sequence(p, b);
-    per_head = LONG ? wave_sequence_units<ROWS, TILE>(p, s) : (unsigned)sequence_units<ROWS, TILE>(p, s);
+    per_head = LONG ? wave_sequence_units<ROWS, TILE, U>(p, s) : sequence_units<ROWS, TILE, U>(p, s);
   }
   it.s = s;
   it.head = 0;
@@ -233,14 +162,15 @@ __device__ inline Item item_of(const AttnArgs& p, unsigned u, int& b, unsigned& 
       const int mine = row0 + lane * ROWS;
       int tile0 = 0;
       const unsigned units = mine < rows ? (unsigned)block_units<ROWS, TILE>(p, s, mine, tile0) : 0u, in = wave_scan(units);
-      const unsigned total = (unsigned)lane_value((int)in, 63);
-      if (u < it.begin + total || row0 + 64 * ROWS >= rows) {
-        const uint64_t here = __ballot(u < it.begin + in);
+      const unsigned total = lane_value(in, 63);
+      const U rest = u - it.begin;
+      if (rest < total || row0 + 64 * ROWS >= rows) {
+        const uint64_t here = __ballot(rest < in);
         const int at = here ? __ffsll((unsigned long long)here) - 1 : 0;
         it.row0 = row0 + at * ROWS;
-        it.units = (unsigned)lane_value((int)units, at);
+        it.units = lane_value(units, at);
         it.tile0 = lane_value(tile0, at);
-        it.begin += (unsigned)lane_value((int)(in - units), at);
+        it.begin += lane_value(in - units, at);
         return it;
       }
       it.begin += total;
@@ -438,13 +368,13 @@ size_t attn_decode_workspace(const AttnArgs& p, int row_tiles);
 // rows: of a block; rows_expected: of a sequence and key head
 hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s);
 // meta, maxima and sums, partial results, in this order
+inline size_t attn_meta_bytes(int workgroups) { return ((size_t)workgroups * sizeof(PartMeta) + 255) / 256 * 256; }
 inline size_t attn_workspace(int rows, int head_dim, int workgroups) {
-  const size_t meta = ((size_t)workgroups * kMeta * 4 + 255) / 256 * 256;
-  return meta + (size_t)workgroups * 2 * rows * (2 + head_dim) * 4;
+  return attn_meta_bytes(workgroups) + (size_t)workgroups * 2 * rows * (2 + head_dim) * 4;
 }
 inline void place_workspace(AttnArgs& p, int rows, int workgroups, void* ws) {
-  p.meta = static_cast<int*>(ws);
-  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + ((size_t)workgroups * kMeta * 4 + 255) / 256 * 256);
+  p.meta = static_cast<PartMeta*>(ws);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + attn_meta_bytes(workgroups));
   p.part_o = p.part_ml + (size_t)workgroups * 2 * rows * 2;
 }
 }  // namespace ave

@@ -119,14 +119,14 @@ struct Queries {
   int s_hi[NT], s_lo[NT];
   v4i x[NT][D / 32];   // eight channels each: pairs of them at 16 g + 64 i
 
-  __device__ inline void request(const AttnArgs& p, const Item& it, int rows) {
+  __device__ inline void request(const AttnArgs& p, const Sequence& s, int head, int row0, int rows) {
     const int lane = threadIdx.x & 63, g = lane / 16;
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      const int row = it.row0 + ct * 16 + lane % 16;
+      const int row = row0 + ct * 16 + lane % 16;
       const bool real = row < rows;
       const int t = real ? p.token_of(row) : 0;
-      const uint16_t* q = p.a.q + (int64_t)(it.s.first + t) * p.a.q_token_stride + (int64_t)(it.head * p.group + (real ? row - t * p.group : 0)) * p.a.q_head_stride;
+      const uint16_t* q = p.a.q + (int64_t)(s.first + t) * p.a.q_token_stride + (int64_t)(head * p.group + (real ? row - t * p.group : 0)) * p.a.q_head_stride;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         x[ct][i] = v4i{0, 0, 0, 0};
@@ -170,7 +170,7 @@ constexpr int workgroups_per_cu() {
   return lds_bytes<D, NT, NW, NS>() <= 78 * 1024 ? 2 : 1;
 }
 
-template <int D, int NT, int NW, int NS, bool ONE_PAGE>
+template <int D, int NT, int NW, int NS, bool ONE_PAGE, typename U>
 __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW / 4)) void attn_decode_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int ROWS = NT * 16, TILE = 64, C = D / 16;   // C: channel tiles of 16
@@ -179,40 +179,37 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
   __shared__ __align__(16) unsigned char smem[lds_bytes<D, NT, NW, NS>()];
   __shared__ float join_ml[NW][ROWS][2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane / 16, col = lane % 16;
-  const Part part = take_part<ROWS, TILE>(p, blockIdx.x, gridDim.x);
+  const Part<U> part = take_part<ROWS, TILE, U>(p, blockIdx.x, gridDim.x);
   const unsigned ring = (unsigned)__builtin_amdgcn_readfirstlane(lds_address(smem)) + wave * NS * S::kStage;
   const unsigned char* ring_ptr = smem + wave * NS * S::kStage;
   const float c = softmax_scale(p.a.scale);
   const Request<D, ONE_PAGE> request;
   int b = part.b;
-  unsigned b_begin = part.b_begin, per_head = part.per_head;
+  U b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
   bool first_item = true;
   if (!p.whole && threadIdx.x == 0 && part.u0 >= part.u1) {   // no work
-    int* m = p.meta + (size_t)blockIdx.x * kMeta;
-    m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
+    PartMeta& m = p.meta[blockIdx.x];
+    m.u0 = m.begin = m.end = part.units;
   }
-  for (unsigned u = part.u0; u < part.u1;) {
-    const Item it = item_of<ROWS, TILE>(p, u, b, b_begin, seq, per_head);
-    const unsigned end = it.begin + it.units;
-    unsigned from = u, to = end < part.u1 ? end : part.u1;
+  for (U u = part.u0; u < part.u1;) {
+    const Item<U> it = item_of<ROWS, TILE, U>(p, u, b, b_begin, seq, per_head);
+    if (u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end)
+    unsigned from = (unsigned)(u - it.begin), to = it.units;   // units of the item
     if (!p.whole) {
-      if (first_item && threadIdx.x == 0) {
-        int* m = p.meta + (size_t)blockIdx.x * kMeta;
-        m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)end, m[kMetaFirst] = it.s.first;
-        m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
-      }
-      u = to;
+      if (part.u1 - it.begin < to) to = (unsigned)(part.u1 - it.begin);
+      if (first_item && threadIdx.x == 0) p.meta[blockIdx.x] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
+      u = it.begin + to;
     } else {   // the items that start in this part, as wholes
-      u = end;
+      u = it.begin + it.units;
       if (it.begin < part.u0) {
         first_item = false;
         continue;
       }
-      to = end;
+      from = 0;
     }
     const int rows = it.s.n * p.group;
-    const int tile0 = it.tile0 + (int)(from - it.begin), tiles = (int)(to - from);
+    const int tile0 = it.tile0 + (int)from, tiles = (int)(to - from);
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
     // what the rows see
@@ -229,7 +226,7 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
     }
     const int mine = it.s.len > 0 && tiles > wave ? (tiles - wave + NW - 1) / NW : 0;   // tiles wave, wave + NW, ...
     Queries<D, NT> q;
-    q.request(p, it, rows);
+    q.request(p, it.s, it.head, it.row0, rows);
     int requested = 0;
     for (; requested < (kEarly ? NS : NS - 1) && requested < mine; ++requested)
       request.stage(p, table, it.s.len, it.head, (tile0 + wave + requested * NW) * TILE, ring + requested * S::kStage);
@@ -440,9 +437,9 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
       for (int k = 0; k < C; ++k) *reinterpret_cast<v4f*>(mine_o + (ct * 16 + col) * kPitch + k * 16 + g * 4) = acc[ct][k];
     }
     __syncthreads();
-    const bool done = from == it.begin && to == end;
+    const bool done = from == 0 && to == it.units;
     const int valid = rows - it.row0 < ROWS ? rows - it.row0 : ROWS;
-    const size_t slot = 2 * (size_t)blockIdx.x + (it.begin >= part.u0 ? 1 : 0);
+    const size_t slot = 2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0);   // the item that the part starts in, the one that it ends in
     for (int at = threadIdx.x; at < valid * (D / 4); at += NW * 64) {
       const int row = at / (D / 4), ch = at % (D / 4) * 4;
       float top = -INFINITY, sum = 0.0f;
@@ -468,7 +465,7 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
   }
 }
 
-template <int D, int NT, int NW, int NS>
+template <int D, int NT, int NW, int NS, typename U = unsigned>
 hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
   constexpr int ROWS = NT * 16;
   const int workgroups = compute_units() * workgroups_per_cu<D, NT, NW, NS>();
@@ -477,8 +474,12 @@ hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
   p.min_units_log2 = p.whole ? 0 : log2_of(NW);
   if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
   const dim3 grid((unsigned)workgroups), block(NW * 64);
-  if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false>), grid, block, 0, s, p);
+  if constexpr (sizeof(U) == 4) {
+    if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true, U>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false, U>), grid, block, 0, s, p);
+  } else {   // (pages of any size by the general form)
+    hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false, U>), grid, block, 0, s, p);
+  }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.whole) return e;
   return launch_attn_combine(p, ROWS, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
 }
@@ -494,14 +495,22 @@ bool keep_whole(const AttnArgs& p, int row_tiles) {
   return (in_window < in_table ? in_window : in_table) <= (p.c.head_dim == 256 ? 512 : 1024) * (many ? 2 : 1);
 }
 
+// More units than 32 bits hold (a call of seconds): one form for each number of channels, of two row tiles
+bool in_64_bits(const AttnArgs& p, int row_tiles) { return units_bound(p, row_tiles * 16, 64) >> 32 != 0; }
+
 }  // namespace
 
 size_t attn_decode_workspace(const AttnArgs& p, int row_tiles) {
-  return keep_whole(p, row_tiles) ? 0 : attn_workspace(row_tiles * 16, p.c.head_dim, 2 * compute_units());
+  return keep_whole(p, row_tiles) ? 0 : attn_workspace((in_64_bits(p, row_tiles) ? 2 : row_tiles) * 16, p.c.head_dim, 2 * compute_units());
 }
 
 hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s) {
   const bool whole = keep_whole(p, row_tiles);
+  if (in_64_bits(p, row_tiles)) {
+    if (p.c.head_dim == 64) return launch_form<64, 2, 4, 4, Units>(p, whole, ws, s);
+    if (p.c.head_dim == 128) return launch_form<128, 2, 4, 2, Units>(p, whole, ws, s);
+    return launch_form<256, 2, 4, 2, Units>(p, whole, ws, s);
+  }
   switch (p.c.head_dim * 8 + row_tiles) {
     case 64 * 8 + 1: return whole ? launch_form<64, 1, 8, 4>(p, whole, ws, s) : launch_form<64, 1, 4, 4>(p, whole, ws, s);
     case 64 * 8 + 2: return whole ? launch_form<64, 2, 8, 4>(p, whole, ws, s) : launch_form<64, 2, 4, 4>(p, whole, ws, s);
@@ -525,10 +534,10 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS)
   __shared__ v4f sums[GROUPS][T];
   __shared__ float ml[GROUPS][2];
   const int g = blockIdx.x + 1;
-  const int* m = p.meta + (size_t)g * kMeta;
-  const unsigned begin = (unsigned)m[kMetaBegin], end = (unsigned)m[kMetaEnd], u0 = (unsigned)m[kMetaU0];
-  if (begin >= u0 || (unsigned)m[kMetaU0 - kMeta] > begin) return;
-  const int rows = m[kMetaRows], row0 = m[kMetaRow0], valid = rows - row0 < ROWS ? rows - row0 : ROWS;
+  const PartMeta* m = p.meta + g;
+  const Units begin = m->begin, end = m->end;
+  if (begin >= m->u0 || m[-1].u0 > begin) return;
+  const int rows = m->rows, row0 = m->row0, valid = rows - row0 < ROWS ? rows - row0 : ROWS;
   const int group = GROUPS > 1 ? threadIdx.x / T : 0, ch = threadIdx.x % T * 4, most = (int)gridDim.x + 1 - g;   // workgroups from g on
   for (int first = blockIdx.y * R; first < valid; first += gridDim.y * R) {
     const int row = first + (GROUPS > 1 ? 0 : threadIdx.x / T);
@@ -538,7 +547,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS)
     if (row < valid) {
 #pragma unroll 4
       for (int i = group; i <= most; i += GROUPS) {
-        if (i > 0 && (unsigned)m[(i - 1) * kMeta + kMetaU0] >= end) break;
+        if (i > 0 && m[i - 1].u0 >= end) break;
         const size_t at = (i == 0 ? 2 * (size_t)(g - 1) + 1 : 2 * (size_t)(g + i - 1)) * ROWS + row;
         const float mi = p.part_ml[at * 2], li = p.part_ml[at * 2 + 1];
         const v4f oi = *reinterpret_cast<const v4f*>(p.part_o + at * D + ch);
@@ -562,11 +571,11 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS)
           sum += ml[k][1] * f;
           o += sums[k][threadIdx.x] * f;
         }
-        finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
+        finish_row(p, row_index(p, m->first, m->head, row0 + row), D, ch, o, top, sum);
       }
       __syncthreads();
     } else if (row < valid) {
-      finish_row(p, row_index(p, m[kMetaFirst], m[kMetaHead], row0 + row), D, ch, o, top, sum);
+      finish_row(p, row_index(p, m->first, m->head, row0 + row), D, ch, o, top, sum);
     }
   }
 }

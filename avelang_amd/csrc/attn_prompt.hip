@@ -98,8 +98,8 @@ __device__ inline unsigned items_below(const AttnArgs& p, const v4i* all, unsign
     for (int b0 = 64; b0 < kSequences; b0 += 64) mine += of_lane(b0);   // (nothing behind the last sequence)
   return (unsigned)p.c.kv_heads * (unsigned)lane_value((int)wave_scan(mine), 63);
 }
-template <int ROWS>
-__device__ inline Item ranked_item(const AttnArgs& p, const v4i* all, unsigned rank, int& b) {   // rank: below the number of items
+template <int ROWS, typename U>
+__device__ inline Item<U> ranked_item(const AttnArgs& p, const v4i* all, unsigned rank, int& b) {   // rank: below the number of items
   const unsigned heads = (unsigned)p.c.kv_heads;
   unsigned level = 0, step = 1;   // the level: the last one with at most `rank` items below it
   while (items_below(p, all, level + step) <= rank) level += step, step *= 2;
@@ -122,7 +122,7 @@ __device__ inline Item ranked_item(const AttnArgs& p, const v4i* all, unsigned r
   const uint64_t found = __ballot((unsigned)mine[3] > level && before == index);
   const int at = uniform(found ? __ffsll((unsigned long long)found) - 1 : 0);
   b = b0 + at;
-  Item it{};
+  Item<U> it{};
   it.s = {lane_value(mine[0], at), lane_value(mine[1], at), lane_value(mine[2], at)};
   it.head = uniform((int)head);
   it.row0 = uniform((lane_value(mine[3], at) - 1 - (int)level) * ROWS);
@@ -132,7 +132,7 @@ __device__ inline Item ranked_item(const AttnArgs& p, const v4i* all, unsigned r
 
 // SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 133 us, with 64-bit
 // bases for every tile 141).
-template <int D, bool SMALL>
+template <int D, bool SMALL, typename U>
 __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
   constexpr int C = S::C;
@@ -159,14 +159,14 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     } else {
       int any;
       const uint64_t all = gridDim.x, last = items - (rounds - 1) * gridDim.x;
-      const uint64_t most = ranked_item<kRows>(p, sequences, (rounds - 1) * gridDim.x, any).units;
-      by_items = most <= 8 || 2 * all * most <= 48 * all + last * (most + ranked_item<kRows>(p, sequences, items - 1, any).units);
+      const uint64_t most = ranked_item<kRows, U>(p, sequences, (rounds - 1) * gridDim.x, any).units;
+      by_items = most <= 8 || 2 * all * most <= 48 * all + last * (most + ranked_item<kRows, U>(p, sequences, items - 1, any).units);
     }
   }
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
-  Part part{};
-  if (!by_items) part = take_part<kRows, kTile, true>(p, g, gridDim.x);
+  Part<U> part{};
+  if (!by_items) part = take_part<kRows, kTile, U, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
   const float c = uniform(softmax_scale(p.a.scale));
   // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
@@ -186,25 +186,25 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     return x;
   };
   int b = part.b;
-  unsigned b_begin = part.b_begin, per_head = part.per_head;
+  U b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
   if (tid == 0 && part.u0 >= part.u1) {   // no part, nothing to join
-    int* m = p.meta + (size_t)g * kMeta;
-    m[kMetaU0] = m[kMetaBegin] = m[kMetaEnd] = (int)part.units;
+    PartMeta& m = p.meta[g];
+    m.u0 = m.begin = m.end = part.units;
   }
   // Among waves that could issue, the oldest goes first, so that of equal parts the workgroups that a compute unit got last would end
   // long after the others (452 us the first, 677 the last).  The later a workgroup came, the more of its tiles it takes at a higher priority.
   const int late = blockIdx.x * waves_per_simd<D>() / gridDim.x;
   int turn = 0;
   bool first_item = true;
-  Item it{};
-  unsigned u = part.u0;
+  Item<U> it{};
+  U u = part.u0;
   for (unsigned round = 0; by_items ? round < rounds : u < part.u1; ++round) {
-    unsigned from = 0, to;
+    unsigned from = 0, to;   // units of the item
     if (by_items) {
       const unsigned rank = round * gridDim.x + (round % 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       if (rank >= items) break;
-      it = ranked_item<kRows>(p, sequences, rank, b);
+      it = ranked_item<kRows, U>(p, sequences, rank, b);
       to = it.units;
     } else {
       if (!first_item && it.row0 + kRows < it.s.n * p.group) {   // the next block of the same key head
@@ -212,19 +212,15 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         it.begin = u;
         it.units = (unsigned)block_units<kRows, kTile>(p, it.s, it.row0, it.tile0);
       } else {
-        it = item_of<kRows, kTile, true>(p, u, b, b_begin, seq, per_head);
+        it = item_of<kRows, kTile, U, true>(p, u, b, b_begin, seq, per_head);
       }
-      from = u, to = it.begin + it.units < part.u1 ? it.begin + it.units : part.u1;
-      u = to;
-      if (first_item && tid == 0) {
-        int* m = p.meta + (size_t)g * kMeta;
-        m[kMetaU0] = (int)part.u0, m[kMetaBegin] = (int)it.begin, m[kMetaEnd] = (int)(it.begin + it.units), m[kMetaFirst] = it.s.first;
-        m[kMetaRows] = it.s.n * p.group, m[kMetaHead] = it.head, m[kMetaRow0] = it.row0;
-      }
+      if (u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end)
+      from = (unsigned)(u - it.begin), to = part.u1 - it.begin < it.units ? (unsigned)(part.u1 - it.begin) : it.units;
+      u = it.begin + to;
+      if (first_item && tid == 0) p.meta[g] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
       first_item = false;
     }
-    const unsigned end = it.begin + it.units;
-    const unsigned start = it.begin + p.item_units;   // unit of the item's first tile
+    const unsigned start = (unsigned)p.item_units;   // unit of the item's first tile
     const unsigned first = from > start ? from : start;
     const int rows = it.s.n * p.group, tile0 = it.tile0 + (int)(first - start);
     const int tiles = it.s.len > 0 && to > first ? (int)(to - first) : 0;
@@ -526,7 +522,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     }
 
     // ---- results: lane (column lane % 32) has channels 32 k + 8 i + 4 (lane / 32) .. + 3 of its row
-    const bool done = from == it.begin && to == end;
+    const bool done = from == 0 && to == it.units;
     if (active) {
       const float sum = cross_sum<false>(l), m2 = m == kNoMax ? -INFINITY : m;
       const int here = lane_here(), row = row0 + here % 32, ch0 = here / 32 * 4;
@@ -558,7 +554,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
           }
         }
       } else if (real) {
-        const size_t slot = 2 * (size_t)g + (it.begin >= part.u0 ? 1 : 0), at = slot * kRows + (row - it.row0);
+        const size_t slot = 2 * (size_t)g + (from == 0 ? 1 : 0), at = slot * kRows + (row - it.row0);
         float* out = p.part_o + at * D + ch0;
 #pragma unroll
         for (int k = 0; k < C; ++k)
@@ -582,8 +578,9 @@ void launch(const AttnArgs& p, int workgroups, hipStream_t s) {
   const int64_t last = p.c.pages - 1, page = (int64_t)p.c.kv_heads * p.c.page_size * D / 2;   // bytes of codes; of scales a 16th
   const auto small = [&](int64_t stride, int64_t bytes) { return last * stride + bytes <= (int64_t)1 << 32; };
   const bool all = small(p.c.k_page_stride, page) && small(p.c.v_page_stride, page) && small(p.c.k_scale_page_stride, page / 16) && small(p.c.v_scale_page_stride, page / 16);
-  if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((attn_prompt_kernel<D, false>), grid, block, 0, s, p);
+  if (units_bound(p, kRows, kTile) >> 32) hipLaunchKernelGGL((attn_prompt_kernel<D, false, Units>), grid, block, 0, s, p);   // (a call of seconds)
+  else if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true, unsigned>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attn_prompt_kernel<D, false, unsigned>), grid, block, 0, s, p);
 }
 
 }  // namespace

@@ -1,0 +1,123 @@
+"""The arithmetic that divides attention among workgroups (``csrc/attn_units.hpp``), compiled for the host: numbers of units beyond 32 bits, equal
+and complete parts, the bound that chooses between 32 and 64, what rows see, and the division by the group size."""
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "avelang_amd", "csrc")
+
+PROGRAM = r"""
+#include <stdio.h>
+#include <stdlib.h>
+#include <initializer_list>
+#include "attn_units.hpp"
+using namespace ave;
+
+// new tokens, keys, group, key heads, window, causal, item units, smallest part (log2), workgroups
+template <int ROWS, typename U>
+int units(char** v) {
+  AttnArgs p{};
+  Sequence s{0, atoi(v[0]), atoi(v[1])};
+  set_group(p, atoi(v[2]));
+  p.a.tokens = s.n, p.a.batch = 1, p.page_shift = 4, p.a.table_pages = (s.len + 15) / 16;
+  p.c.kv_heads = atoi(v[3]);
+  p.a.window = atoi(v[4]), p.a.causal = atoi(v[5]), p.item_units = atoi(v[6]), p.min_units_log2 = atoi(v[7]);
+  const unsigned workgroups = (unsigned)atoi(v[8]);
+  Part<U> r{};
+  r.units = (unsigned)p.c.kv_heads * sequence_units<ROWS, 64, U>(p, s);
+  U at = 0, most = 0, least = ~(U)0;
+  for (unsigned g = 0; g < workgroups; ++g) {
+    cut(p, r, g, workgroups);
+    if (r.u0 != at || r.u1 < r.u0) return printf("part %u starts at %llu behind %llu\n", g, (unsigned long long)r.u0, (unsigned long long)at), 1;
+    at = r.u1;
+    if (g < r.parts) {
+      if (r.u1 - r.u0 > most) most = r.u1 - r.u0;
+      if (r.u1 - r.u0 < least) least = r.u1 - r.u0;
+    }
+  }
+  printf("%llu %llu %llu %llu %u %llu\n", (unsigned long long)r.units, (unsigned long long)at, (unsigned long long)most, (unsigned long long)least, r.parts,
+         (unsigned long long)units_bound(p, ROWS, 64));
+  return 0;
+}
+template <int ROWS>
+int both(char** v) { return units<ROWS, Units>(v) + units<ROWS, unsigned>(v); }
+int groups(int from, int to) {
+  for (int d = from; d < to; ++d) {
+    AttnArgs p{};
+    set_group(p, d);
+    const int64_t top = 2147483647;
+    for (int64_t k = 0; k < 64; ++k)
+      for (int64_t n : {k, k * d - 1, k * d, k * d + 1, top - k, top / d * d - 1, top / d * d, top / d * d - k * d - 1, (top >> (k % 31)) * 1})
+        if (n >= 0 && n <= top && p.token_of((int)n) != n / d) return printf("%lld / %d\n", (long long)n, d), 1;
+  }
+  return 0;
+}
+int main(int n, char** v) {
+  if (n == 3) return groups(atoi(v[1]), atoi(v[2]));
+  switch (atoi(v[1])) {
+    case 16: return both<16>(v + 2);
+    case 32: return both<32>(v + 2);
+    case 64: return both<64>(v + 2);
+    default: return both<128>(v + 2);
+  }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def program(tmp_path_factory):
+    where = tmp_path_factory.mktemp("units")
+    (where / "units.cc").write_text(PROGRAM)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", "-ftrapv", f"-I{CSRC}", str(where / "units.cc"), "-o", str(where / "units")], check=True)
+    return str(where / "units")
+
+
+def _expected(rows_of_block, new, keys, group, heads, window, causal, item):
+    total = 0
+    for row0 in range(0, new * group, rows_of_block):
+        first, last = row0 // group, (min(row0 + rows_of_block, new * group) - 1) // group
+        hi = max(0, keys - new + last + 1) if causal else keys
+        at = keys - new + first
+        lo = at - window + 1 if window and at >= window else 0
+        total += ((hi + 63) // 64 - lo // 64 if hi > lo else 1) + item
+    return total * heads
+
+
+CASES = [
+    (128, 600000, 600000, 16, 8, 0, 0, 3, 2, 768),        # 5.6e9: beyond 32 bits
+    (128, 520000, 1 << 20, 16, 8, 0, 1, 3, 2, 768),
+    (128, 786448, 786448, 8, 8, 0, 0, 2, 2, 1024),
+    (128, 100, 2000, 16, 8, 0, 1, 3, 2, 768),
+    (128, 5000, 300, 3, 5, 0, 1, 3, 2, 768),              # more new tokens than keys
+    (128, 5000, 90000, 3, 5, 1000, 1, 3, 2, 1000),
+    (16, 1, 1 << 20, 1, 4096, 0, 1, 0, 2, 512),
+    (16, 1, (1 << 31) - 4096, 8, 1024, 0, 1, 0, 2, 512),  # one token on as many keys as a table covers: 3.4e10
+    (32, 1, 0, 32, 8, 0, 1, 0, 2, 512),
+    (64, 2, 131072, 32, 1, 0, 1, 0, 2, 256),
+    (16, 4, 1500, 8, 8, 128, 1, 0, 3, 512),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_units_and_parts(program, case):
+    done = subprocess.run([program, *map(str, case)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
+    wide, narrow = (list(map(int, line.split())) for line in done.stdout.splitlines())
+    units, covered, most, least, parts, bound = wide
+    rows, new, keys, group, heads, window, causal, item, smallest, workgroups = case
+    assert units == _expected(rows, new, keys, group, heads, window, causal, item)
+    assert covered == units and most - least <= 1
+    assert parts == max(1, min(workgroups, -(-units // (1 << smallest))))
+    # the bound by which the host chooses: never below, so that 32 bits hold what they are given
+    assert units <= bound
+    assert bound >= 1 << 32 or narrow == wide
+
+
+def test_some_of_these_pass_32_bits():
+    assert sum(_expected(c[0], *c[1:8]) > 1 << 32 for c in CASES) >= 4
+
+
+def test_division_by_the_group(program):
+    done = subprocess.run([program, "1", "1025"], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr

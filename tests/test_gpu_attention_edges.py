@@ -1,0 +1,56 @@
+"""Attention over an MXFP4 cache and the kernels around it at the edges of what they accept."""
+import numpy as np
+import pytest
+import torch
+
+import avelang_amd as ave
+from tests import attention_helpers as A
+
+pytestmark = pytest.mark.gpu
+
+
+def test_more_than_2_to_the_32_units(gpu):
+    """257 single tokens of 1024 heads over 2^20 keys, which are the same 64 keys again and again (one page): units of 64 keys."""
+    heads, d, page, batch, keys = 1024, 64, 64, 257, 1 << 20
+    g = torch.Generator().manual_seed(34)
+    cache = ave.kv_cache_mxfp4(1, heads, page, d, gpu)
+    kv = torch.randn(2, page, heads, d, generator=g).to(gpu)
+    ave.append_kv_mxfp4(kv[0], kv[1], cache, torch.arange(page, dtype=torch.int32, device=gpu))
+    q = torch.randn(1, heads, d, generator=g).bfloat16().to(gpu)
+    lens = torch.full((batch,), keys, dtype=torch.int32, device=gpu)
+    lens[::7] += 1 - page                                      # not every one of them a whole number of pages
+    table = torch.zeros(1, keys // page, dtype=torch.int32, device=gpu).expand(batch, -1)
+    out = torch.full((batch, heads, d), float("nan"), dtype=torch.bfloat16, device=gpu)
+    ave.attention_mxfp4(q.expand(batch, -1, -1), cache, table, lens, out=out)
+    k, v = (x.double().cpu() for x in ave.gather_kv_mxfp4(cache, torch.arange(page, dtype=torch.int32, device=gpu)))
+    p = torch.softmax((k * q.double().cpu()).sum(-1) * d ** -0.5, 0)[..., None]
+    want, weight = (p * v).sum(0), (p * v.abs()).sum(0)
+    # the result's rounding and a probability's; two fp32 sums of 2^16 steps a lane; the last page counting in part, one of 2^14
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * 2.0 ** -24 * 2 ** 16) * weight + 2.0 ** -13 * (weight + v.abs().amax(0))
+    err = (out.double().cpu() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 2, 40])
+def test_tables_wide_enough_for_units_beyond_32_bits(gpu, d, new):
+    """The width of the page table alone decides how units are numbered, so that short sequences reach the 64-bit forms, too."""
+    hq, hkv, page = 16, 8, 4096
+    rows = [(new, (2400 if new > 2 else 600) - 7 * i) for i in range(12)] + [(new, 3000), (0, 9), (new, 3), (new, 64)]
+    batch = A.Batch(rows, hq, hkv, d, page, seed=35)
+    t = batch.tensors(gpu)
+    wide = torch.full((len(rows), (1 << 31) // page - 1), 1 << 30, dtype=torch.int32, device=gpu)
+    wide[:, :t["page_table"].shape[1]] = t["page_table"]
+    want, want_lse, tol, lse_tol = batch.reference()
+    outs = []
+    for table in (t["page_table"], wide):
+        lse = torch.full(batch.q.shape[:2], float("nan"), device=gpu)
+        out = torch.full(batch.q.shape, float("nan"), dtype=torch.bfloat16, device=gpu)
+        ave.attention_mxfp4(t["q"], t["cache"], table, t["seq_lens"], t["cu_q"], out, lse, max_q=new)
+        assert (np.abs(out.float().cpu().numpy() - want) <= tol).all()
+        some = np.isfinite(want_lse)
+        assert np.array_equal(lse.cpu().numpy()[~some], want_lse[~some])
+        assert (np.abs(lse.cpu().numpy()[some] - want_lse[some]) <= lse_tol[some]).all()
+        outs.append(out)
+    if new == 40:
+        assert torch.equal(*outs)      # the kernel for prompts: the same parts either way
