@@ -135,9 +135,11 @@ static int check_attention(const ave_fp4_attention* a, const ave_fp4_kv_cache* c
   if (a->heads <= 0 || a->heads % cache->kv_heads != 0)
     return fail_inval("query heads must be a multiple of the cache's %d, got %d.", cache->kv_heads, a->heads);
   if (a->heads / cache->kv_heads > 1024) return fail_inval("at most 1024 query heads share a key head, got %d.", a->heads / cache->kv_heads);
-  if ((int64_t)a->tokens * a->heads > INT32_MAX) return fail_inval("tokens times heads must fit 31 bits, got %d x %d.", a->tokens, a->heads);
-  if (a->table_pages < 0 || (int64_t)a->table_pages * cache->page_size > INT32_MAX)
-    return fail_inval("the page table must cover less than 2^31 tokens, got %d pages of %d.", a->table_pages, cache->page_size);
+  // the kernels' ints also count what lies behind the last row (the blocks of 64 lanes) and the last key (two tiles that are looked for ahead)
+  if ((int64_t)a->tokens * a->heads > INT32_MAX - (1 << 14))
+    return fail_inval("tokens times heads must fit 31 bits with 2^14 to spare, got %d x %d.", a->tokens, a->heads);
+  if (a->table_pages < 0 || (int64_t)a->table_pages * cache->page_size > INT32_MAX - 255)
+    return fail_inval("the page table must cover at most 2^31 - 256 tokens, got %d pages of %d.", a->table_pages, cache->page_size);
   if (a->max_q < 0) return fail_inval("max_q must be non-negative, got %d.", a->max_q);
   if (a->window < 0) return fail_inval("window must be non-negative, got %d.", a->window);
   if (a->window > 0 && !a->causal) return fail_inval("a window needs causal attention.");

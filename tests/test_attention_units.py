@@ -1,9 +1,12 @@
 """The arithmetic that divides attention among workgroups (``csrc/attn_units.hpp``), compiled for the host: numbers of units beyond 32 bits, equal
 and complete parts, the bound that chooses between 32 and 64, what rows see, and the division by the group size."""
+import ctypes
 import os
 import subprocess
 
 import pytest
+
+from avelang_amd import _lib
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "avelang_amd", "csrc")
 
@@ -93,6 +96,8 @@ CASES = [
     (128, 5000, 90000, 3, 5, 1000, 1, 3, 2, 1000),
     (16, 1, 1 << 20, 1, 4096, 0, 1, 0, 2, 512),
     (16, 1, (1 << 31) - 4096, 8, 1024, 0, 1, 0, 2, 512),  # one token on as many keys as a table covers: 3.4e10
+    (16, 1, (1 << 31) - 256, 8, 1, 0, 1, 0, 2, 512),      # ... with pages of 256 and less
+    (128, 3000, (1 << 31) - 256, 2, 1, 0, 1, 3, 2, 768),
     (32, 1, 0, 32, 8, 0, 1, 0, 2, 512),
     (64, 2, 131072, 32, 1, 0, 1, 0, 2, 256),
     (16, 4, 1500, 8, 8, 128, 1, 0, 3, 512),
@@ -121,3 +126,22 @@ def test_some_of_these_pass_32_bits():
 def test_division_by_the_group(program):
     done = subprocess.run([program, "1", "1025"], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("page,pages,tokens,heads,text", [
+    (16, (1 << 27) - 1, 1, 8, "2^31 - 256"), (128, (1 << 24) - 1, 1, 8, "2^31 - 256"), (256, (1 << 23) - 1, 1, 8, None), (4096, (1 << 19) - 1, 1, 8, None),
+    (16, 1, (1 << 28) - 1, 8, "2^14 to spare"), (16, 1, (1 << 28) - 2049, 8, None), (16, 1, (1 << 28) - 2048, 8, "2^14 to spare")])
+def test_sizes_next_to_2_to_the_31(page, pages, tokens, heads, text):
+    """What is looked for behind the last key or row has to have a number, too: at 2^31 - 16 keys the next tile's was negative, and the page table was
+    read in front of its start."""
+    p = 1 << 20   # any aligned address: nothing is launched
+    c = _lib.KVCache(k=p, k_scale=p, v=p, v_scale=p, k_page_stride=page * 64, k_scale_page_stride=page * 4, v_page_stride=page * 64, v_scale_page_stride=page * 4,
+                     pages=3, kv_heads=1, page_size=page, head_dim=128)
+    a = _lib.Attention(q=p, out=p, page_table=p, seq_lens=p, cu_q=p, tokens=tokens, batch=1, heads=heads, table_pages=pages, max_q=1, causal=1, scale=1)
+    lib = _lib.load()
+    if text is None:   # (a call would launch)
+        lib.ave_fp4_attention_mxfp4_workspace_bytes(ctypes.byref(a), ctypes.byref(c))
+        assert _lib.last_error() == ""
+    else:
+        assert lib.ave_fp4_attention_mxfp4(ctypes.byref(a), ctypes.byref(c), None, 0, None) == -1
+        assert text in _lib.last_error(), _lib.last_error()
