@@ -193,16 +193,18 @@ __device__ inline const uint8_t* uniform_pointer(const uint8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
   return reinterpret_cast<const uint8_t*>((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)v) | (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
 }
+// A wave-uniform base in scalar registers: five wait states have to pass if a vector instruction (uniform_pointer, a register spilled to lanes) wrote
+// them just before, and the compiler, which counts those for its own loads, does not look inside: one by s_mov, four by s_nop.
 template <bool ONCE = false>   // ONCE: nobody else will want it (non-temporal)
 __device__ inline void to_lds16(const uint8_t* base, unsigned offset, unsigned lds) {   // base is wave-uniform
-  if constexpr (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
-  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
+  if constexpr (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ inline void to_lds4(const uint8_t* src, unsigned lds) {   // (scales for few rows, which nobody else will want either)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off nt" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "m0", "memory");
 }
 __device__ inline void to_lds4(const uint8_t* base, unsigned offset, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "m0", "memory");
 }
 template <int N>
 __device__ inline void wait_loads() {
