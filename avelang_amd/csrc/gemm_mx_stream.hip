@@ -85,14 +85,20 @@ __device__ inline void load_scale_rows(const uint8_t* from, unsigned to) {
       : "m0", "memory");
 }
 
-// dma16 for the lanes of `lanes` only (with no lane left it counts on vmcnt all the same)
+// dma16 with a base that a vector instruction may have written just before (uniform, below): the load may read it five wait states later, which the
+// compiler does not see to inside asm.  s_mov and s_nop 3 are five.
+__device__ inline void dma16_uniform(const void* gbase, unsigned voff, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voff), "s"(gbase) : "m0");
+}
+
+// The same for the lanes of `lanes` only (with no lane left it counts on vmcnt all the same)
 __device__ inline void dma16_lanes(const void* gbase, unsigned voff, unsigned lds_addr, unsigned long long lanes) {
   unsigned long long saved;
   asm volatile(
       "s_mov_b32 m0, %[to]\n\t"
       "s_mov_b64 %[sv], exec\n\t"
       "s_mov_b64 exec, %[mask]\n\t"
-      "s_nop 0\n\t"
+      "s_nop 1\n\t"
       "global_load_lds_dwordx4 %[off], %[base]\n\t"
       "s_mov_b64 exec, %[sv]\n\t"
       : [sv] "=&s"(saved)
@@ -338,9 +344,9 @@ __device__ __forceinline__ void stream_tiles(const MxArgs& p, int n_tiles, const
         for (int i = 0; i < 4; ++i) dma16_lanes(uniform(gb), b_off[i], to + G::kOffB + (unsigned)(wi * 4 + i) * 1024, mine(b_late, i, b_chunk[i]));
       } else {
 #pragma unroll
-        for (int i = 0; i < G::kALoads; ++i) dma16(uniform(ga), a_off[i], to + (unsigned)(wi * G::kALoads + i) * 1024);
+        for (int i = 0; i < G::kALoads; ++i) dma16_uniform(uniform(ga), a_off[i], to + (unsigned)(wi * G::kALoads + i) * 1024);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dma16(uniform(gb), b_off[i], to + G::kOffB + (unsigned)(wi * 4 + i) * 1024);
+        for (int i = 0; i < 4; ++i) dma16_uniform(uniform(gb), b_off[i], to + G::kOffB + (unsigned)(wi * 4 + i) * 1024);
       }
       ga += kRowBytes;
       gb += kRowBytes;

@@ -3,12 +3,14 @@ wrote it (five) have to be there already.  A kernel in which such an instruction
 import os
 import re
 import shutil
+import struct
 import subprocess
 
 import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "avelang_amd", "csrc")
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
 
 KERNEL = r"""
 #include "attn_common.hpp"
@@ -61,3 +63,48 @@ def test_wait_states_in_front_of_loads_with_a_scalar_base(tmp_path):
             assert states >= 5, (line, states)
             seen += 1
     assert seen == 3
+
+
+def _code_objects(library):
+    """The gfx950 code objects of a library built by hipcc: bundles of (offset, size, target) entries, one for each source."""
+    data = open(library, "rb").read()
+    magic = b"__CLANG_OFFLOAD_BUNDLE__"
+    at = data.find(magic)
+    while at >= 0:
+        count, = struct.unpack_from("<Q", data, at + len(magic))
+        entry = at + len(magic) + 8
+        for _ in range(count):
+            offset, size, length = struct.unpack_from("<QQQ", data, entry)
+            target = data[entry + 24:entry + 24 + length]
+            entry += 24 + length
+            if b"gfx950" in target:
+                yield data[at + offset:at + offset + size]
+        at = data.find(magic, at + 1)
+
+
+def test_wait_states_in_the_built_library(tmp_path):
+    """Every load and store of the library's kernels that names a scalar base: no vector instruction within five wait states in front of it writes that
+    base.  (In order of address: a branch in between only adds to them.)"""
+    if not os.path.exists(OBJDUMP):
+        pytest.skip("no llvm-objdump")
+    loads, bad = 0, []
+    for n, code in enumerate(_code_objects(os.path.join(os.path.dirname(CSRC), "libave_fp4.so"))):
+        (tmp_path / "code").write_bytes(code)
+        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", "--no-leading-addr", str(tmp_path / "code")], check=True, capture_output=True, text=True).stdout
+        kernel, last = "", []
+        for line in text.splitlines():
+            if line.endswith(">:"):
+                kernel, last = line, []
+                continue
+            line = line.split("//")[0].strip()
+            if line.startswith(("global_", "buffer_", "scratch_")):
+                wanted = set().union(*map(_scalars, line.replace(",", " ").split()[1:]))
+                if wanted:
+                    loads += 1
+                    states = _wait_states(last, len(last), wanted)
+                    if states is not None and states < 5:
+                        bad.append((kernel, line, states))
+            if line:
+                last = last[-7:] + [line]
+    assert loads > 10000
+    assert not bad, (len(bad), bad[:3])
