@@ -378,19 +378,29 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
           return __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + 0x00010001u * (blk % 4));
         }
       };
-      if (nan) {   // a row to which a value with a NaN scale counts: its block of channels is NaN
+      if (nan) {   // a row that sees a value with a NaN scale, however little it counts: its block of channels is NaN
+        unsigned seen[NT];   // a bit for each of this group's 16 tokens
 #pragma unroll
-        for (int blk = 0; blk < S::kBlocks; ++blk)
+        for (int ct = 0; ct < NT; ++ct) {
+          const int from = lo_row[ct] - t0 - 16 * g, to = hi_row[ct] - t0 - 16 * g;
+          seen[ct] = (to > 15 ? 0xFFFFu : to > 0 ? (1u << to) - 1 : 0u) & (from > 15 ? 0u : from > 0 ? ~0u << from : ~0u);
+        }
+#pragma unroll
+        for (int blk = 0; blk < S::kBlocks; ++blk) {
+          unsigned bad = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const unsigned over = pk_sub_sat(scale_pair(blk, k), 0x00FC00FCu);   // 1 to 3 in a half where NaN
+            const unsigned two = (over | over >> 1) & 0x00010001u;
+            bad |= ((two | two >> 15) & 3u) << 2 * k;
+          }
 #pragma unroll
           for (int ct = 0; ct < NT; ++ct) {
-            unsigned hit = 0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              hit |= as_u32(as_us2(pk_sub_sat(scale_pair(blk, k), 0x00FC00FCu)) * __builtin_elementwise_min(as_us2(prob[ct][k]), us2{1, 1}));
-            const float poison = cross_max<true>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
+            const float poison = cross_max<true>(bad & seen[ct] ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
             acc[ct][2 * blk] += poison;
             acc[ct][2 * blk + 1] += poison;
           }
+        }
       }
 #pragma unroll
       for (int blk = 0; blk < S::kBlocks; ++blk) {

@@ -448,14 +448,16 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       }
       l += sum;
     };
-    const auto add_values = [&](int buffer, auto which, const unsigned (&prob)[8], int nan, const v4i& place, v8bf (&v)[kAhead], Keys& keys) {
+    const auto add_values = [&](int tile, int buffer, auto which, const unsigned (&prob)[8], int nan, const v4i& place, v8bf (&v)[kAhead], Keys& keys) {
       const unsigned at = place[2] + buffer % S::kValueBuffers * S::kValues;
       constexpr int j = decltype(which)::value;
-      // ---- values with a NaN scale, zeros in LDS: NaN for the rows to which they count
+      // ---- values with a NaN scale, zeros in LDS: NaN for the rows that see them, however little they count
       if (nan) {
-        uint64_t some = 0;   // four bits for each of this lane's keys, set where its probability is not zero
-#pragma unroll
-        for (int t = 0; t < 16; ++t) some |= (prob[t / 2] >> (16 * (t % 2))) & 0xFFFFu ? (uint64_t)15 << (4 * t) : 0;
+        const int here = lane_here(), key = tile * kTile + 32 * j + here / 32 * 16;
+        int lo, hi;
+        visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);
+        const int from = lo - key, to = hi - key;   // four bits for each of this lane's 16 keys
+        const uint64_t some = (to > 15 ? ~0ull : to > 0 ? (1ull << 4 * to) - 1 : 0ull) & (from > 15 ? 0ull : from > 0 ? ~0ull << 4 * from : ~0ull);
 #pragma unroll
         for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
           const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (j == 0) nan = uniform(any[0] | any[1] | any[2] | any[3]);
       probabilities(tile, which, first, s, prob);
-      add_values(buffer, which, prob, nan, place, v, keys);
+      add_values(tile, buffer, which, prob, nan, place, v, keys);
     };
 
     if (tiles > 0) store_values(tile0, 0);

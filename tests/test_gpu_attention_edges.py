@@ -9,6 +9,32 @@ from tests import attention_helpers as A
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [[(1, 300), (1, 90)], [(5, 300), (3, 90)], [(150, 300), (70, 90)], [(1, 5000)], [(70, 5000)]], ids=str)
+def test_a_seen_value_with_a_nan_scale_counts_however_small_its_probability(gpu, d, rows):
+    """Scores of hundreds: almost every probability is zero as a number, and still 0 * NaN is NaN.  Rows that do not see the key, and the
+    other blocks of channels, keep their bits."""
+    hq, hkv, window = 4, 2, 40
+    new, keys = rows[0]
+    for at_key in (keys - 60, keys - 30, keys - 1):
+        for how in ({}, {"window": window}):
+            batch, clean = (A.Batch(rows, hq, hkv, d, 32, seed=31, q_std=60.0) for _ in range(2))
+            page, at = batch.place(0, at_key)
+            batch.cache[3][page, 1, at, d // 32 - 1] = 253
+            got, want = (ave.attention_mxfp4(t["q"], t["cache"], t["page_table"], t["seq_lens"], t["cu_q"], max_q=max(n for n, _ in rows), **how)
+                         for t in (batch.tensors(gpu), clean.tensors(gpu)))
+            position = keys - new + torch.arange(new, device=gpu)
+            sees = position >= at_key
+            if how:
+                sees = sees & (position - window < at_key)
+            nan = torch.zeros(got.shape, dtype=torch.bool, device=gpu)
+            block = torch.zeros(hq, d, dtype=torch.bool, device=gpu)
+            block[2:, d - 32:] = True
+            nan[:new] = sees[:, None, None] & block
+            assert torch.equal(got.isnan(), nan), (at_key, how)
+            assert torch.equal(got[~nan], want[~nan])
+
+
 def test_more_than_2_to_the_32_units(gpu):
     """257 single tokens of 1024 heads over 2^20 keys, which are the same 64 keys again and again (one page): units of 64 keys."""
     heads, d, page, batch, keys = 1024, 64, 64, 257, 1 << 20
