@@ -174,10 +174,10 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadArgs p, int q_heads, int
 }
 
 template <typename T, int D>
-hipError_t launch_heads_as(const HeadArgs& p, hipStream_t s) {
+hipError_t launch_some_heads(const HeadArgs& p, hipStream_t s) {
   const int q = p.q.data ? p.q.heads : 0, all = q + (p.k.data ? p.k.heads : 0) + (p.v.data ? p.v.heads : 0);
   const int groups = (all + 2048 / D - 1) / (2048 / D);
-  if (p.tokens == 0 || all == 0) return hipSuccess;
+  if (all == 0) return hipSuccess;
   // few tokens: a workgroup for every group of heads; many: the fewest, which load their cosines once (32 + 8 + 8 heads of 128, 64 tokens 3.8 us
   // so, 5.7 otherwise; 512 5.8 and 6.7, 1024 9.1 and 8.7, 8192 50 and 43)
   const int want = (groups + kEach - 1) / kEach, each = p.tokens >= 1024 ? (groups + want - 1) / want : 1;
@@ -189,6 +189,24 @@ hipError_t launch_heads_as(const HeadArgs& p, hipStream_t s) {
   if (wide(p.q) && wide(p.k) && wide(p.v)) hipLaunchKernelGGL((heads_kernel<T, D, true>), grid, dim3(256), 0, s, p, q, all, each, shift);
   else hipLaunchKernelGGL((heads_kernel<T, D, false>), grid, dim3(256), 0, s, p, q, all, each, shift);
   return hipGetLastError();
+}
+
+// A workgroup of 256 for every token: a launch has less than 2^32 threads (with more HIP starts some of them and reports nothing), so that 2^23
+// tokens go at once.
+template <typename T, int D>
+hipError_t launch_heads_as(HeadArgs p, hipStream_t s) {
+  constexpr int kMost = 1 << 23;
+  for (int left = p.tokens; left > 0; left -= kMost) {
+    p.tokens = left < kMost ? left : kMost;
+    if (hipError_t e = launch_some_heads<T, D>(p, s); e != hipSuccess) return e;
+    const auto on = [&](ave_fp4_heads& h, size_t element) {
+      if (h.data) h.data = static_cast<char*>(h.data) + h.token_stride * kMost * (int64_t)element;
+    };
+    on(p.q, sizeof(T)), on(p.k, sizeof(T)), on(p.v, sizeof(T)), on(p.q_out, 2), on(p.k_out, 2);
+    if (p.how.positions) p.how.positions += kMost;
+    if (p.slots) p.slots += kMost;
+  }
+  return hipSuccess;
 }
 
 // A lane takes eight channels of one head of one token.

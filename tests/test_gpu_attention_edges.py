@@ -35,6 +35,29 @@ def test_a_seen_value_with_a_nan_scale_counts_however_small_its_probability(gpu,
             assert torch.equal(got[~nan], want[~nan])
 
 
+def test_more_than_2_to_the_24_tokens(gpu):
+    """Head kernels take a workgroup a token: more workgroups than one launch may have threads for."""
+    t, d, rows = (1 << 24) + 37, 64, 64
+    x = torch.randn(rows, 1, d, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+    cos, sin = (torch.from_numpy(c).to(gpu) for c in A.tables(rows, d))
+    pos = (torch.arange(t, device=gpu) % rows).int()
+    many = x.repeat(t // rows + 1, 1, 1)[:t]
+    out, _ = ave.qk_norm_rope(many, None, cos, sin, pos)
+    want, _ = ave.qk_norm_rope(x, None, cos, sin, pos[:rows].contiguous())
+    whole = t // rows * rows
+    assert (out[:whole].view(-1, rows, 1, d) == want).all() and torch.equal(out[whole:], want[:t - whole])
+    del out
+    # appended: the last tokens alone are stored
+    cache = ave.kv_cache_mxfp4(4, 1, 16, d, gpu)
+    slots = torch.full((t,), -1, dtype=torch.int32, device=gpu)
+    slots[-rows:] = torch.arange(rows, dtype=torch.int32, device=gpu)
+    ave.append_kv_mxfp4(many, many, cache, slots, cos, sin, pos)
+    last = many[-rows:].contiguous()
+    small = ave.kv_cache_mxfp4(4, 1, 16, d, gpu)
+    ave.append_kv_mxfp4(last, last, small, torch.arange(rows, dtype=torch.int32, device=gpu), cos, sin, pos[-rows:].contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(cache, small))
+
+
 def test_more_than_2_to_the_32_units(gpu):
     """257 single tokens of 1024 heads over 2^20 keys, which are the same 64 keys again and again (one page): units of 64 keys."""
     heads, d, page, batch, keys = 1024, 64, 64, 257, 1 << 20
