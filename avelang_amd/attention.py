@@ -35,12 +35,19 @@ def kv_cache_mxfp4(pages, kv_heads, page_size, head_dim, device="cuda"):
     return make(head_dim // 2), make(head_dim // 32), make(head_dim // 2), make(head_dim // 32)
 
 
+def _sizes(t, name):
+    """``t``, whose sizes the C ABI takes as 32-bit numbers."""
+    if any(n > 2 ** 31 - 1 for n in t.shape):
+        raise ValueError(f"{name} must have sizes below 2^31, got {tuple(t.shape)}.")
+    return t
+
+
 def _cache(cache):
     """The C ABI's view of a cache; also its device.  (The library itself checks sizes and alignment.)"""
     if not isinstance(cache, (tuple, list)) or len(cache) != 4:
         raise TypeError("cache must be the tuple (k, k_scale, v, v_scale) of kv_cache_mxfp4.")
     names = ("k_cache", "k_scale", "v_cache", "v_scale")
-    parts = [_as_bytes(t, n) for t, n in zip(cache, names)]
+    parts = [_sizes(_as_bytes(t, n), n) for t, n in zip(cache, names)]
     k = parts[0]
     if k.dim() != 4:
         raise ValueError(f"k_cache must be 4-D [pages, kv_heads, page_size, head_dim/2], got {k.dim()}-D.")
@@ -68,6 +75,7 @@ def _heads(t, name, heads, head_dim, tokens, device, dtypes=(torch.bfloat16, tor
         raise ValueError(f"{name} must have dtype {' or '.join(map(str, dtypes))}, got {t.dtype}.")
     if t.dim() != 3:
         raise ValueError(f"{name} must be 3-D [tokens, heads, head_dim], got {t.dim()}-D.")
+    _sizes(t, name)
     want = (t.shape[0] if tokens is None else tokens, t.shape[1] if heads is None else heads, head_dim)
     if tuple(t.shape) != want:
         raise ValueError(f"{name} must have shape {want}, got {tuple(t.shape)}.")
@@ -81,7 +89,7 @@ def _heads(t, name, heads, head_dim, tokens, device, dtypes=(torch.bfloat16, tor
 def _vector(t, name, dtype, length, device):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise ValueError(f"{name} must be a {dtype} tensor.")
-    if tuple(t.shape) != (length,):
+    if tuple(_sizes(t, name).shape) != (length,):
         raise ValueError(f"{name} must have shape {(length,)}, got {tuple(t.shape)}.")
     if t.device != device:
         raise ValueError(f"{name} must be on device {device}, got {t.device}.")
@@ -98,6 +106,7 @@ def _how(cos, sin, positions, q_weight, k_weight, eps, neighbours, tokens, head_
         for t, name in ((cos, "cos"), (sin, "sin")):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 2:
                 raise ValueError(f"{name} must be a 2-D torch.float32 tensor [positions, rotary_dim/2].")
+            _sizes(t, name)
             if t.shape != cos.shape or t.device != device or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous, on device {device} and of cos's shape {tuple(cos.shape)}.")
         if positions is None:
@@ -121,6 +130,11 @@ def _bf16_out(t, name, like, head_dim, device):
 
 def _ref(x):
     return ctypes.byref(x) if x is not None else None
+
+
+def _int32(x):
+    """``x``, or the nearest number of 32 bits: no length comes near, and ctypes would drop the bits above."""
+    return max(-2 ** 31, min(int(x), 2 ** 31 - 1))
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None, q_out=None, k_out=None, *, eps=1e-6,
@@ -236,14 +250,14 @@ def attention_mxfp4(q, cache, page_table, seq_lens, cu_q=None, out=None, lse=Non
     t, heads, _ = q.shape
     if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or page_table.dim() != 2:
         raise ValueError("page_table must be a 2-D torch.int32 tensor [sequences, pages].")
-    b, width = page_table.shape
+    b, width = _sizes(page_table, "page_table").shape
     if page_table.device != dev:
         raise ValueError(f"page_table must be on device {dev}, got {page_table.device}.")
     if width > 1 and page_table.stride(1) != 1:
         raise ValueError("page_table must have consecutive entries in a row.")
     a = _lib.Attention(q=q.data_ptr(), q_token_stride=q.stride(0), q_head_stride=q.stride(1), page_table=page_table.data_ptr(),
-                       page_table_stride=page_table.stride(0), tokens=t, batch=b, heads=heads, table_pages=width, max_q=int(max_q),
-                       window=int(window or 0), causal=int(bool(causal)), scale=d ** -0.5 if scale is None else scale)
+                       page_table_stride=page_table.stride(0), tokens=t, batch=b, heads=heads, table_pages=width, max_q=_int32(max_q),
+                       window=_int32(window or 0), causal=int(bool(causal)), scale=d ** -0.5 if scale is None else scale)
     if not math.isfinite(a.scale):
         raise ValueError(f"scale must be finite, got {scale}.")
     a.seq_lens = _vector(seq_lens, "seq_lens", torch.int32, b, dev)

@@ -5,8 +5,9 @@ import os
 import subprocess
 
 import pytest
+import torch
 
-from avelang_amd import _lib
+from avelang_amd import _lib, attention as mod
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "avelang_amd", "csrc")
 
@@ -145,3 +146,16 @@ def test_sizes_next_to_2_to_the_31(page, pages, tokens, heads, text):
     else:
         assert lib.ave_fp4_attention_mxfp4(ctypes.byref(a), ctypes.byref(c), None, 0, None) == -1
         assert text in _lib.last_error(), _lib.last_error()
+
+
+def test_sizes_beyond_31_bits_are_refused():
+    """The C ABI's numbers of tokens, heads and pages have 32 bits: a larger size must not reach it cut to them."""
+    many = lambda *shape, dtype=torch.bfloat16: torch.empty(1, dtype=dtype, device="meta").expand(*shape)   # noqa: E731
+    with pytest.raises(ValueError, match="sizes below 2.31"):
+        mod._heads(many((1 << 32) + 1, 1, 64), "k", None, 64, None, torch.device("meta"))
+    with pytest.raises(ValueError, match="sizes below 2.31"):
+        mod._vector(many(1 << 31, dtype=torch.int32), "slots", torch.int32, 1 << 31, torch.device("meta"))
+    with pytest.raises(ValueError, match="sizes below 2.31"):
+        mod._cache([many(1 << 33, 1, 16, n, dtype=torch.uint8) for n in (64, 4, 64, 4)])
+    with pytest.raises(ValueError, match="sizes below 2.31"):
+        mod._how(*[many(1 << 31, 32, dtype=torch.float32)] * 2, None, None, None, 1e-6, False, 1, 64, torch.device("meta"))

@@ -35,6 +35,48 @@ def test_a_seen_value_with_a_nan_scale_counts_however_small_its_probability(gpu,
             assert torch.equal(got[~nan], want[~nan])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [[(1, 200)], [(20, 200)], [(150, 200)], [(1, 4000)], [(70, 4000)]], ids=str)
+@pytest.mark.parametrize("power", [10, 28, -100])
+def test_large_and_small_scores(gpu, d, rows, power):
+    """Every key is the same and every product -2^power: the mean of the values that a row sees.  (Beyond 2^30 fp32 has no bits left for what
+    a score differs by.)"""
+    hq, hkv = 4, 2
+    batch = A.Batch(rows, hq, hkv, d, 32, seed=32)
+    batch.cache[0][:] = 0x22                      # ones
+    batch.cache[1][:] = 127
+    batch.q[:] = -(2.0 ** power / d)
+    new, keys = rows[0]
+    n = keys - new + 1 + np.arange(new)
+    for scale in (0.125, 1.0, float(np.log(2.0))):
+        t = batch.tensors(gpu)
+        lse = torch.full(batch.q.shape[:2], float("nan"), device=gpu)
+        got = ave.attention_mxfp4(t["q"], t["cache"], t["page_table"], t["seq_lens"], t["cu_q"], None, lse, max_q=new, scale=scale)
+        got = got.double().cpu().numpy().reshape(new, hkv, -1, d)
+        for i in range(new):
+            v, size = (x[:n[i]].mean(0)[:, None] for x in (batch.v[0], np.abs(batch.v[0])))       # [hkv, 1, d]
+            # all probabilities are equal, one rounding (2^-9 of the numerator at most) apart from the sum's; fp32 sums of at most 128 steps
+            # a lane and the result's rounding
+            assert (np.abs(got[i] - v) <= 2.0 ** -8 * np.abs(v) + (2.0 ** -8 + 2.0 ** -16) * size).all(), (i, scale)
+        want = -scale * 2.0 ** power + np.log(n)
+        assert np.allclose(lse.double().cpu().numpy(), want[:, None], rtol=2.0 ** -20, atol=2.0 ** -16)
+
+
+def test_windows_beyond_31_bits(gpu):
+    batch = A.Batch([(1, 300), (40, 90)], 4, 2, 64, 16, seed=33)
+    t = batch.tensors(gpu)
+    call = lambda **kw: ave.attention_mxfp4(t["q"], t["cache"], t["page_table"], t["seq_lens"], t["cu_q"], **{"max_q": 40, **kw})   # noqa: E731
+    want = call()
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40 + 1, 2 ** 70):
+        assert torch.equal(call(window=window), want), window
+    assert torch.equal(call(max_q=2 ** 32 + 40), want)
+    for window in (-1, -2 ** 31 - 1, -2 ** 32, 1 - 2 ** 32):
+        with pytest.raises(ValueError, match="window must be non-negative"):
+            call(window=window)
+    with pytest.raises(ValueError, match="max_q"):
+        call(max_q=-2 ** 32 + 1)
+
+
 def test_more_than_2_to_the_24_tokens(gpu):
     """Head kernels take a workgroup a token: more workgroups than one launch may have threads for."""
     t, d, rows = (1 << 24) + 37, 64, 64
