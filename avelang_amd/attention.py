@@ -177,7 +177,8 @@ def append_kv_mxfp4(k, v, cache, slots, cos=None, sin=None, positions=None, k_we
                     eps=1e-6, neighbours=False):
     """Append keys and values of ``T`` tokens to a cache, with the keys' norm and rotation on the way.
 
-    ``k``, ``v`` ``[T, kv_heads, head_dim]`` bf16 or fp32; ``slots`` int32 ``[T]``: a slot outside the cache (-1) stores nothing.
+    ``k``, ``v`` ``[T, kv_heads, head_dim]`` bf16 or fp32; ``slots`` int32 ``[T]``: a slot outside the cache (-1) stores nothing;
+    those inside it must differ (what two tokens of a call share is undefined: a mix of both).
     ``cos``, ``sin``, ``positions``, ``k_weight``, ``eps``, ``neighbours`` as in :func:`qk_norm_rope` (all ``None``: the keys as they are).
     Codes and scales are those that :func:`quantize_mxfp4` gives for the fp32 values of the normed and rotated keys, and for the values.
     With ``q`` ``[T, heads, head_dim]`` the same launch norms (``q_weight``) and rotates the queries and returns them as bf16;

@@ -418,7 +418,8 @@ int ave_fp4_qk_norm_rope(const ave_fp4_heads* q, const ave_fp4_heads* k, int tok
 /*
  * Keys (normed and rotated as `how` says; null: as they are) and values of a batch of tokens into the cache at slots
  * [tokens]: the quantiser of ave_fp4_quantize_mxfp4_* per 32 channels, from fp32.  A slot outside the cache stores nothing (padding);
- * of two tokens with one slot either may stay.  With q the same launch norms and rotates the queries into q_out (bf16).
+ * what a slot inside it holds that two tokens of a call share is undefined -- tokens are written by workgroups of their own, codes and scales apart,
+ * so that it may be neither token -- and other slots are as they should be.  With q the same launch norms and rotates the queries into q_out (bf16).
  */
 int ave_fp4_append_kv_mxfp4(const ave_fp4_heads* k, const ave_fp4_heads* v, int tokens, const int32_t* slots, const ave_fp4_norm_rope* how,
                             const ave_fp4_kv_cache* cache, const ave_fp4_heads* q, const ave_fp4_heads* q_out, void* hip_stream);

@@ -145,3 +145,21 @@ def test_tables_wide_enough_for_units_beyond_32_bits(gpu, d, new):
         outs.append(out)
     if new == 40:
         assert torch.equal(*outs)      # the kernel for prompts: the same parts either way
+
+
+def test_tokens_that_share_a_slot_leave_the_others_alone(gpu):
+    """Padding that is all sent to one slot: that one's contents are undefined, every other token is in its place."""
+    heads, d, page, t = 3, 128, 16, 1500
+    g = torch.Generator().manual_seed(36)
+    k, v = (torch.randn(t, heads, d, generator=g).bfloat16().to(gpu) for _ in range(2))
+    slots = torch.randperm(2000, generator=g)[:t].int().to(gpu)
+    shared = int(slots[0])
+    slots[::3] = shared
+    one, other = (ave.kv_cache_mxfp4(125, heads, page, d, gpu) for _ in range(2))
+    ave.append_kv_mxfp4(k, v, one, slots)
+    keep = slots != shared
+    ave.append_kv_mxfp4(k[keep].contiguous(), v[keep].contiguous(), other, slots[keep].contiguous())
+    for a, b in zip(one, other):
+        a, b = (x.transpose(1, 2).flatten(0, 1) for x in (a, b))
+        a, b = (torch.cat([x[:shared], x[shared + 1:]]) for x in (a, b))
+        assert torch.equal(a, b)
