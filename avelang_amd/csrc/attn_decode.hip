@@ -194,11 +194,11 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
   }
   for (U u = part.u0; u < part.u1;) {
     const Item<U> it = item_of<ROWS, TILE, U>(p, u, b, b_begin, seq, per_head);
-    if (u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end)
+    if (!p.whole && first_item && threadIdx.x == 0) p.meta[blockIdx.x] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
+    if (u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end, and the second launch finds its record)
     unsigned from = (unsigned)(u - it.begin), to = it.units;   // units of the item
     if (!p.whole) {
       if (part.u1 - it.begin < to) to = (unsigned)(part.u1 - it.begin);
-      if (first_item && threadIdx.x == 0) p.meta[blockIdx.x] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
       u = it.begin + to;
     } else {   // the items that start in this part, as wholes
       u = it.begin + it.units;

@@ -214,10 +214,10 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       } else {
         it = item_of<kRows, kTile, U, true>(p, u, b, b_begin, seq, per_head);
       }
-      if (u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end)
+      if (first_item && tid == 0) p.meta[g] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
+      if (u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end, and the second launch finds its record)
       from = (unsigned)(u - it.begin), to = part.u1 - it.begin < it.units ? (unsigned)(part.u1 - it.begin) : it.units;
       u = it.begin + to;
-      if (first_item && tid == 0) p.meta[g] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
       first_item = false;
     }
     const unsigned start = (unsigned)p.item_units;   // unit of the item's first tile

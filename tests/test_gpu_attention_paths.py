@@ -76,3 +76,15 @@ def test_norm_and_rotation_of_every_shape_against_fp64(gpu, t, hq, hkv, d, rot, 
         # of 2^-24; one to bf16
         bound = 2.0 ** -8 * want.abs() + 32 * 2.0 ** -24 * 1.01 * size
         assert ((out.double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (10, 2, 128), (6, 2, 256), (40, 1, 128)], ids=str)
+def test_a_wrong_bound_on_new_tokens_costs_time_only(gpu, heads):
+    for rows in ([(150, 300), (1, 40), (20, 2500)], [(1, 70), (1, 3000)], [(0, 50), (2, 0), (9, 9)]):
+        batch = A.Batch(rows, *heads, 32, seed=46)
+        t = batch.tensors(gpu)
+        for how in ({}, {"window": 70}):
+            want, _, tol, _ = batch.reference(**how)
+            for max_q in (0, 1, 2, 9, 1000, 2 ** 31 - 1):
+                got = ave.attention_mxfp4(t["q"], t["cache"], t["page_table"], t["seq_lens"], t["cu_q"], max_q=max_q, **how)
+                assert (np.abs(got.float().cpu().numpy() - want) <= tol).all(), (rows, how, max_q)
