@@ -14,8 +14,10 @@ AttnArgs args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
 }
 
 // Row tiles of 16 of the kernel for few rows; 0: the kernel for prompts.  Up to 32 rows the former is ahead (64 sequences of 4096 keys,
-// 8 new tokens, 32 query heads on 8 of 128: 87 us to 117), from 33 the latter (64 query heads: 310 to 166), but for single tokens on
-// one key head of 128 channels (48 query heads, 16 sequences of 16384 keys: 47 to 56 us, one of 131072: 67 to 106).
+// 8 new tokens, 32 query heads on 8 of 128: 82 us to 122), from 33 the latter (64 query heads: 265 to 147), but for single tokens on
+// one key head of 128 channels (48 query heads, 16 sequences of 16384 keys: 45 to 46 us, one of 131072: 61 to 101).
+// Between 17 and 127 rows neither is near its floor: reads and products of these four take 46, 57, 6 and 3 us.  Four row tiles leave one wave a
+// SIMD and many parts of one item to join; a block of 128 rows with 64 in it leaves two of four waves without work.
 int decode_row_tiles(const AttnArgs& p) {
   const int new_tokens = p.a.cu_q ? p.a.max_q : 1;
   const int64_t rows = (int64_t)new_tokens * p.group;

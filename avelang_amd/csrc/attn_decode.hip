@@ -16,11 +16,11 @@
 // P is rounded to bf16 because the values' codes reach the matrix cores as bf16 without loss and the result is bf16 anyway: 2^-9 of a
 // probability, averaged over the keys.  Scores, maxima, sums and results are fp32.
 //
-// 32 heads on 8 of 128: 64 sequences of 2048 to 4096 keys 54 us (4.0 TB/s; of 16384 keys each 5.8, of 256 channels 5.7, of 64 4.9), one of
-// 131072 39.5 us.  Non-temporal hints on what nobody else reads are 4 of them (58.5 and 43 us without, 16384 keys 215 and 199).  About 15 us are
-// no traffic: the launches (5 each), and the way from the lengths by the table to the first keys.  For up to 16 rows four waves with two stages
-// each, two workgroups a compute unit, read ahead best (eight waves, one workgroup: 63 and 45 us); items that stay whole get eight waves, which
-// halve their way.
+// 32 heads on 8 of 128: 64 sequences of 2048 to 4096 keys 52 us (4.1 TB/s; of 16384 keys each 6.0, of 256 channels 6.1, of 64 5.4), one of
+// 131072 38 us.  A plain read of as many bytes takes 36 and 25 us; the rest is the second launch (7 with the gap in front of it) and the way from the
+// lengths by the table to the first keys.  Non-temporal hints on what nobody else reads gave 4 us (58.5 and 43 before, 16384 keys 215 to 199).  For
+// up to 16 rows four waves with two stages each, two workgroups a compute unit, read ahead best (eight waves, one workgroup: 63 and 45 us where this
+// came to 58 and 42); items that stay whole get eight waves, which halve their way.
 #include "attn_common.hpp"
 #include "kernels.hpp"
 
@@ -43,7 +43,7 @@ struct Shape {
 __device__ inline const uint8_t* pick(bool first, const uint8_t* a, const uint8_t* b) { return first ? a : b; }
 
 // Requests for stages.  ONE_PAGE: pages of 64 tokens and more, so that a stage lies in one page and its addresses are a scalar base and
-// a lane's fixed offset (four groups of 16 tokens in pages of their own cost four times the scalar arithmetic: 64 sequences of 16384 keys 197 us in pages of 64, 203 in
+// a lane's fixed offset (four groups of 16 tokens in pages of their own cost four times the scalar arithmetic: 64 sequences of 16384 keys 190 us in pages of 64, 204 in
 // pages of 16).
 template <int D, bool ONE_PAGE>
 struct Request {
@@ -496,9 +496,9 @@ hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
 
 // Short items stay whole: one launch, no partial results.  Cut in parts they cost a second launch and 128 bytes of partial results for each
 // row and 32 channels; whole they keep one workgroup each busy, which matters where there are few of them.  32 query heads on 8 of 128, one
-// sequence: single tokens 500 keys 9.6 us whole, 11.3 cut, 1500 keys 13.2 and 11.3; 8 tokens 13.7 and 16.8, 20.7 and 16.6; of 256 channels 500
-// keys 23.1 and 22.0.  16 sequences, 8 tokens, 1500 keys: 22.5 and 28.9, of 64 channels 17.5 and 28.9, of 256 45.0 and 39.8; 64 sequences of
-// 1500, single tokens: 30.9 and 27.3.  The bound on an item's keys is what the page table or the window can hold.
+// sequence: single tokens 500 keys 8.5 us whole, 11.1 cut, 1500 keys 13.5 and 11.0; 8 tokens 12.5 and 16.3, 19.0 and 16.1; of 256 channels 500
+// keys 13.2 and 12.9.  16 sequences, 8 tokens, 1500 keys: 21.2 and 30.8, of 64 channels 15.8 and 26.9, of 256 44.0 and 40.9; 64 sequences of
+// 1500, single tokens: 31.9 and 27.4.  The bound on an item's keys is what the page table or the window can hold.
 bool keep_whole(const AttnArgs& p, int row_tiles) {
   const int64_t in_table = (int64_t)p.a.table_pages << p.page_shift, in_window = p.a.window > 0 ? (int64_t)p.a.window + p.a.max_q : in_table;
   const bool many = 2 * (int64_t)p.a.batch * p.c.kv_heads >= compute_units() && (row_tiles > 1 || p.c.head_dim == 64);
@@ -593,8 +593,9 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs p, int ROWS)
 template <int D>
 void launch_combine_of(const AttnArgs& p, int rows, int64_t expected, int workgroups, hipStream_t s) {
   const unsigned x = (unsigned)workgroups - 1, at_once = 1024 / D, of_block = (unsigned)(expected < rows ? expected : rows);
-  // Many threads for a row of many parts (48 query heads on one, 131072 keys, 512 parts of one item: 106 us against 268), many rows at once
-  // for prompts (8192 tokens: 17 us against 110).  Items as far as the host knows; a part is at most one workgroup's.
+  // Many threads for a row of many parts (48 query heads on one, 131072 keys, 256 parts of one item: the call takes 61 us so, 132 with a thread
+  // for a row's four channels), many rows at once for prompts (600 new tokens of 4 sequences to 16000 keys: 356 us so, 394 with many threads for a
+  // row).  Items as far as the host knows; a part is at most one workgroup's.
   const int64_t items = (int64_t)p.a.batch * p.c.kv_heads * ((expected + rows - 1) / rows);
   if (of_block <= 32 || workgroups >= 8 * items)
     hipLaunchKernelGGL((attn_combine_kernel<D, 1024 / D>), dim3(x, of_block < 32 ? of_block : 32), dim3(256), 0, s, p, rows);

@@ -22,7 +22,7 @@
 //   - whole items instead of parts where that leaves little waiting (503 -> 480; six prompts of about 1000 tokens 88 -> 72).
 // (Cards differ by some per cent; a figure and the one it is compared with are of one card.)
 // 8192 tokens, 32 heads on 8 of 128: 459 us, 1.20 PFLOP/s of 4 D flop a score (the matrix cores also multiply the queries' second part, half as much
-// again); 4 sequences of up to 16000 keys, 600 new tokens, 40 heads on 8: 325 us, 1.09 PFLOP/s; six prompts of about 1000 tokens, 64 heads on 8 of 64:
+// again); 4 sequences of up to 16000 keys, 600 new tokens, 40 heads on 8: 320 us, 1.11 PFLOP/s; six prompts of about 1000 tokens, 64 heads on 8 of 64:
 // 67 us, where an item of 128 rows has but 8 tiles for its start and end, and half the work is exponentials.
 #include "attn_common.hpp"
 #include "kernels.hpp"
@@ -130,8 +130,8 @@ __device__ inline Item<U> ranked_item(const AttnArgs& p, const v4i* all, unsigne
   return it;
 }
 
-// SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 133 us, with 64-bit
-// bases for every tile 141).
+// SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 84 us, with 64-bit
+// bases for every tile 89).
 template <int D, bool SMALL, typename U>
 __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(AttnArgs p) {
   using S = Shape<D>;
@@ -592,9 +592,11 @@ size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p
 hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   const int workgroups = workgroups_of(p);
   p.whole = 0;
-  p.item_units = p.c.head_dim == 64 ? 2 : 3;   // (8192 tokens, 128 channels: with 1 674 us, 2 647, 3 and 4 633; prompts of 400, 64 channels: 2 80, 4 83)
+  // In parts: 2048 new tokens of 2 sequences of 16384 keys, 128 channels, with 1 950 us, 2 950, 3 947, 4 948; 300 prompts of 60 tokens, whose items have
+  // but one tile, 100, 107, 118, 118; 64 channels 106, 113, 112, 115.  (It also counts in the choice of whole items, whose bound was measured with it.)
+  p.item_units = p.c.head_dim == 64 ? 2 : 3;
   p.min_units_log2 = 2;
-  p.few_long = p.a.batch <= 8;   // (6 prompts of 1000: 135 us so, 142 otherwise; 16 of 500: 112 and 106)
+  p.few_long = p.a.batch <= 8;   // (one sequence, 4096 new tokens on 65536 keys: 3734 us so, 3771 otherwise; 8 with 40 on 2300: 54 and 49; 300 prompts of 60: 315 and 118)
   place_workspace(p, kRows, workgroups, ws);
   if (p.c.head_dim == 64) launch<64>(p, workgroups, s);
   else if (p.c.head_dim == 128) launch<128>(p, workgroups, s);

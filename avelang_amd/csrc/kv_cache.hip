@@ -9,7 +9,8 @@
 //
 // Bound by HBM for a prompt (each input read once, each output written once), by latency for a decode batch: one launch for
 // all roles of heads.  8192 tokens, 32 query and 8 key heads of 128, norm and rotation: 41 us, 4.2 TB/s; the append of 64 + 8 + 8 heads of 64:
-// 31 us, 5.1 TB/s (a large copy reaches 5.2); the way back 4.3 TB/s.  64 tokens of 32 + 8 + 8 heads of 128: 3.8 us in a graph.
+// 32 us, 5.0 TB/s (a large copy reaches 5.2); the way back 4.3 TB/s.  64 tokens of 32 + 8 + 8 heads of 128: 3.8 us in a graph.  From fp32 54 us
+// (4.8 TB/s) and 45 us (5.4).
 #include "fp4_common.hpp"
 #include "kv_cache.hpp"
 

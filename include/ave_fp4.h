@@ -441,8 +441,10 @@ int ave_fp4_gather_kv_mxfp4(const ave_fp4_kv_cache* cache, const int32_t* slots,
  * in its 32 channels, a scale of a value it sees from 253 on (beyond what bf16 holds; the quantiser writes 252 at most).
  * Rows of q behind cu_q[batch] are left alone.  Device data is never trusted with addresses: lengths are cut to the page
  * table's width, rows to q's, pages outside the cache are read as its nearest page.  Lengths, offsets and tables are read more than once: they must
- * not change before the call has run (then results are anybody's, and no access leaves q, out, table or cache).  Limits: tokens * heads below 2^31 - 2^14, a table of at
- * most 2^31 - 256 tokens, at most 1024 query heads on a key head.
+ * not change before the call has run (if they do, results are anybody's, and no access leaves q, out, table or cache).
+ * Limits: tokens * heads below 2^31 - 2^14, a table of at most 2^31 - 256 tokens, at most 1024 query heads on a key head.  In fp32 two scores beyond
+ * 2^30 no longer differ by less than 64, and a row's numerator, which is summed before it is divided and at up to 2^8 times the probabilities, may
+ * overflow for values beyond 2^100.
  * max_q: a bound on the new tokens of a sequence, by which the kernel is chosen (a wrong one costs time only).
  * The workspace (16-byte aligned, no initialisation, garbage afterwards; calls that may overlap need their own) takes the
  * partial results of sequences that several workgroups share; results do not depend on what it held.
