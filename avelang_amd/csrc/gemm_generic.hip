@@ -13,10 +13,11 @@ namespace ave {
 // SWIGLU: B holds 2N rows (gate rows, then up rows); a second accumulator takes the up projection of
 // the same columns and C = silu(gate) * up.
 template <bool SWIGLU>
-__global__ __launch_bounds__(256) void mx_generic_kernel(MxArgs p, unsigned n_blocks) {
+__global__ __launch_bounds__(256) void mx_generic_kernel(MxArgs p, unsigned n_blocks, unsigned first) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int r = lane & 31, h = lane >> 5;
-  const int bx = (int)(blockIdx.x % n_blocks), by = (int)(blockIdx.x / n_blocks);
+  const unsigned block = first + blockIdx.x;
+  const int bx = (int)(block % n_blocks), by = (int)(block / n_blocks);
   int m_begin = by * 32, m_end = p.M, expert = 0;
   if (p.row_offsets) {
     if (!locate_group_tile(p.row_offsets, p.E, p.M, 32, by, expert, m_begin, m_end)) return;
@@ -86,11 +87,12 @@ __device__ inline v8h dequant8_f16(unsigned codes, v2h s2) {
 // registers.  Per trip the wave consumes 64 k: lane (r, h) owns k in [64*i + 32*h, +32)
 // of row r = two 16-element scale blocks, fed to four MFMAs eight elements at a time
 // (A and B use the same assignment, so the K order inside a trip is immaterial).
-__global__ __launch_bounds__(256) void nv_generic_kernel(NvArgs p, unsigned n_blocks) {
+__global__ __launch_bounds__(256) void nv_generic_kernel(NvArgs p, unsigned n_blocks, unsigned first) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int r = lane & 31, h = lane >> 5;
-  const int m0 = (int)(blockIdx.x / n_blocks) * 32;
-  const int n0 = (int)(blockIdx.x % n_blocks) * 128 + wave * 32;
+  const unsigned block = first + blockIdx.x;
+  const int m0 = (int)(block / n_blocks) * 32;
+  const int n0 = (int)(block % n_blocks) * 128 + wave * 32;
   if (n0 >= p.N) return;
   const size_t row_bytes = (size_t)p.K / 2, row_scales = (size_t)p.K / kNvBlock;
   const int m = m0 + r, n = n0 + r;
@@ -138,11 +140,22 @@ __global__ __launch_bounds__(256) void nv_generic_kernel(NvArgs p, unsigned n_bl
 }
 
 // Workgroups of the shape-agnostic kernels for m_tiles 32-row tiles: ceil(N/128) * m_tiles in grid.x, 0 when that
-// exceeds what one grid dimension holds (2^31 - 1).
+// exceeds 2^31 - 1.
 unsigned generic_grid(int N, uint64_t m_tiles, unsigned* n_blocks) {
   *n_blocks = ((unsigned)N + 127u) / 128u;
   const uint64_t total = (uint64_t)*n_blocks * m_tiles;
   return total <= 0x7FFFFFFFull ? (unsigned)total : 0u;
+}
+
+// 2^23 workgroups of 256 at once: of 2^32 threads and more a launch starts a part and reports nothing.
+template <typename F>
+static hipError_t launch_some(unsigned grid, F launch) {
+  constexpr unsigned kMost = 1u << 23;
+  for (unsigned first = 0; first < grid; first += kMost) {
+    launch(first, grid - first < kMost ? grid - first : kMost);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_mx_generic(const MxArgs& p, hipStream_t s) {
@@ -150,9 +163,10 @@ hipError_t launch_mx_generic(const MxArgs& p, hipStream_t s) {
   unsigned n_blocks;
   const unsigned grid = generic_grid(p.N, ((uint64_t)p.M + 31) / 32 + (p.row_offsets ? (uint64_t)p.E : 0u), &n_blocks);
   if (grid == 0) return hipErrorInvalidConfiguration;
-  if (p.swiglu) hipLaunchKernelGGL(mx_generic_kernel<true>, dim3(grid), dim3(256), 0, s, p, n_blocks);
-  else hipLaunchKernelGGL(mx_generic_kernel<false>, dim3(grid), dim3(256), 0, s, p, n_blocks);
-  return hipGetLastError();
+  return launch_some(grid, [&](unsigned first, unsigned some) {
+    if (p.swiglu) hipLaunchKernelGGL(mx_generic_kernel<true>, dim3(some), dim3(256), 0, s, p, n_blocks, first);
+    else hipLaunchKernelGGL(mx_generic_kernel<false>, dim3(some), dim3(256), 0, s, p, n_blocks, first);
+  });
 }
 
 hipError_t launch_nv_generic(const NvArgs& p, hipStream_t s) {
@@ -160,8 +174,9 @@ hipError_t launch_nv_generic(const NvArgs& p, hipStream_t s) {
   unsigned n_blocks;
   const unsigned grid = generic_grid(p.N, ((uint64_t)p.M + 31) / 32, &n_blocks);
   if (grid == 0) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(nv_generic_kernel, dim3(grid), dim3(256), 0, s, p, n_blocks);
-  return hipGetLastError();
+  return launch_some(grid, [&](unsigned first, unsigned some) {
+    hipLaunchKernelGGL(nv_generic_kernel, dim3(some), dim3(256), 0, s, p, n_blocks, first);
+  });
 }
 
 }  // namespace ave
