@@ -18,9 +18,12 @@ from .attention import (  # noqa: F401
     append_kv_mxfp4,
     attention_mxfp4,
     gather_kv_mxfp4,
+    keep_kv_mxfp4,
     kv_cache_mxfp4,
     qk_norm_rope,
+    tree_attention_mxfp4,
 )
+from .drafts import draft_tree, verify_draft  # noqa: F401
 from .moe import gather_rows_mxfp4, moe_combine_top2, moe_route_top2  # noqa: F401
 from .scale_layout import blocked_numel, scales_from_blocked, scales_to_blocked  # noqa: F401
 
@@ -46,6 +49,10 @@ __all__ = [
     "append_kv_mxfp4",
     "gather_kv_mxfp4",
     "attention_mxfp4",
+    "draft_tree",
+    "tree_attention_mxfp4",
+    "verify_draft",
+    "keep_kv_mxfp4",
     "blocked_numel",
     "scales_to_blocked",
     "scales_from_blocked",

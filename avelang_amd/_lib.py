@@ -66,7 +66,24 @@ class Attention(ctypes.Structure):
         (n, _i32) for n in ("tokens", "batch", "heads", "table_pages", "max_q", "window", "causal")] + [("scale", ctypes.c_float)]
 
 
-_heads, _cache, _how, _attn = (ctypes.POINTER(c) for c in (Heads, KVCache, NormRope, Attention))
+class Tree(ctypes.Structure):
+    """``ave_fp4_tree``"""
+    _fields_ = [("seen", _vp), ("stride", _i64), ("words", _i32)]
+
+
+class Draft(ctypes.Structure):
+    """``ave_fp4_draft``"""
+    _fields_ = [("logits", _vp), ("logits_stride", _i64)] + [(n, _vp) for n in ("tokens", "parents", "cu_q", "uniform", "temperature", "draft_probs")] + [
+        ("draft_probs_stride", _i64)] + [(n, _vp) for n in ("accepted", "path", "emitted")] + [(n, _i32) for n in ("rows", "batch", "vocab", "logits_f32")]
+
+
+class Keep(ctypes.Structure):
+    """``ave_fp4_keep``"""
+    _fields_ = [("page_table", _vp), ("page_table_stride", _i64)] + [(n, _vp) for n in ("seq_lens", "cu_q", "path", "accepted", "kept_lens")] + [
+        (n, _i32) for n in ("tokens", "batch", "table_pages", "max_q")]
+
+
+_heads, _cache, _how, _attn, _tree, _draft, _keep = (ctypes.POINTER(c) for c in (Heads, KVCache, NormRope, Attention, Tree, Draft, Keep))
 
 #: symbol -> argtypes; every symbol ``include/ave_fp4.h`` and ``include/ave_fp4_debug.h`` declare
 SIGNATURES = {
@@ -126,6 +143,12 @@ SIGNATURES = {
     "ave_fp4_gather_kv_mxfp4": [_cache, _vp, _int, _vp, _vp, _vp],
     "ave_fp4_attention_mxfp4_workspace_bytes": [_attn, _cache],
     "ave_fp4_attention_mxfp4": [_attn, _cache, _vp, ctypes.c_size_t, _vp],
+    "ave_fp4_draft_tree": [_vp, _vp, _vp, _int, _int, _vp, _int, _vp, _vp],
+    "ave_fp4_tree_attention_mxfp4_workspace_bytes": [_attn, _tree, _cache],
+    "ave_fp4_tree_attention_mxfp4": [_attn, _tree, _cache, _vp, ctypes.c_size_t, _vp],
+    "ave_fp4_verify_draft_workspace_bytes": [_draft],
+    "ave_fp4_verify_draft": [_draft, _vp, ctypes.c_size_t, _vp],
+    "ave_fp4_keep_kv_mxfp4": [_cache, _int, _keep, _vp],
     "ave_fp4_last_error": [],
     "ave_fp4_abi_version": [],
     "ave_fp4_debug_weights_from_hbm": [_vp, ctypes.c_size_t],
@@ -149,7 +172,9 @@ _RESTYPES = {"ave_fp4_last_error": ctypes.c_char_p, "ave_fp4_gemm_mxfp4_workspac
              "ave_fp4_gemm_mxfp4_swiglu_workspace_bytes": ctypes.c_size_t,
              "ave_fp4_gemm_nvfp4_workspace_bytes": ctypes.c_size_t,
              "ave_fp4_moe_route_top2_workspace_bytes": ctypes.c_size_t,
-             "ave_fp4_attention_mxfp4_workspace_bytes": ctypes.c_size_t}
+             "ave_fp4_attention_mxfp4_workspace_bytes": ctypes.c_size_t,
+             "ave_fp4_tree_attention_mxfp4_workspace_bytes": ctypes.c_size_t,
+             "ave_fp4_verify_draft_workspace_bytes": ctypes.c_size_t}
 
 
 def library_path() -> str:

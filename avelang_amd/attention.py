@@ -245,6 +245,37 @@ def attention_mxfp4(q, cache, page_table, seq_lens, cu_q=None, out=None, lse=Non
     done = _native.attention_mxfp4(q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, causal)
     if done is not None:
         return done
+    return _attention(q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, causal)
+
+
+def tree_attention_mxfp4(q, cache, page_table, seq_lens, cu_q, seen, out=None, lse=None, *, max_q=None, scale=None, window=0, sinks=None):
+    """:func:`attention_mxfp4` of drafted tokens that are not a chain: with ``n`` new tokens (nodes) in a sequence, each sees the tokens before all
+    of them and, of the nodes, those whose bit is set in its row of ``seen`` (int64 ``[T, words]``, as :func:`draft_tree` makes it; rows may be strided;
+    bit ``j % 64`` of word ``j // 64``: node ``j`` of the sequence).  ``window``: the last ``window`` of what a node sees (nodes are seen as the bits
+    say, and ``window`` less their number of the tokens before them).  The rest, and what is returned, as there."""
+    if max_q is None:
+        max_q = 1 if cu_q is None else q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
+    done = _native.tree_attention_mxfp4(q, cache, page_table, seq_lens, cu_q, seen, out, lse, max_q, scale, window, sinks)
+    if done is not None:
+        return done
+    if seen is None:
+        raise ValueError("seen is required.")
+    return _attention(q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, True, seen)
+
+
+def _tree(seen, tokens, device):
+    if not isinstance(seen, torch.Tensor) or seen.dtype != torch.int64 or seen.dim() != 2:
+        raise ValueError("seen must be a 2-D torch.int64 tensor [nodes, words].")
+    if _sizes(seen, "seen").shape[0] != tokens or seen.shape[1] < 1:
+        raise ValueError(f"seen must have {tokens} rows of at least one word, got {tuple(seen.shape)}.")
+    if seen.device != device:
+        raise ValueError(f"seen must be on device {device}, got {seen.device}.")
+    if seen.shape[1] > 1 and seen.stride(1) != 1:
+        raise ValueError("seen must have consecutive words in a row.")
+    return _lib.Tree(seen.data_ptr(), seen.stride(0) if tokens > 1 else seen.shape[1], seen.shape[1])
+
+
+def _attention(q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, causal, seen=None):
     c, dev = _cache(cache)
     d = c.head_dim
     _heads(q, "q", None, d, None, dev, (torch.bfloat16,))
@@ -277,9 +308,53 @@ def attention_mxfp4(q, cache, page_table, seq_lens, cu_q=None, out=None, lse=Non
             raise ValueError(f"lse must be a contiguous torch.float32 tensor of shape {(t, heads)} on device {dev}.")
         a.lse = lse.data_ptr()
     lib = _lib.load()
+    given = (_ref(a), _ref(c)) if seen is None else (_ref(a), _ref(_tree(seen, t, dev)), _ref(c))
+    name = "ave_fp4_attention_mxfp4" if seen is None else "ave_fp4_tree_attention_mxfp4"
     with torch.cuda.device(dev):
-        bytes_ = lib.ave_fp4_attention_mxfp4_workspace_bytes(_ref(a), _ref(c))
+        bytes_ = getattr(lib, name + "_workspace_bytes")(*given)
         workspace = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
-        rc = lib.ave_fp4_attention_mxfp4(_ref(a), _ref(c), workspace.data_ptr() if bytes_ else None, bytes_, _stream_ptr(dev))
+        rc = getattr(lib, name)(*given, workspace.data_ptr() if bytes_ else None, bytes_, _stream_ptr(dev))
     _lib.check(rc)
     return out
+
+
+def keep_kv_mxfp4(caches, page_table, seq_lens, cu_q, path, accepted, kept_lens=None, *, max_q=None):
+    """Move the kept ones of each sequence's last tokens together, in the caches of all layers at once.  Returns int32 ``kept_lens`` ``[B]``.
+
+    ``caches``: one cache, or a list of them of one shape.  Of the last ``n = cu_q[b+1] - cu_q[b]`` tokens of sequence ``b``, those at ``path[cu_q[b] + i]``,
+    ``i < accepted[b]`` (int32 ``[T]`` and ``[B]``; rising), go to places ``seq_lens[b] - n + i``, keys, values and scales as they are; ``kept_lens`` is
+    ``seq_lens - n + accepted``, the lengths that are left (it must not be one of the inputs).  With what :func:`verify_draft` returns a checked draft
+    becomes part of its sequence; with ``n`` the whole sequence, tokens that a policy gives up leave the cache.  What stands behind the kept
+    tokens stays as it was.  Pages that hold moved tokens must belong to one sequence only.  ``max_q``: a bound on ``n``, if the host knows one; it
+    helps to choose the kernel."""
+    done = _native.keep_kv_mxfp4(caches, page_table, seq_lens, cu_q, path, accepted, kept_lens, max_q)
+    if done is not None:
+        return done
+    if isinstance(caches, (tuple, list)) and len(caches) == 4 and all(isinstance(t, torch.Tensor) for t in caches):
+        caches = [caches]
+    if not isinstance(caches, (tuple, list)) or not caches:
+        raise TypeError("caches must be a cache or a list of caches.")
+    views = [_cache(c) for c in caches]
+    dev = views[0][1]
+    if any(d != dev for _, d in views):
+        raise ValueError(f"all caches must be on device {dev}.")
+    if not isinstance(path, torch.Tensor) or path.dim() != 1 or not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError("path must be a 1-D and page_table a 2-D torch.int32 tensor.")
+    b, width = _sizes(page_table, "page_table").shape
+    if page_table.device != dev:
+        raise ValueError(f"page_table must be on device {dev}, got {page_table.device}.")
+    if width > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table must have consecutive entries in a row.")
+    t = path.shape[0]
+    k = _lib.Keep(page_table=page_table.data_ptr(), page_table_stride=page_table.stride(0), tokens=t, batch=b, table_pages=width,
+                  max_q=_int32(t if max_q is None else max_q))
+    k.seq_lens, k.cu_q = _vector(seq_lens, "seq_lens", torch.int32, b, dev), _vector(cu_q, "cu_q", torch.int32, b + 1, dev)
+    k.path, k.accepted = _vector(path, "path", torch.int32, t, dev), _vector(accepted, "accepted", torch.int32, b, dev)
+    if kept_lens is None:
+        kept_lens = torch.empty(b, dtype=torch.int32, device=dev)
+    k.kept_lens = _vector(kept_lens, "kept_lens", torch.int32, b, dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        rc = lib.ave_fp4_keep_kv_mxfp4((_lib.KVCache * len(views))(*(c for c, _ in views)), len(views), _ref(k), _stream_ptr(dev))
+    _lib.check(rc)
+    return kept_lens

@@ -4,8 +4,9 @@
 namespace ave {
 namespace {
 
-AttnArgs args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
-  AttnArgs p{};
+template <typename A = AttnArgs>
+A args_of(const ave_fp4_attention& a, const ave_fp4_kv_cache& c) {
+  A p{};
   p.a = a, p.c = c;
   set_group(p, a.heads / c.kv_heads);
   p.q_aligned = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
@@ -35,6 +36,26 @@ size_t attention_workspace_bytes(const ave_fp4_attention& a, const ave_fp4_kv_ca
 
 hipError_t launch_attention(const ave_fp4_attention& a, const ave_fp4_kv_cache& c, void* workspace, hipStream_t s) {
   const AttnArgs args = args_of(a, c);
+  if (const int tiles = decode_row_tiles(args)) return launch_attn_decode(args, tiles, workspace, s);
+  return launch_attn_prompt(args, workspace, s);
+}
+
+namespace {
+TreeArgs tree_args(const ave_fp4_attention& a, const ave_fp4_tree& t, const ave_fp4_kv_cache& c) {
+  TreeArgs p = args_of<TreeArgs>(a, c);
+  p.seen = t.seen, p.seen_stride = t.stride, p.words = t.words;
+  return p;
+}
+}  // namespace
+
+size_t tree_attention_workspace_bytes(const ave_fp4_attention& a, const ave_fp4_tree& t, const ave_fp4_kv_cache& c) {
+  const TreeArgs p = tree_args(a, t, c);
+  if (const int tiles = decode_row_tiles(p)) return attn_decode_workspace(p, tiles);
+  return attn_prompt_workspace(p);
+}
+
+hipError_t launch_tree_attention(const ave_fp4_attention& a, const ave_fp4_tree& t, const ave_fp4_kv_cache& c, void* workspace, hipStream_t s) {
+  const TreeArgs args = tree_args(a, t, c);
   if (const int tiles = decode_row_tiles(args)) return launch_attn_decode(args, tiles, workspace, s);
   return launch_attn_prompt(args, workspace, s);
 }

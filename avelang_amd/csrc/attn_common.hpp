@@ -62,8 +62,8 @@ __device__ inline Units wave_scan(Units v) {   // of numbers whose sum is below 
   return wave_scan((unsigned)v & 0x3FFFFFFu) + ((Units)wave_scan((unsigned)(v >> 26)) << 26);
 }
 // Units of one key head of a sequence of many blocks, which the lanes of a wave share
-template <int ROWS, int TILE, typename U>
-__device__ inline U wave_sequence_units(const AttnArgs& p, const Sequence& s) {
+template <int ROWS, int TILE, typename U, typename A>
+__device__ inline U wave_sequence_units(const A& p, const Sequence& s) {
   U u = 0;
   int tile0;
   const int rows = s.n * p.group, lane = threadIdx.x & 63;
@@ -76,8 +76,8 @@ __device__ inline U wave_sequence_units(const AttnArgs& p, const Sequence& s) {
 
 // The part of workgroup g.  Every wave finds it by itself (no barrier): 64 sequences at a time, a lane each.
 // LONG: sequences may have many blocks of rows; where p.few_long says so the wave takes one sequence after the other.
-template <int ROWS, int TILE, typename U, bool LONG = false>
-__device__ inline Part<U> take_part(const AttnArgs& p, unsigned g, unsigned workgroups) {
+template <int ROWS, int TILE, typename U, bool LONG = false, typename A>
+__device__ inline Part<U> take_part(const A& p, unsigned g, unsigned workgroups) {
   if constexpr (LONG) {
     if (p.few_long) {
       Part<U> r{};
@@ -142,8 +142,8 @@ struct Item {
 };
 // The item that holds unit u >= b_begin; moves b, b_begin, the sequence s and its units of one head on to it.  (Where lengths change under the call
 // it may end before u, and never begins behind it.)
-template <int ROWS, int TILE, typename U, bool LONG = false>
-__device__ inline Item<U> item_of(const AttnArgs& p, U u, int& b, U& b_begin, Sequence& s, U& per_head) {
+template <int ROWS, int TILE, typename U, bool LONG = false, typename A>
+__device__ inline Item<U> item_of(const A& p, U u, int& b, U& b_begin, Sequence& s, U& per_head) {
   Item<U> it;
   // (u is below the number of all units; the bounds on b and row0 hold if lengths change under the call, too)
   while (u >= b_begin + per_head * (unsigned)p.c.kv_heads && b + 1 < p.a.batch) {
@@ -222,6 +222,38 @@ __device__ inline int page_of(const AttnArgs& p, int entry) {
   return page < p.c.pages ? page : p.c.pages - 1;
 }
 __device__ inline int page_at(const AttnArgs& p, ConstInts row, int token, int len) { return page_of(p, page_entry(p, row, token, len)); }
+
+// ---- a tree of drafted tokens ---------------------------------------------------------------------------------------------------
+template <typename A>
+inline constexpr bool kTree = false;
+template <>
+inline constexpr bool kTree<TreeArgs> = true;
+
+// Bits `at` .. `at` + 15 of a row of words, counted from 0 at its first; what lies outside the words or from bit n on is not set
+__device__ inline unsigned bits_of(const TreeArgs& p, const uint64_t* row, int n, int at) {
+  if (n <= 0 || at <= -16 || at >= n) return 0u;
+  const int word = at >> 6, bit = at & 63;   // (word -1: bits below the first)
+  const uint64_t a = word >= 0 && word < p.words ? row[word] : 0, b = bit > 48 && word + 1 < p.words ? row[word + 1] : 0;
+  unsigned r = (unsigned)(a >> bit);
+  if (bit > 48) r |= (unsigned)(b << (64 - bit));
+  return r & (n - at >= 16 ? 0xFFFFu : (1u << (n - at)) - 1);
+}
+__device__ inline const uint64_t* row_bits(const TreeArgs& p, const Sequence& s, int t) { return p.seen + (int64_t)(s.first + t) * p.seen_stride; }
+// First key that a row may see: the window counts back from the last of what it sees, the new tokens among it
+__device__ inline int first_seen(const TreeArgs& p, const Sequence& s, int t) {
+  if (p.a.window <= 0) return 0;
+  const uint64_t* row = row_bits(p, s, t);
+  int many = 0;
+  for (int w = 0; w < p.words && 64 * w < s.n; ++w) many += __popcll(s.n - 64 * w >= 64 ? row[w] : row[w] & ((1ull << (s.n - 64 * w)) - 1));
+  const int64_t lo = (int64_t)s.len - s.n + many - p.a.window;
+  return lo < 0 ? 0 : (int)lo;
+}
+// Which of the 16 keys from `key` on new token t sees, lo = first_seen: those before the new tokens from lo on, and its bits
+__device__ inline unsigned seen_of(const TreeArgs& p, const Sequence& s, int t, int lo, int key) {
+  const int base = s.len - s.n, from = lo - key, to = base - key;
+  const unsigned before = (to > 15 ? 0xFFFFu : to > 0 ? (1u << to) - 1 : 0u) & (from > 15 ? 0u : from > 0 ? ~0u << from : ~0u);
+  return before | (key + 15 >= base ? bits_of(p, row_bits(p, s, t), s.n, key - base) : 0u);
+}
 
 // A value that all lanes hold, in a scalar register
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -363,10 +395,13 @@ __device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int chan
   if (p.a.lse && channel == 0) p.a.lse[row] = e.lse;
 }
 
-hipError_t launch_attn_prompt(AttnArgs p, void* workspace, hipStream_t s);
+template <typename A>
+hipError_t launch_attn_prompt(A p, void* workspace, hipStream_t s);
 size_t attn_prompt_workspace(const AttnArgs& p);
-hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* workspace, hipStream_t s);
-size_t attn_decode_workspace(const AttnArgs& p, int row_tiles);
+template <typename A>
+hipError_t launch_attn_decode(A p, int row_tiles, void* workspace, hipStream_t s);
+template <typename A>
+size_t attn_decode_workspace(const A& p, int row_tiles);
 // rows: of a block; rows_expected: of a sequence and key head
 hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s);
 // meta, maxima and sums, partial results, in this order

@@ -170,8 +170,8 @@ constexpr int workgroups_per_cu() {
   return lds_bytes<D, NT, NW, NS>() <= 78 * 1024 ? 2 : 1;
 }
 
-template <int D, int NT, int NW, int NS, bool ONE_PAGE, typename U>
-__global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW / 4)) void attn_decode_kernel(AttnArgs p) {
+template <int D, int NT, int NW, int NS, bool ONE_PAGE, typename U, typename A>
+__global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW / 4)) void attn_decode_kernel(A p) {
   using S = Shape<D>;
   constexpr int ROWS = NT * 16, TILE = 64, C = D / 16;   // C: channel tiles of 16
   constexpr bool kEarly = NT == 1;            // registers for a whole stage beside the rest
@@ -213,15 +213,16 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
     // what the rows see
-    int lo_row[NT], hi_row[NT], lo_max, hi_min, dummy;
+    int lo_row[NT], hi_row[NT], lo_max, hi_min;   // hi_row: of a tree the row's token
     {
       const int last = it.row0 + ROWS < rows ? it.row0 + ROWS - 1 : rows - 1;
-      visible(p, it.s, p.token_of(it.row0), dummy, hi_min);
-      visible(p, it.s, p.token_of(last), lo_max, dummy);
+      const Bounds all = bounds(p, it.s, p.token_of(it.row0), p.token_of(last));
+      lo_max = all.lo_max, hi_min = all.hi_min;
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
-        const int row = it.row0 + ct * 16 + col;
-        visible(p, it.s, p.token_of(row < rows ? row : last), lo_row[ct], hi_row[ct]);
+        const int row = it.row0 + ct * 16 + col, t = p.token_of(row < rows ? row : last);
+        if constexpr (kTree<A>) lo_row[ct] = rows > 0 ? first_seen(p, it.s, t) : 0, hi_row[ct] = t;
+        else visible(p, it.s, t, lo_row[ct], hi_row[ct]);
       }
     }
     const int mine = it.s.len > 0 && tiles > wave ? (tiles - wave + NW - 1) / NW : 0;   // tiles wave, wave + NW, ...
@@ -318,9 +319,17 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
       // ---- probabilities
       const bool all_seen = t0 >= lo_max && t0 + TILE <= hi_min;
       unsigned prob[NT][8], bias[NT][8];   // pairs of tokens 16 g + 2 i, + 1; what is taken from their exponents
+      unsigned seen[NT];                   // of a tree: a bit for each of this group's 16 tokens
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
-        if (!all_seen) {
+        seen[ct] = 0xFFFFu;
+        if constexpr (kTree<A>) {
+          if (!all_seen) {
+            seen[ct] = seen_of(p, it.s, hi_row[ct], lo_row[ct], t0 + 16 * g);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[ct][j / 4][j % 4] = seen[ct] >> j & 1 ? s[ct][j / 4][j % 4] : kNone;
+          }
+        } else if (!all_seen) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -379,9 +388,8 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
         }
       };
       if (nan) {   // a row that sees a value with a NaN scale, however little it counts: its block of channels is NaN
-        unsigned seen[NT];   // a bit for each of this group's 16 tokens
 #pragma unroll
-        for (int ct = 0; ct < NT; ++ct) {
+        for (int ct = 0; ct < NT && !kTree<A>; ++ct) {
           const int from = lo_row[ct] - t0 - 16 * g, to = hi_row[ct] - t0 - 16 * g;
           seen[ct] = (to > 15 ? 0xFFFFu : to > 0 ? (1u << to) - 1 : 0u) & (from > 15 ? 0u : from > 0 ? ~0u << from : ~0u);
         }
@@ -475,8 +483,8 @@ __global__ __launch_bounds__(NW * 64, (workgroups_per_cu<D, NT, NW, NS>() * NW /
   }
 }
 
-template <int D, int NT, int NW, int NS, typename U = unsigned>
-hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
+template <int D, int NT, int NW, int NS, typename U = unsigned, typename A>
+hipError_t launch_form(A p, bool whole, void* ws, hipStream_t s) {
   constexpr int ROWS = NT * 16;
   const int workgroups = compute_units() * workgroups_per_cu<D, NT, NW, NS>();
   p.whole = whole;
@@ -485,10 +493,10 @@ hipError_t launch_form(AttnArgs p, bool whole, void* ws, hipStream_t s) {
   if (!p.whole) place_workspace(p, ROWS, workgroups, ws);
   const dim3 grid((unsigned)workgroups), block(NW * 64);
   if constexpr (sizeof(U) == 4) {
-    if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true, U>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false, U>), grid, block, 0, s, p);
+    if (p.c.page_size >= 64) hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, true, U, A>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false, U, A>), grid, block, 0, s, p);
   } else {   // (pages of any size by the general form)
-    hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false, U>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((attn_decode_kernel<D, NT, NW, NS, false, U, A>), grid, block, 0, s, p);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.whole) return e;
   return launch_attn_combine(p, ROWS, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
@@ -506,15 +514,18 @@ bool keep_whole(const AttnArgs& p, int row_tiles) {
 }
 
 // More units than 32 bits hold (a call of seconds): one form for each number of channels, of two row tiles
-bool in_64_bits(const AttnArgs& p, int row_tiles) { return units_bound(p, row_tiles * 16, 64) >> 32 != 0; }
+template <typename A>
+bool in_64_bits(const A& p, int row_tiles) { return units_bound(p, row_tiles * 16, 64) >> 32 != 0; }
 
 }  // namespace
 
-size_t attn_decode_workspace(const AttnArgs& p, int row_tiles) {
+template <typename A>
+size_t attn_decode_workspace(const A& p, int row_tiles) {
   return keep_whole(p, row_tiles) ? 0 : attn_workspace((in_64_bits(p, row_tiles) ? 2 : row_tiles) * 16, p.c.head_dim, 2 * compute_units());
 }
 
-hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s) {
+template <typename A>
+hipError_t launch_attn_decode(A p, int row_tiles, void* ws, hipStream_t s) {
   const bool whole = keep_whole(p, row_tiles);
   if (in_64_bits(p, row_tiles)) {
     if (p.c.head_dim == 64) return launch_form<64, 2, 4, 4, Units>(p, whole, ws, s);
@@ -531,6 +542,11 @@ hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s
     default: return launch_form<256, 2, 4, 2>(p, whole, ws, s);
   }
 }
+
+template size_t attn_decode_workspace(const AttnArgs& p, int row_tiles);
+template hipError_t launch_attn_decode(AttnArgs p, int row_tiles, void* ws, hipStream_t s);
+template size_t attn_decode_workspace(const TreeArgs& p, int row_tiles);
+template hipError_t launch_attn_decode(TreeArgs p, int row_tiles, void* ws, hipStream_t s);
 
 // ---- parts of split items, joined -----------------------------------------------------------------------------------------------
 namespace {

@@ -98,8 +98,8 @@ __device__ inline unsigned items_below(const AttnArgs& p, const v4i* all, unsign
     for (int b0 = 64; b0 < kSequences; b0 += 64) mine += of_lane(b0);   // (nothing behind the last sequence)
   return (unsigned)p.c.kv_heads * (unsigned)lane_value((int)wave_scan(mine), 63);
 }
-template <int ROWS, typename U>
-__device__ inline Item<U> ranked_item(const AttnArgs& p, const v4i* all, unsigned rank, int& b) {   // rank: below the number of items
+template <int ROWS, typename U, typename A>
+__device__ inline Item<U> ranked_item(const A& p, const v4i* all, unsigned rank, int& b) {   // rank: below the number of items
   const unsigned heads = (unsigned)p.c.kv_heads;
   unsigned level = 0, step = 1;   // the level: the last one with at most `rank` items below it
   while (items_below(p, all, level + step) <= rank) level += step, step *= 2;
@@ -130,10 +130,16 @@ __device__ inline Item<U> ranked_item(const AttnArgs& p, const v4i* all, unsigne
   return it;
 }
 
+// Of a tree: which of the 16 keys from `key` on a row of a sequence sees (a row behind the last: what that one does)
+__device__ inline unsigned tree_bits(const TreeArgs& p, const Sequence& s, int row, int rows, int key) {
+  const int t = p.token_of(row < rows ? row : rows - 1);
+  return seen_of(p, s, t, first_seen(p, s, t), key);
+}
+
 // SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 84 us, with 64-bit
 // bases for every tile 89).
-template <int D, bool SMALL, typename U>
-__global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(AttnArgs p) {
+template <int D, bool SMALL, typename U, typename A>
+__global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(A p) {
   using S = Shape<D>;
   constexpr int C = S::C;
   __shared__ __align__(512) unsigned char smem[S::kLds];
@@ -230,8 +236,13 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     const int row0 = uniform(it.row0 + 32 * wave);
     const bool active = row0 < uniform(rows);
     int lo_max, hi_min, lo_min, hi_max;
-    visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
-    visible(p, it.s, p.token_of(row0 + 32 < rows ? row0 + 31 : rows - 1), lo_max, hi_max);
+    if constexpr (kTree<A>) {
+      const Bounds all = bounds(p, it.s, 0, 0);
+      lo_max = all.lo_max, hi_min = all.hi_min, lo_min = all.lo_min, hi_max = all.hi_max;
+    } else {
+      visible(p, it.s, p.token_of(active ? row0 : 0), lo_min, hi_min);
+      visible(p, it.s, p.token_of(row0 + 32 < rows ? row0 + 31 : rows - 1), lo_max, hi_max);
+    }
     lo_max = uniform(lo_max), hi_min = uniform(hi_min), lo_min = uniform(lo_min), hi_max = uniform(hi_max);
 
     // ---- a tile's requests: keys and their scales to LDS, values to registers; a wave takes 16 tokens, which lie in one page
@@ -413,12 +424,18 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       const int key0 = tile * kTile + 32 * j;
       if (key0 < lo_max || key0 + 32 > hi_min) {
         const int here = lane_here();
-        int lo, hi;
-        visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);   // (a row behind the last: whatever)
-        const int from = lo - key0 - here / 32 * 16;
-        const unsigned many = (unsigned)(hi > lo ? hi - lo : 0);
+        if constexpr (kTree<A>) {
+          const unsigned seen = tree_bits(p, it.s, row0 + here % 32, rows, key0 + here / 32 * 16);
 #pragma unroll
-        for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
+          for (int t = 0; t < 16; ++t) s[t] = seen >> t & 1 ? s[t] : kNone;
+        } else {
+          int lo, hi;
+          visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);   // (a row behind the last: whatever)
+          const int from = lo - key0 - here / 32 * 16;
+          const unsigned many = (unsigned)(hi > lo ? hi - lo : 0);
+#pragma unroll
+          for (int t = 0; t < 16; ++t) s[t] = (unsigned)(t - from) < many ? s[t] : kNone;
+        }
       }
       float sum;
       const auto exponentials = [&](float reference) {
@@ -454,10 +471,18 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       // ---- values with a NaN scale, zeros in LDS: NaN for the rows that see them, however little they count
       if (nan) {
         const int here = lane_here(), key = tile * kTile + 32 * j + here / 32 * 16;
-        int lo, hi;
-        visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);
-        const int from = lo - key, to = hi - key;   // four bits for each of this lane's 16 keys
-        const uint64_t some = (to > 15 ? ~0ull : to > 0 ? (1ull << 4 * to) - 1 : 0ull) & (from > 15 ? 0ull : from > 0 ? ~0ull << 4 * from : ~0ull);
+        uint64_t some;   // four bits for each of this lane's 16 keys
+        if constexpr (kTree<A>) {
+          const unsigned seen = tree_bits(p, it.s, row0 + here % 32, rows, key);
+          some = 0;
+#pragma unroll
+          for (int t = 0; t < 16; ++t) some |= (seen >> t & 1 ? 0xFull : 0ull) << 4 * t;
+        } else {
+          int lo, hi;
+          visible(p, it.s, p.token_of(row0 + here % 32), lo, hi);
+          const int from = lo - key, to = hi - key;
+          some = (to > 15 ? ~0ull : to > 0 ? (1ull << 4 * to) - 1 : 0ull) & (from > 15 ? 0ull : from > 0 ? ~0ull << 4 * from : ~0ull);
+        }
 #pragma unroll
         for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
           const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
@@ -574,22 +599,23 @@ int workgroups_of(const AttnArgs& p) {
   const int d = p.c.head_dim;
   return compute_units() * (d == 64 ? waves_per_simd<64>() : d == 128 ? waves_per_simd<128>() : waves_per_simd<256>());
 }
-template <int D>
-void launch(const AttnArgs& p, int workgroups, hipStream_t s) {
+template <int D, typename A>
+void launch(const A& p, int workgroups, hipStream_t s) {
   const dim3 grid((unsigned)workgroups), block(kWaves * 64);
   const int64_t last = p.c.pages - 1, page = (int64_t)p.c.kv_heads * p.c.page_size * D / 2;   // bytes of codes; of scales a 16th
   const auto small = [&](int64_t stride, int64_t bytes) { return last * stride + bytes <= (int64_t)1 << 32; };
   const bool all = small(p.c.k_page_stride, page) && small(p.c.v_page_stride, page) && small(p.c.k_scale_page_stride, page / 16) && small(p.c.v_scale_page_stride, page / 16);
-  if (units_bound(p, kRows, kTile) >> 32) hipLaunchKernelGGL((attn_prompt_kernel<D, false, Units>), grid, block, 0, s, p);   // (a call of seconds)
-  else if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true, unsigned>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((attn_prompt_kernel<D, false, unsigned>), grid, block, 0, s, p);
+  if (units_bound(p, kRows, kTile) >> 32) hipLaunchKernelGGL((attn_prompt_kernel<D, false, Units, A>), grid, block, 0, s, p);   // (a call of seconds)
+  else if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true, unsigned, A>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attn_prompt_kernel<D, false, unsigned, A>), grid, block, 0, s, p);
 }
 
 }  // namespace
 
 size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p.c.head_dim, workgroups_of(p)); }
 
-hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
+template <typename A>
+hipError_t launch_attn_prompt(A p, void* ws, hipStream_t s) {
   const int workgroups = workgroups_of(p);
   p.whole = 0;
   // In parts: 2048 new tokens of 2 sequences of 16384 keys, 128 channels, with 1 950 us, 2 950, 3 947, 4 948; 300 prompts of 60 tokens, whose items have
@@ -604,5 +630,8 @@ hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s) {
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   return launch_attn_combine(p, kRows, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
 }
+
+template hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s);
+template hipError_t launch_attn_prompt(TreeArgs p, void* ws, hipStream_t s);
 
 }  // namespace ave

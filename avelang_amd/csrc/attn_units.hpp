@@ -37,6 +37,13 @@ struct AttnArgs {
 
   AVE_BOTH inline int token_of(int row) const { return group == 1 ? row : (int)((unsigned)((uint64_t)(unsigned)row * group_mul >> 32) >> group_shift); }
 };
+// The same for a tree of drafted tokens: the new tokens of a sequence see all keys before them, or the last p.a.window of what they see, and of each
+// other those that their row of bits says.
+struct TreeArgs : AttnArgs {
+  const uint64_t* seen;   // bit j % 64 of word j / 64 of a token's row: new token j of its sequence
+  int64_t seen_stride;    // words between rows
+  int words;              // of a row
+};
 // 2^(31+s) / d rounded up with s = ceil(log2 d) has an error below 2^-31 of a quotient, so that n < 2^31 is divided exactly.
 inline void set_group(AttnArgs& p, int group) {
   p.group = group;
@@ -65,22 +72,37 @@ AVE_BOTH inline void visible(const AttnArgs& p, const Sequence& s, int t, int& l
   lo = p.a.window > 0 && pos >= p.a.window ? pos - p.a.window + 1 : 0;
 }
 
+// Rows t_first to t_last: [lo_min, hi_max) is what any of them sees at most, all of them see [lo_max, hi_min)
+struct Bounds {
+  int lo_min, lo_max, hi_min, hi_max;
+};
+AVE_BOTH inline Bounds bounds(const AttnArgs& p, const Sequence& s, int t_first, int t_last) {
+  Bounds r;
+  visible(p, s, t_first, r.lo_min, r.hi_min);
+  visible(p, s, t_last, r.lo_max, r.hi_max);
+  return r;
+}
+AVE_BOTH inline Bounds bounds(const TreeArgs& p, const Sequence& s, int, int) {   // (a row sees none to all of the n new tokens)
+  const int base = s.len - s.n, before = base < 0 ? 0 : base, w = p.a.window;
+  const int lo_min = w > 0 && base > w ? base - w : 0, lo_max = w > 0 && s.len > w ? s.len - w : 0;
+  return {lo_min, lo_max, before, s.len};
+}
+
 // A block of rows: units (those for its start come before its tiles), and the first tile
-template <int ROWS, int TILE>
-AVE_BOTH inline int block_units(const AttnArgs& p, const Sequence& s, int row0, int& tile0) {
+template <int ROWS, int TILE, typename A>
+AVE_BOTH inline int block_units(const A& p, const Sequence& s, int row0, int& tile0) {
   const int rows = s.n * p.group, last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
-  int lo, hi, other;
   if (rows <= 0) {
     tile0 = 0;
     return 1 + p.item_units;
   }
-  visible(p, s, p.token_of(row0), lo, other);
-  visible(p, s, p.token_of(last), other, hi);
+  const Bounds b = bounds(p, s, p.token_of(row0), p.token_of(last));
+  const int lo = b.lo_min, hi = b.hi_max;
   tile0 = lo / TILE;
   return (hi > lo ? (hi + TILE - 1) / TILE - tile0 : 1) + p.item_units;
 }
-template <int ROWS, int TILE, typename U>
-AVE_BOTH inline U sequence_units(const AttnArgs& p, const Sequence& s) {   // of one key head
+template <int ROWS, int TILE, typename U, typename A>
+AVE_BOTH inline U sequence_units(const A& p, const Sequence& s) {   // of one key head
   U u = 0;
   int tile0;
   for (int row0 = 0; row0 < s.n * p.group; row0 += ROWS) u += (unsigned)block_units<ROWS, TILE>(p, s, row0, tile0);
@@ -93,6 +115,12 @@ inline Units units_bound(const AttnArgs& p, int rows_of_block, int tile) {
   const Units in_table = ((Units)p.a.table_pages << p.page_shift) / tile + 1, in_window = ((Units)p.a.window + rows_of_block) / tile + 2;
   const Units tiles = p.a.window > 0 && in_window < in_table ? in_window : in_table;
   return blocks * p.c.kv_heads * (tiles + p.item_units);
+}
+
+inline Units units_bound(const TreeArgs& p, int rows_of_block, int tile) {   // (a block also sees all new tokens of its sequence)
+  AttnArgs q = p;
+  if (p.a.window > 0) q.a.window = p.a.window > INT32_MAX - p.a.tokens ? INT32_MAX : p.a.window + p.a.tokens;
+  return units_bound(q, rows_of_block, tile);
 }
 
 // The part of a workgroup: units [u0, u1) of all `units`, cut into `parts` equal ones; sequence b holds u0, b_begin is its first unit and

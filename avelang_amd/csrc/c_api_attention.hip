@@ -167,4 +167,103 @@ int ave_fp4_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_kv_cache* 
   return finish(ave::launch_attention(*a, *cache, workspace, static_cast<hipStream_t>(hip_stream)), "attention kernel");
 }
 
+static int check_tree(const ave_fp4_attention* a, const ave_fp4_tree* t, const ave_fp4_kv_cache* cache, ave_fp4_attention* with_causal) {
+  if (!a || !t) return fail_inval("null arguments.");
+  *with_causal = *a;
+  with_causal->causal = 1;
+  if (int rc = check_attention(with_causal, cache)) return rc;
+  if (t->words <= 0 || t->words > 1 << 25) return fail_inval("seen must have between 1 and 2^25 words a row, got %d.", t->words);
+  if (t->stride < 0 || (t->stride > 0 && t->stride < t->words)) return fail_inval("rows of seen overlap: %d words, %lld apart.", t->words, (long long)t->stride);
+  return 0;
+}
+
+size_t ave_fp4_tree_attention_mxfp4_workspace_bytes(const ave_fp4_attention* a, const ave_fp4_tree* tree, const ave_fp4_kv_cache* cache) {
+  ave::clear_error();
+  ave_fp4_attention args;
+  if (check_tree(a, tree, cache, &args) != 0 || args.tokens == 0 || args.batch == 0) return 0;
+  return ave::tree_attention_workspace_bytes(args, *tree, *cache);
+}
+
+int ave_fp4_tree_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_tree* tree, const ave_fp4_kv_cache* cache, void* workspace,
+                                 size_t workspace_bytes, void* hip_stream) {
+  ave::clear_error();
+  ave_fp4_attention args;
+  if (int rc = check_tree(a, tree, cache, &args)) return rc;
+  if (args.tokens == 0 || args.batch == 0) return 0;
+  if (!args.q || !args.out || !args.seq_lens || !tree->seen || (!args.page_table && args.table_pages > 0)) return fail_inval("null device pointer.");
+  if (!aligned(args.q, 2) || !aligned(args.out, 4) || !aligned(tree->seen, 8)) return fail_inval("q must be 2-byte, out 4-byte and seen 8-byte aligned.");
+  const size_t need = ave::tree_attention_workspace_bytes(args, *tree, *cache);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail_inval("the workspace must have %zu bytes, got %zu.", need, workspace ? workspace_bytes : (size_t)0);
+  if (need > 0 && !aligned(workspace, 16)) return fail_inval("the workspace must be 16-byte aligned.");
+  return finish(ave::launch_tree_attention(args, *tree, *cache, workspace, static_cast<hipStream_t>(hip_stream)), "tree attention kernel");
+}
+
+int ave_fp4_draft_tree(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens, int batch, uint64_t* seen, int words,
+                       int32_t* positions, void* hip_stream) {
+  ave::clear_error();
+  if (tokens < 0 || batch < 0) return fail_inval("tokens and batch must be non-negative, got %d and %d.", tokens, batch);
+  if (seen && (words <= 0 || words > 1 << 25)) return fail_inval("seen must have between 1 and 2^25 words a row, got %d.", words);
+  if (tokens == 0 || batch == 0 || (!seen && !positions)) return 0;
+  if (!parents || !cu_q || (positions && !seq_lens)) return fail_inval("null device pointer.");
+  if (!aligned(seen, 8)) return fail_inval("seen must be 8-byte aligned.");
+  return finish(ave::launch_draft_tree(parents, cu_q, seq_lens, tokens, batch, seen, seen ? words : 0, positions, static_cast<hipStream_t>(hip_stream)),
+                "draft tree kernel");
+}
+
+static int check_draft(const ave_fp4_draft* d) {
+  if (!d) return fail_inval("null arguments.");
+  if (d->rows < 0 || d->batch < 0) return fail_inval("rows and batch must be non-negative, got %d and %d.", d->rows, d->batch);
+  if (d->vocab <= 0 || d->vocab > 1 << 30) return fail_inval("vocab must be from 1 to 2^30, got %d.", d->vocab);
+  if ((int64_t)d->rows * ((d->vocab + ave::kVocabPiece - 1) / ave::kVocabPiece) >= 1 << 24)   // workgroups of a launch
+    return fail_inval("rows times vocab / %d must be below 2^24, got %d x %d.", ave::kVocabPiece, d->rows, d->vocab);
+  return 0;
+}
+
+size_t ave_fp4_verify_draft_workspace_bytes(const ave_fp4_draft* draft) {
+  ave::clear_error();
+  if (check_draft(draft) != 0 || draft->batch == 0) return 0;
+  return ave::verify_draft_workspace_bytes(*draft);
+}
+
+int ave_fp4_verify_draft(const ave_fp4_draft* draft, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  ave::clear_error();
+  if (int rc = check_draft(draft)) return rc;
+  const ave_fp4_draft& d = *draft;
+  if (d.batch == 0) return 0;
+  if (!d.cu_q || !d.accepted || (d.rows > 0 && (!d.logits || !d.tokens || !d.parents || !d.uniform || !d.path || !d.emitted)))
+    return fail_inval("null device pointer.");
+  if (!aligned(d.logits, d.logits_f32 ? 4 : 2) || !aligned(d.draft_probs, 4)) return fail_inval("logits and draft_probs must be aligned to their elements.");
+  const size_t need = ave::verify_draft_workspace_bytes(d);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail_inval("the workspace must have %zu bytes, got %zu.", need, workspace ? workspace_bytes : (size_t)0);
+  if (need > 0 && !aligned(workspace, 16)) return fail_inval("the workspace must be 16-byte aligned.");
+  return finish(ave::launch_verify_draft(d, workspace, static_cast<hipStream_t>(hip_stream)), "draft verification kernel");
+}
+
+int ave_fp4_keep_kv_mxfp4(const ave_fp4_kv_cache* caches, int layers, const ave_fp4_keep* keep, void* hip_stream) {
+  ave::clear_error();
+  if (layers <= 0) return fail_inval("there must be layers, got %d.", layers);
+  if (!caches || !keep) return fail_inval("null arguments.");
+  for (int i = 0; i < layers; ++i) {
+    const ave_fp4_kv_cache &c = caches[i], &c0 = caches[0];
+    if (int rc = check_cache(&c)) return rc;
+    if (c.pages != c0.pages || c.kv_heads != c0.kv_heads || c.page_size != c0.page_size || c.head_dim != c0.head_dim)
+      return fail_inval("all caches must have one shape: layer %d differs from layer 0.", i);
+    for (int j = 0; j < i; ++j)
+      if (caches[j].k == c.k || caches[j].v == c.v) return fail_inval("layers %d and %d have the same cache.", j, i);
+  }
+  const ave_fp4_keep& k = *keep;
+  if (k.tokens < 0 || k.batch < 0 || k.table_pages < 0 || k.max_q < 0)
+    return fail_inval("tokens, batch, table_pages and max_q must be non-negative, got %d, %d, %d and %d.", k.tokens, k.batch, k.table_pages, k.max_q);
+  if ((int64_t)k.table_pages * caches->page_size > INT32_MAX)
+    return fail_inval("the page table must cover at most 2^31 - 1 tokens, got %d pages of %d.", k.table_pages, caches->page_size);
+  if (k.batch == 0) return 0;
+  if (!k.seq_lens || !k.cu_q || !k.accepted || (k.tokens > 0 && !k.path) || (k.table_pages > 0 && !k.page_table)) return fail_inval("null device pointer.");
+  const auto overlaps = [&](const int32_t* p, int64_t n) { return k.kept_lens && p < k.kept_lens + k.batch && k.kept_lens < p + n; };
+  if (overlaps(k.seq_lens, k.batch) || overlaps(k.cu_q, (int64_t)k.batch + 1) || overlaps(k.path, k.tokens) || overlaps(k.accepted, k.batch))
+    return fail_inval("kept_lens must not overlap an input.");
+  return finish(ave::launch_keep_kv(caches, layers, k, static_cast<hipStream_t>(hip_stream)), "key/value keep kernel");
+}
+
 }  // extern "C"

@@ -579,51 +579,173 @@ PyObject* gather_kv_mxfp4(PyObject* const* arg) {
   return ok ? pair_of(k, v) : nullptr;
 }
 
-// q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, causal
-PyObject* attention_mxfp4(PyObject* const* arg) {
+// [rows, columns] with consecutive elements in a row
+bool strided_rows(const Tensor& t, c10::Device dev, at::ScalarType dtype) {
+  return t.scalar_type() == dtype && t.dim() == 2 && t.device() == dev && fits(t.size(0)) && fits(t.size(1)) && (t.size(1) <= 1 || t.stride(1) == 1);
+}
+
+// q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks; seen: null without a tree
+PyObject* attention_of(PyObject* q_, PyObject* cache_, PyObject* table_, PyObject* lens_, PyObject* cu_, PyObject* out_, PyObject* lse_, PyObject* max_q,
+                       PyObject* scale, PyObject* window, PyObject* sinks_, bool causal, PyObject* seen_) {
   Cache cache;
-  const Tensor *q = tensor(arg[0]), *table = tensor(arg[2]), *lens = tensor(arg[3]);
-  if (!cache.take(arg[1]) || !q || !table || !lens) NOT_MINE;
+  const Tensor *q = tensor(q_), *table = tensor(table_), *lens = tensor(lens_);
+  if (!cache.take(cache_) || !q || !table || !lens) NOT_MINE;
   const auto dev = cache.dev;
   const int64_t d = cache.c.head_dim;
   if (q->scalar_type() != at::kBFloat16 || q->dim() != 3 || q->device() != dev || q->size(2) != d || q->stride(2) != 1 || !fits(q->size(0)) || !fits(q->size(1)))
     NOT_MINE;
-  if (table->scalar_type() != at::kInt || table->dim() != 2 || table->device() != dev || (table->size(1) > 1 && table->stride(1) != 1) ||
-      !fits(table->size(0)) || !fits(table->size(1)))
-    NOT_MINE;
+  if (!strided_rows(*table, dev, at::kInt)) NOT_MINE;
   const int64_t t = q->size(0), heads = q->size(1), b = table->size(0);
   if (!vec(*lens, dev, b, at::kInt)) NOT_MINE;
   ave_fp4_attention a{};
   a.q = ptr_as<uint16_t>(*q), a.q_token_stride = q->stride(0), a.q_head_stride = q->stride(1);
   a.page_table = ptr_as<int32_t>(*table), a.page_table_stride = table->stride(0), a.seq_lens = ptr_as<int32_t>(*lens);
   a.tokens = (int)t, a.batch = (int)b, a.heads = (int)heads, a.table_pages = (int)table->size(1);
-  if (arg[4] != Py_None) {
-    const Tensor* cu = tensor(arg[4]);
+  if (cu_ != Py_None) {
+    const Tensor* cu = tensor(cu_);
     if (!cu || !vec(*cu, dev, b + 1, at::kInt)) NOT_MINE;
     a.cu_q = ptr_as<int32_t>(*cu);
   }
-  if (arg[10] != Py_None) {
-    const Tensor* sinks = tensor(arg[10]);
+  if (sinks_ != Py_None) {
+    const Tensor* sinks = tensor(sinks_);
     if (!sinks || !vec(*sinks, dev, heads, at::kFloat)) NOT_MINE;
     a.sinks = ptr_as<float>(*sinks);
   }
-  if (arg[6] != Py_None) {
-    const Tensor* lse = tensor(arg[6]);
+  if (lse_ != Py_None) {
+    const Tensor* lse = tensor(lse_);
     if (!lse || lse->scalar_type() != at::kFloat || !matrix(*lse, dev, t, heads)) NOT_MINE;
     a.lse = ptr_as<float>(*lse);
   }
-  if (!as_int(arg[7], &a.max_q) || !as_int(arg[9], &a.window) || !PyBool_Check(arg[11])) NOT_MINE;
-  a.causal = arg[11] == Py_True;
-  if (arg[8] == Py_None) a.scale = d == 64 ? 0.125f : d == 256 ? 0.0625f : 0.08838834764831845f;
-  else if (!as_float(arg[8], &a.scale) || !std::isfinite(a.scale)) NOT_MINE;
+  if (!as_int(max_q, &a.max_q) || !as_int(window, &a.window)) NOT_MINE;
+  a.causal = causal;
+  if (scale == Py_None) a.scale = d == 64 ? 0.125f : d == 256 ? 0.0625f : 0.08838834764831845f;
+  else if (!as_float(scale, &a.scale) || !std::isfinite(a.scale)) NOT_MINE;
+  ave_fp4_tree tree{};
+  if (seen_) {
+    const Tensor* seen = tensor(seen_);
+    if (!seen || !strided_rows(*seen, dev, at::kLong) || seen->size(0) != t || seen->size(1) < 1) NOT_MINE;
+    tree = {ptr_as<uint64_t>(*seen), t > 1 ? seen->stride(0) : seen->size(1), (int32_t)seen->size(1)};
+  }
   Out out;
-  if (!out.take(arg[5], {t, heads, d}, at::kBFloat16, dev)) NOT_MINE;
+  if (!out.take(out_, {t, heads, d}, at::kBFloat16, dev)) NOT_MINE;
   a.out = ptr_as<uint16_t>(out.t);
-  const size_t bytes = on_device(dev, [&] { return ave_fp4_attention_mxfp4_workspace_bytes(&a, &cache.c); });
+  const size_t bytes = on_device(dev, [&] {
+    return seen_ ? ave_fp4_tree_attention_mxfp4_workspace_bytes(&a, &tree, &cache.c) : ave_fp4_attention_mxfp4_workspace_bytes(&a, &cache.c);
+  });
   Tensor ws;
   if (bytes) ws = empty({(int64_t)bytes}, at::kByte, dev);
-  const bool ok = launch(dev, [&](void* s) { return ave_fp4_attention_mxfp4(&a, &cache.c, bytes ? ptr(ws) : nullptr, bytes, s); });
+  const bool ok = launch(dev, [&](void* s) {
+    return seen_ ? ave_fp4_tree_attention_mxfp4(&a, &tree, &cache.c, bytes ? ptr(ws) : nullptr, bytes, s)
+                 : ave_fp4_attention_mxfp4(&a, &cache.c, bytes ? ptr(ws) : nullptr, bytes, s);
+  });
   return ok ? out.object() : nullptr;
+}
+// q, cache, page_table, seq_lens, cu_q, out, lse, max_q, scale, window, sinks, causal
+PyObject* attention_mxfp4(PyObject* const* arg) {
+  if (!PyBool_Check(arg[11])) NOT_MINE;
+  return attention_of(arg[0], arg[1], arg[2], arg[3], arg[4], arg[5], arg[6], arg[7], arg[8], arg[9], arg[10], arg[11] == Py_True, nullptr);
+}
+// q, cache, page_table, seq_lens, cu_q, seen, out, lse, max_q, scale, window, sinks
+PyObject* tree_attention_mxfp4(PyObject* const* arg) {
+  return attention_of(arg[0], arg[1], arg[2], arg[3], arg[4], arg[6], arg[7], arg[8], arg[9], arg[10], arg[11], true, arg[5]);
+}
+
+// ---- a tree of drafted tokens ---------------------------------------------------------------------------------------------------------
+// parents, cu_q, seq_lens, seen, positions, max_q
+PyObject* draft_tree(PyObject* const* arg) {
+  const Tensor *parents = tensor(arg[0]), *cu = tensor(arg[1]), *lens = tensor(arg[2]);
+  int max_q;
+  if (!parents || !cu || !lens || !parents->is_cuda() || parents->dim() != 1 || !fits(parents->size(0)) || cu->dim() != 1 || cu->size(0) < 1 ||
+      !fits(cu->size(0)) || !as_int(arg[5], &max_q) || max_q < 1)
+    NOT_MINE;
+  const auto dev = parents->device();
+  const int64_t t = parents->size(0), b = cu->size(0) - 1, words = ((int64_t)max_q + 63) / 64;
+  if (words > 1 << 25 || !vec(*parents, dev, t, at::kInt) || !vec(*cu, dev, b + 1, at::kInt) || !vec(*lens, dev, b, at::kInt)) NOT_MINE;
+  Out seen, positions;
+  if (!seen.take(arg[3], {t, words}, at::kLong, dev) || !positions.take(arg[4], {t}, at::kInt, dev)) NOT_MINE;
+  const bool ok = launch(dev, [&](void* s) {
+    return ave_fp4_draft_tree(ptr_as<int32_t>(*parents), ptr_as<int32_t>(*cu), ptr_as<int32_t>(*lens), (int)t, (int)b, ptr_as<uint64_t>(seen.t), (int)words,
+                              ptr_as<int32_t>(positions.t), s);
+  });
+  return ok ? pair_of(seen, positions) : nullptr;
+}
+
+// logits, tokens, parents, cu_q, uniform, temperature, draft_probs, accepted, path, emitted
+PyObject* verify_draft(PyObject* const* arg) {
+  const Tensor *logits = tensor(arg[0]), *tokens = tensor(arg[1]), *parents = tensor(arg[2]), *cu = tensor(arg[3]), *uniform = tensor(arg[4]);
+  if (!logits || !tokens || !parents || !cu || !uniform || !logits->is_cuda() || !is_float(*logits) || cu->dim() != 1 || cu->size(0) < 1 || !fits(cu->size(0)))
+    NOT_MINE;
+  const auto dev = logits->device();
+  if (!strided_rows(*logits, dev, logits->scalar_type())) NOT_MINE;
+  const int64_t t = logits->size(0), v = logits->size(1), b = cu->size(0) - 1;
+  if (!vec(*tokens, dev, t, at::kInt) || !vec(*parents, dev, t, at::kInt) || !vec(*cu, dev, b + 1, at::kInt) || !vec(*uniform, dev, t, at::kFloat)) NOT_MINE;
+  ave_fp4_draft d{};
+  d.logits = ptr(*logits), d.logits_stride = logits->stride(0), d.logits_f32 = logits->scalar_type() == at::kFloat;
+  d.tokens = ptr_as<int32_t>(*tokens), d.parents = ptr_as<int32_t>(*parents), d.cu_q = ptr_as<int32_t>(*cu), d.uniform = ptr_as<float>(*uniform);
+  d.rows = (int)t, d.batch = (int)b, d.vocab = (int)v;
+  if (arg[5] != Py_None) {
+    const Tensor* temperature = tensor(arg[5]);
+    if (!temperature || !vec(*temperature, dev, b, at::kFloat)) NOT_MINE;
+    d.temperature = ptr_as<float>(*temperature);
+  }
+  if (arg[6] != Py_None) {
+    const Tensor* probs = tensor(arg[6]);
+    if (!probs || !strided_rows(*probs, dev, at::kFloat) || probs->size(0) != t || probs->size(1) != v) NOT_MINE;
+    d.draft_probs = ptr_as<float>(*probs), d.draft_probs_stride = probs->stride(0);
+  }
+  Out accepted, path, emitted;
+  if (!accepted.take(arg[7], {b}, at::kInt, dev) || !path.take(arg[8], {t}, at::kInt, dev) || !emitted.take(arg[9], {t}, at::kInt, dev)) NOT_MINE;
+  d.accepted = ptr_as<int32_t>(accepted.t), d.path = ptr_as<int32_t>(path.t), d.emitted = ptr_as<int32_t>(emitted.t);
+  const size_t bytes = ave_fp4_verify_draft_workspace_bytes(&d);
+  Tensor ws;
+  if (bytes) ws = empty({(int64_t)bytes}, at::kByte, dev);
+  if (!launch(dev, [&](void* s) { return ave_fp4_verify_draft(&d, bytes ? ptr(ws) : nullptr, bytes, s); })) return nullptr;
+  PyObject* x = accepted.object();
+  PyObject* y = x ? path.object() : nullptr;
+  PyObject* z = y ? emitted.object() : nullptr;
+  PyObject* r = z ? PyTuple_Pack(3, x, y, z) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  Py_XDECREF(z);
+  return r;
+}
+
+// caches, page_table, seq_lens, cu_q, path, accepted, kept_lens, max_q
+PyObject* keep_kv_mxfp4(PyObject* const* arg) {
+  constexpr int kMost = 256;   // layers; more go through Python
+  const Tensor *table = tensor(arg[1]), *lens = tensor(arg[2]), *cu = tensor(arg[3]), *path = tensor(arg[4]), *accepted = tensor(arg[5]);
+  if (!table || !lens || !cu || !path || !accepted || path->dim() != 1 || !fits(path->size(0))) NOT_MINE;
+  ave_fp4_kv_cache caches[kMost];
+  int layers = 1;
+  Cache one;
+  if (one.take(arg[0])) {
+    caches[0] = one.c;
+  } else {
+    if (!PyList_CheckExact(arg[0]) && !PyTuple_CheckExact(arg[0])) NOT_MINE;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(arg[0]);
+    if (n < 1 || n > kMost) NOT_MINE;
+    layers = (int)n;
+    for (int i = 0; i < layers; ++i) {
+      Cache c;
+      if (!c.take(PySequence_Fast_GET_ITEM(arg[0], i)) || (i > 0 && c.dev != one.dev)) NOT_MINE;
+      caches[i] = c.c;
+      one.dev = c.dev;
+    }
+  }
+  const auto dev = one.dev;
+  if (!strided_rows(*table, dev, at::kInt)) NOT_MINE;
+  const int64_t t = path->size(0), b = table->size(0);
+  if (!vec(*lens, dev, b, at::kInt) || !vec(*cu, dev, b + 1, at::kInt) || !vec(*path, dev, t, at::kInt) || !vec(*accepted, dev, b, at::kInt)) NOT_MINE;
+  ave_fp4_keep k{};
+  k.page_table = ptr_as<int32_t>(*table), k.page_table_stride = table->stride(0), k.table_pages = (int)table->size(1);
+  k.seq_lens = ptr_as<int32_t>(*lens), k.cu_q = ptr_as<int32_t>(*cu), k.path = ptr_as<int32_t>(*path), k.accepted = ptr_as<int32_t>(*accepted);
+  k.tokens = (int)t, k.batch = (int)b, k.max_q = (int)t;
+  if (arg[7] != Py_None && !as_int(arg[7], &k.max_q)) NOT_MINE;
+  Out kept;
+  if (!kept.take(arg[6], {b}, at::kInt, dev)) NOT_MINE;
+  k.kept_lens = ptr_as<int32_t>(kept.t);
+  if (!launch(dev, [&](void* s) { return ave_fp4_keep_kv_mxfp4(caches, layers, &k, s); })) return nullptr;
+  return kept.object();
 }
 
 // ---- the module -------------------------------------------------------------------------------------------------------------
@@ -657,6 +779,10 @@ PyMethodDef kMethods[] = {
     ENTRY(append_kv_mxfp4, 13),
     ENTRY(gather_kv_mxfp4, 4),
     ENTRY(attention_mxfp4, 12),
+    ENTRY(tree_attention_mxfp4, 12),
+    ENTRY(draft_tree, 6),
+    ENTRY(verify_draft, 10),
+    ENTRY(keep_kv_mxfp4, 8),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_calls", "the package's entry points on torch tensors, in C++", -1, kMethods, nullptr, nullptr, nullptr, nullptr};

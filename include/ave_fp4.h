@@ -465,6 +465,91 @@ size_t ave_fp4_attention_mxfp4_workspace_bytes(const ave_fp4_attention* a, const
 int ave_fp4_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_kv_cache* cache, void* workspace, size_t workspace_bytes,
                             void* hip_stream);
 
+/*
+ * ---- Checking a tree of drafted tokens ----
+ *
+ * A draft proposes several tokens behind the last decided one, possibly with alternatives: a tree.  Its nodes are appended to the cache as the
+ * last tokens of their sequence (nodes cu_q[b] .. cu_q[b+1]-1 of all nodes, a parent before its children, node 0 the decided token), the
+ * target model runs on all of them at once, and the nodes that it would have drawn itself are kept.  No counterpart in the reference.
+ *
+ * From the nodes' parents ([tokens], an index within the sequence; one that is not in [0, the node's own index) means none): `seen`, `words` 64-bit
+ * words a node, bit j % 64 of word j / 64 is set where node j of the sequence is the node itself or one that it descends from (nodes from 64 * words on
+ * have no bit), and the position of each node, seq_lens[b] less the number of nodes plus the number of nodes above it.  Either output may be null.
+ * Rows behind cu_q[batch] are left alone.
+ */
+int ave_fp4_draft_tree(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens, int batch, uint64_t* seen, int words,
+                       int32_t* positions, void* hip_stream);
+
+/* What the new tokens of a sequence see of each other: bits as ave_fp4_draft_tree makes them, or any others. */
+typedef struct ave_fp4_tree {
+  const uint64_t* seen; /* [tokens, words], 8-byte aligned */
+  int64_t stride;       /* words between rows; 0: one row for all */
+  int32_t words;        /* new tokens from 64 * words on are seen by nobody */
+} ave_fp4_tree;
+
+/*
+ * ave_fp4_attention_mxfp4 where the new tokens are not a chain: with n of them row i sees the keys before them, j < seq_lens[b] - n, and of the new ones
+ * those whose bit is set in its row of `seen` (its own, too).  window > 0: the last `window` of what it sees -- of the keys before, those
+ * from seq_lens[b] - n + (bits set) - window on; the new tokens are seen as their bits say.  `causal` is ignored.  Everything else, workspace
+ * included, is as there.  With the bits of a chain (node i sees 0 .. i) the result is that of the causal call with the same window, up to the order
+ * of sums.
+ */
+size_t ave_fp4_tree_attention_mxfp4_workspace_bytes(const ave_fp4_attention* a, const ave_fp4_tree* tree, const ave_fp4_kv_cache* cache);
+int ave_fp4_tree_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_tree* tree, const ave_fp4_kv_cache* cache, void* workspace,
+                                 size_t workspace_bytes, void* hip_stream);
+
+/*
+ * Which nodes of a draft are kept, so that the tokens are distributed as if the target model had drawn them one by one (temperature > 0), or are the ones
+ * that it would choose (temperature 0, or not above it).  From node 0 on: p is the softmax of the node's logits over the temperature; its children c, in
+ * the order of their indices, are tried one after the other until one is accepted; from that one on the same again.
+ *   draft_probs null (children are given, not drawn): r is p without the tokens of rejected siblings, over its sum; c is accepted if uniform[c] < r(token)
+ *   draft_probs (children of a node were drawn from its row q): r starts as p and becomes max(r - q, 0) over its sum with each rejection; c is accepted
+ *   if uniform[c] q(token) < r(token)
+ *   temperature 0: the child whose token has the largest logit (the lowest of equal ones) is accepted
+ * Where no child is accepted, the next token is drawn from r: the first index where the running sum of r is above uniform[node 0] times the whole (temperature 0:
+ * the token of the largest logit).  If rejections leave nothing of r, it is p (draft_probs: c is then rejected; tokens: r(token) is 0).
+ * accepted[b]: nodes kept, node 0 among them (0 for a sequence without nodes); path[cu_q[b] + i], i < accepted[b]: their indices, rising; emitted: as many
+ * tokens, those of the kept nodes from the second on, then the drawn one.  Both are -1 for the other nodes of the sequence.
+ * Softmax, sums and products in 64 bits (a choice lies between sums of very many probabilities).  A NaN among the logits counts as -inf, +inf as the largest
+ * finite number; a row without any number accepts no child and draws -1.  uniform is taken into [0, 1], NaN as 0; a token that is no index of the
+ * vocabulary is never accepted; NaN and negative numbers in draft_probs count as 0, as they are otherwise (no sum of 1 is asked for).
+ * Rows behind cu_q[batch] are neither read nor written.  Offsets are cut to the rows; nothing in device memory leads out of the arrays.
+ * The workspace (16-byte aligned, no initialisation) belongs to one call at a time.  Equal inputs give equal outputs.
+ */
+typedef struct ave_fp4_draft {
+  const void* logits;        /* [rows, vocab] bf16, or fp32 where logits_f32: the target's, row t behind node t */
+  int64_t logits_stride;     /* elements between rows */
+  const int32_t *tokens, *parents; /* [rows] */
+  const int32_t* cu_q;       /* [batch + 1] */
+  const float* uniform;      /* [rows] */
+  const float* temperature;  /* [batch] or null (1) */
+  const float* draft_probs;  /* [rows, vocab] or null; rows of nodes without children are not read */
+  int64_t draft_probs_stride;
+  int32_t *accepted, *path, *emitted; /* [batch], [rows], [rows] */
+  int32_t rows, batch, vocab, logits_f32;
+} ave_fp4_draft;
+size_t ave_fp4_verify_draft_workspace_bytes(const ave_fp4_draft* draft);
+int ave_fp4_verify_draft(const ave_fp4_draft* draft, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/*
+ * Of the last n = cu_q[b+1] - cu_q[b] tokens of each sequence, those at path[cu_q[b] + i], i < accepted[b] (rising, each at least i), are moved together in the
+ * caches of `layers` layers, codes and scales as they are: token seq_lens[b] - n + path[cu_q[b] + i] to place seq_lens[b] - n + i.  kept_lens[b] (null: not
+ * asked for; must not overlap the inputs) = seq_lens[b] - n + accepted[b], the length that is left.  With the outputs of ave_fp4_verify_draft a checked
+ * draft becomes part of its sequence; with n = seq_lens[b] tokens that a policy gives up leave a cache.
+ * All caches have one shape (pages, kv_heads, page_size, head_dim) and the page table in common; pages that hold moved tokens belong to one sequence
+ * only.  What stands behind the kept tokens is left as it was.  An index outside [0, n), a token outside the page table and a page outside the cache
+ * move nothing; indices that do not rise leave a mix of the tokens that they name.
+ * max_q: a bound on n, by which the kernel is chosen (a wrong one costs time only).
+ */
+typedef struct ave_fp4_keep {
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t *seq_lens, *cu_q, *path, *accepted; /* [batch], [batch + 1], [tokens], [batch] */
+  int32_t* kept_lens;
+  int32_t tokens, batch, table_pages, max_q;
+} ave_fp4_keep;
+int ave_fp4_keep_kv_mxfp4(const ave_fp4_kv_cache* caches, int layers, const ave_fp4_keep* keep, void* hip_stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* ave_fp4_last_error(void);
 
