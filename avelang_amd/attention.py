@@ -325,8 +325,8 @@ def keep_kv_mxfp4(caches, page_table, seq_lens, cu_q, path, accepted, kept_lens=
     ``i < accepted[b]`` (int32 ``[T]`` and ``[B]``; rising), go to places ``seq_lens[b] - n + i``, keys, values and scales as they are; ``kept_lens`` is
     ``seq_lens - n + accepted``, the lengths that are left (it must not be one of the inputs).  With what :func:`verify_draft` returns a checked draft
     becomes part of its sequence; with ``n`` the whole sequence, tokens that a policy gives up leave the cache.  What stands behind the kept
-    tokens stays as it was.  Pages that hold moved tokens must belong to one sequence only.  ``max_q``: a bound on ``n``, if the host knows one; it
-    helps to choose the kernel."""
+    tokens stays as it was.  Pages that hold moved tokens must belong to one sequence only.  ``max_q``: a bound on ``n``, if the host knows one (without, the mean is
+    taken); it helps to choose the kernel."""
     done = _native.keep_kv_mxfp4(caches, page_table, seq_lens, cu_q, path, accepted, kept_lens, max_q)
     if done is not None:
         return done
@@ -347,7 +347,7 @@ def keep_kv_mxfp4(caches, page_table, seq_lens, cu_q, path, accepted, kept_lens=
         raise ValueError("page_table must have consecutive entries in a row.")
     t = path.shape[0]
     k = _lib.Keep(page_table=page_table.data_ptr(), page_table_stride=page_table.stride(0), tokens=t, batch=b, table_pages=width,
-                  max_q=_int32(t if max_q is None else max_q))
+                  max_q=_int32(-(-t // max(b, 1)) if max_q is None else max_q))
     k.seq_lens, k.cu_q = _vector(seq_lens, "seq_lens", torch.int32, b, dev), _vector(cu_q, "cu_q", torch.int32, b + 1, dev)
     k.path, k.accepted = _vector(path, "path", torch.int32, t, dev), _vector(accepted, "accepted", torch.int32, b, dev)
     if kept_lens is None:

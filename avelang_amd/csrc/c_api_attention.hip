@@ -215,8 +215,9 @@ static int check_draft(const ave_fp4_draft* d) {
   if (!d) return fail_inval("null arguments.");
   if (d->rows < 0 || d->batch < 0) return fail_inval("rows and batch must be non-negative, got %d and %d.", d->rows, d->batch);
   if (d->vocab <= 0 || d->vocab > 1 << 30) return fail_inval("vocab must be from 1 to 2^30, got %d.", d->vocab);
-  if ((int64_t)d->rows * ((d->vocab + ave::kVocabPiece - 1) / ave::kVocabPiece) >= 1 << 24)   // workgroups of a launch
-    return fail_inval("rows times vocab / %d must be below 2^24, got %d x %d.", ave::kVocabPiece, d->rows, d->vocab);
+  const int64_t pieces = (d->vocab + ave::kVocabPiece - 1) / ave::kVocabPiece;
+  if (d->rows * pieces >= 1 << 22 || d->batch * pieces >= 1 << 22)   // workgroups of a launch, of up to 1024 threads
+    return fail_inval("rows and batch times vocab / %d must be below 2^22, got %d, %d and %d.", ave::kVocabPiece, d->rows, d->batch, d->vocab);
   return 0;
 }
 

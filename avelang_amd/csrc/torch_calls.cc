@@ -739,7 +739,7 @@ PyObject* keep_kv_mxfp4(PyObject* const* arg) {
   ave_fp4_keep k{};
   k.page_table = ptr_as<int32_t>(*table), k.page_table_stride = table->stride(0), k.table_pages = (int)table->size(1);
   k.seq_lens = ptr_as<int32_t>(*lens), k.cu_q = ptr_as<int32_t>(*cu), k.path = ptr_as<int32_t>(*path), k.accepted = ptr_as<int32_t>(*accepted);
-  k.tokens = (int)t, k.batch = (int)b, k.max_q = (int)t;
+  k.tokens = (int)t, k.batch = (int)b, k.max_q = b > 0 ? (int)((t + b - 1) / b) : 0;
   if (arg[7] != Py_None && !as_int(arg[7], &k.max_q)) NOT_MINE;
   Out kept;
   if (!kept.take(arg[6], {b}, at::kInt, dev)) NOT_MINE;

@@ -1,37 +1,65 @@
 // Which nodes of a drafted tree the target model accepts, and the token behind them.
 //
-//   row sums     one launch over all rows and pieces of the vocabulary: largest logit, its lowest index, sum of exp((x - largest) / temperature)
-//   rejections   (drafts with distributions only) sum of max(p - q, 0) of the rows whose first child is rejected, then, a workgroup a row, the
-//                children that are left
-//   walk         a workgroup a sequence: whether a node is accepted once its parent is and its elder siblings are not does not depend on the
-//                rest of the walk, so all nodes' probabilities are fetched at once; then the path, then the token: among the sums of the
-//                pieces first, and in one piece element by element
+//   row sums   a workgroup for a piece of a row: largest logit, its lowest index, sum of exp((x - largest) / temperature)
+//   children   (drafts with distributions only) rows whose first child is rejected and that have more: sums of max(p - t q, 0), child after child
+//   walk       every workgroup of a piece goes the way from node to node by itself -- whether a node is accepted, once its parent is and its elder
+//              siblings are not, does not depend on the rest of the way, so all nodes' probabilities are fetched at once -- and then sums up, in
+//              fp64, what its piece of the last node's row leaves to draw from; the last one of a sequence draws: the piece in which the random
+//              number lies, then the element
 //
-// Everything behind a logit is fp64: a token is chosen by where a number lies among the running sums of 10^5 probabilities, and in fp32 one
-// draw in some hundred to thousand would go to a neighbour by rounding.
+// Bound by HBM where there is much to read, by the latency of the launches where there is not.  With much to read the children of node 0 are decided on first,
+// from its row alone, and then only rows that descend from the accepted one are read.
+//
+// Precision.  A token is drawn by where a number lies among the running sums of 10^5 probabilities; in fp32 one draw in some hundred to
+// thousand would go to a neighbour by rounding, so what is drawn from is summed in fp64.  A node's acceptance is one comparison: the row sums behind it are
+// formed in fp32 (kSumError), and where the comparison comes out nearer than that, the row is summed again in fp64.
 #include <algorithm>
 
 #include "fp4_common.hpp"
+#include "kernels.hpp"
 #include "kv_cache.hpp"
 
 namespace ave {
 namespace {
 
 constexpr int kPiece = kVocabPiece;
-constexpr int kRowThreads = 256, kWalkThreads = 1024;
+constexpr int kThreads = 256, kRowThreads = 1024;
+constexpr int kEach = kPiece / kThreads, kOnce = 8;   // elements of a thread, together in memory
 
 struct PieceSum {
   double sum;   // of exp((x - top) / temperature)
   float top;    // -inf: no number
   int at;       // the lowest index of top
 };
+constexpr int kGone = 16;
+// What a sequence's token is drawn from
+struct Draw {
+  double times;   // t of max(p - t q, 0)
+  double sum;     // of the row, in units of its largest weight
+  float top;
+  int gone[kGone], many;   // the children's tokens, so many; -1: more, to be looked for
+  int row, how, out;       // out: of `emitted`; how: kAll: p, kWithout: p without the children's tokens, kRest: max(p - t q, 0); kNothing: the token is there already
+};
+enum { kAll, kWithout, kRest, kNothing };
+constexpr int kMany = -2;
+
+struct Wanted {
+  double per;   // inverse temperature
+  int row;
+};
+
 struct VerifyArgs {
   ave_fp4_draft d;
   int pieces;
-  PieceSum* sums;      // [rows][pieces]
-  double* rest;        // [rows][pieces]: sums of max(p - t q, 0), where a row's children are rejected
-  double* times;       // [rows]: that t, 0 without rejections
-  int* choice;         // [rows]: the accepted child, -1
+  PieceSum* sums;   // [rows][pieces]
+  double* left;     // [batch][pieces]: of what is drawn from
+  Draw* draws;      // [batch]
+  double* rest;     // [rows][pieces]: sums of max(p - q, 0)
+  double* times;    // [rows]: t when all children are rejected
+  int* choice;      // [rows]: the accepted child, -1: none; kMany: there are several and nobody has looked
+  Wanted* wanted;   // [rows]: the rows that descend from the accepted children of nodes 0, in any order, and
+  int* many;        // how many
+  int* done;        // [batch]: pieces of the last row that are summed up
 };
 
 struct Span {
@@ -46,6 +74,7 @@ __device__ inline Span span_of(const VerifyArgs& p, int b) {
   s.n = end - s.first;
   return s;
 }
+__device__ inline int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // The sequence of a row (every wave by itself), -1: nobody's.  64 probes at a time; if offsets fall, any sequence that has the row, or none.
 __device__ inline int sequence_of(const VerifyArgs& p, int row) {
   const int lane = threadIdx.x & 63;
@@ -60,8 +89,8 @@ __device__ inline int sequence_of(const VerifyArgs& p, int row) {
   }
   if (p.d.batch <= 0) return -1;
   // (an empty sequence starts where the next one does, and comes before it)
-  const Span s = span_of(p, __builtin_amdgcn_readfirstlane(from));
-  return row >= s.first && row < s.first + s.n ? __builtin_amdgcn_readfirstlane(from) : -1;
+  const Span s = span_of(p, uniform_int(from));
+  return row >= s.first && row < s.first + s.n ? uniform_int(from) : -1;
 }
 // 1 / temperature in units of log2(e); 0: the largest logit
 __device__ inline double inverse_temperature(const VerifyArgs& p, int b) {
@@ -69,69 +98,117 @@ __device__ inline double inverse_temperature(const VerifyArgs& p, int b) {
   return t > 0.0f ? 1.4426950408889634 / (double)fminf(t, 3.402823466e38f) : 0.0;
 }
 
-// 2^y for y <= 0: 2^n times the Taylor polynomial of e^f, |f| <= ln 2 / 2, whose first missing term is below 2e-16
-__device__ inline double exp2_of(double y) {
-  y = fmax(y, -1100.0);
-  const double n = rint(y), f = (y - n) * 0.6931471805599453;
-  double r = 1.0 / 479001600.0;
-  r = fma(r, f, 1.0 / 39916800.0);
-  r = fma(r, f, 1.0 / 3628800.0);
-  r = fma(r, f, 1.0 / 362880.0);
-  r = fma(r, f, 1.0 / 40320.0);
-  r = fma(r, f, 1.0 / 5040.0);
-  r = fma(r, f, 1.0 / 720.0);
-  r = fma(r, f, 1.0 / 120.0);
-  r = fma(r, f, 1.0 / 24.0);
-  r = fma(r, f, 1.0 / 6.0);
-  r = fma(r, f, 0.5);
+// exp((x - top) / temperature) for x <= top; 0 for -inf.  2^y = 2^n 2^f with n the nearest integer (out of the low bits of y + 1.5 2^52) and the Taylor
+// polynomial of 2^f, |f| <= 1/2, whose first missing term is 2^-42 of it; 2^n by adding to the exponent.  What is below 2^-1000 counts as that.
+__device__ inline double weight_of(float x, double top, double per) {
+  constexpr double kRound = 6755399441055744.0;
+  const double y = fmax(((double)x - top) * per, -1000.0), up = y + kRound, f = y - (up - kRound);
+  double r = 7.0549116208011233e-9;   // (ln 2)^k / k!
+  r = fma(r, f, 1.0178086009239699e-7);
+  r = fma(r, f, 1.3215486790144307e-6);
+  r = fma(r, f, 1.5252733804059841e-5);
+  r = fma(r, f, 1.5403530393381609e-4);
+  r = fma(r, f, 1.3333558146428443e-3);
+  r = fma(r, f, 9.6181291076284772e-3);
+  r = fma(r, f, 5.5504108664821580e-2);
+  r = fma(r, f, 0.24022650695910071);
+  r = fma(r, f, 0.69314718055994531);
   r = fma(r, f, 1.0);
-  r = fma(r, f, 1.0);
-  return ldexp(r, (int)n);
-}
-// exp((x - top) / temperature); x <= top, either may be -inf (then 0)
-__device__ inline double weight_of(float x, float top, double per) {
-  return x == -INFINITY ? 0.0 : exp2_of(((double)x - (double)top) * per);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, r) + ((uint64_t)(unsigned)__builtin_bit_cast(uint64_t, up) << 52);
+  return x == -INFINITY ? 0.0 : __builtin_bit_cast(double, bits);
 }
 
-__device__ inline float number(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
+// A NaN counts as -inf, infinity as the largest number
+// (the middle of three with a NaN is the least of the others)
+__device__ inline float number(float x) { return __builtin_amdgcn_fmed3f(x, -INFINITY, 3.402823466e38f); }
 template <bool F32>
 __device__ inline float logit(const VerifyArgs& p, int row, int i) {
-  if constexpr (F32) return number(static_cast<const float*>(p.d.logits)[(int64_t)row * p.d.logits_stride + i]);
-  else return number(__builtin_bit_cast(float, (unsigned)static_cast<const uint16_t*>(p.d.logits)[(int64_t)row * p.d.logits_stride + i] << 16));
+  if constexpr (F32) return static_cast<const float*>(p.d.logits)[(int64_t)row * p.d.logits_stride + i];
+  else return __builtin_bit_cast(float, (unsigned)static_cast<const uint16_t*>(p.d.logits)[(int64_t)row * p.d.logits_stride + i] << 16);
 }
-// N consecutive logits from index i on, -inf behind the last
-template <bool F32, int N>
-__device__ inline void logits(const VerifyArgs& p, int row, int i, float (&x)[N]) {
-  constexpr int kOf = F32 ? 4 : 8;   // elements of 16 bytes
-  static_assert(N % kOf == 0, "");
-  const int64_t at = (int64_t)row * p.d.logits_stride + i;
-  const char* from = static_cast<const char*>(p.d.logits) + at * (F32 ? 4 : 2);
-  if (i + N <= p.d.vocab && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
-    v4i raw[N / kOf];
+// Eight consecutive logits from index i on as they are in memory, -inf behind the last
+template <bool F32>
+struct Eight {
+  int word[F32 ? 8 : 4];
+};
+template <bool F32>
+__device__ inline Eight<F32> load8(const VerifyArgs& p, int row, int i) {
+  typedef int Four __attribute__((ext_vector_type(4), aligned(2)));   // (rows of an odd vocabulary start anywhere)
+  const char* from = static_cast<const char*>(p.d.logits) + ((int64_t)row * p.d.logits_stride + i) * (F32 ? 4 : 2);
+  Eight<F32> r;
+  if (i + kOnce <= p.d.vocab) {
 #pragma unroll
-    for (int k = 0; k < N / kOf; ++k) raw[k] = reinterpret_cast<const v4i*>(from)[k];
+    for (int k = 0; k < (F32 ? 2 : 1); ++k) {
+      const Four x = reinterpret_cast<const Four*>(from)[k];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if constexpr (F32) x[k] = number(__builtin_bit_cast(float, (int)raw[k / 4][k % 4]));
-      else x[k] = number(__builtin_bit_cast(float, k % 2 ? (unsigned)raw[k / 8][k % 8 / 2] & 0xFFFF0000u : (unsigned)raw[k / 8][k % 8 / 2] << 16));
+      for (int e = 0; e < 4; ++e) r.word[4 * k + e] = x[e];
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = i + k < p.d.vocab ? logit<F32>(p, row, i + k) : -INFINITY;
+    for (int k = 0; k < kOnce; ++k) {
+      const int x = __builtin_bit_cast(int, i + k < p.d.vocab ? logit<F32>(p, row, i + k) : -INFINITY);
+      if constexpr (F32) r.word[k] = x;
+      else r.word[k / 2] = k % 2 ? r.word[k / 2] | x : (int)((unsigned)x >> 16);
+    }
   }
+  return r;
+}
+template <bool F32>
+__device__ inline void unpack(const Eight<F32>& r, float (&x)[kOnce]) {
+#pragma unroll
+  for (int k = 0; k < kOnce; ++k) {
+    if constexpr (F32) x[k] = __builtin_bit_cast(float, r.word[k]);
+    else x[k] = __builtin_bit_cast(float, k % 2 ? (unsigned)r.word[k / 2] & 0xFFFF0000u : (unsigned)r.word[k / 2] << 16);
+  }
+}
+template <bool F32>
+__device__ inline void logits(const VerifyArgs& p, int row, int i, float (&x)[kOnce]) {
+  unpack<F32>(load8<F32>(p, row, i), x);
 }
 __device__ inline double draft_prob(const VerifyArgs& p, int row, int i) {
   const float q = p.d.draft_probs[(int64_t)row * p.d.draft_probs_stride + i];
   return q > 0.0f ? (double)q : 0.0;
 }
+__device__ inline void draft_probs(const VerifyArgs& p, int row, int i, float (&q)[kOnce]) {   // eight, 0 behind the last
+  typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+  const float* from = p.d.draft_probs + (int64_t)row * p.d.draft_probs_stride + i;
+  if (i + kOnce <= p.d.vocab) {
+    const Four a = reinterpret_cast<const Four*>(from)[0], b = reinterpret_cast<const Four*>(from)[1];
+#pragma unroll
+    for (int k = 0; k < kOnce; ++k) q[k] = k < 4 ? a[k] : b[k - 4];
+  } else {
+#pragma unroll
+    for (int k = 0; k < kOnce; ++k) q[k] = i + k < p.d.vocab ? from[k] : 0.0f;
+  }
+}
+__device__ inline double random_of(const VerifyArgs& p, int row) {
+  const float u = p.d.uniform[row];
+  return u > 0.0f ? fmin((double)u, 1.0) : 0.0;
+}
 
-// ---- over a workgroup ------------------------------------------------------------------------------------------------------------------
+// Children of node v of a sequence from node `from` on: the next one, or n (every wave by itself)
+__device__ inline int next_child(const VerifyArgs& p, const Span& s, int v, int from) {
+  const int lane = threadIdx.x & 63;
+  for (int c0 = from; c0 < s.n; c0 += 64) {
+    const int c = c0 + lane;
+    const uint64_t any = __ballot(c < s.n && c > v && p.d.parents[s.first + c] == v);
+    if (any) return c0 + __ffsll((unsigned long long)any) - 1;
+  }
+  return s.n;
+}
+
+// ---- over a wave, over a workgroup ---------------------------------------------------------------------------------------------------------
 __device__ inline double wave_sum(double v) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
   return v;
 }
-// of every thread's v, in all threads; `scratch` has an element a wave and is free again when the next call's barrier has passed
+__device__ inline double lane_double(double v, int lane) {   // lane: the same in all lanes
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, lane) |
+                                        (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), lane) << 32);
+}
+// of every thread's v, in all threads; `scratch` has an element a wave
 template <int THREADS>
 __device__ inline double block_sum(double v, double* scratch) {
   v = wave_sum(v);
@@ -144,43 +221,104 @@ __device__ inline double block_sum(double v, double* scratch) {
   return all;
 }
 
-// ---- a row's sums ------------------------------------------------------------------------------------------------------------------------
-template <bool F32>
-__global__ __launch_bounds__(kRowThreads) void row_sums_kernel(VerifyArgs p) {
-  constexpr int kEach = kPiece / kRowThreads, kOnce = 8;   // elements of a thread, together in memory
-  __shared__ double scratch[kRowThreads / 64];
-  __shared__ float tops[kRowThreads / 64];
-  __shared__ int ats[kRowThreads / 64];
-  const int row = blockIdx.x / (unsigned)p.pieces, piece = blockIdx.x % (unsigned)p.pieces, b = sequence_of(p, row);
-  if (b < 0) return;
-  const double per = inverse_temperature(p, b);
-  float x[kEach / kOnce][kOnce];
-#pragma unroll
-  for (int k = 0; k < kEach / kOnce; ++k) logits<F32>(p, row, piece * kPiece + (k * kRowThreads + threadIdx.x) * kOnce, x[k]);
-  float top = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) top = fmaxf(top, x[k / kOnce][k % kOnce]);
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x / 64] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 64; ++w) top = fmaxf(top, tops[w]);
-  int at = INT32_MAX;
-  double sum = 0.0;
-#pragma unroll
-  for (int k = kEach - 1; k >= 0; --k) {
-    if (x[k / kOnce][k % kOnce] == top) at = piece * kPiece + (k / kOnce * kRowThreads + threadIdx.x) * kOnce + k % kOnce;
-    if (per > 0.0) sum += weight_of(x[k / kOnce][k % kOnce], top, per);
+// ---- a row's sums ----------------------------------------------------------------------------------------------------------------------------
+// The relative error of a row's sum in fp32: a difference and a product of a rounding each before an exponential of an argument down to -126 (3 2^-24 126
+// ln 2), the exponential's own and 32 additions (2^-23, 2^-19): 1.8e-5 at most.
+constexpr double kSumError = 1.0 / 32768.0;
+
+// EXACT: in fp64.  ROWS: 0 all, 1 the first of each sequence, 2 those that are wanted (by a workgroup one after the other)
+template <bool F32, bool EXACT, int ROWS>
+__global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
+  __shared__ double scratch[kThreads / 64];
+  __shared__ float tops[kThreads / 64];
+  __shared__ int lowest;
+  if constexpr (ROWS < 2) {   // for the launches behind this one
+    for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < (unsigned)p.d.batch; i += gridDim.x * kThreads) p.done[i] = 0;
+    if (ROWS == 1 && blockIdx.x == 0 && threadIdx.x == 0) *p.many = 0;
   }
+  const unsigned all = ROWS == 2 ? (unsigned)min(*p.many, p.d.rows) * (unsigned)p.pieces : blockIdx.x + 1;
+  Wanted now{};
+  Eight<F32> next[kEach / kOnce];
+  const auto fetch = [&](unsigned item) {
+    now = p.wanted[item / (unsigned)p.pieces];
 #pragma unroll
-  for (int m = 32; m > 0; m >>= 1) at = min(at, __shfl_xor(at, m, 64));
-  if ((threadIdx.x & 63) == 0) ats[threadIdx.x / 64] = at;
-  sum = block_sum<kRowThreads>(sum, scratch);
-  if (threadIdx.x == 0) {
+    for (int k = 0; k < kEach / kOnce; ++k) next[k] = load8<F32>(p, now.row, (int)(item % (unsigned)p.pieces) * kPiece + (k * kThreads + threadIdx.x) * kOnce);
+  };
+  if (ROWS == 2 && blockIdx.x < all) fetch(blockIdx.x);
+  for (unsigned item = blockIdx.x; item < all; item += gridDim.x) {
+    const int piece = (int)(item % (unsigned)p.pieces);
+    int row = (int)(item / (unsigned)p.pieces), b = row;
+    if constexpr (ROWS == 1) {
+      const Span s = span_of(p, b);
+      if (s.n == 0) return;
+      row = s.first;
+    }
+    double per;
+    float x[kEach / kOnce][kOnce];
+    if constexpr (ROWS == 2) {   // the present row's are here, the next one's under way
+      row = now.row, per = now.per;
 #pragma unroll
-    for (int w = 0; w < kRowThreads / 64; ++w) at = min(at, ats[w]);
-    p.sums[(size_t)row * p.pieces + piece] = {sum, top, at};
+      for (int k = 0; k < kEach / kOnce; ++k) unpack<F32>(next[k], x[k]);
+      if (item + gridDim.x < all) fetch(item + gridDim.x);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kEach / kOnce; ++k) logits<F32>(p, row, piece * kPiece + (k * kThreads + threadIdx.x) * kOnce, x[k]);
+      if constexpr (ROWS == 0) b = sequence_of(p, row);
+      if (b < 0) return;
+      per = inverse_temperature(p, b);
+    }
+    if (threadIdx.x == 0) lowest = INT32_MAX;
+    float top;
+    double sum;
+    const auto reduce = [&] {
+      float mine = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) mine = fmaxf(mine, x[k / kOnce][k % kOnce]);
+      top = mine;
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+      if ((threadIdx.x & 63) == 0) tops[threadIdx.x / 64] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, tops[w]);
+      sum = 0.0;
+      if (per > 0.0 && top != -INFINITY) {
+        if constexpr (EXACT) {
+#pragma unroll
+          for (int k = 0; k < kEach; ++k) sum += weight_of(x[k / kOnce][k % kOnce], top, per);
+        } else {
+          const float per32 = (float)fmin(per, 3.4e38);
+          float s = 0.0f;
+#pragma unroll
+          for (int k = 0; k < kEach; ++k) s += __builtin_amdgcn_exp2f((x[k / kOnce][k % kOnce] - top) * per32);
+          sum = (double)s;
+        }
+      }
+      sum = block_sum<kThreads>(sum, scratch);
+      return mine;
+    };
+    float mine = reduce();
+    if (!(sum < 1e300) || top == INFINITY) {   // a NaN or an infinity in the piece
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) x[k / kOnce][k % kOnce] = number(x[k / kOnce][k % kOnce]);
+      mine = reduce();
+    }
+    if (mine == top) {
+      int at = INT32_MAX;
+#pragma unroll
+      for (int k = kEach - 1; k >= 0; --k)
+        if (x[k / kOnce][k % kOnce] == top) at = piece * kPiece + (k / kOnce * kThreads + threadIdx.x) * kOnce + k % kOnce;
+      atomicMin(&lowest, at);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.sums[(size_t)row * p.pieces + piece] = {sum, top, lowest};
+    if constexpr (ROWS == 2) __syncthreads();   // before the next one's `lowest`
+    if (EXACT && piece == 0 && threadIdx.x < 64) {   // (with distributions)
+      const Span s = span_of(p, b);
+      const int v = row - s.first, child = next_child(p, s, v, v + 1);
+      const bool several = child < s.n && next_child(p, s, v, child + 1) < s.n;
+      if (threadIdx.x == 0) p.choice[row] = several && per > 0.0 ? kMany : -1;
+    }
   }
 }
 
@@ -189,295 +327,451 @@ struct RowSum {
   float top;
   int at;
 };
-// Of all pieces, by one wave, in all of its lanes.  (The order of the sum depends on the number of pieces alone.)
+template <bool EXACT>
+__device__ inline void add_piece(RowSum& r, const PieceSum& q, double per) {
+  if (q.top == -INFINITY) return;
+  const bool higher = q.top > r.top;
+  if (per > 0.0) {
+    const float low = higher ? r.top : q.top, high = higher ? q.top : r.top;
+    const double w = EXACT ? weight_of(low, high, per) : (double)__builtin_amdgcn_exp2f((low - high) * (float)fmin(per, 3.4e38));
+    r.sum = higher ? r.sum * w + q.sum : r.sum + q.sum * w;
+  }
+  if (higher) r.top = q.top, r.at = q.at;
+}
+// Of all pieces, by a lane: sixteen at a time under way.  (The order of the sum depends on the number of pieces alone.)
+template <bool EXACT>
 __device__ inline RowSum row_sum(const VerifyArgs& p, int row, double per) {
   const PieceSum* s = p.sums + (size_t)row * p.pieces;
-  const int lane = threadIdx.x & 63;
   RowSum r{0.0, -INFINITY, INT32_MAX};
-  for (int c = lane; c < p.pieces; c += 64)
+  for (int c0 = 0; c0 < p.pieces; c0 += 16) {
+    PieceSum q[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) q[c] = s[min(c0 + c, p.pieces - 1)];
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      if (c0 + c < p.pieces) add_piece<EXACT>(r, q[c], per);
+  }
+  return r;
+}
+// Largest logit and its lowest index, by a wave
+__device__ inline RowSum row_top(const VerifyArgs& p, int row) {
+  const PieceSum* s = p.sums + (size_t)row * p.pieces;
+  RowSum r{0.0, -INFINITY, INT32_MAX};
+  for (int c = threadIdx.x & 63; c < p.pieces; c += 64)
     if (s[c].top > r.top) r.top = s[c].top, r.at = s[c].at;
   float top = r.top;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  r.at = r.top == top && top != -INFINITY ? r.at : INT32_MAX;
-  r.top = top;
+  if (r.top != top || top == -INFINITY) r.at = INT32_MAX;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) r.at = min(r.at, __shfl_xor(r.at, m, 64));
-  if (per > 0.0) {
-    for (int c = lane; c < p.pieces; c += 64) r.sum += s[c].top == -INFINITY ? 0.0 : s[c].sum * weight_of(s[c].top, top, per);
-    r.sum = wave_sum(r.sum);
-  }
+  r.top = top;
   return r;
 }
-
-// ---- rejections, where drafts come with distributions ----------------------------------------------------------------------------------------
-// Children of node v of a sequence from node `from` on: the next one, or n (every wave by itself)
-__device__ inline int next_child(const VerifyArgs& p, const Span& s, int v, int from) {
-  const int lane = threadIdx.x & 63;
-  for (int c0 = from; c0 < s.n; c0 += 64) {
-    const int c = c0 + lane;
-    const uint64_t any = __ballot(c < s.n && c > v && p.d.parents[s.first + c] == v);
-    if (any) return c0 + __ffsll((unsigned long long)any) - 1;
-  }
-  return s.n;
-}
-__device__ inline double uniform_of(const VerifyArgs& p, int row) {
-  const float u = p.d.uniform[row];
-  return u > 0.0f ? fmin((double)u, 1.0) : 0.0;
-}
-// Is child c accepted, with t and s = sum of max(p - t q, 0)?
+// Sum of a row in fp64, by a wave
 template <bool F32>
-__device__ inline bool accepts(const VerifyArgs& p, int row, const RowSum& r, double per, int child_row, double t, double s) {
+__device__ inline double exact_sum(const VerifyArgs& p, int row, float top, double per) {
+  double sum = 0.0;
+  for (int i = (threadIdx.x & 63) * kOnce; i < p.d.vocab; i += 64 * kOnce) {
+    float x[kOnce];
+    logits<F32>(p, row, i, x);
+#pragma unroll
+    for (int k = 0; k < kOnce; ++k) sum += weight_of(number(x[k]), top, per);
+  }
+  return wave_sum(sum);
+}
+
+// ---- the way through the tree ------------------------------------------------------------------------------------------------------------------
+struct Way {
+  int at, kept, tried, token;   // the last node, how many are kept, how many of its children were rejected; temperature 0: the token
+  double times;                 // with distributions: t
+};
+// By one wave.  FIRST: one step only (at: the accepted child of node 0, or 0).  write: this workgroup writes path and emitted.  draw: where the tokens of the
+// last node's children go.
+template <bool F32, bool FIRST>
+__device__ inline Way walk(const VerifyArgs& p, const Span& s, double per, bool write, Draw* draw = nullptr) {
+  const int lane = threadIdx.x & 63;
+  const bool probs = p.d.draft_probs != nullptr;
+  Way w{0, 1, 0, -1, 0.0};
+  double taken = 0.0;   // by rejected children, of the present row
+  write = write && lane == 0;
+  if (write) p.d.path[s.first] = 0;
+  for (int c0 = 0; c0 < s.n; c0 += 64) {
+    // a node a lane: its parent's row, what the target gives its token, what the draft gave it
+    const int j = c0 + lane;
+    int parent = -1, token = -1;
+    double u = 0.0, mine = 0.0, q = 0.0;
+    RowSum r{0.0, -INFINITY, INT32_MAX};
+    if (j < s.n && j > 0) {
+      parent = p.d.parents[s.first + j], token = p.d.tokens[s.first + j];
+      if (parent >= j) parent = -1;
+    }
+    if (parent >= w.at && (!FIRST || parent == 0)) {   // (the others cannot be reached)
+      const int row = s.first + parent;
+      u = random_of(p, s.first + j);
+      const bool there = token >= 0 && token < p.d.vocab;
+      const float x = there ? number(logit<F32>(p, row, token)) : -INFINITY;
+      if (there && probs) q = draft_prob(p, row, token);
+      r = probs ? row_sum<true>(p, row, per) : row_sum<false>(p, row, per);
+      if (per > 0.0) mine = r.sum > 0.0 ? weight_of(x, r.top, per) / r.sum : 0.0;
+      if (!there) token = -1;
+    } else {
+      parent = -1;
+    }
+    uint64_t mask = __ballot(parent == w.at);
+    while (mask) {
+      const int k = __ffsll((unsigned long long)mask) - 1, child = c0 + k, child_token = __builtin_amdgcn_readlane(token, k);
+      mask &= mask - 1;
+      bool accepted = false;
+      const double p_child = lane_double(mine, k), u_child = lane_double(u, k);
+      if (per == 0.0) {
+        accepted = child_token >= 0 && child_token == __builtin_amdgcn_readlane(r.at, k);
+      } else if (probs) {
+        if (w.tried == 0) {
+          accepted = child_token >= 0 && u_child * lane_double(q, k) < p_child;
+        } else {   // by children_kernel
+          const int chosen = p.choice[s.first + w.at];
+          if (chosen > w.at && chosen < s.n) {   // this child or a later one
+            if (chosen > child) continue;
+            accepted = chosen == child;
+          }
+        }
+      } else if (child_token >= 0) {   // a token that an elder sibling had has been taken out
+        bool again = __any(lane < k && parent == w.at && token == child_token);
+        for (int b0 = w.at + 1; b0 < c0 && !again; b0 += 64)
+          again = __any(b0 + lane < c0 && p.d.parents[s.first + b0 + lane] == w.at && p.d.tokens[s.first + b0 + lane] == child_token);
+        if (!again) {
+          const double bound = u_child * (1.0 - taken);
+          double now = p_child, against = bound;
+          if (fabs(bound - p_child) <= kSumError * (bound + p_child + u_child * taken)) {
+            // nearer than the row's sum is exact: all of it again, over the same tokens
+            const int row = s.first + w.at;
+            const RowSum of_row = row_top(p, row);
+            const double sum = exact_sum<F32>(p, row, of_row.top, per);
+            double gone = 0.0;
+            for (int b0 = w.at + 1; b0 < child; b0 += 64) {
+              const int c = b0 + lane;
+              const int t = c < child && p.d.parents[s.first + c] == w.at ? p.d.tokens[s.first + c] : -1;
+              bool first = t >= 0 && t < p.d.vocab;
+              for (int e = w.at + 1; first && e < c; ++e) first = p.d.parents[s.first + e] != w.at || p.d.tokens[s.first + e] != t;
+              gone += wave_sum(first ? weight_of(number(logit<F32>(p, row, t)), of_row.top, per) / sum : 0.0);
+            }
+            now = weight_of(number(logit<F32>(p, row, child_token)), of_row.top, per) / sum;
+            against = u_child * (1.0 - gone);
+          }
+          accepted = against < now;
+          if (!accepted) taken += p_child;
+        }
+      }
+      if (accepted) {
+        if (write) p.d.path[s.first + w.kept] = child, p.d.emitted[s.first + w.kept - 1] = child_token;
+        w.at = child, ++w.kept, w.tried = 0, taken = 0.0;
+        if constexpr (FIRST) return w;
+        mask = __ballot(parent == w.at && lane > k);
+      } else {
+        ++w.tried;
+      }
+    }
+    if (!FIRST && s.n <= 64) {
+      const uint64_t children = __ballot(parent == w.at && token >= 0);
+      const int many = __popcll(children), to = __popcll(children & ((1ull << lane) - 1));
+      if (many <= kGone && (children >> lane & 1)) draw->gone[to] = token;
+      if (lane == 0) draw->many = many <= kGone ? many : -1;
+    }
+  }
+  if (!FIRST && s.n > 64 && lane == 0) draw->many = -1;
+  if (probs && per > 0.0) w.times = w.tried > 1 ? p.times[s.first + w.at] : (double)w.tried;   // (p.times is there with distributions only)
+  return w;
+}
+
+// With much to read: which rows are wanted after node 0's
+template <bool F32>
+__global__ __launch_bounds__(64) void first_step_kernel(VerifyArgs p) {
+  const int b = blockIdx.x;
+  const Span s = span_of(p, b);
+  if (s.n == 0) return;
+  const double per = inverse_temperature(p, b);
+  const int top = walk<F32, true>(p, s, per, false).at;
+  for (int i = threadIdx.x; i < s.n; i += 64) {
+    int at = i;   // up to the accepted child, or past it
+    while (at > top) {
+      const int up = p.d.parents[s.first + at];
+      at = up < at ? up : -1;
+    }
+    const uint64_t mine = __ballot(top > 0 && at == top);   // (the wave's lanes that are here: the first ones)
+    if (mine) {
+      const int lane = threadIdx.x;
+      int to = 0;
+      if (lane == 0) to = atomicAdd(p.many, __popcll(mine));
+      to = uniform_int(to) + __popcll(mine & ((1ull << lane) - 1));
+      if ((mine >> lane & 1) && to >= 0 && to < p.d.rows) p.wanted[to] = {per, s.first + i};
+    }
+  }
+}
+
+// Element i.. of what is drawn from, in units of the row's largest weight (kRest: of 1)
+template <bool F32, int N>
+__device__ inline void weights_of(const VerifyArgs& p, const Span& s, const Draw& d, double per, int i, double (&w)[N]) {
+  static_assert(N % kOnce == 0, "");
+  const double over = 1.0 / d.sum;
+#pragma unroll
+  for (int k = 0; k < N; k += kOnce) {
+    float x[kOnce], q[kOnce];
+    logits<F32>(p, d.row, i + k, x);
+    if (d.how == kRest) draft_probs(p, d.row, i + k, q);
+#pragma unroll
+    for (int j = 0; j < kOnce; ++j) w[k + j] = weight_of(number(x[j]), d.top, per);
+    if (d.how == kRest) {
+#pragma unroll
+      for (int j = 0; j < kOnce; ++j) w[k + j] = fmax(w[k + j] * over - d.times * (q[j] > 0.0f ? (double)q[j] : 0.0), 0.0);
+    }
+  }
+  if (d.how == kWithout && d.many >= 0) {
+    for (int c = 0; c < d.many; ++c) {
+      const int gone = d.gone[c] - i;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (gone == j) w[j] = 0.0;
+    }
+  } else if (d.how == kWithout) {
+    const int at = d.row - s.first;
+    for (int c = next_child(p, s, at, at + 1); c < s.n; c = next_child(p, s, at, c + 1)) {
+      const int gone = p.d.tokens[s.first + c] - i;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (gone == j) w[j] = 0.0;
+    }
+  }
+}
+
+// Inclusive running sum over the wave's lanes
+__device__ inline double wave_running(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double other = __shfl_up(v, m, 64);
+    if ((threadIdx.x & 63) >= m) v += other;
+  }
+  return v;
+}
+// The next token, by a workgroup, whose threads share the piece in which it lies
+template <bool F32, int THREADS>
+__device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw& of, double per, int b) {
+  constexpr int kMine = kPiece / THREADS;
+  __shared__ double wave_at[THREADS / 64];
+  __shared__ int firsts[THREADS / 64], lasts[THREADS / 64];
+  __shared__ Draw all_of_it;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  bool nothing_left = false;
+  const auto piece_sum = [&](int c) -> double {
+    if (c >= p.pieces) return 0.0;
+    if (!nothing_left) return p.left[(size_t)b * p.pieces + c];
+    const PieceSum q = p.sums[(size_t)of.row * p.pieces + c];   // all of the row
+    return q.top == -INFINITY ? 0.0 : q.sum * weight_of(q.top, (double)of.top, per);
+  };
+  // every wave: pieces a lane, 64 at a time
+  const auto sum_of_all = [&] {
+    double sum = 0.0;
+    for (int c0 = 0; c0 < p.pieces; c0 += 64) sum += lane_double(wave_running(piece_sum(c0 + lane)), 63);
+    return sum;
+  };
+  double all = sum_of_all();
+  if (!(all > 0.0)) {
+    nothing_left = true;
+    all = sum_of_all();
+  }
+  const double want = random_of(p, s.first) * all;
+  int piece = 0;
+  double before = 0.0, sum = 0.0;   // before: the sum of the pieces in front
+  for (int c0 = 0; c0 < p.pieces; c0 += 64) {
+    const double mine = piece_sum(c0 + lane), upto = wave_running(mine);
+    const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && sum + upto > want);
+    if (some) {   // (the last one with anything, if rounding leaves `want` at the sum of all)
+      const int k = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+      piece = c0 + k, before = sum + lane_double(upto, k) - lane_double(mine, k);
+    }
+    if (over) break;
+    sum += lane_double(upto, 63);
+  }
+  if (threadIdx.x == 0) {
+    all_of_it = of;
+    if (nothing_left) all_of_it.how = kAll;
+  }
+  __syncthreads();
+  const Draw& d = all_of_it;
+  double w[kMine], mine = 0.0;
+  weights_of<F32>(p, s, d, per, piece * kPiece + (int)threadIdx.x * kMine, w);
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) mine += w[j];
+  const double upto = wave_running(mine);
+  if (lane == 63) wave_at[wave] = upto;
+  __syncthreads();
+  double run = before;
+  for (int k = 0; k < wave; ++k) run += wave_at[k];
+  run += upto - mine;
+  // the first element whose running sum is above `want`; if rounding leaves none, the last one that has a weight
+  int first = -1, last = -1;
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    run += w[j];
+    if (w[j] > 0.0) {
+      last = piece * kPiece + (int)threadIdx.x * kMine + j;
+      if (run > want && first < 0) first = last;
+    }
+  }
+  const uint64_t over = __ballot(first >= 0), some = __ballot(last >= 0);
+  if (over ? lane == __ffsll((unsigned long long)over) - 1 : lane == 0) firsts[wave] = first;
+  if (some ? lane == 63 - __clzll((long long)some) : lane == 0) lasts[wave] = last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int token = -1;
+    for (int k = 0; k < THREADS / 64 && token < 0; ++k) token = firsts[k];
+    for (int k = THREADS / 64 - 1; k >= 0 && token < 0; --k) token = lasts[k];
+    p.d.emitted[d.out] = token;
+  }
+}
+
+// ONE_LAUNCH: the last workgroup of a sequence draws
+template <bool F32, bool ONE_LAUNCH>
+__global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs p) {
+  constexpr int THREADS = kThreads;
+  __shared__ double scratch[THREADS / 64];
+  __shared__ Draw draw;
+  __shared__ int before_me;
+  const int piece = blockIdx.x % (unsigned)p.pieces, b = blockIdx.x / (unsigned)p.pieces, lane = threadIdx.x & 63;
+  const Span s = span_of(p, b);
+  const double per = inverse_temperature(p, b);
+  if (s.n == 0) {
+    if (piece == 0 && threadIdx.x == 0) {
+      p.d.accepted[b] = 0;
+      if constexpr (!ONE_LAUNCH) p.draws[b].how = kNothing;
+    }
+    return;
+  }
+  if (threadIdx.x < 64) {
+    const Way w = walk<F32, false>(p, s, per, piece == 0, &draw);
+    RowSum r = row_top(p, s.first + w.at);
+    if (w.times > 0.0) r.sum = row_sum<true>(p, s.first + w.at, per).sum;
+    const bool none = per == 0.0 || r.top == -INFINITY;
+    const int out = s.first + w.kept - 1;
+    if (lane == 0) {
+      draw.times = w.times, draw.sum = r.sum, draw.top = r.top, draw.row = s.first + w.at, draw.out = out;
+      draw.how = none ? kNothing : w.times > 0.0 ? kRest : w.tried > 0 && !p.d.draft_probs ? kWithout : kAll;
+    }
+    if (piece == 0) {
+      for (int i = w.kept + lane; i < s.n; i += 64) p.d.path[s.first + i] = -1, p.d.emitted[s.first + i] = -1;
+      if (lane == 0) {
+        p.d.accepted[b] = w.kept;
+        if (none) p.d.emitted[out] = r.top == -INFINITY ? -1 : r.at;
+        if constexpr (!ONE_LAUNCH) p.draws[b] = draw;
+      }
+    }
+  }
+  __syncthreads();
+  const Draw& d = draw;
+  if (d.how == kNothing) return;
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < kPiece / THREADS / kOnce; ++k) {
+    double w[kOnce];
+    weights_of<F32>(p, s, d, per, piece * kPiece + (k * THREADS + threadIdx.x) * kOnce, w);
+#pragma unroll
+    for (int j = 0; j < kOnce; ++j) sum += w[j];
+  }
+  sum = block_sum<THREADS>(sum, scratch);
+  if (threadIdx.x == 0) p.left[(size_t)b * p.pieces + piece] = sum;
+  if constexpr (ONE_LAUNCH) {
+    if (threadIdx.x == 0) {
+      __threadfence();   // the sum, before the count says that it is there
+      before_me = atomicAdd(p.done + b, 1);
+    }
+    __syncthreads();
+    if (before_me != p.pieces - 1) return;
+    __threadfence();   // the others' sums
+    draw_token<F32, THREADS>(p, s, d, per, b);
+  }
+}
+
+template <bool F32>
+__global__ __launch_bounds__(kRowThreads) void draw_kernel(VerifyArgs p) {
+  const int b = blockIdx.x;
+  if (p.draws[b].how != kNothing) draw_token<F32, kRowThreads>(p, span_of(p, b), p.draws[b], inverse_temperature(p, b), b);
+}
+
+// ---- children one after the other, where drafts come with distributions ----------------------------------------------------------------------------
+template <bool F32>
+__device__ inline bool accepts(const VerifyArgs& p, int row, const RowSum& r, double per, int child_row, double t, double left) {
   const int token = p.d.tokens[child_row];
   if (token < 0 || token >= p.d.vocab || !(r.sum > 0.0)) return false;
-  const double q = draft_prob(p, row, token), w = weight_of(logit<F32>(p, row, token), r.top, per) / r.sum;
-  return uniform_of(p, child_row) * q * s < fmax(w - t * q, 0.0);
+  const double q = draft_prob(p, row, token), w = weight_of(number(logit<F32>(p, row, token)), r.top, per) / r.sum;
+  return random_of(p, child_row) * q * left < fmax(w - t * q, 0.0);
+}
+// Sum of a thread's elements of max(p - t q, 0)
+template <bool F32, int N>
+__device__ inline double rest_of(const VerifyArgs& p, const Span& s, const RowSum& r, double per, double t, int row, int i) {
+  double w[N], sum = 0.0;
+  Draw rest{};
+  rest.times = t, rest.sum = r.sum, rest.top = r.top, rest.row = row, rest.how = kRest;
+  weights_of<F32>(p, s, rest, per, i, w);
+#pragma unroll
+  for (int j = 0; j < N; ++j) sum += w[j];
+  return sum;
 }
 
 template <bool F32>
-__global__ __launch_bounds__(kRowThreads) void rest_sums_kernel(VerifyArgs p) {
-  constexpr int kEach = kPiece / kRowThreads, kOnce = 8;
-  __shared__ double scratch[kRowThreads / 64];
-  const int row = blockIdx.x / (unsigned)p.pieces, piece = blockIdx.x % (unsigned)p.pieces, b = sequence_of(p, row);
+__global__ __launch_bounds__(kThreads) void rest_sums_kernel(VerifyArgs p) {
+  __shared__ double scratch[kThreads / 64];
+  const int row = blockIdx.x / (unsigned)p.pieces, piece = blockIdx.x % (unsigned)p.pieces;
+  if (p.choice[row] != kMany) return;
+  const int b = sequence_of(p, row);
   if (b < 0) return;
   const double per = inverse_temperature(p, b);
   const Span s = span_of(p, b);
   const int v = row - s.first, child = next_child(p, s, v, v + 1);
-  if (child >= s.n || per == 0.0) return;
-  const RowSum r = row_sum(p, row, per);
+  if (child >= s.n) return;
+  const RowSum r = row_sum<true>(p, row, per);
   if (!(r.sum > 0.0) || accepts<F32>(p, row, r, per, s.first + child, 0.0, 1.0)) return;
   double sum = 0.0;
 #pragma unroll
-  for (int k = 0; k < kEach / kOnce; ++k) {
-    const int i = piece * kPiece + (k * kRowThreads + threadIdx.x) * kOnce;
-    float x[kOnce];
-    logits<F32>(p, row, i, x);
-#pragma unroll
-    for (int j = 0; j < kOnce; ++j)
-      if (i + j < p.d.vocab) sum += fmax(weight_of(x[j], r.top, per) / r.sum - draft_prob(p, row, i + j), 0.0);
-  }
-  sum = block_sum<kRowThreads>(sum, scratch);
+  for (int k = 0; k < kEach / kOnce; ++k) sum += rest_of<F32, kOnce>(p, s, r, per, 1.0, row, piece * kPiece + (k * kThreads + threadIdx.x) * kOnce);
+  sum = block_sum<kThreads>(sum, scratch);
   if (threadIdx.x == 0) p.rest[(size_t)row * p.pieces + piece] = sum;
 }
 
-// A row's children one after the other
+// Rows of two children and more whose first one is rejected: the others
 template <bool F32>
-__global__ __launch_bounds__(kWalkThreads) void children_kernel(VerifyArgs p) {
-  constexpr int kEach = kPiece / kWalkThreads;
-  __shared__ double scratch[kWalkThreads / 64];
-  const int row = blockIdx.x, b = sequence_of(p, row);
+__global__ __launch_bounds__(kRowThreads) void children_kernel(VerifyArgs p) {
+  constexpr int kMine = kPiece / kRowThreads;
+  __shared__ double scratch[kRowThreads / 64];
+  const int row = blockIdx.x;
+  if (p.choice[row] != kMany) return;
+  const int b = sequence_of(p, row);
   if (b < 0) return;
   const double per = inverse_temperature(p, b);
-  if (per == 0.0) return;
   const Span s = span_of(p, b);
   const int v = row - s.first;
-  const RowSum r = row_sum(p, row, per);
-  double t = 0.0, left = 1.0;
-  int found = -1, tried = 0;
-  for (int child = next_child(p, s, v, v + 1); child < s.n; child = next_child(p, s, v, child + 1)) {
-    if (tried == 1) {
-      t = 1.0, left = 0.0;
-      for (int c = 0; c < p.pieces; ++c) left += p.rest[(size_t)row * p.pieces + c];
-    } else if (tried > 1) {
-      t += left, left = 0.0;
-      for (int c = 0; c < p.pieces; ++c) {
-        double sum = 0.0;
-        const int i = c * kPiece + threadIdx.x * kEach;
-        float x[kEach];
-        logits<F32>(p, row, i, x);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (i + j < p.d.vocab) sum += fmax(weight_of(x[j], r.top, per) / r.sum - t * draft_prob(p, row, i + j), 0.0);
-        left += block_sum<kWalkThreads>(sum, scratch);
-      }
-    }
+  int child = next_child(p, s, v, v + 1);
+  if (child >= s.n) return;
+  const int second = next_child(p, s, v, child + 1);
+  if (second >= s.n) return;
+  const RowSum r = row_sum<true>(p, row, per);
+  if (accepts<F32>(p, row, r, per, s.first + child, 0.0, 1.0)) return;
+  double t = 1.0, left = 0.0;
+  if (r.sum > 0.0)
+    for (int c = 0; c < p.pieces; ++c) left += p.rest[(size_t)row * p.pieces + c];
+  int found = -1;
+  for (child = second; child < s.n;) {
     if (accepts<F32>(p, row, r, per, s.first + child, t, left)) {
       found = child;
       break;
     }
-    ++tried;
-  }
-  // nothing accepted: what the next token is drawn from
-  if (found < 0 && r.sum > 0.0 && tried > 1) {
     t += left;
-    for (int c = 0; c < p.pieces; ++c) {
-      double sum = 0.0;
-      const int i = c * kPiece + threadIdx.x * kEach;
-      float x[kEach];
-      logits<F32>(p, row, i, x);
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (i + j < p.d.vocab) sum += fmax(weight_of(x[j], r.top, per) / r.sum - t * draft_prob(p, row, i + j), 0.0);
-      sum = block_sum<kWalkThreads>(sum, scratch);
-      if (threadIdx.x == 0) p.rest[(size_t)row * p.pieces + c] = sum;
-    }
-  } else if (tried == 1) {
-    t = 1.0;
+    child = next_child(p, s, v, child + 1);
+    if (child >= s.n || !(r.sum > 0.0)) continue;
+    left = 0.0;
+    for (int c = 0; c < p.pieces; ++c) left += block_sum<kRowThreads>(rest_of<F32, kMine>(p, s, r, per, t, row, c * kPiece + threadIdx.x * kMine), scratch);
   }
-  if (threadIdx.x == 0) p.choice[row] = found, p.times[row] = found < 0 ? t : 0.0;
-}
-
-// ---- the walk ----------------------------------------------------------------------------------------------------------------------------------
-template <bool F32>
-__global__ __launch_bounds__(kWalkThreads) void walk_kernel(VerifyArgs p) {
-  constexpr int kEach = kPiece / kWalkThreads, kWaves = kWalkThreads / 64;
-  __shared__ double scratch[kWaves];
-  __shared__ double wave_at[kWaves + 1];
-  __shared__ int said[4];
-  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const Span s = span_of(p, b);
-  const double per = inverse_temperature(p, b);
-  if (s.n == 0) {
-    if (threadIdx.x == 0) p.d.accepted[b] = 0;
-    return;
-  }
-  if (wave == 0) {
-    int at = 0, kept = 1;
-    double taken = 0.0;
-    RowSum r = row_sum(p, s.first, per);
-    const auto accept = [&](int child) {
-      at = child, taken = 0.0;
-      if (lane == 0) {
-        p.d.path[s.first + kept] = child;
-        p.d.emitted[s.first + kept - 1] = p.d.tokens[s.first + child];
-      }
-      ++kept;
-      r = row_sum(p, s.first + child, per);
-    };
-    if (lane == 0) p.d.path[s.first] = 0;
-    if (p.d.draft_probs && per > 0.0) {
-      for (int child; (child = p.choice[s.first + at]) > at && child < s.n;) accept(child);
-    } else {
-      for (int child = next_child(p, s, 0, 1); child < s.n; child = next_child(p, s, at, child + 1)) {
-        const int token = p.d.tokens[s.first + child];
-        if (token < 0 || token >= p.d.vocab) continue;
-        if (per == 0.0) {
-          if (token == r.at) accept(child);
-          continue;
-        }
-        // a token that an elder sibling had has been taken out
-        bool again = false;
-        for (int c0 = at + 1; c0 < child; c0 += 64) {
-          const int c = c0 + lane;
-          again = again || __any(c < child && p.d.parents[s.first + c] == at && p.d.tokens[s.first + c] == token);
-        }
-        if (again || !(r.sum > 0.0)) continue;
-        const double mine = weight_of(logit<F32>(p, s.first + at, token), r.top, per) / r.sum;
-        if (uniform_of(p, s.first + child) * (1.0 - taken) < mine) accept(child);
-        else taken += mine;
-      }
-    }
-    for (int i = kept + lane; i < s.n; i += 64) p.d.path[s.first + i] = -1, p.d.emitted[s.first + i] = -1;
-    if (lane == 0) p.d.accepted[b] = kept, said[0] = at, said[1] = kept, said[2] = r.at;
-    if (lane == 0) scratch[0] = r.sum, scratch[1] = (double)r.top;
-  }
-  __syncthreads();
-  const int at = said[0], kept = said[1], row = s.first + at;
-  int32_t* out = p.d.emitted + s.first + kept - 1;
-  RowSum r{scratch[0], (float)scratch[1], said[2]};
-  __syncthreads();
-  if (per == 0.0 || !(r.sum > 0.0)) {
-    if (threadIdx.x == 0) *out = r.top == -INFINITY ? -1 : r.at;
-    return;
-  }
-  // The next token: weights in units of the row's largest, which are p r.sum.  `how`: 0 p, 1 p without the children's tokens, 2 max(p - t q, 0)
-  const double t = p.d.draft_probs ? p.times[row] : 0.0;
-  int how = p.d.draft_probs ? (t > 0.0 ? 2 : 0) : next_child(p, s, at, at + 1) < s.n ? 1 : 0;
-  const auto weights = [&](int c, double (&w)[kEach]) {   // of this thread's elements of piece c
-    const int i = c * kPiece + threadIdx.x * kEach;
-    float x[kEach];
-    logits<F32>(p, row, i, x);
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      w[j] = i + j < p.d.vocab ? weight_of(x[j], r.top, per) / r.sum : 0.0;
-      if (how == 2 && i + j < p.d.vocab) w[j] = fmax(w[j] - t * draft_prob(p, row, i + j), 0.0);
-    }
-    if (how == 1)
-      for (int k = next_child(p, s, at, at + 1); k < s.n; k = next_child(p, s, at, k + 1)) {
-        const int gone = p.d.tokens[s.first + k] - i;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (gone == j) w[j] = 0.0;
-      }
-  };
-  const auto piece_sum = [&](int c) -> double {
-    if (how == 2) return p.rest[(size_t)row * p.pieces + c];
-    if (how == 1) {   // recomputed where a token is gone
-      bool hit = false;
-      for (int k = next_child(p, s, at, at + 1); k < s.n; k = next_child(p, s, at, k + 1)) {
-        const int token = p.d.tokens[s.first + k];
-        hit = hit || (token >= 0 && token / kPiece == c);
-      }
-      if (hit) {
-        double w[kEach], sum = 0.0;
-        weights(c, w);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) sum += w[j];
-        return block_sum<kWalkThreads>(sum, scratch);
-      }
-    }
-    const PieceSum q = p.sums[(size_t)row * p.pieces + c];
-    return q.top == -INFINITY ? 0.0 : q.sum * weight_of(q.top, r.top, per) / r.sum;
-  };
-  double all = 0.0;
-  for (int c = 0; c < p.pieces; ++c) all += piece_sum(c);
-  if (!(all > 0.0) && how > 0) {
-    how = 0;
-    for (int c = 0; c < p.pieces; ++c) all += piece_sum(c);
-  }
-  const double want = uniform_of(p, s.first) * all;
-  int piece = -1;
-  double before = 0.0, sum = 0.0;
-  for (int c = 0; c < p.pieces; ++c) {
-    const double mine = piece_sum(c);
-    if (mine > 0.0) {   // (the last one with anything, if rounding leaves `want` at the sum of all)
-      if (piece >= 0) before = sum;
-      piece = c;
-    }
-    sum += mine;
-    if (sum > want) break;
-  }
-  if (piece < 0) {
-    if (threadIdx.x == 0) *out = -1;
-    return;
-  }
-  double w[kEach], mine = 0.0;
-  weights(piece, w);
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) mine += w[j];
-  double upto = mine;   // inclusive running sum over the wave's lanes
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double other = __shfl_up(upto, m, 64);
-    if (lane >= m) upto += other;
-  }
-  if (lane == 63) wave_at[wave] = upto;
-  if (threadIdx.x == 0) said[3] = -1;
-  __syncthreads();
-  double start = before;
-  for (int k = 0; k < wave; ++k) start += wave_at[k];
-  start += upto - mine;
-  // the first element whose running sum is above `want`; if rounding leaves none, the last one that has a weight
-  int first = INT32_MAX, last = -1;
-  double run = start;
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    run += w[j];
-    if (w[j] > 0.0) {
-      last = piece * kPiece + (int)threadIdx.x * kEach + j;
-      if (run > want) first = min(first, last);
-    }
-  }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) first = min(first, __shfl_xor(first, m, 64)), last = max(last, __shfl_xor(last, m, 64));
-  __syncthreads();
-  int* const firsts = reinterpret_cast<int*>(scratch);   // (two ints an element)
-  if (lane == 0) firsts[2 * wave] = first, firsts[2 * wave + 1] = last;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 0; k < kWaves; ++k) first = min(first, firsts[2 * k]), last = max(last, firsts[2 * k + 1]);
-    *out = first != INT32_MAX ? first : last;
-  }
+  __syncthreads();   // (all have read it)
+  if (threadIdx.x == 0) p.choice[row] = found, p.times[row] = t;
 }
 
 VerifyArgs args_of(const ave_fp4_draft& d, void* ws, size_t* bytes) {
@@ -493,25 +787,48 @@ VerifyArgs args_of(const ave_fp4_draft& d, void* ws, size_t* bytes) {
   };
   const size_t all = (size_t)d.rows * p.pieces;
   p.sums = reinterpret_cast<PieceSum*>(take(all * sizeof(PieceSum)));
+  p.left = reinterpret_cast<double*>(take((size_t)d.batch * p.pieces * sizeof(double)));
+  p.draws = reinterpret_cast<Draw*>(take((size_t)d.batch * sizeof(Draw)));
   if (d.draft_probs) {
     p.rest = reinterpret_cast<double*>(take(all * sizeof(double)));
     p.times = reinterpret_cast<double*>(take((size_t)d.rows * sizeof(double)));
     p.choice = reinterpret_cast<int*>(take((size_t)d.rows * sizeof(int)));
+  } else {
+    p.wanted = reinterpret_cast<Wanted*>(take((size_t)d.rows * sizeof(Wanted)));
+    p.many = reinterpret_cast<int*>(take(sizeof(int)));
   }
+  p.done = reinterpret_cast<int*>(take((size_t)d.batch * sizeof(int)));
   if (bytes) *bytes = used;
   return p;
 }
 
+// Node 0's rows first and then those that are wanted, instead of all at once: two launches more, against what need not be read.
+bool in_two_steps(const VerifyArgs& p) {
+  return (int64_t)p.d.rows * p.d.vocab * (p.d.logits_f32 ? 4 : 2) > (int64_t)64 << 20 && p.d.rows >= 3 * (int64_t)p.d.batch;
+}
+
 template <bool F32>
 hipError_t launch(const VerifyArgs& p, hipStream_t s) {
-  const int rows = p.d.rows;
-  const dim3 each((unsigned)p.pieces * (unsigned)rows);
-  if (rows > 0) hipLaunchKernelGGL((row_sums_kernel<F32>), each, dim3(kRowThreads), 0, s, p);
-  if (rows > 0 && p.d.draft_probs) {
-    hipLaunchKernelGGL((rest_sums_kernel<F32>), each, dim3(kRowThreads), 0, s, p);
-    hipLaunchKernelGGL((children_kernel<F32>), dim3((unsigned)rows), dim3(kWalkThreads), 0, s, p);
+  const unsigned rows = (unsigned)p.d.rows, batch = (unsigned)p.d.batch, pieces = (unsigned)p.pieces;
+  if (p.d.draft_probs) {
+    if (rows > 0) {
+      hipLaunchKernelGGL((row_sums_kernel<F32, true, 0>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
+      hipLaunchKernelGGL((rest_sums_kernel<F32>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
+      hipLaunchKernelGGL((children_kernel<F32>), dim3(rows), dim3(kRowThreads), 0, s, p);
+    }
+  } else if (in_two_steps(p)) {
+    hipLaunchKernelGGL((row_sums_kernel<F32, false, 1>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((first_step_kernel<F32>), dim3(batch), dim3(64), 0, s, p);
+    hipLaunchKernelGGL((row_sums_kernel<F32, false, 2>), dim3(std::min(rows * pieces, 8u * (unsigned)compute_units())), dim3(kThreads), 0, s, p);
+  } else if (rows > 0) {
+    hipLaunchKernelGGL((row_sums_kernel<F32, false, 0>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
   }
-  hipLaunchKernelGGL((walk_kernel<F32>), dim3((unsigned)p.d.batch), dim3(kWalkThreads), 0, s, p);
+  if (batch * pieces <= (unsigned)compute_units()) {
+    hipLaunchKernelGGL((walk_kernel<F32, true>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((walk_kernel<F32, false>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((draw_kernel<F32>), dim3(batch), dim3(kRowThreads), 0, s, p);
+  }
   return hipGetLastError();
 }
 

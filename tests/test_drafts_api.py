@@ -68,7 +68,7 @@ def test_workspaces_and_empty_calls():
 
 @pytest.mark.parametrize("bad,text", [
     (dict(rows=-1), "non-negative"), (dict(batch=-1), "non-negative"), (dict(vocab=0), "vocab must be"), (dict(vocab=(1 << 30) + 1), "vocab must be"),
-    (dict(rows=1 << 24), "below 2^24"), (dict(rows=1 << 14, vocab=1 << 23), "below 2^24"), (dict(cu_q=0), "null device pointer"), (dict(logits=0), "null device"),
+    (dict(rows=1 << 22), "below 2^22"), (dict(batch=1 << 22), "below 2^22"), (dict(rows=1 << 12, vocab=1 << 23), "below 2^22"), (dict(cu_q=0), "null device pointer"), (dict(logits=0), "null device"),
     (dict(uniform=0), "null device pointer"), (dict(emitted=0), "null device pointer"), (dict(logits=P + 1), "aligned"),
     (dict(logits=P + 2, logits_f32=1), "aligned"), (dict(draft_probs=P + 2), "aligned")], ids=str)
 def test_drafts_that_are_refused(bad, text):

@@ -316,6 +316,32 @@ def test_numbers_next_to_a_border(gpu):
     _verify(gpu, d, [1.0] * 64)
 
 
+@pytest.mark.parametrize("f32", [False, True])
+def test_acceptance_next_to_a_border(gpu, f32):
+    """The number of a child is the fp32 one nearest to the probability that it is compared with: of a first child, and of a second one behind a rejected one."""
+    d = _draft(22, [4] * 48, 20011, f32=f32, sharp=2.0)
+    hits = 0
+    for b in range(48):
+        r = slice(4 * b, 4 * b + 4)
+        d["parents"][r] = [-1, 0, 0, 1 + b % 2]
+        d["tokens"][r] = np.argsort(-d["logits"][4 * b], kind="stable")[:4]
+        p = D.softmax(d["logits"][4 * b], 1.0)[d["tokens"][r]]
+        exact = [0, p[1], p[2] / (1 - p[1]), 0]
+        d["uniform"][r] = [0.5, p[1] if b % 2 else 1.0, exact[2], 0.5]
+        at = 1 if b % 2 else 2
+        hits += abs(float(d["uniform"][4 * b + at]) - exact[at]) < 2.0 ** -24 * exact[at]
+    assert hits == 48
+    want = _verify(gpu, d, [1.0] * 48)
+    assert 5 < (want[0] > 1).sum() < 43
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_much_to_read(gpu, f32):
+    """Rows of more than 64 MB: node 0's first, then those behind the accepted child."""
+    d = _draft(31, [14, 1, 20, 12, 17, 0, 9], 270003 if f32 else 500009, f32=f32)
+    _verify(gpu, d, [1.0, 0.9, 0.0, 1.0, 0.7, 1.0, 1.0], extra=3)
+
+
 def test_strided_rows_and_no_temperature(gpu):
     d = _draft(4, [6, 5], 1001, probs=True)
     logits, probs = D.tensor(d["logits"], gpu).bfloat16(), D.tensor(d["probs"], gpu)
