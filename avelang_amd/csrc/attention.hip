@@ -48,15 +48,24 @@ TreeArgs tree_args(const ave_fp4_attention& a, const ave_fp4_tree& t, const ave_
 }
 }  // namespace
 
+namespace {
+// For trees the kernel for prompts has blocks of 64 rows, too, and is ahead from 17 rows on (8 nodes, 32 heads on 8 of 128: 64 sequences of 4096 keys 78 us
+// to 97, 64 of 1000 35 to 45, one of 131072 45 to 55), but for few short sequences, whose items stay whole (one of 700: 17 to 14).
+int tree_row_tiles(const TreeArgs& p) {
+  const int64_t rows = (int64_t)(p.a.cu_q ? p.a.max_q : 1) * p.group, keys = (int64_t)p.a.table_pages << p.page_shift;
+  return rows <= 16 ? 1 : rows <= 32 && keys <= 1024 && p.a.batch * (int64_t)p.c.kv_heads <= 32 ? 2 : 0;
+}
+}  // namespace
+
 size_t tree_attention_workspace_bytes(const ave_fp4_attention& a, const ave_fp4_tree& t, const ave_fp4_kv_cache& c) {
   const TreeArgs p = tree_args(a, t, c);
-  if (const int tiles = decode_row_tiles(p)) return attn_decode_workspace(p, tiles);
+  if (const int tiles = tree_row_tiles(p)) return attn_decode_workspace(p, tiles);
   return attn_prompt_workspace(p);
 }
 
 hipError_t launch_tree_attention(const ave_fp4_attention& a, const ave_fp4_tree& t, const ave_fp4_kv_cache& c, void* workspace, hipStream_t s) {
   const TreeArgs args = tree_args(a, t, c);
-  if (const int tiles = decode_row_tiles(args)) return launch_attn_decode(args, tiles, workspace, s);
+  if (const int tiles = tree_row_tiles(args)) return launch_attn_decode(args, tiles, workspace, s);
   return launch_attn_prompt(args, workspace, s);
 }
 

@@ -44,6 +44,10 @@ __device__ inline Sequence sequence(const AttnArgs& p, int b) {
   return s;
 }
 
+// A value that all lanes hold, in a scalar register
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
+
 __device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ inline unsigned wave_scan(unsigned v) {   // inclusive prefix sums over the lanes
   v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // one, two, four, eight lanes to the right in a row of 16
@@ -184,6 +188,106 @@ __device__ inline Item<U> item_of(const A& p, U u, int& b, U& b_begin, Sequence&
   return it;
 }
 
+// ---- the division of a call with a tree, whose blocks of rows all have the same units ------------------------------------------------
+// Where a workgroup's walk stands: a block of rows of key head `head` of sequence b, its tiles from tile0 on, its first unit
+template <typename U>
+struct TreeWalk {
+  Sequence s;
+  int b, head, row0, tile0;
+  unsigned units, blocks;
+  U begin;
+};
+template <int ROWS, int TILE>
+__device__ inline unsigned tree_units(const TreeArgs& p, const Sequence& s, unsigned& blocks, int& tile0) {   // of a block
+  blocks = (unsigned)(s.n * p.group + ROWS - 1) / ROWS;
+  const Bounds r = bounds(p, s, 0, 0);
+  tile0 = r.lo_min / TILE;
+  return (unsigned)((r.hi_max > r.lo_min ? (r.hi_max + TILE - 1) / TILE - tile0 : 1) + p.item_units);
+}
+// Units [u0, u1) of workgroup g, and where they start.  `whole`: one item a workgroup (the walk of those without one has no units); the item number is
+// its unit.  Every wave by itself, 64 sequences at a time, a lane each.
+template <int ROWS, int TILE, typename U>
+__device__ inline TreeWalk<U> tree_part(const TreeArgs& p, unsigned g, unsigned workgroups, unsigned slack, bool& whole, U& u0, U& u1, U& all) {
+  const int lane = threadIdx.x & 63;
+  const unsigned heads = (unsigned)p.c.kv_heads;
+  Sequence s{0, 0, 0};
+  unsigned blocks = 0, units = 0;
+  int tile0 = 0;
+  const auto load = [&](int b0) {
+    blocks = units = 0;
+    if (b0 + lane < p.a.batch) {
+      s = sequence(p, b0 + lane);
+      units = tree_units<ROWS, TILE>(p, s, blocks, tile0);
+    }
+  };
+  load(0);
+  U items = lane_value(wave_scan((U)blocks * heads), 63);
+  all = lane_value(wave_scan((U)blocks * heads * units), 63);
+  unsigned most = units;
+  for (int b0 = 64; b0 < p.a.batch; b0 += 64) {
+    load(b0);
+    items += lane_value(wave_scan((U)blocks * heads), 63);
+    all += lane_value(wave_scan((U)blocks * heads * units), 63);
+    most = units > most ? units : most;
+  }
+  if (p.a.batch > 64) load(0);
+  Part<U> part{};
+  part.units = all;
+  cut(p, part, g, workgroups);
+  // Whole items where there is one a workgroup at most, and the longest is not much longer than equal parts would be
+  const unsigned equal = (unsigned)(all / workgroups);
+  whole = items <= workgroups && !__any(most > equal + slack);
+  u0 = whole ? (U)g : part.u0, u1 = whole ? (U)g + 1 : part.u1;
+  TreeWalk<U> w{};
+  if (whole ? (U)g >= items : part.u0 >= part.u1) {
+    u1 = u0;
+    return w;
+  }
+  U base = 0, mine, upto;
+  for (int b0 = 0;;) {
+    mine = (U)blocks * heads * (whole ? 1u : units), upto = wave_scan(mine);
+    const U sum = lane_value(upto, 63);
+    if (u0 < base + sum || b0 + 64 >= p.a.batch) {
+      w.b = b0;
+      break;
+    }
+    base += sum, b0 += 64;
+    load(b0);
+  }
+  const uint64_t here = __ballot(u0 - base < upto);
+  const int at = here ? __ffsll((unsigned long long)here) - 1 : 0;
+  w.b += at;
+  w.s = {lane_value(s.first, at), lane_value(s.n, at), lane_value(s.len, at)};
+  w.units = lane_value(units, at), w.blocks = lane_value(blocks, at), w.tile0 = lane_value(tile0, at);
+  const U begin = base + lane_value(upto - mine, at);
+  const unsigned of_item = whole || w.units == 0 ? 1u : w.units, index = (unsigned)((u0 - begin) / of_item);
+  w.head = (int)(w.blocks ? index / w.blocks : 0);
+  const unsigned block = index - (unsigned)w.head * w.blocks;
+  w.head = uniform(w.head < p.c.kv_heads ? w.head : p.c.kv_heads - 1);   // (the bounds hold if lengths change under the call, too)
+  w.row0 = uniform((int)(block < w.blocks ? block : 0) * ROWS);
+  w.begin = begin + (U)index * of_item;
+  return w;
+}
+// The next block of rows
+template <int ROWS, int TILE, typename U>
+__device__ inline void tree_next(const TreeArgs& p, TreeWalk<U>& w) {
+  w.begin += w.units;
+  w.row0 += ROWS;
+  if (w.row0 < (int)w.blocks * ROWS) return;
+  w.row0 = 0;
+  if (++w.head < p.c.kv_heads) return;
+  w.head = 0;
+  do {
+    if (w.b + 1 >= p.a.batch) {   // (lengths that change under the call)
+      w.units = 0;
+      return;
+    }
+    w.b = uniform(w.b + 1);
+    w.s = sequence(p, w.b);
+    w.units = tree_units<ROWS, TILE>(p, w.s, w.blocks, w.tile0);
+  } while (w.blocks == 0);
+}
+
 // ---- loads ---------------------------------------------------------------------------------------------------------------------
 // Lane l of the wave writes its 16 (4) bytes at LDS address lds + 16 l (4 l), straight from memory; counts on vmcnt.
 __device__ inline void to_lds16(const uint8_t* src, unsigned lds) {
@@ -254,10 +358,6 @@ __device__ inline unsigned seen_of(const TreeArgs& p, const Sequence& s, int t, 
   const unsigned before = (to > 15 ? 0xFFFFu : to > 0 ? (1u << to) - 1 : 0u) & (from > 15 ? 0u : from > 0 ? ~0u << from : ~0u);
   return before | (key + 15 >= base ? bits_of(p, row_bits(p, s, t), s.n, key - base) : 0u);
 }
-
-// A value that all lanes hold, in a scalar register
-__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ inline float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 
 // Eight bf16, from any address where `aligned` is not set
 __device__ inline v4i load8_bf16(const uint16_t* q, bool aligned) {
@@ -398,12 +498,14 @@ __device__ inline void finish_row(const AttnArgs& p, size_t row, int D, int chan
 template <typename A>
 hipError_t launch_attn_prompt(A p, void* workspace, hipStream_t s);
 size_t attn_prompt_workspace(const AttnArgs& p);
+size_t attn_prompt_workspace(const TreeArgs& p);
 template <typename A>
 hipError_t launch_attn_decode(A p, int row_tiles, void* workspace, hipStream_t s);
 template <typename A>
 size_t attn_decode_workspace(const A& p, int row_tiles);
 // rows: of a block; rows_expected: of a sequence and key head
 hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s);
+hipError_t launch_attn_join(const TreeArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s);
 // meta, maxima and sums, partial results, in this order
 inline size_t attn_meta_bytes(int workgroups) { return ((size_t)workgroups * sizeof(PartMeta) + 255) / 256 * 256; }
 inline size_t attn_workspace(int rows, int head_dim, int workgroups) {

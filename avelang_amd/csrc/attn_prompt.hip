@@ -33,7 +33,7 @@ namespace {
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr float kNoMax = -1.0e30f;   // a maximum of nothing
-constexpr int kTile = 64, kWaves = 4, kRows = 32 * kWaves, kBuffers = 2;
+constexpr int kTile = 64, kWaves = 4, kMostRows = 32 * kWaves, kBuffers = 2;
 
 template <int D>
 struct Shape {
@@ -69,6 +69,7 @@ struct Index {
 typedef __attribute__((address_space(3))) v4i LdsInt4;
 typedef __attribute__((address_space(3))) unsigned LdsInt;
 typedef __attribute__((address_space(3))) v2i LdsInt2;
+typedef __attribute__((address_space(3))) v4f LdsFloat4;
 typedef __attribute__((address_space(3))) uint16_t LdsShort;
 typedef __attribute__((address_space(3))) v4s LdsShort4;
 typedef __attribute__((address_space(3))) v8bf Lds8Bf16;
@@ -138,22 +139,24 @@ __device__ inline unsigned tree_bits(const TreeArgs& p, const Sequence& s, int r
 
 // SMALL: no tensor of the cache spans more than 4 GB, so that 32 bits hold a byte offset (64 prompts of 200 tokens: 84 us, with 64-bit
 // bases for every tile 89).
-template <int D, bool SMALL, typename U, typename A>
+// SPLIT 2: blocks of 64 rows; waves 0 and 1 take the first 32 keys of a tile, 2 and 3 the others, and the two results of a row meet at the item's end.
+template <int D, bool SMALL, typename U, typename A, int SPLIT = 1>
 __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_prompt_kernel(A p) {
   using S = Shape<D>;
-  constexpr int C = S::C;
+  constexpr int C = S::C, kRows = kMostRows / SPLIT;
   __shared__ __align__(512) unsigned char smem[S::kLds];
   __shared__ uint64_t nan_in[kBuffers][Values<D>::kScaleBytes][kWaves];   // which lanes of a wave hold a value with a NaN scale
   __shared__ __align__(16) int nan_any[kBuffers][kWaves];
+  __shared__ float other_ml[SPLIT == 2 ? 2 : 1][32][2];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid & 63, h = lane / 32, col = lane % 32;
   // Equal parts, or whole items: then a workgroup takes one of the first gridDim.x, in the next round the one as far from the end, and so on to
   // and fro.  What that may cost is the largest item of the last round (`most` units), less a workgroup's share of that round;
   // up to 24 units it is below the cost of partial results, their launch and the items' second starts (six prompts of 1000 tokens, 64 channels: 71 us,
   // in parts 88; 4 of 2000, 256 channels 173 and 222; one of 8192, 128 channels, 22 units: 591 and 624; 150 of 100 89 and 108).
-  __shared__ __align__(16) v4i sequences[kSequences];
+  __shared__ __align__(16) v4i sequences[kTree<A> ? 1 : kSequences];
   unsigned items = 0, rounds = 0;
   bool by_items = false;
-  if (p.a.batch <= kSequences) {
+  if (!kTree<A> && p.a.batch <= kSequences) {
     Sequence s{0, 0, 0};
     if (tid < p.a.batch) s = sequence(p, tid);
     sequences[tid] = v4i{s.first, s.n, s.len, (s.n * p.group + kRows - 1) / kRows};
@@ -172,7 +175,9 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
   const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
   Part<U> part{};
-  if (!by_items) part = take_part<kRows, kTile, U, true>(p, g, gridDim.x);
+  TreeWalk<U> walk{};
+  if constexpr (kTree<A>) walk = tree_part<kRows, kTile, U>(p, g, gridDim.x, 8, by_items, part.u0, part.u1, part.units);
+  else if (!by_items) part = take_part<kRows, kTile, U, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
   const float c = uniform(softmax_scale(p.a.scale));
   // this lane's places in LDS, of the first half of the first buffer: its key (row 8 i + 4 h' + t' of a result is key 16 h' + 4 i + t'), the
@@ -194,7 +199,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   int b = part.b;
   U b_begin = part.b_begin, per_head = part.per_head;
   Sequence seq = part.s;
-  if (tid == 0 && part.u0 >= part.u1) {   // no part, nothing to join
+  if (tid == 0 && (part.u0 >= part.u1 || (kTree<A> && by_items))) {   // no part, nothing to join
     PartMeta& m = p.meta[g];
     m.u0 = m.begin = m.end = part.units;
   }
@@ -205,9 +210,19 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   bool first_item = true;
   Item<U> it{};
   U u = part.u0;
-  for (unsigned round = 0; by_items ? round < rounds : u < part.u1; ++round) {
+  for (unsigned round = 0; by_items && !kTree<A> ? round < rounds : u < part.u1; ++round) {
     unsigned from = 0, to;   // units of the item
-    if (by_items) {
+    if constexpr (kTree<A>) {
+      if (!first_item) tree_next<kRows, kTile, U>(p, walk);
+      b = walk.b;
+      it.s = walk.s, it.head = walk.head, it.row0 = walk.row0, it.tile0 = walk.tile0, it.units = walk.units, it.begin = walk.begin;
+      if (!by_items && first_item && tid == 0) p.meta[g] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
+      if (!by_items && u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end, and the second launch finds its record)
+      from = by_items ? 0 : (unsigned)(u - it.begin);
+      to = by_items || part.u1 - it.begin >= it.units ? it.units : (unsigned)(part.u1 - it.begin);
+      u = by_items ? part.u1 : it.begin + to;
+      first_item = false;
+    } else if (by_items) {
       const unsigned rank = round * gridDim.x + (round % 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       if (rank >= items) break;
       it = ranked_item<kRows, U>(p, sequences, rank, b);
@@ -233,7 +248,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     const ConstInts table = (ConstInts)(p.a.page_table + (int64_t)b * p.a.page_table_stride);
 
     // what this wave's rows see: [lo_max, hi_min) all of them, [lo_min, hi_max) any
-    const int row0 = uniform(it.row0 + 32 * wave);
+    const int row0 = uniform(it.row0 + 32 * (SPLIT == 1 ? wave : wave % 2)), keys_from = SPLIT == 1 ? 0 : wave / 2 * 32;   // of a tile
     const bool active = row0 < uniform(rows);
     int lo_max, hi_min, lo_min, hi_max;
     if constexpr (kTree<A>) {
@@ -421,7 +436,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     // steps go without.
     const auto probabilities = [&](int tile, auto which, bool first, v16f& s, unsigned (&prob)[8]) {   // first: of the item
       constexpr int j = decltype(which)::value;
-      const int key0 = tile * kTile + 32 * j;
+      const int key0 = tile * kTile + 32 * j + keys_from;
       if (key0 < lo_max || key0 + 32 > hi_min) {
         const int here = lane_here();
         if constexpr (kTree<A>) {
@@ -470,7 +485,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       constexpr int j = decltype(which)::value;
       // ---- values with a NaN scale, zeros in LDS: NaN for the rows that see them, however little they count
       if (nan) {
-        const int here = lane_here(), key = tile * kTile + 32 * j + here / 32 * 16;
+        const int here = lane_here(), key = tile * kTile + 32 * j + keys_from + here / 32 * 16;
         uint64_t some;   // four bits for each of this lane's 16 keys
         if constexpr (kTree<A>) {
           const unsigned seen = tree_bits(p, it.s, row0 + here % 32, rows, key);
@@ -486,7 +501,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
 #pragma unroll
         for (int k = 0; k < C; ++k) {   // lane 4 t + quarter of a wave holds channels of block k
           const int quarter = D == 64 ? 2 * k : D == 128 ? k : k / 2;
-          const uint64_t* lanes = nan_in[buffer][D == 256 ? k % 2 : 0] + 2 * j;
+          const uint64_t* lanes = nan_in[buffer][D == 256 ? k % 2 : 0] + 2 * j + keys_from / 16;
           const bool hit = ((lane < 32 ? lanes[0] : lanes[1]) & some & (0x1111111111111111ull << quarter)) != 0;
           acc[k] += cross_max<false>(hit ? 1.0f : 0.0f) != 0.0f ? __builtin_nanf("") : 0.0f;
         }
@@ -498,7 +513,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         acc[n % C] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % kAhead], __builtin_bit_cast(v8bf, w), acc[n % C], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (n + kAhead < 2 * C) v[n % kAhead] = read_values(at, j, n + kAhead);
-        if (j == 0 && n + kAhead == 2 * C) read_keys(buffer, 1, place, keys);
+        if (SPLIT == 1 && j == 0 && n + kAhead == 2 * C) read_keys(buffer, 1, place, keys);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -524,7 +539,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       const int tile = tile0 + i, buffer = i & 1;
-      const v4i place = places[lane];
+      v4i place = places[lane];
+      if constexpr (SPLIT == 2) place += v4i{keys_from * S::kRow, keys_from * S::kBlocks, keys_from * 2 * D, 0};
       if constexpr (waves_per_simd<D>() > 1) {
         if (turn < late) __builtin_amdgcn_s_setprio(1);
         else __builtin_amdgcn_s_setprio(0);
@@ -536,7 +552,13 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
         request_keys(tile + 1, page, buffer ^ 1);
         entry = entry_of(tile + 2);
       }
-      if (active && tile * kTile < hi_max && tile * kTile + kTile > lo_min) {
+      if constexpr (SPLIT == 2) {
+        if (active && tile * kTile + keys_from < hi_max && tile * kTile + keys_from + 32 > lo_min) {
+          int nan = 0;
+          Keys keys;
+          half_tile(tile, buffer, Index<0>{}, i == 0, nan, place, keys);
+        }
+      } else if (active && tile * kTile < hi_max && tile * kTile + kTile > lo_min) {
         int nan = 0;
         Keys keys;
         half_tile(tile, buffer, Index<0>{}, i == 0, nan, place, keys);
@@ -548,9 +570,46 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       __syncthreads();
     }
 
+    if constexpr (SPLIT == 2) {   // waves 2 and 3 leave their sums in the values' place, waves 0 and 1 add them to their own
+      constexpr int kAtOnce = S::kValues * S::kValueBuffers / (2 * 64 * 64);   // blocks of 32 channels that fit there
+      const unsigned at = lds + kBuffers * S::kBuffer + wave % 2 * (kAtOnce * 4096) + lane * 16;
+      const float sum = cross_sum<false>(l);
+      float(&ml)[32][2] = other_ml[wave % 2];
+      if (wave >= 2 && lane < 32) ml[lane][0] = m, ml[lane][1] = sum;
+      float f0 = 0.0f, f1 = 0.0f;
+#pragma unroll
+      for (int first = 0; first < C; first += kAtOnce) {
+        if (wave >= 2) {
+#pragma unroll
+          for (int k = first; k < first + kAtOnce && k < C; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *lds_at<LdsFloat4>(at + (4 * (k - first) + i) * 1024) = v4f{acc[k][4 * i], acc[k][4 * i + 1], acc[k][4 * i + 2], acc[k][4 * i + 3]};
+        }
+        __syncthreads();
+        if (wave < 2) {
+          if (first == 0) {
+            const float m1 = ml[lane % 32][0], top = fmaxf(m, m1);
+            f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+            l = lane < 32 ? sum * f0 + ml[lane % 32][1] * f1 : 0.0f;   // (both halves of the wave are added up below)
+            m = top;
+          }
+#pragma unroll
+          for (int k = first; k < first + kAtOnce && k < C; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const v4f x = *lds_at<const LdsFloat4>(at + (4 * (k - first) + i) * 1024);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[k][4 * i + e] = acc[k][4 * i + e] * f0 + x[e] * f1;
+            }
+        }
+        __syncthreads();   // (the next ones, and the results, go by way of the same LDS)
+      }
+    }
+
     // ---- results: lane (column lane % 32) has channels 32 k + 8 i + 4 (lane / 32) .. + 3 of its row
     const bool done = from == 0 && to == it.units;
-    if (active) {
+    if (active && (SPLIT == 1 || wave < 2)) {
       const float sum = cross_sum<false>(l), m2 = m == kNoMax ? -INFINITY : m;
       const int here = lane_here(), row = row0 + here % 32, ch0 = here / 32 * 4;
       const bool real = row < rows;
@@ -599,38 +658,70 @@ int workgroups_of(const AttnArgs& p) {
   const int d = p.c.head_dim;
   return compute_units() * (d == 64 ? waves_per_simd<64>() : d == 128 ? waves_per_simd<128>() : waves_per_simd<256>());
 }
-template <int D, typename A>
+template <int D, int SPLIT, typename A>
 void launch(const A& p, int workgroups, hipStream_t s) {
   const dim3 grid((unsigned)workgroups), block(kWaves * 64);
   const int64_t last = p.c.pages - 1, page = (int64_t)p.c.kv_heads * p.c.page_size * D / 2;   // bytes of codes; of scales a 16th
   const auto small = [&](int64_t stride, int64_t bytes) { return last * stride + bytes <= (int64_t)1 << 32; };
   const bool all = small(p.c.k_page_stride, page) && small(p.c.v_page_stride, page) && small(p.c.k_scale_page_stride, page / 16) && small(p.c.v_scale_page_stride, page / 16);
-  if (units_bound(p, kRows, kTile) >> 32) hipLaunchKernelGGL((attn_prompt_kernel<D, false, Units, A>), grid, block, 0, s, p);   // (a call of seconds)
-  else if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true, unsigned, A>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((attn_prompt_kernel<D, false, unsigned, A>), grid, block, 0, s, p);
+  if (units_bound(p, kMostRows / SPLIT, kTile) >> 32) hipLaunchKernelGGL((attn_prompt_kernel<D, false, Units, A, SPLIT>), grid, block, 0, s, p);   // (a call of seconds)
+  else if (all) hipLaunchKernelGGL((attn_prompt_kernel<D, true, unsigned, A, SPLIT>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attn_prompt_kernel<D, false, unsigned, A, SPLIT>), grid, block, 0, s, p);
 }
 
 }  // namespace
 
-size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kRows, p.c.head_dim, workgroups_of(p)); }
+size_t attn_prompt_workspace(const AttnArgs& p) { return attn_workspace(kMostRows, p.c.head_dim, workgroups_of(p)); }
 
-template <typename A>
-hipError_t launch_attn_prompt(A p, void* ws, hipStream_t s) {
+namespace {
+int64_t rows_of(const AttnArgs& p) { return p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group; }
+// Rows of a block, for trees: 64 where there are no more, and where few blocks of few tiles leave waves without work.  us in blocks of 64 and of 128, 32
+// heads on 8 of 128: 16 sequences of 4096 keys, 16 nodes (64 rows) 40 and 42; 4 of 4096, 64 nodes (256 rows) 40 and 45, 16 of them 86 and 79; one of
+// 131072, 64 nodes 132 and 116; 64 heads on 8 of 64, 64 sequences of 1000, 16 nodes (128 rows) 37 and 47, 128 of 300 49 and 29.  (The bound on a sequence's keys is
+// what the page table or the window can hold.)
+int tree_block(const TreeArgs& p) {
+  const int64_t rows = rows_of(p), items = (int64_t)p.a.batch * p.c.kv_heads * ((rows + kMostRows - 1) / kMostRows), slots = workgroups_of(p);
+  const int64_t in_table = (int64_t)p.a.table_pages << p.page_shift, in_window = p.a.window > 0 ? (int64_t)p.a.window + p.a.max_q : in_table;
+  const int64_t tiles = (in_window < in_table ? in_window : in_table) / kTile + 1;
+  return rows <= kMostRows / 2 || (2 * items <= slots && items * tiles <= 8 * slots) ? kMostRows / 2 : kMostRows;
+}
+
+template <int D>
+hipError_t launch_of(AttnArgs p, void* ws, hipStream_t s) {
   const int workgroups = workgroups_of(p);
   p.whole = 0;
   // In parts: 2048 new tokens of 2 sequences of 16384 keys, 128 channels, with 1 950 us, 2 950, 3 947, 4 948; 300 prompts of 60 tokens, whose items have
   // but one tile, 100, 107, 118, 118; 64 channels 106, 113, 112, 115.  (It also counts in the choice of whole items, whose bound was measured with it.)
-  p.item_units = p.c.head_dim == 64 ? 2 : 3;
+  p.item_units = D == 64 ? 2 : 3;
   p.min_units_log2 = 2;
   p.few_long = p.a.batch <= 8;   // (one sequence, 4096 new tokens on 65536 keys: 3734 us so, 3771 otherwise; 8 with 40 on 2300: 54 and 49; 300 prompts of 60: 315 and 118)
-  place_workspace(p, kRows, workgroups, ws);
-  if (p.c.head_dim == 64) launch<64>(p, workgroups, s);
-  else if (p.c.head_dim == 128) launch<128>(p, workgroups, s);
-  else launch<256>(p, workgroups, s);
+  place_workspace(p, kMostRows, workgroups, ws);
+  launch<D, 1>(p, workgroups, s);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  return launch_attn_combine(p, kRows, p.a.cu_q ? (int64_t)p.a.max_q * p.group : p.group, workgroups, s);
+  return launch_attn_combine(p, kMostRows, rows_of(p), workgroups, s);
 }
+template <int D>
+hipError_t launch_of(TreeArgs p, void* ws, hipStream_t s) {
+  const int workgroups = workgroups_of(p), rows = tree_block(p);
+  p.whole = 0;
+  p.item_units = 3;
+  p.min_units_log2 = 2;
+  place_workspace(p, rows, workgroups, ws);
+  if (rows < kMostRows) launch<D, 2>(p, workgroups, s);
+  else launch<D, 1>(p, workgroups, s);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  return launch_attn_join(p, rows, rows_of(p), workgroups, s);
+}
+}  // namespace
 
+size_t attn_prompt_workspace(const TreeArgs& p) { return attn_workspace(tree_block(p), p.c.head_dim, workgroups_of(p)); }
+
+template <typename A>
+hipError_t launch_attn_prompt(A p, void* ws, hipStream_t s) {
+  if (p.c.head_dim == 64) return launch_of<64>(p, ws, s);
+  if (p.c.head_dim == 128) return launch_of<128>(p, ws, s);
+  return launch_of<256>(p, ws, s);
+}
 template hipError_t launch_attn_prompt(AttnArgs p, void* ws, hipStream_t s);
 template hipError_t launch_attn_prompt(TreeArgs p, void* ws, hipStream_t s);
 

@@ -108,6 +108,13 @@ AVE_BOTH inline U sequence_units(const A& p, const Sequence& s) {   // of one ke
   for (int row0 = 0; row0 < s.n * p.group; row0 += ROWS) u += (unsigned)block_units<ROWS, TILE>(p, s, row0, tile0);
   return u;
 }
+// All blocks of a tree's rows have the same units
+template <int ROWS, int TILE, typename U>
+AVE_BOTH inline U sequence_units(const TreeArgs& p, const Sequence& s) {
+  int tile0;
+  const unsigned rows = (unsigned)(s.n * p.group);
+  return (U)((rows + ROWS - 1) / ROWS) * (unsigned)block_units<ROWS, TILE>(p, s, 0, tile0);
+}
 // No call has more, whatever its lengths are, as long as its sequences do not share rows of q (if they do, results are anybody's, and no walk
 // leaves its bounds): blocks of rows, times the tiles that the page table or the window has for one
 inline Units units_bound(const AttnArgs& p, int rows_of_block, int tile) {
