@@ -508,6 +508,7 @@ hipError_t launch_attn_combine(const AttnArgs& p, int rows, int64_t rows_expecte
 hipError_t launch_attn_join(const TreeArgs& p, int rows, int64_t rows_expected, int workgroups, hipStream_t s);
 // meta, maxima and sums, partial results, in this order
 inline size_t attn_meta_bytes(int workgroups) { return ((size_t)workgroups * sizeof(PartMeta) + 255) / 256 * 256; }
+inline size_t attn_starts_bytes(int workgroups) { return ((size_t)workgroups * sizeof(PartStart) + 255) / 256 * 256; }
 inline size_t attn_workspace(int rows, int head_dim, int workgroups) {
   return attn_meta_bytes(workgroups) + (size_t)workgroups * 2 * rows * (2 + head_dim) * 4;
 }

@@ -639,32 +639,38 @@ namespace {
 constexpr int kMostItems = 1024;   // boundaries: workgroups of the first launch
 
 template <int D, int GROUPS>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs p, int ROWS, int workgroups) {
+__global__ __launch_bounds__(256) void attn_join_kernel(TreeArgs p, int ROWS, int workgroups) {
   constexpr int T = D / 4, R = 256 / T / GROUPS;
   __shared__ v4f sums[GROUPS][R][T];
   __shared__ float ml[GROUPS][R][2];
   __shared__ uint16_t items[kMostItems];
-  __shared__ int counts[kMostItems / 64];
+  __shared__ uint64_t counts[kMostItems / 64];   // which of 64 workgroups
+  __shared__ Units u0[kMostItems];
   const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
   bool first[kMostItems / 256];
-  uint64_t here[kMostItems / 256];
+  PartStart start[kMostItems / 256];
 #pragma unroll
   for (int k = 0; k < kMostItems / 256; ++k) {
-    const int g = 1 + k * 256 + threadIdx.x, at = g < workgroups ? g : 1;
-    const Units begin = p.meta[at].begin, u0 = p.meta[at].u0, before = p.meta[at - 1].u0;
-    first[k] = g < workgroups && begin < u0 && before <= begin;
+    const int g = k * 256 + threadIdx.x;
+    start[k] = p.starts[g < workgroups ? g : workgroups - 1];
   }
 #pragma unroll
+  for (int k = 0; k < kMostItems / 256; ++k) u0[k * 256 + threadIdx.x] = start[k].u0;
+  __syncthreads();
+#pragma unroll
   for (int k = 0; k < kMostItems / 256; ++k) {
-    here[k] = __ballot(first[k]);
-    if (lane == 0) counts[k * 4 + wave] = __popcll(here[k]);
+    const int g = k * 256 + threadIdx.x;
+    first[k] = g > 0 && g < workgroups && start[k].begin < start[k].u0 && u0[g > 0 ? g - 1 : 0] <= start[k].begin;
+    const uint64_t here = __ballot(first[k]);
+    if (lane == 0) counts[k * 4 + wave] = here;
   }
   __syncthreads();
   int many = 0;
 #pragma unroll
   for (int k = 0; k < kMostItems / 64; ++k) {
-    if (k % 4 == wave && first[k / 4]) items[many + __popcll(here[k / 4] & ((1ull << lane) - 1))] = (uint16_t)(1 + k / 4 * 256 + threadIdx.x);
-    many += counts[k];
+    const uint64_t here = counts[k];
+    if (k % 4 == wave && first[k / 4]) items[many + __popcll(here & ((1ull << lane) - 1))] = (uint16_t)(k * 64 + lane);
+    many += __popcll(here);
   }
   __syncthreads();
   const int blocks = (ROWS + R - 1) / R, group = threadIdx.x / T / R, mine = threadIdx.x / T % R, ch = threadIdx.x % T * 4;
@@ -676,7 +682,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs p, int ROWS, in
     // parts: of the workgroup that the item starts in, and of those from g on that start inside the item
     int parts = 1;
     for (int g0 = 0; g0 < most; g0 += 64) {
-      const int more = __popcll(__ballot(g0 + lane < most && m[g0 + lane < most ? g0 + lane : 0].u0 < end));
+      const int more = __popcll(__ballot(g0 + lane < most && u0[g0 + lane < most ? g + g0 + lane : g] < end));
       parts += more;
       if (more < 64) break;
     }

@@ -202,6 +202,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
   if (tid == 0 && (part.u0 >= part.u1 || (kTree<A> && by_items))) {   // no part, nothing to join
     PartMeta& m = p.meta[g];
     m.u0 = m.begin = m.end = part.units;
+    if constexpr (kTree<A>) p.starts[g] = {part.units, part.units};
   }
   // Among waves that could issue, the oldest goes first, so that of equal parts the workgroups that a compute unit got last would end
   // long after the others (452 us the first, 677 the last).  The later a workgroup came, the more of its tiles it takes at a higher priority.
@@ -216,7 +217,10 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
       if (!first_item) tree_next<kRows, kTile, U>(p, walk);
       b = walk.b;
       it.s = walk.s, it.head = walk.head, it.row0 = walk.row0, it.tile0 = walk.tile0, it.units = walk.units, it.begin = walk.begin;
-      if (!by_items && first_item && tid == 0) p.meta[g] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
+      if (!by_items && first_item && tid == 0) {
+        p.meta[g] = {part.u0, it.begin, it.begin + it.units, it.s.first, it.s.n * p.group, it.head, it.row0};
+        p.starts[g] = {part.u0, it.begin};
+      }
       if (!by_items && u - it.begin >= it.units) break;   // (lengths that change under the call: no walk without end, and the second launch finds its record)
       from = by_items ? 0 : (unsigned)(u - it.begin);
       to = by_items || part.u1 - it.begin >= it.units ? it.units : (unsigned)(part.u1 - it.begin);
@@ -706,7 +710,8 @@ hipError_t launch_of(TreeArgs p, void* ws, hipStream_t s) {
   p.whole = 0;
   p.item_units = 3;
   p.min_units_log2 = 2;
-  place_workspace(p, rows, workgroups, ws);
+  p.starts = static_cast<PartStart*>(ws);
+  place_workspace(p, rows, workgroups, static_cast<char*>(ws) + attn_starts_bytes(workgroups));
   if (rows < kMostRows) launch<D, 2>(p, workgroups, s);
   else launch<D, 1>(p, workgroups, s);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -714,7 +719,7 @@ hipError_t launch_of(TreeArgs p, void* ws, hipStream_t s) {
 }
 }  // namespace
 
-size_t attn_prompt_workspace(const TreeArgs& p) { return attn_workspace(tree_block(p), p.c.head_dim, workgroups_of(p)); }
+size_t attn_prompt_workspace(const TreeArgs& p) { return attn_starts_bytes(workgroups_of(p)) + attn_workspace(tree_block(p), p.c.head_dim, workgroups_of(p)); }
 
 template <typename A>
 hipError_t launch_attn_prompt(A p, void* ws, hipStream_t s) {

@@ -39,7 +39,9 @@ struct AttnArgs {
 };
 // The same for a tree of drafted tokens: the new tokens of a sequence see all keys before them, or the last p.a.window of what they see, and of each
 // other those that their row of bits says.
+struct PartStart;
 struct TreeArgs : AttnArgs {
+  PartStart* starts;      // workspace: [workgroups]
   const uint64_t* seen;   // bit j % 64 of word j / 64 of a token's row: new token j of its sequence
   int64_t seen_stride;    // words between rows
   int words;              // of a row
@@ -58,6 +60,11 @@ inline void set_group(AttnArgs& p, int group) {
 struct PartMeta {
   Units u0, begin, end;
   int first, rows, head, row0;
+};
+
+// Of a tree also by itself, for whoever looks through all of them
+struct PartStart {
+  Units u0, begin;
 };
 
 struct Sequence {
