@@ -204,10 +204,21 @@ __device__ inline unsigned tree_units(const TreeArgs& p, const Sequence& s, unsi
   tile0 = r.lo_min / TILE;
   return (unsigned)((r.hi_max > r.lo_min ? (r.hi_max + TILE - 1) / TILE - tile0 : 1) + p.item_units);
 }
-// Units [u0, u1) of workgroup g, and where they start.  `whole`: one item a workgroup (the walk of those without one has no units); the item number is
-// its unit.  Every wave by itself, 64 sequences at a time, a lane each.
-template <int ROWS, int TILE, typename U>
-__device__ inline TreeWalk<U> tree_part(const TreeArgs& p, unsigned g, unsigned workgroups, unsigned slack, bool& whole, U& u0, U& u1, U& all) {
+// How many workgroups a compute unit take part, for so many units (of 64 rows) a compute unit: a few work on small calls faster than many (the ones that start
+// together hinder each other, and every part is written, read and joined).  us with one, two and three: 128 channels, one sequence of 8000 keys, 16 nodes (4
+// units) 23, 27, 31, 64 nodes (16) 33, 33, 35; 16 of 4096, 16 nodes (27) 47, 41, 41; one of 131072, 8 nodes (64) 66, 47, 44; 64 channels, 8000 keys, 16 nodes
+// (8) 20, 21, 25, 4 of 4096, 25 nodes (27) 34, 29, 30, 64 nodes (55) 59, 44, 42; 256 channels, 16 of 4096, 64 nodes (22) 69, 75, 64 of 4096, 25 nodes
+// (44) 108, 91.
+template <int D>
+__device__ inline unsigned tree_workgroups(unsigned units) {
+  if (D == 64) return units <= 8 ? 1 : units <= 32 ? 2 : units <= 64 ? 3 : 4;
+  if (D == 128) return units <= 12 ? 1 : units <= 28 ? 2 : 3;
+  return units <= 24 ? 1 : 2;
+}
+// The number g of workgroup `block` of `most_of_cu` a compute unit, its units [u0, u1), and where they start.  `whole`: one item a workgroup (the walk of those without
+// one has no units); the item number is its unit.  Every wave by itself, 64 sequences at a time, a lane each.
+template <int D, int ROWS, int TILE, typename U>
+__device__ inline TreeWalk<U> tree_part(const TreeArgs& p, unsigned block_index, unsigned grid, unsigned most_of_cu, unsigned& g, bool& whole, U& u0, U& u1, U& all) {
   const int lane = threadIdx.x & 63;
   const unsigned heads = (unsigned)p.c.kv_heads;
   Sequence s{0, 0, 0};
@@ -231,12 +242,23 @@ __device__ inline TreeWalk<U> tree_part(const TreeArgs& p, unsigned g, unsigned 
     most = units > most ? units : most;
   }
   if (p.a.batch > 64) load(0);
+  // Whole items where there is one a workgroup at most, and the longest is not much longer than equal parts would be: parts cost a start each and their
+  // joining, about eight tiles
+  const unsigned cus = grid / most_of_cu;
+  const auto bounded = [](U x) { return x < (1u << 29) ? (unsigned)x : 1u << 29; };
+  unsigned workgroups = tree_workgroups<D>(bounded(all / cus) * (ROWS / 64));
+  workgroups = (workgroups < most_of_cu ? workgroups : most_of_cu) * cus;
+  whole = items <= grid;
+  if (whole) {
+    const unsigned even = ((unsigned)items + cus - 1) / cus * cus, of = even ? even : cus;
+    whole = !__any(most > bounded(all / of) + 8);
+    workgroups = whole ? of : workgroups;
+  }
+  // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
+  g = block_index < workgroups && workgroups % 8 == 0 ? block_index % 8 * (workgroups / 8) + block_index / 8 : block_index;
   Part<U> part{};
   part.units = all;
   cut(p, part, g, workgroups);
-  // Whole items where there is one a workgroup at most, and the longest is not much longer than equal parts would be
-  const unsigned equal = (unsigned)(all / workgroups);
-  whole = items <= workgroups && !__any(most > equal + slack);
   u0 = whole ? (U)g : part.u0, u1 = whole ? (U)g + 1 : part.u1;
   TreeWalk<U> w{};
   if (whole ? (U)g >= items : part.u0 >= part.u1) {

@@ -173,10 +173,10 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<D>())) void attn_promp
     }
   }
   // workgroups of an XCD (every eighth) take neighbouring parts, which read the same keys
-  const unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+  unsigned g = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
   Part<U> part{};
   TreeWalk<U> walk{};
-  if constexpr (kTree<A>) walk = tree_part<kRows, kTile, U>(p, g, gridDim.x, 8, by_items, part.u0, part.u1, part.units);
+  if constexpr (kTree<A>) walk = tree_part<D, kRows, kTile, U>(p, blockIdx.x, gridDim.x, waves_per_simd<D>(), g, by_items, part.u0, part.u1, part.units);
   else if (!by_items) part = take_part<kRows, kTile, U, true>(p, g, gridDim.x);
   const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_address(smem));
   const float c = uniform(softmax_scale(p.a.scale));
