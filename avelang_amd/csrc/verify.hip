@@ -23,8 +23,8 @@ namespace ave {
 namespace {
 
 constexpr int kPiece = kVocabPiece;
-constexpr int kThreads = 256, kRowThreads = 1024;
-constexpr int kEach = kPiece / kThreads, kOnce = 8;   // elements of a thread, together in memory
+constexpr int kThreads = 256, kOnce = 8;          // elements of a thread that are together in memory
+constexpr int kShort = kThreads * kOnce;           // elements that a workgroup draws from
 
 struct PieceSum {
   double sum;   // of exp((x - top) / temperature)
@@ -50,16 +50,16 @@ struct Wanted {
 
 struct VerifyArgs {
   ave_fp4_draft d;
-  int pieces;
+  int pieces, shorts;   // of kPiece and of kShort elements
   PieceSum* sums;   // [rows][pieces]
-  double* left;     // [batch][pieces]: of what is drawn from
+  double* left;     // [batch][shorts]: sums of what is drawn from
   Draw* draws;      // [batch]
   double* rest;     // [rows][pieces]: sums of max(p - q, 0)
   double* times;    // [rows]: t when all children are rejected
   int* choice;      // [rows]: the accepted child, -1: none; kMany: there are several and nobody has looked
   Wanted* wanted;   // [rows]: the rows that descend from the accepted children of nodes 0, in any order, and
   int* many;        // how many
-  int* done;        // [batch]: pieces of the last row that are summed up
+  int* done;        // [batch]: pieces of the last row that are summed up; with distributions also [rows] behind that: pieces of `rest`
 };
 
 struct Span {
@@ -228,12 +228,14 @@ constexpr double kSumError = 1.0 / 32768.0;
 
 // EXACT: in fp64.  ROWS: 0 all, 1 the first of each sequence, 2 those that are wanted (by a workgroup one after the other)
 template <bool F32, bool EXACT, int ROWS>
-__global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
-  __shared__ double scratch[kThreads / 64];
-  __shared__ float tops[kThreads / 64];
+__global__ __launch_bounds__((EXACT ? 2 : 1) * kThreads) void row_sums_kernel(VerifyArgs p) {
+  constexpr int THREADS = (EXACT ? 2 : 1) * kThreads, kEach = kPiece / THREADS;
+  __shared__ double scratch[THREADS / 64];
+  __shared__ float tops[THREADS / 64];
   __shared__ int lowest;
   if constexpr (ROWS < 2) {   // for the launches behind this one
-    for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < (unsigned)p.d.batch; i += gridDim.x * kThreads) p.done[i] = 0;
+    const unsigned counts = (unsigned)p.d.batch + (EXACT ? (unsigned)p.d.rows : 0u);
+    for (unsigned i = blockIdx.x * THREADS + threadIdx.x; i < counts; i += gridDim.x * THREADS) p.done[i] = 0;
     if (ROWS == 1 && blockIdx.x == 0 && threadIdx.x == 0) *p.many = 0;
   }
   const unsigned all = ROWS == 2 ? (unsigned)min(*p.many, p.d.rows) * (unsigned)p.pieces : blockIdx.x + 1;
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
   const auto fetch = [&](unsigned item) {
     now = p.wanted[item / (unsigned)p.pieces];
 #pragma unroll
-    for (int k = 0; k < kEach / kOnce; ++k) next[k] = load8<F32>(p, now.row, (int)(item % (unsigned)p.pieces) * kPiece + (k * kThreads + threadIdx.x) * kOnce);
+    for (int k = 0; k < kEach / kOnce; ++k) next[k] = load8<F32>(p, now.row, (int)(item % (unsigned)p.pieces) * kPiece + (k * THREADS + threadIdx.x) * kOnce);
   };
   if (ROWS == 2 && blockIdx.x < all) fetch(blockIdx.x);
   for (unsigned item = blockIdx.x; item < all; item += gridDim.x) {
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
       if (item + gridDim.x < all) fetch(item + gridDim.x);
     } else {
 #pragma unroll
-      for (int k = 0; k < kEach / kOnce; ++k) logits<F32>(p, row, piece * kPiece + (k * kThreads + threadIdx.x) * kOnce, x[k]);
+      for (int k = 0; k < kEach / kOnce; ++k) logits<F32>(p, row, piece * kPiece + (k * THREADS + threadIdx.x) * kOnce, x[k]);
       if constexpr (ROWS == 0) b = sequence_of(p, row);
       if (b < 0) return;
       per = inverse_temperature(p, b);
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
       if ((threadIdx.x & 63) == 0) tops[threadIdx.x / 64] = top;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, tops[w]);
+      for (int w = 0; w < THREADS / 64; ++w) top = fmaxf(top, tops[w]);
       sum = 0.0;
       if (per > 0.0 && top != -INFINITY) {
         if constexpr (EXACT) {
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
           sum = (double)s;
         }
       }
-      sum = block_sum<kThreads>(sum, scratch);
+      sum = block_sum<THREADS>(sum, scratch);
       return mine;
     };
     float mine = reduce();
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void row_sums_kernel(VerifyArgs p) {
       int at = INT32_MAX;
 #pragma unroll
       for (int k = kEach - 1; k >= 0; --k)
-        if (x[k / kOnce][k % kOnce] == top) at = piece * kPiece + (k / kOnce * kThreads + threadIdx.x) * kOnce + k % kOnce;
+        if (x[k / kOnce][k % kOnce] == top) at = piece * kPiece + (k / kOnce * THREADS + threadIdx.x) * kOnce + k % kOnce;
       atomicMin(&lowest, at);
     }
     __syncthreads();
@@ -553,36 +555,46 @@ __device__ inline double wave_running(double v) {
   }
   return v;
 }
-// The next token, by a workgroup, whose threads share the piece in which it lies
-template <bool F32, int THREADS>
+// The next token, by a workgroup, whose threads share the kShort elements among which it lies
+template <bool F32>
 __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw& of, double per, int b) {
-  constexpr int kMine = kPiece / THREADS;
-  __shared__ double wave_at[THREADS / 64];
-  __shared__ int firsts[THREADS / 64], lasts[THREADS / 64];
+  __shared__ double wave_at[kThreads / 64];
+  __shared__ int firsts[kThreads / 64], lasts[kThreads / 64];
   __shared__ Draw all_of_it;
   const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
   bool nothing_left = false;
-  const auto piece_sum = [&](int c) -> double {
-    if (c >= p.pieces) return 0.0;
-    if (!nothing_left) return p.left[(size_t)b * p.pieces + c];
-    const PieceSum q = p.sums[(size_t)of.row * p.pieces + c];   // all of the row
-    return q.top == -INFINITY ? 0.0 : q.sum * weight_of(q.top, (double)of.top, per);
-  };
+  const auto piece_sum = [&](int c) -> double { return c < p.shorts ? p.left[(size_t)b * p.shorts + c] : 0.0; };
   // every wave: pieces a lane, 64 at a time
   const auto sum_of_all = [&] {
     double sum = 0.0;
-    for (int c0 = 0; c0 < p.pieces; c0 += 64) sum += lane_double(wave_running(piece_sum(c0 + lane)), 63);
+    for (int c0 = 0; c0 < p.shorts; c0 += 64) sum += lane_double(wave_running(piece_sum(c0 + lane)), 63);
     return sum;
   };
   double all = sum_of_all();
-  if (!(all > 0.0)) {
+  if (!(all > 0.0)) {   // nothing is left: all of the row, summed up here
     nothing_left = true;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      all_of_it = of;
+      all_of_it.how = kAll;
+    }
+    __syncthreads();
+    for (int c = 0; c < p.shorts; ++c) {
+      double w[kOnce], sum = 0.0;
+      weights_of<F32>(p, s, all_of_it, per, c * kShort + (int)threadIdx.x * kOnce, w);
+#pragma unroll
+      for (int j = 0; j < kOnce; ++j) sum += w[j];
+      sum = block_sum<kThreads>(sum, wave_at);
+      if (threadIdx.x == 0) p.left[(size_t)b * p.shorts + c] = sum;
+    }
+    __threadfence();
+    __syncthreads();
     all = sum_of_all();
   }
   const double want = random_of(p, s.first) * all;
   int piece = 0;
   double before = 0.0, sum = 0.0;   // before: the sum of the pieces in front
-  for (int c0 = 0; c0 < p.pieces; c0 += 64) {
+  for (int c0 = 0; c0 < p.shorts; c0 += 64) {
     const double mine = piece_sum(c0 + lane), upto = wave_running(mine);
     const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && sum + upto > want);
     if (some) {   // (the last one with anything, if rounding leaves `want` at the sum of all)
@@ -592,16 +604,11 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
     if (over) break;
     sum += lane_double(upto, 63);
   }
-  if (threadIdx.x == 0) {
-    all_of_it = of;
-    if (nothing_left) all_of_it.how = kAll;
-  }
-  __syncthreads();
-  const Draw& d = all_of_it;
-  double w[kMine], mine = 0.0;
-  weights_of<F32>(p, s, d, per, piece * kPiece + (int)threadIdx.x * kMine, w);
+  const Draw& d = nothing_left ? all_of_it : of;
+  double w[kOnce], mine = 0.0;
+  weights_of<F32>(p, s, d, per, piece * kShort + (int)threadIdx.x * kOnce, w);
 #pragma unroll
-  for (int j = 0; j < kMine; ++j) mine += w[j];
+  for (int j = 0; j < kOnce; ++j) mine += w[j];
   const double upto = wave_running(mine);
   if (lane == 63) wave_at[wave] = upto;
   __syncthreads();
@@ -611,10 +618,10 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
   // the first element whose running sum is above `want`; if rounding leaves none, the last one that has a weight
   int first = -1, last = -1;
 #pragma unroll
-  for (int j = 0; j < kMine; ++j) {
+  for (int j = 0; j < kOnce; ++j) {
     run += w[j];
     if (w[j] > 0.0) {
-      last = piece * kPiece + (int)threadIdx.x * kMine + j;
+      last = piece * kShort + (int)threadIdx.x * kOnce + j;
       if (run > want && first < 0) first = last;
     }
   }
@@ -624,77 +631,106 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
   __syncthreads();
   if (threadIdx.x == 0) {
     int token = -1;
-    for (int k = 0; k < THREADS / 64 && token < 0; ++k) token = firsts[k];
-    for (int k = THREADS / 64 - 1; k >= 0 && token < 0; --k) token = lasts[k];
+    for (int k = 0; k < kThreads / 64 && token < 0; ++k) token = firsts[k];
+    for (int k = kThreads / 64 - 1; k >= 0 && token < 0; --k) token = lasts[k];
     p.d.emitted[d.out] = token;
   }
 }
 
-// ONE_LAUNCH: the last workgroup of a sequence draws
-template <bool F32, bool ONE_LAUNCH>
-__global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs p) {
-  constexpr int THREADS = kThreads;
-  __shared__ double scratch[THREADS / 64];
-  __shared__ Draw draw;
-  __shared__ int before_me;
-  const int piece = blockIdx.x % (unsigned)p.pieces, b = blockIdx.x / (unsigned)p.pieces, lane = threadIdx.x & 63;
-  const Span s = span_of(p, b);
-  const double per = inverse_temperature(p, b);
-  if (s.n == 0) {
-    if (piece == 0 && threadIdx.x == 0) {
-      p.d.accepted[b] = 0;
-      if constexpr (!ONE_LAUNCH) p.draws[b].how = kNothing;
-    }
-    return;
+// A sequence's way, by one wave, and what its token is drawn from; write: also path, accepted, emitted
+template <bool F32>
+__device__ inline void find_way(const VerifyArgs& p, const Span& s, double per, int b, bool write, Draw& draw) {
+  const int lane = threadIdx.x & 63;
+  const Way w = walk<F32, false>(p, s, per, write, &draw);
+  RowSum r = row_top(p, s.first + w.at);
+  if (w.times > 0.0) r.sum = row_sum<true>(p, s.first + w.at, per).sum;
+  const bool none = per == 0.0 || r.top == -INFINITY;
+  const int out = s.first + w.kept - 1;
+  if (lane == 0) {
+    draw.times = w.times, draw.sum = r.sum, draw.top = r.top, draw.row = s.first + w.at, draw.out = out;
+    draw.how = none ? kNothing : w.times > 0.0 ? kRest : w.tried > 0 && !p.d.draft_probs ? kWithout : kAll;
   }
-  if (threadIdx.x < 64) {
-    const Way w = walk<F32, false>(p, s, per, piece == 0, &draw);
-    RowSum r = row_top(p, s.first + w.at);
-    if (w.times > 0.0) r.sum = row_sum<true>(p, s.first + w.at, per).sum;
-    const bool none = per == 0.0 || r.top == -INFINITY;
-    const int out = s.first + w.kept - 1;
+  if (write) {
+    for (int i = w.kept + lane; i < s.n; i += 64) p.d.path[s.first + i] = -1, p.d.emitted[s.first + i] = -1;
     if (lane == 0) {
-      draw.times = w.times, draw.sum = r.sum, draw.top = r.top, draw.row = s.first + w.at, draw.out = out;
-      draw.how = none ? kNothing : w.times > 0.0 ? kRest : w.tried > 0 && !p.d.draft_probs ? kWithout : kAll;
-    }
-    if (piece == 0) {
-      for (int i = w.kept + lane; i < s.n; i += 64) p.d.path[s.first + i] = -1, p.d.emitted[s.first + i] = -1;
-      if (lane == 0) {
-        p.d.accepted[b] = w.kept;
-        if (none) p.d.emitted[out] = r.top == -INFINITY ? -1 : r.at;
-        if constexpr (!ONE_LAUNCH) p.draws[b] = draw;
-      }
+      p.d.accepted[b] = w.kept;
+      if (none) p.d.emitted[out] = r.top == -INFINITY ? -1 : r.at;
     }
   }
-  __syncthreads();
-  const Draw& d = draw;
-  if (d.how == kNothing) return;
-  double sum = 0.0;
+}
+// Sums of SHORTS pieces of kShort elements from `first` on, by a workgroup
+template <bool F32, int SHORTS>
+__device__ inline void sum_shorts(const VerifyArgs& p, const Span& s, const Draw& d, double per, int b, int first) {
+  __shared__ double scratch[kThreads / 64][SHORTS];
 #pragma unroll
-  for (int k = 0; k < kPiece / THREADS / kOnce; ++k) {
-    double w[kOnce];
-    weights_of<F32>(p, s, d, per, piece * kPiece + (k * THREADS + threadIdx.x) * kOnce, w);
+  for (int k = 0; k < SHORTS; ++k) {
+    double w[kOnce], sum = 0.0;
+    weights_of<F32>(p, s, d, per, (first + k) * kShort + (int)threadIdx.x * kOnce, w);
 #pragma unroll
     for (int j = 0; j < kOnce; ++j) sum += w[j];
+    sum = wave_sum(sum);
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x / 64][k] = sum;
   }
-  sum = block_sum<THREADS>(sum, scratch);
-  if (threadIdx.x == 0) p.left[(size_t)b * p.pieces + piece] = sum;
-  if constexpr (ONE_LAUNCH) {
-    if (threadIdx.x == 0) {
-      __threadfence();   // the sum, before the count says that it is there
-      before_me = atomicAdd(p.done + b, 1);
-    }
-    __syncthreads();
-    if (before_me != p.pieces - 1) return;
-    __threadfence();   // the others' sums
-    draw_token<F32, THREADS>(p, s, d, per, b);
+  __syncthreads();
+  if (threadIdx.x < SHORTS) {
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) all += scratch[w][threadIdx.x];
+    const int c = first + (int)threadIdx.x;
+    if (c < p.shorts) p.left[(size_t)b * p.shorts + c] = all;
   }
 }
 
+// Few pieces: every workgroup finds the way by itself and sums up one piece, and the last one of a sequence draws
 template <bool F32>
-__global__ __launch_bounds__(kRowThreads) void draw_kernel(VerifyArgs p) {
+__global__ __launch_bounds__(kThreads) void walk_and_draw_kernel(VerifyArgs p) {
+  __shared__ Draw draw;
+  __shared__ int before_me;
+  const int piece = blockIdx.x % (unsigned)p.shorts, b = blockIdx.x / (unsigned)p.shorts;
+  const Span s = span_of(p, b);
+  const double per = inverse_temperature(p, b);
+  if (s.n == 0) {
+    if (piece == 0 && threadIdx.x == 0) p.d.accepted[b] = 0;
+    return;
+  }
+  if (threadIdx.x < 64) find_way<F32>(p, s, per, b, piece == 0, draw);
+  __syncthreads();
+  if (draw.how == kNothing) return;
+  sum_shorts<F32, 1>(p, s, draw, per, b, piece);
+  if (threadIdx.x == 0) {
+    __threadfence();   // the sum, before the count says that it is there
+    before_me = atomicAdd(p.done + b, 1);
+  }
+  __syncthreads();
+  if (before_me != p.shorts - 1) return;
+  __threadfence();   // the others' sums
+  draw_token<F32>(p, s, draw, per, b);
+}
+
+// Many: a launch each
+template <bool F32>
+__global__ __launch_bounds__(64) void walk_kernel(VerifyArgs p) {
+  __shared__ Draw draw;
   const int b = blockIdx.x;
-  if (p.draws[b].how != kNothing) draw_token<F32, kRowThreads>(p, span_of(p, b), p.draws[b], inverse_temperature(p, b), b);
+  const Span s = span_of(p, b);
+  if (s.n > 0) find_way<F32>(p, s, inverse_temperature(p, b), b, true, draw);
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  if (s.n == 0) p.d.accepted[b] = 0, p.draws[b].how = kNothing;
+  else p.draws[b] = draw;
+}
+constexpr int kShorts = kPiece / kShort;
+template <bool F32>
+__global__ __launch_bounds__(kThreads) void left_sums_kernel(VerifyArgs p) {
+  const unsigned of_sequence = (unsigned)(p.shorts + kShorts - 1) / kShorts;
+  const int piece = blockIdx.x % of_sequence, b = blockIdx.x / of_sequence;
+  const Draw& d = p.draws[b];
+  if (d.how != kNothing) sum_shorts<F32, kShorts>(p, span_of(p, b), d, inverse_temperature(p, b), b, piece * kShorts);
+}
+template <bool F32>
+__global__ __launch_bounds__(kThreads) void draw_kernel(VerifyArgs p) {
+  const int b = blockIdx.x;
+  if (p.draws[b].how != kNothing) draw_token<F32>(p, span_of(p, b), p.draws[b], inverse_temperature(p, b), b);
 }
 
 // ---- children one after the other, where drafts come with distributions ----------------------------------------------------------------------------
@@ -717,32 +753,13 @@ __device__ inline double rest_of(const VerifyArgs& p, const Span& s, const RowSu
   return sum;
 }
 
+// Rows of two children and more whose first one is rejected: the sum of max(p - q, 0), a piece a workgroup; the last one goes on with the other children.
 template <bool F32>
-__global__ __launch_bounds__(kThreads) void rest_sums_kernel(VerifyArgs p) {
+__global__ __launch_bounds__(kThreads) void children_kernel(VerifyArgs p) {
+  constexpr int kParts = kPiece / kShort;
   __shared__ double scratch[kThreads / 64];
+  __shared__ int before_me;
   const int row = blockIdx.x / (unsigned)p.pieces, piece = blockIdx.x % (unsigned)p.pieces;
-  if (p.choice[row] != kMany) return;
-  const int b = sequence_of(p, row);
-  if (b < 0) return;
-  const double per = inverse_temperature(p, b);
-  const Span s = span_of(p, b);
-  const int v = row - s.first, child = next_child(p, s, v, v + 1);
-  if (child >= s.n) return;
-  const RowSum r = row_sum<true>(p, row, per);
-  if (!(r.sum > 0.0) || accepts<F32>(p, row, r, per, s.first + child, 0.0, 1.0)) return;
-  double sum = 0.0;
-#pragma unroll
-  for (int k = 0; k < kEach / kOnce; ++k) sum += rest_of<F32, kOnce>(p, s, r, per, 1.0, row, piece * kPiece + (k * kThreads + threadIdx.x) * kOnce);
-  sum = block_sum<kThreads>(sum, scratch);
-  if (threadIdx.x == 0) p.rest[(size_t)row * p.pieces + piece] = sum;
-}
-
-// Rows of two children and more whose first one is rejected: the others
-template <bool F32>
-__global__ __launch_bounds__(kRowThreads) void children_kernel(VerifyArgs p) {
-  constexpr int kMine = kPiece / kRowThreads;
-  __shared__ double scratch[kRowThreads / 64];
-  const int row = blockIdx.x;
   if (p.choice[row] != kMany) return;
   const int b = sequence_of(p, row);
   if (b < 0) return;
@@ -751,33 +768,46 @@ __global__ __launch_bounds__(kRowThreads) void children_kernel(VerifyArgs p) {
   const int v = row - s.first;
   int child = next_child(p, s, v, v + 1);
   if (child >= s.n) return;
-  const int second = next_child(p, s, v, child + 1);
-  if (second >= s.n) return;
   const RowSum r = row_sum<true>(p, row, per);
   if (accepts<F32>(p, row, r, per, s.first + child, 0.0, 1.0)) return;
+  const auto sum_of = [&](int c, double t) {   // of piece c
+    double sum = 0.0;
+    if (r.sum > 0.0) {
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) sum += rest_of<F32, kOnce>(p, s, r, per, t, row, c * kPiece + (k * kThreads + (int)threadIdx.x) * kOnce);
+    }
+    return block_sum<kThreads>(sum, scratch);
+  };
+  const double first = sum_of(piece, 1.0);
+  if (threadIdx.x == 0) {
+    p.rest[(size_t)row * p.pieces + piece] = first;
+    __threadfence();   // the sum, before the count says that it is there
+    before_me = atomicAdd(p.done + p.d.batch + row, 1);
+  }
+  __syncthreads();
+  if (before_me != p.pieces - 1) return;
+  __threadfence();   // the others' sums
   double t = 1.0, left = 0.0;
-  if (r.sum > 0.0)
-    for (int c = 0; c < p.pieces; ++c) left += p.rest[(size_t)row * p.pieces + c];
+  for (int c = 0; c < p.pieces; ++c) left += p.rest[(size_t)row * p.pieces + c];
   int found = -1;
-  for (child = second; child < s.n;) {
+  for (child = next_child(p, s, v, child + 1); child < s.n;) {
     if (accepts<F32>(p, row, r, per, s.first + child, t, left)) {
       found = child;
       break;
     }
     t += left;
     child = next_child(p, s, v, child + 1);
-    if (child >= s.n || !(r.sum > 0.0)) continue;
+    if (child >= s.n) break;
     left = 0.0;
-    for (int c = 0; c < p.pieces; ++c) left += block_sum<kRowThreads>(rest_of<F32, kMine>(p, s, r, per, t, row, c * kPiece + threadIdx.x * kMine), scratch);
+    for (int c = 0; c < p.pieces; ++c) left += sum_of(c, t);
   }
-  __syncthreads();   // (all have read it)
   if (threadIdx.x == 0) p.choice[row] = found, p.times[row] = t;
 }
 
 VerifyArgs args_of(const ave_fp4_draft& d, void* ws, size_t* bytes) {
   VerifyArgs p{};
   p.d = d;
-  p.pieces = (d.vocab + kPiece - 1) / kPiece;
+  p.pieces = (d.vocab + kPiece - 1) / kPiece, p.shorts = (d.vocab + kShort - 1) / kShort;
   char* at = static_cast<char*>(ws);
   size_t used = 0;
   const auto take = [&](size_t n) {
@@ -787,7 +817,7 @@ VerifyArgs args_of(const ave_fp4_draft& d, void* ws, size_t* bytes) {
   };
   const size_t all = (size_t)d.rows * p.pieces;
   p.sums = reinterpret_cast<PieceSum*>(take(all * sizeof(PieceSum)));
-  p.left = reinterpret_cast<double*>(take((size_t)d.batch * p.pieces * sizeof(double)));
+  p.left = reinterpret_cast<double*>(take((size_t)d.batch * p.shorts * sizeof(double)));
   p.draws = reinterpret_cast<Draw*>(take((size_t)d.batch * sizeof(Draw)));
   if (d.draft_probs) {
     p.rest = reinterpret_cast<double*>(take(all * sizeof(double)));
@@ -797,7 +827,7 @@ VerifyArgs args_of(const ave_fp4_draft& d, void* ws, size_t* bytes) {
     p.wanted = reinterpret_cast<Wanted*>(take((size_t)d.rows * sizeof(Wanted)));
     p.many = reinterpret_cast<int*>(take(sizeof(int)));
   }
-  p.done = reinterpret_cast<int*>(take((size_t)d.batch * sizeof(int)));
+  p.done = reinterpret_cast<int*>(take(((size_t)d.batch + (d.draft_probs ? d.rows : 0)) * sizeof(int)));
   if (bytes) *bytes = used;
   return p;
 }
@@ -812,9 +842,8 @@ hipError_t launch(const VerifyArgs& p, hipStream_t s) {
   const unsigned rows = (unsigned)p.d.rows, batch = (unsigned)p.d.batch, pieces = (unsigned)p.pieces;
   if (p.d.draft_probs) {
     if (rows > 0) {
-      hipLaunchKernelGGL((row_sums_kernel<F32, true, 0>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
-      hipLaunchKernelGGL((rest_sums_kernel<F32>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
-      hipLaunchKernelGGL((children_kernel<F32>), dim3(rows), dim3(kRowThreads), 0, s, p);
+      hipLaunchKernelGGL((row_sums_kernel<F32, true, 0>), dim3(rows * pieces), dim3(2 * kThreads), 0, s, p);
+      hipLaunchKernelGGL((children_kernel<F32>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
     }
   } else if (in_two_steps(p)) {
     hipLaunchKernelGGL((row_sums_kernel<F32, false, 1>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
@@ -823,11 +852,12 @@ hipError_t launch(const VerifyArgs& p, hipStream_t s) {
   } else if (rows > 0) {
     hipLaunchKernelGGL((row_sums_kernel<F32, false, 0>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
   }
-  if (batch * pieces <= (unsigned)compute_units()) {
-    hipLaunchKernelGGL((walk_kernel<F32, true>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
+  if (batch * (unsigned)p.shorts <= 2u * (unsigned)compute_units()) {
+    hipLaunchKernelGGL((walk_and_draw_kernel<F32>), dim3(batch * (unsigned)p.shorts), dim3(kThreads), 0, s, p);
   } else {
-    hipLaunchKernelGGL((walk_kernel<F32, false>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
-    hipLaunchKernelGGL((draw_kernel<F32>), dim3(batch), dim3(kRowThreads), 0, s, p);
+    hipLaunchKernelGGL((walk_kernel<F32>), dim3(batch), dim3(64), 0, s, p);
+    hipLaunchKernelGGL((left_sums_kernel<F32>), dim3(batch * pieces), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((draw_kernel<F32>), dim3(batch), dim3(kThreads), 0, s, p);
   }
   return hipGetLastError();
 }
