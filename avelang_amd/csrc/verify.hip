@@ -2,17 +2,25 @@
 //
 //   row sums   a workgroup for a piece of a row: largest logit, its lowest index, sum of exp((x - largest) / temperature)
 //   children   (drafts with distributions only) rows whose first child is rejected and that have more: sums of max(p - t q, 0), child after child
-//   walk       every workgroup of a piece goes the way from node to node by itself -- whether a node is accepted, once its parent is and its elder
-//              siblings are not, does not depend on the rest of the way, so all nodes' probabilities are fetched at once -- and then sums up, in
-//              fp64, what its piece of the last node's row leaves to draw from; the last one of a sequence draws: the piece in which the random
-//              number lies, then the element
+//   way        a wave goes from node to node: whether a node is accepted, once its parent is and its elder siblings are not, does not depend on the rest
+//              of the way, so the probabilities of 64 nodes are fetched at once, a lane each
+//   left sums  what pieces of the last node's row leave to draw from, in fp64
+//   draw       the piece in which the random number lies, then the element
 //
-// Bound by HBM where there is much to read, by the latency of the launches where there is not.  With much to read the children of node 0 are decided on first,
+// With little to read the last three are one launch, whose workgroups find the way each by itself.  With much, the children of node 0 are decided on first,
 // from its row alone, and then only rows that descend from the accepted one are read.
 //
+// Bound by HBM where there is much to read: 64 trees of 16 nodes, 131072 tokens in bf16, 64 us of which 23 are the wanted 377 of 1024 rows at 4.2 TB/s
+// (all rows at 4.9 TB/s would be 55); else by the way from one launch to the next and by chains of loads: six nodes of 32768 tokens 9 us; eight chains of six
+// with distributions, 50001 tokens, 25.  Beside that, fp64: the sums over 64 rows of 131072 take 16 us, about 25 instructions an element.
+//
+// Rejections with distributions: r_0 = p, r_(k+1) = max(r_k - q, 0) / sum is max(p - t_k q, 0) / s_k with t_0 = 0, s_0 = 1, t_(k+1) = t_k + s_k and
+// s_k = sum max(p - t_k q, 0), so that a row needs its logits, q and two numbers.
+//
 // Precision.  A token is drawn by where a number lies among the running sums of 10^5 probabilities; in fp32 one draw in some hundred to
-// thousand would go to a neighbour by rounding, so what is drawn from is summed in fp64.  A node's acceptance is one comparison: the row sums behind it are
-// formed in fp32 (kSumError), and where the comparison comes out nearer than that, the row is summed again in fp64.
+// thousand would go to a neighbour by rounding, so what is drawn from is summed in fp64, and with distributions the row sums are, too.  Without, a node's
+// acceptance is one comparison: the row sums behind it are formed in fp32 (kSumError), and where the comparison comes out nearer than that, the row
+// is summed again in fp64.
 #include <algorithm>
 
 #include "fp4_common.hpp"
@@ -832,7 +840,9 @@ VerifyArgs args_of(const ave_fp4_draft& d, void* ws, size_t* bytes) {
   return p;
 }
 
-// Node 0's rows first and then those that are wanted, instead of all at once: two launches more, against what need not be read.
+// Node 0's rows first and then those that are wanted, instead of all at once: two launches more, against what need not be read.  us so and at once, trees of
+// 16 nodes, 131072 tokens: 8 sequences (32 MB) 37 and 31, 16 40 and 40, 32 48 and 54, 64 65 and 80; 16 sequences of 64 nodes 60 and 74; chains of six, 64
+// sequences 51 and 50.
 bool in_two_steps(const VerifyArgs& p) {
   return (int64_t)p.d.rows * p.d.vocab * (p.d.logits_f32 ? 4 : 2) > (int64_t)64 << 20 && p.d.rows >= 3 * (int64_t)p.d.batch;
 }
@@ -852,7 +862,9 @@ hipError_t launch(const VerifyArgs& p, hipStream_t s) {
   } else if (rows > 0) {
     hipLaunchKernelGGL((row_sums_kernel<F32, false, 0>), dim3(rows * pieces), dim3(kThreads), 0, s, p);
   }
-  if (batch * (unsigned)p.shorts <= 2u * (unsigned)compute_units()) {
+  // The way, its sums and the draw at once where that makes no more than one workgroup a compute unit (each finds the way by itself, and its fence costs the
+  // others time): one sequence, 131072 tokens, 17 us, with a launch each 23; four 23 and 26, eight 34 and 31, 16 55 and 40.
+  if (batch * (unsigned)p.shorts <= (unsigned)compute_units()) {
     hipLaunchKernelGGL((walk_and_draw_kernel<F32>), dim3(batch * (unsigned)p.shorts), dim3(kThreads), 0, s, p);
   } else {
     hipLaunchKernelGGL((walk_kernel<F32>), dim3(batch), dim3(64), 0, s, p);
