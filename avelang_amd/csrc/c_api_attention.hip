@@ -61,6 +61,29 @@ int check_how(const ave_fp4_norm_rope* how, int head_dim) {
 
 }  // namespace
 
+namespace {
+struct Range {
+  uintptr_t from, to;
+};
+template <typename T>
+Range range(const T* p, int64_t n) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+  return {from, p ? from + (uintptr_t)n * sizeof(T) : from};
+}
+bool overlap(const Range& a, const Range& b) { return a.from < b.to && b.from < a.to; }
+// Does an output overlap an input or another output?
+template <size_t I, size_t O>
+bool overlap(const Range (&in)[I], const Range (&out)[O]) {
+  for (size_t o = 0; o < O; ++o) {
+    for (size_t i = 0; i < I; ++i)
+      if (overlap(in[i], out[o])) return true;
+    for (size_t other = 0; other < o; ++other)
+      if (overlap(out[other], out[o])) return true;
+  }
+  return false;
+}
+}  // namespace
+
 extern "C" {
 
 int ave_fp4_qk_norm_rope(const ave_fp4_heads* q, const ave_fp4_heads* k, int tokens, int head_dim, const ave_fp4_norm_rope* how,
@@ -207,6 +230,9 @@ int ave_fp4_draft_tree(const int32_t* parents, const int32_t* cu_q, const int32_
   if (tokens == 0 || batch == 0 || (!seen && !positions)) return 0;
   if (!parents || !cu_q || (positions && !seq_lens)) return fail_inval("null device pointer.");
   if (!aligned(seen, 8)) return fail_inval("seen must be 8-byte aligned.");
+  const Range in[] = {range(parents, tokens), range(cu_q, (int64_t)batch + 1), range(seq_lens, batch)};
+  const Range out[] = {range(seen, (int64_t)tokens * words), range(positions, tokens)};
+  if (overlap(in, out)) return fail_inval("seen and positions must not overlap the inputs, nor each other.");
   return finish(ave::launch_draft_tree(parents, cu_q, seq_lens, tokens, batch, seen, seen ? words : 0, positions, static_cast<hipStream_t>(hip_stream)),
                 "draft tree kernel");
 }
@@ -235,6 +261,9 @@ int ave_fp4_verify_draft(const ave_fp4_draft* draft, void* workspace, size_t wor
   if (!d.cu_q || !d.accepted || (d.rows > 0 && (!d.logits || !d.tokens || !d.parents || !d.uniform || !d.path || !d.emitted)))
     return fail_inval("null device pointer.");
   if (!aligned(d.logits, d.logits_f32 ? 4 : 2) || !aligned(d.draft_probs, 4)) return fail_inval("logits and draft_probs must be aligned to their elements.");
+  const Range in[] = {range(d.tokens, d.rows), range(d.parents, d.rows), range(d.cu_q, (int64_t)d.batch + 1), range(d.uniform, d.rows), range(d.temperature, d.batch)};
+  const Range out[] = {range(d.accepted, d.batch), range(d.path, d.rows), range(d.emitted, d.rows)};
+  if (overlap(in, out)) return fail_inval("accepted, path and emitted must not overlap the inputs, nor each other.");
   const size_t need = ave::verify_draft_workspace_bytes(d);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail_inval("the workspace must have %zu bytes, got %zu.", need, workspace ? workspace_bytes : (size_t)0);
@@ -261,9 +290,9 @@ int ave_fp4_keep_kv_mxfp4(const ave_fp4_kv_cache* caches, int layers, const ave_
     return fail_inval("the page table must cover at most 2^31 - 1 tokens, got %d pages of %d.", k.table_pages, caches->page_size);
   if (k.batch == 0) return 0;
   if (!k.seq_lens || !k.cu_q || !k.accepted || (k.tokens > 0 && !k.path) || (k.table_pages > 0 && !k.page_table)) return fail_inval("null device pointer.");
-  const auto overlaps = [&](const int32_t* p, int64_t n) { return k.kept_lens && p < k.kept_lens + k.batch && k.kept_lens < p + n; };
-  if (overlaps(k.seq_lens, k.batch) || overlaps(k.cu_q, (int64_t)k.batch + 1) || overlaps(k.path, k.tokens) || overlaps(k.accepted, k.batch))
-    return fail_inval("kept_lens must not overlap an input.");
+  const Range in[] = {range(k.seq_lens, k.batch), range(k.cu_q, (int64_t)k.batch + 1), range(k.path, k.tokens), range(k.accepted, k.batch)};
+  const Range out[] = {range(k.kept_lens, k.batch)};
+  if (overlap(in, out)) return fail_inval("kept_lens must not overlap an input.");
   return finish(ave::launch_keep_kv(caches, layers, k, static_cast<hipStream_t>(hip_stream)), "key/value keep kernel");
 }
 

@@ -13,10 +13,9 @@ namespace {
 // last first.  Bound by latency: the parents lie in LDS, where a step takes about 100 cycles.
 constexpr int kTreeThreads = 256, kTreeNodes = 8192;   // nodes whose parents LDS holds; the rest are looked up in memory
 
-__global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens,
-                                                                  uint64_t* seen, int words, int32_t* positions) {
+__device__ inline void tree_of(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens, uint64_t* seen, int words,
+                               int32_t* positions, int b) {
   __shared__ int32_t up[kTreeNodes];
-  const int b = blockIdx.x;
   int first = cu_q[b], end = cu_q[b + 1];
   first = first < 0 ? 0 : first > tokens ? tokens : first;
   end = end < first ? first : end > tokens ? tokens : end;
@@ -43,6 +42,13 @@ __global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const int32_t*
     if (positions) positions[first + i] = base + above;
   }
 }
+__global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens, int batch,
+                                                                  uint64_t* seen, int words, int32_t* positions) {
+  for (int64_t b = blockIdx.x; b < batch; b += gridDim.x) {
+    if (b >= gridDim.x) __syncthreads();   // the parents of the one before have been read
+    tree_of(parents, cu_q, seq_lens, tokens, seen, words, positions, (int)b);
+  }
+}
 
 // ---- kept tokens moved together -----------------------------------------------------------------------------------------------------
 // A sequence's tokens of one head, keys or values, of one layer are a list; 16 bytes of codes and a byte of scale a thread.  A token comes from no place
@@ -58,7 +64,8 @@ struct KeepArgs {
   } layer[kLayers];
 };
 struct KeepSpan {
-  int first, n, many, base;   // first entry of `path`, nodes, kept ones, place of the first node
+  int first, n, many;   // first entry of `path`, nodes, kept ones
+  int64_t base;         // place of the first node
 };
 __device__ inline KeepSpan keep_span(const KeepArgs& p, int b) {
   KeepSpan s;
@@ -75,8 +82,9 @@ __device__ inline KeepSpan keep_span(const KeepArgs& p, int b) {
 struct Place {
   int page, row;
 };
-__device__ inline Place keep_place(const KeepArgs& p, int b, int position) {
-  if (position < 0 || position >= p.k.table_pages << p.page_shift) return {-1, 0};
+__device__ inline Place keep_place(const KeepArgs& p, int b, int64_t at) {
+  if (at < 0 || at >= p.k.table_pages << p.page_shift) return {-1, 0};
+  const int position = (int)at;
   const int page = p.k.page_table[(int64_t)b * p.k.page_table_stride + (position >> p.page_shift)];
   return {page < p.pages ? page : -1, position & (p.page_size - 1)};
 }
@@ -96,7 +104,7 @@ __global__ __launch_bounds__(256) void keep_few_kernel(KeepArgs p, int layers, i
   constexpr int kAtOnce = 64 / PIECES, kUnits = 4;   // units (head, keys or values, layer) of a wave under way
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x / 64, piece = lane % PIECES;
   const KeepSpan s = keep_span(p, b);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && p.k.kept_lens) p.k.kept_lens[b] = s.base + s.many;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.k.kept_lens) p.k.kept_lens[b] = (int32_t)(s.base + s.many);
   const int layer0 = blockIdx.x * each, now = min(each, layers - layer0), units = now * p.kv_heads * 2;
   for (int i0 = 0; i0 < s.many; i0 += kAtOnce) {
     Place from, to;
@@ -143,7 +151,7 @@ __global__ __launch_bounds__(512) void keep_many_kernel(KeepArgs p) {
   const int b = blockIdx.y, piece = threadIdx.x % PIECES, mine = threadIdx.x / PIECES, kv = 2 * (blockIdx.x & 1), head = blockIdx.x >> 1;
   const auto& layer = p.layer[blockIdx.z];
   const KeepSpan s = keep_span(p, b);
-  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.k.kept_lens) p.k.kept_lens[b] = s.base + s.many;
+  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.k.kept_lens) p.k.kept_lens[b] = (int32_t)(s.base + s.many);
   uint8_t* const codes = layer.data[kv];
   uint8_t* const scales = layer.data[kv + 1];
   const int64_t code_stride = layer.stride[kv], scale_stride = layer.stride[kv + 1];
@@ -216,7 +224,8 @@ void launch_keep(const KeepArgs& p, int layers, hipStream_t s) {
 
 hipError_t launch_draft_tree(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens, int batch, uint64_t* seen, int words,
                              int32_t* positions, hipStream_t s) {
-  hipLaunchKernelGGL(draft_tree_kernel, dim3((unsigned)batch), dim3(kTreeThreads), 0, s, parents, cu_q, seq_lens, tokens, seen, words, positions);
+  hipLaunchKernelGGL(draft_tree_kernel, dim3((unsigned)std::min(batch, 1 << 16)), dim3(kTreeThreads), 0, s, parents, cu_q, seq_lens, tokens, batch, seen, words,
+                     positions);
   return hipGetLastError();
 }
 

@@ -475,7 +475,7 @@ int ave_fp4_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_kv_cache* 
  * From the nodes' parents ([tokens], an index within the sequence; one that is not in [0, the node's own index) means none): `seen`, `words` 64-bit
  * words a node, bit j % 64 of word j / 64 is set where node j of the sequence is the node itself or one that it descends from (nodes from 64 * words on
  * have no bit), and the position of each node, seq_lens[b] less the number of nodes plus the number of nodes above it.  Either output may be null.
- * Rows behind cu_q[batch] are left alone.
+ * Rows behind cu_q[batch] are left alone.  No output may overlap an input.
  */
 int ave_fp4_draft_tree(const int32_t* parents, const int32_t* cu_q, const int32_t* seq_lens, int tokens, int batch, uint64_t* seen, int words,
                        int32_t* positions, void* hip_stream);
@@ -513,7 +513,7 @@ int ave_fp4_tree_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_tree*
  * Softmax, sums and products in 64 bits (a choice lies between sums of very many probabilities).  A NaN among the logits counts as -inf, +inf as the largest
  * finite number; a row without any number accepts no child and draws -1.  uniform is taken into [0, 1], NaN as 0; a token that is no index of the
  * vocabulary is never accepted; NaN and negative numbers in draft_probs count as 0, as they are otherwise (no sum of 1 is asked for).
- * Rows behind cu_q[batch] are neither read nor written.  Offsets are cut to the rows; nothing in device memory leads out of the arrays.
+ * Rows behind cu_q[batch] are not written, and what they hold does not matter.  No output may overlap another or the small inputs.  Offsets are cut to the rows; nothing in device memory leads out of the arrays.
  * The workspace (16-byte aligned, no initialisation) belongs to one call at a time.  Equal inputs give equal outputs.
  */
 typedef struct ave_fp4_draft {

@@ -21,7 +21,8 @@ def _tree(**kw):
 
 
 def _draft(**kw):
-    return _lib.Draft(**{**dict(logits=P, logits_stride=100, tokens=P, parents=P, cu_q=P, uniform=P, accepted=P, path=P, emitted=P, rows=8, batch=2, vocab=100), **kw})
+    return _lib.Draft(**{**dict(logits=P, logits_stride=100, tokens=P, parents=P, cu_q=P, uniform=P, accepted=2 * P, path=3 * P, emitted=4 * P, rows=8, batch=2, vocab=100),
+                         **kw})
 
 
 def _keep(**kw):
@@ -70,7 +71,8 @@ def test_workspaces_and_empty_calls():
     (dict(rows=-1), "non-negative"), (dict(batch=-1), "non-negative"), (dict(vocab=0), "vocab must be"), (dict(vocab=(1 << 30) + 1), "vocab must be"),
     (dict(rows=1 << 22), "below 2^22"), (dict(batch=1 << 22), "below 2^22"), (dict(rows=1 << 12, vocab=1 << 23), "below 2^22"), (dict(cu_q=0), "null device pointer"), (dict(logits=0), "null device"),
     (dict(uniform=0), "null device pointer"), (dict(emitted=0), "null device pointer"), (dict(logits=P + 1), "aligned"),
-    (dict(logits=P + 2, logits_f32=1), "aligned"), (dict(draft_probs=P + 2), "aligned")], ids=str)
+    (dict(logits=P + 2, logits_f32=1), "aligned"), (dict(draft_probs=P + 2), "aligned"), (dict(emitted=P), "overlap"), (dict(path=P + 28), "overlap"),
+    (dict(accepted=P + 8), "overlap"), (dict(path=4 * P - 28), "overlap"), (dict(accepted=3 * P + 28), "overlap")], ids=str)
 def test_drafts_that_are_refused(bad, text):
     lib = _lib.load()
     _refused(lib.ave_fp4_verify_draft(_ref(_draft(**bad)), P, 1 << 40, None), text)
@@ -84,6 +86,9 @@ def test_parents_that_are_refused():
     _refused(lib.ave_fp4_draft_tree(None, P, P, 4, 1, P, 1, P, None), "null device pointer")
     _refused(lib.ave_fp4_draft_tree(P, P, None, 4, 1, P, 1, P, None), "null device pointer")
     _refused(lib.ave_fp4_draft_tree(P, P, P, 4, 1, P + 4, 1, P, None), "8-byte")
+    _refused(lib.ave_fp4_draft_tree(P, P, P, 4, 1, 2 * P, 1, P, None), "overlap")
+    _refused(lib.ave_fp4_draft_tree(P, P, P, 4, 1, P - 24, 1, 3 * P, None), "overlap")
+    _refused(lib.ave_fp4_draft_tree(P, P, P, 4, 1, 2 * P, 1, 2 * P + 28, None), "overlap")
 
 
 @pytest.mark.parametrize("bad,text", [

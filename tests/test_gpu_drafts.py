@@ -23,9 +23,12 @@ def _parents(batch, seed, chain=False):
     return [D.random_parents(rng, n, chain) for n, _ in batch.rows]
 
 
-def _attend(gpu, batch, above, *, words=None, window=0, sinks=None, scale=None, max_q=None):
-    """The call, and its comparison; `above`: bool [nodes, nodes] of each sequence."""
+def _attend(gpu, batch, above, *, words=None, window=0, sinks=None, scale=None, max_q=None, wide=False):
+    """The call, and its comparison; `above`: bool [nodes, nodes] of each sequence.  wide: a page table for 2^17 tokens, by which other kernels are chosen
+    (blocks of 128 rows; no items kept whole)."""
     t = batch.tensors(gpu)
+    if wide:
+        t["page_table"] = torch.nn.functional.pad(t["page_table"], (0, 2 ** 17 // batch.page), value=-7)
     most = max(1, max(n for n, _ in batch.rows))
     words = -(-most // 64) if words is None else words
     seen = D.tensor(np.concatenate([D.words_of(a, words) for a in above]), gpu)
@@ -49,7 +52,30 @@ def _attend(gpu, batch, above, *, words=None, window=0, sinks=None, scale=None, 
 @pytest.mark.parametrize("heads", HEADS)
 def test_attention_over_trees(gpu, heads, page, rows):
     batch = A.Batch(rows, *HEADS[heads], page, seed=page + rows[0][1])
-    _attend(gpu, batch, [D.ancestors(p) for p in _parents(batch, rows[0][0])])
+    above = [D.ancestors(p) for p in _parents(batch, rows[0][0])]
+    _attend(gpu, batch, above)
+    _attend(gpu, batch, above, wide=True)
+
+
+@pytest.mark.parametrize("heads", ["gqa64", "gqa128", "gqa256", "mha128", "mqa64"])
+@pytest.mark.parametrize("count,nodes,keys", [(70, 3, 40), (150, 9, 60), (300, 20, 50), (9, 64, 700)])
+def test_many_sequences(gpu, heads, count, nodes, keys):
+    """More sequences than a wave has lanes, more items than workgroups, items whole and in parts, some sequences empty."""
+    rng = np.random.default_rng(count)
+    rows = [(int(n), int(n) + int(k)) if n else (0, int(k)) for n, k in zip(rng.integers(0, nodes + 1, count), rng.integers(0, keys + 1, count))]
+    batch = A.Batch(rows, *HEADS[heads], 16, seed=count)
+    above = [D.ancestors(p) for p in _parents(batch, 3)]
+    _attend(gpu, batch, above)
+    _attend(gpu, batch, above, wide=True, window=33)
+
+
+def test_a_bound_that_is_wrong(gpu):
+    """max_q below and far above the nodes that there are chooses other kernels and costs time only."""
+    batch = A.Batch([(40, 300), (3, 90), (64, 64)], *HEADS["gqa128"], 16, seed=9)
+    above = [D.ancestors(p) for p in _parents(batch, 4)]
+    for bound in (0, 1, 3, 9, 5000):
+        _attend(gpu, batch, above, max_q=bound)
+        _attend(gpu, batch, above, max_q=bound, wide=True)
 
 
 @pytest.mark.parametrize("rows", [[(6, 400), (3, 30)], [(40, 300), (20, 21), (64, 130)]], ids=str)
@@ -58,7 +84,9 @@ def test_attention_over_trees(gpu, heads, page, rows):
 @pytest.mark.parametrize("heads", ["gqa64", "gqa128", "gqa256", "group5"])
 def test_windows_sinks_scales(gpu, heads, how, rows):
     batch = A.Batch(rows, *HEADS[heads], 32, seed=3)
-    _attend(gpu, batch, [D.ancestors(p) for p in _parents(batch, 5)], **{k: batch.sinks if k == "sinks" else v for k, v in how.items()})
+    how = {k: batch.sinks if k == "sinks" else v for k, v in how.items()}
+    for wide in (False, True):
+        _attend(gpu, batch, [D.ancestors(p) for p in _parents(batch, 5)], wide=wide, **how)
 
 
 @pytest.mark.parametrize("heads", ["gqa64", "gqa128", "gqa256", "group40"])
@@ -72,8 +100,9 @@ def test_any_bits(gpu, heads):
         a[::3] = False
     _, _, out = _attend(gpu, batch, above)
     assert out[0].eq(0).all() and out[5].eq(0).all()
-    _attend(gpu, batch, above, words=1)
-    _attend(gpu, batch, above, window=40, sinks=batch.sinks)
+    for wide in (False, True):
+        _attend(gpu, batch, above, words=1, wide=wide)
+        _attend(gpu, batch, above, window=40, sinks=batch.sinks, wide=wide)
     wide = [np.concatenate([a, np.ones((a.shape[0], 300), bool)], 1) for a in above]      # bits of nodes that are not there
     t = batch.tensors(gpu)
     a, b = (ave.tree_attention_mxfp4(t["q"], t["cache"], t["page_table"], t["seq_lens"], t["cu_q"], D.tensor(np.concatenate([D.words_of(x, 4) for x in m]), gpu), max_q=130,
@@ -127,21 +156,23 @@ def test_strides_other_rows_and_streams(gpu):
     assert torch.equal(one, ave.attention_mxfp4(t["q"][:2], t["cache"], t["page_table"], t["seq_lens"]))
 
 
-@pytest.mark.parametrize("nodes", [6, 40])
+@pytest.mark.parametrize("nodes", [2, 6, 40])
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("heads", ["gqa64", "gqa128", "gqa256"])
-def test_hidden_nodes_do_not_matter(gpu, heads, nodes):
+def test_hidden_nodes_do_not_matter(gpu, heads, wide, nodes):
     """NaN scales of keys and values in nodes that a row does not see leave it alone; those that it sees make it NaN."""
     batch = A.Batch([(nodes, nodes + 70)], *HEADS[heads], 16, seed=7)
     above = np.eye(nodes, dtype=bool)
     above[:, 0] = True
-    t, seen, out = _attend(gpu, batch, [above])
+    t, seen, out = _attend(gpu, batch, [above], wide=wide)
     for part in (1, 3):
         cache = [c.clone() for c in t["cache"]]
-        p, o = batch.place(0, 70 + 3)
+        hidden = min(3, nodes - 1)
+        p, o = batch.place(0, 70 + hidden)
         cache[part][int(p), :, int(o)] = 0xFF
         got = ave.tree_attention_mxfp4(t["q"], tuple(cache), t["page_table"], t["seq_lens"], t["cu_q"], seen, max_q=nodes)
-        others = [i for i in range(nodes) if i != 3]
-        assert torch.equal(got[others], out[others]) and got[3].isnan().all()
+        others = [i for i in range(nodes) if i != hidden]
+        assert torch.equal(got[others], out[others]) and got[hidden].isnan().all()
 
 
 def test_workspaces_that_do_not_do(gpu):
@@ -183,9 +214,33 @@ def test_tree_of_parents(gpu, counts, chain):
     at = np.concatenate([k - len(p) + D.ancestors(p).sum(1) - 1 for p, k in zip(parents, lens)])
     assert np.array_equal(seen.cpu().numpy()[:t], want) and np.array_equal(positions.cpu().numpy()[:t], at)
     assert seen[t:].eq(77).all() and positions[t:].eq(77).all()
-    if most > 64:      # fewer bits than nodes
+    if 64 < most < 1000:      # fewer bits than nodes
         narrow, same = ave.draft_tree(D.tensor(flat, gpu), D.tensor(cu, gpu), D.tensor(lens, gpu), max_q=64)
         assert np.array_equal(narrow.cpu().numpy()[:t, 0], want[:, 0]) and torch.equal(same[:t], positions[:t])
+
+
+def test_more_trees_than_workgroups(gpu):
+    """Chains of 0 to 2 nodes for 70000 sequences: a workgroup takes a second one."""
+    count = 70000
+    n = np.arange(count) % 3
+    cu = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    place = np.arange(cu[-1]) - np.repeat(cu[:-1], n)
+    lens = (n + np.arange(count) % 7).astype(np.int32)
+    seen, positions = ave.draft_tree(D.tensor((place - 1).astype(np.int32), gpu), D.tensor(cu, gpu), D.tensor(lens, gpu), max_q=2)
+    assert np.array_equal(seen.cpu().numpy()[:, 0], 2 ** (place + 1) - 1)
+    assert np.array_equal(positions.cpu().numpy(), np.repeat(lens - n, n) + place)
+
+
+def test_trees_beyond_what_lds_holds(gpu):
+    rng = np.random.default_rng(5)
+    n = 9001
+    parents = np.array([-1] + [int(rng.integers(0, j)) for j in range(1, n)], np.int32)
+    cu, lens = np.array([0, 5, 5 + n], np.int32), np.array([5, n + 10], np.int32)
+    seen, positions = ave.draft_tree(D.tensor(np.concatenate([[-1, 0, 1, 2, 3], parents]).astype(np.int32), gpu), D.tensor(cu, gpu), D.tensor(lens, gpu), max_q=n)
+    seen, positions, lines = seen.cpu().numpy(), positions.cpu().numpy(), D.lines_of(parents)
+    for i in range(0, n, 7):
+        bits = np.flatnonzero(np.unpackbits(seen[5 + i].view(np.uint8), bitorder="little"))
+        assert bits.tolist() == lines[i] and positions[5 + i] == 10 + len(lines[i]) - 1
 
 
 # ---- acceptance -----------------------------------------------------------------------------------------------------------------------------
