@@ -513,7 +513,8 @@ int ave_fp4_tree_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_tree*
  * Softmax, sums and products in 64 bits (a choice lies between sums of very many probabilities).  A NaN among the logits counts as -inf, +inf as the largest
  * finite number; a row without any number accepts no child and draws -1.  uniform is taken into [0, 1], NaN as 0; a token that is no index of the
  * vocabulary is never accepted; NaN and negative numbers in draft_probs count as 0, as they are otherwise (no sum of 1 is asked for).
- * Rows behind cu_q[batch] are not written, and what they hold does not matter.  No output may overlap another or the small inputs.  Offsets are cut to the rows; nothing in device memory leads out of the arrays.
+ * Rows behind cu_q[batch] are not written, and what they hold does not matter.  No output may overlap another output or an input.  Offsets are cut to the
+ * rows; nothing in device memory leads out of the arrays.
  * The workspace (16-byte aligned, no initialisation) belongs to one call at a time.  Equal inputs give equal outputs.
  */
 typedef struct ave_fp4_draft {

@@ -558,6 +558,63 @@ def test_a_step_replayed(gpu):
     assert total > 5 * b and int(lens[0].sum()) == total + int(starts.sum())
 
 
+def _acceptance(gpu, seed, counts, vocab, probs):
+    d = _draft(seed, counts, vocab, probs=probs)
+    args = [D.tensor(d["logits"], gpu).bfloat16()] + [D.tensor(d[k], gpu) for k in ("tokens", "parents", "cu", "uniform")]
+    return args + [torch.ones(len(counts), device=gpu), D.tensor(d["probs"], gpu) if probs else None]
+
+
+@pytest.mark.parametrize("counts,vocab,probs", [([6], 9000, False), ([6], 9000, True), ([6] * 70, 20000, False), ([5] * 40, 20000, True), ([14, 1, 20, 12, 17, 0, 9], 500009, False)],
+                         ids=["one", "one-probs", "many", "many-probs", "two-steps"])
+def test_acceptance_replayed(gpu, counts, vocab, probs):
+    """Every order of launches in a graph, on inputs that change between replays."""
+    inputs = [_acceptance(gpu, seed, counts, vocab, probs) for seed in (1, 2)]
+    held = [None if x is None else x.clone() for x in inputs[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ave.verify_draft(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = ave.verify_draft(*held)
+    for i in (1, 0, 1, 1):
+        for to, x in zip(held, inputs[i]):
+            if x is not None:
+                to.copy_(x)
+        graph.replay()
+        eager = ave.verify_draft(*inputs[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, eager)), i
+
+
+def test_calls_at_once(gpu):
+    """Two streams, each with calls of its own that share nothing, give what the calls give alone."""
+    batches = [A.Batch([(40, 300), (9, 2000), (64, 64)], *HEADS["gqa128"], 16, seed=1), A.Batch([(3, 5000), (6, 70)], *HEADS["gqa64"], 64, seed=2)]
+    work = []
+    for i, batch in enumerate(batches):
+        t = batch.tensors(gpu)
+        seen, _ = ave.draft_tree(D.tensor(np.concatenate(_parents(batch, 7 + i)), gpu), t["cu_q"], t["seq_lens"], max_q=64)
+        work.append((t, seen, _acceptance(gpu, 3 + i, [6] * (70 if i else 2), 20000, bool(i))))
+
+    def calls(t, seen, accept):
+        return ave.tree_attention_mxfp4(t["q"], t["cache"], t["page_table"], t["seq_lens"], t["cu_q"], seen, max_q=64), *ave.verify_draft(*accept)
+
+    alone = [[x.clone() for x in calls(*w)] for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results[i].append(calls(*work[i]))
+    torch.cuda.synchronize()
+    for got, want in zip(results, alone):
+        for run in got:
+            live = [torch.equal(a, b) for a, b in zip(run, want)]
+            assert all(live), live
+
+
 def test_both_bindings_agree(gpu, monkeypatch):
     """The entry points in C++ and through ctypes."""
     batch = A.Batch([(9, 60), (20, 200)], *HEADS["gqa128"], 16, seed=6)
