@@ -24,6 +24,12 @@
 // 8192 tokens, 32 heads on 8 of 128: 459 us, 1.20 PFLOP/s of 4 D flop a score (the matrix cores also multiply the queries' second part, half as much
 // again); 4 sequences of up to 16000 keys, 600 new tokens, 40 heads on 8: 320 us, 1.11 PFLOP/s; six prompts of about 1000 tokens, 64 heads on 8 of 64:
 // 67 us, where an item of 128 rows has but 8 tiles for its start and end, and half the work is exponentials.
+//
+// Trees of drafted tokens (TreeArgs): a row sees its sequence's keys before the nodes, and of the nodes those with a bit; bits are looked at in tiles that hold
+// nodes only.  Drafts make 17 to 128 rows a key head, so there are blocks of 64 rows, too (SPLIT 2: waves 0 and 1 take the first 32 keys of a tile, 2 and 3 the
+// others, with sums of their own that meet in LDS at the item's end), and always parts: 16 sequences of up to 4096 keys, 16 nodes, 32 heads on 8 of 128 33 us and
+// 7.5 the join (vector units 29 % busy, matrix cores 13 %; 6 to 10 us are the start); 8 of up to 3000, 64 nodes, 64 heads on 8 of 64, window 1000 28 and 7.4; one of
+// 131072, 64 nodes (blocks of 128 rows) 129 and 12.5, 1.06 PFLOP/s in the first.
 #include "attn_common.hpp"
 #include "kernels.hpp"
 
