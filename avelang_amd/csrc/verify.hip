@@ -272,10 +272,12 @@ __global__ __launch_bounds__((EXACT ? 2 : 1) * kThreads) void row_sums_kernel(Ve
       if (item + gridDim.x < all) fetch(item + gridDim.x);
     } else {
 #pragma unroll
-      for (int k = 0; k < kEach / kOnce; ++k) logits<F32>(p, row, piece * kPiece + (k * THREADS + threadIdx.x) * kOnce, x[k]);
+      for (int k = 0; k < kEach / kOnce; ++k) next[k] = load8<F32>(p, row, piece * kPiece + (k * THREADS + threadIdx.x) * kOnce);   // all under way
       if constexpr (ROWS == 0) b = sequence_of(p, row);
       if (b < 0) return;
       per = inverse_temperature(p, b);
+#pragma unroll
+      for (int k = 0; k < kEach / kOnce; ++k) unpack<F32>(next[k], x[k]);
     }
     if (threadIdx.x == 0) lowest = INT32_MAX;
     float top;
@@ -519,37 +521,44 @@ __global__ __launch_bounds__(64) void first_step_kernel(VerifyArgs p) {
   }
 }
 
-// Element i.. of what is drawn from, in units of the row's largest weight (kRest: of 1)
-template <bool F32, int N>
-__device__ inline void weights_of(const VerifyArgs& p, const Span& s, const Draw& d, double per, int i, double (&w)[N]) {
-  static_assert(N % kOnce == 0, "");
-  const double over = 1.0 / d.sum;
+// Elements i .. i + 7 of what is drawn from: what they are made of, to be asked for before any is used,
+template <bool F32>
+struct Source {
+  Eight<F32> x;
+  float q[kOnce];
+};
+template <bool F32>
+__device__ inline Source<F32> source_of(const VerifyArgs& p, const Draw& d, int i) {
+  Source<F32> r;
+  r.x = load8<F32>(p, d.row, i);
+  if (d.how == kRest) draft_probs(p, d.row, i, r.q);
+  return r;
+}
+// and they, in units of the row's largest weight (kRest: of 1).  By whole waves, whose lanes' elements follow each other.
+template <bool F32>
+__device__ inline void weights_of(const VerifyArgs& p, const Span& s, const Draw& d, double per, int i, const Source<F32>& from, double (&w)[kOnce]) {
+  float x[kOnce];
+  unpack<F32>(from.x, x);
 #pragma unroll
-  for (int k = 0; k < N; k += kOnce) {
-    float x[kOnce], q[kOnce];
-    logits<F32>(p, d.row, i + k, x);
-    if (d.how == kRest) draft_probs(p, d.row, i + k, q);
+  for (int j = 0; j < kOnce; ++j) w[j] = weight_of(number(x[j]), d.top, per);
+  if (d.how == kRest) {
+    const double over = 1.0 / d.sum;
 #pragma unroll
-    for (int j = 0; j < kOnce; ++j) w[k + j] = weight_of(number(x[j]), d.top, per);
-    if (d.how == kRest) {
-#pragma unroll
-      for (int j = 0; j < kOnce; ++j) w[k + j] = fmax(w[k + j] * over - d.times * (q[j] > 0.0f ? (double)q[j] : 0.0), 0.0);
-    }
+    for (int j = 0; j < kOnce; ++j) w[j] = fmax(w[j] * over - d.times * (from.q[j] > 0.0f ? (double)from.q[j] : 0.0), 0.0);
   }
-  if (d.how == kWithout && d.many >= 0) {
-    for (int c = 0; c < d.many; ++c) {
-      const int gone = d.gone[c] - i;
+  if (d.how == kWithout) {
+    const int first = uniform_int(i);
+    const auto without = [&](int token) {
+      if ((unsigned)token - (unsigned)first >= 64u * kOnce) return;   // none of this wave's
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (gone == j) w[j] = 0.0;
-    }
-  } else if (d.how == kWithout) {
-    const int at = d.row - s.first;
-    for (int c = next_child(p, s, at, at + 1); c < s.n; c = next_child(p, s, at, c + 1)) {
-      const int gone = p.d.tokens[s.first + c] - i;
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (gone == j) w[j] = 0.0;
+      for (int j = 0; j < kOnce; ++j)
+        w[j] = token - i == j ? 0.0 : w[j];
+    };
+    if (d.many >= 0) {
+      for (int c = 0; c < d.many; ++c) without(d.gone[c]);
+    } else {
+      const int at = d.row - s.first;
+      for (int c = next_child(p, s, at, at + 1); c < s.n; c = next_child(p, s, at, c + 1)) without(p.d.tokens[s.first + c]);
     }
   }
 }
@@ -589,7 +598,8 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
     __syncthreads();
     for (int c = 0; c < p.shorts; ++c) {
       double w[kOnce], sum = 0.0;
-      weights_of<F32>(p, s, all_of_it, per, c * kShort + (int)threadIdx.x * kOnce, w);
+      const int i = c * kShort + (int)threadIdx.x * kOnce;
+      weights_of<F32>(p, s, all_of_it, per, i, source_of<F32>(p, all_of_it, i), w);
 #pragma unroll
       for (int j = 0; j < kOnce; ++j) sum += w[j];
       sum = block_sum<kThreads>(sum, wave_at);
@@ -614,7 +624,8 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
   }
   const Draw& d = nothing_left ? all_of_it : of;
   double w[kOnce], mine = 0.0;
-  weights_of<F32>(p, s, d, per, piece * kShort + (int)threadIdx.x * kOnce, w);
+  const int i = piece * kShort + (int)threadIdx.x * kOnce;
+  weights_of<F32>(p, s, d, per, i, source_of<F32>(p, d, i), w);
 #pragma unroll
   for (int j = 0; j < kOnce; ++j) mine += w[j];
   const double upto = wave_running(mine);
@@ -670,10 +681,13 @@ __device__ inline void find_way(const VerifyArgs& p, const Span& s, double per, 
 template <bool F32, int SHORTS>
 __device__ inline void sum_shorts(const VerifyArgs& p, const Span& s, const Draw& d, double per, int b, int first) {
   __shared__ double scratch[kThreads / 64][SHORTS];
+  Source<F32> from[SHORTS];
+#pragma unroll
+  for (int k = 0; k < SHORTS; ++k) from[k] = source_of<F32>(p, d, (first + k) * kShort + (int)threadIdx.x * kOnce);
 #pragma unroll
   for (int k = 0; k < SHORTS; ++k) {
     double w[kOnce], sum = 0.0;
-    weights_of<F32>(p, s, d, per, (first + k) * kShort + (int)threadIdx.x * kOnce, w);
+    weights_of<F32>(p, s, d, per, (first + k) * kShort + (int)threadIdx.x * kOnce, from[k], w);
 #pragma unroll
     for (int j = 0; j < kOnce; ++j) sum += w[j];
     sum = wave_sum(sum);
@@ -749,17 +763,6 @@ __device__ inline bool accepts(const VerifyArgs& p, int row, const RowSum& r, do
   const double q = draft_prob(p, row, token), w = weight_of(number(logit<F32>(p, row, token)), r.top, per) / r.sum;
   return random_of(p, child_row) * q * left < fmax(w - t * q, 0.0);
 }
-// Sum of a thread's elements of max(p - t q, 0)
-template <bool F32, int N>
-__device__ inline double rest_of(const VerifyArgs& p, const Span& s, const RowSum& r, double per, double t, int row, int i) {
-  double w[N], sum = 0.0;
-  Draw rest{};
-  rest.times = t, rest.sum = r.sum, rest.top = r.top, rest.row = row, rest.how = kRest;
-  weights_of<F32>(p, s, rest, per, i, w);
-#pragma unroll
-  for (int j = 0; j < N; ++j) sum += w[j];
-  return sum;
-}
 
 // Rows of two children and more whose first one is rejected: the sum of max(p - q, 0), a piece a workgroup; the last one goes on with the other children.
 template <bool F32>
@@ -781,8 +784,19 @@ __global__ __launch_bounds__(kThreads) void children_kernel(VerifyArgs p) {
   const auto sum_of = [&](int c, double t) {   // of piece c
     double sum = 0.0;
     if (r.sum > 0.0) {
+      Draw rest{};
+      rest.times = t, rest.sum = r.sum, rest.top = r.top, rest.row = row, rest.how = kRest;
+      Source<F32> from[kParts];
+      const int i = c * kPiece + (int)threadIdx.x * kOnce;
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) sum += rest_of<F32, kOnce>(p, s, r, per, t, row, c * kPiece + (k * kThreads + (int)threadIdx.x) * kOnce);
+      for (int k = 0; k < kParts; ++k) from[k] = source_of<F32>(p, rest, i + k * kShort);
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) {
+        double w[kOnce];
+        weights_of<F32>(p, s, rest, per, i + k * kShort, from[k], w);
+#pragma unroll
+        for (int j = 0; j < kOnce; ++j) sum += w[j];
+      }
     }
     return block_sum<kThreads>(sum, scratch);
   };
