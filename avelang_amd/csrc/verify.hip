@@ -10,9 +10,9 @@
 // With little to read the last three are one launch, whose workgroups find the way each by itself.  With much, the children of node 0 are decided on first,
 // from its row alone, and then only rows that descend from the accepted one are read.
 //
-// Bound by HBM where there is much to read: 64 trees of 16 nodes, 131072 tokens in bf16, 64 us of which 23 are the wanted 377 of 1024 rows at 4.2 TB/s
+// Bound by HBM where there is much to read: 64 trees of 16 nodes, 131072 tokens in bf16, 65 us of which 23 are the wanted 377 of 1024 rows at 4.2 TB/s
 // (all rows at 4.9 TB/s would be 55); else by the way from one launch to the next and by chains of loads: six nodes of 32768 tokens 9 us; eight chains of six
-// with distributions, 50001 tokens, 25.  Beside that, fp64: the sums over 64 rows of 131072 take 16 us, about 25 instructions an element.
+// with distributions, 50001 tokens, 23.  Beside that, fp64: the sums over 64 rows of 131072 take 14 us, about 25 instructions an element.
 //
 // Rejections with distributions: r_0 = p, r_(k+1) = max(r_k - q, 0) / sum is max(p - t_k q, 0) / s_k with t_0 = 0, s_0 = 1, t_(k+1) = t_k + s_k and
 // s_k = sum max(p - t_k q, 0), so that a row needs its logits, q and two numbers.
@@ -339,31 +339,72 @@ struct RowSum {
   float top;
   int at;
 };
-template <bool EXACT>
-__device__ inline void add_piece(RowSum& r, const PieceSum& q, double per) {
-  if (q.top == -INFINITY) return;
-  const bool higher = q.top > r.top;
-  if (per > 0.0) {
-    const float low = higher ? r.top : q.top, high = higher ? q.top : r.top;
-    const double w = EXACT ? weight_of(low, high, per) : (double)__builtin_amdgcn_exp2f((low - high) * (float)fmin(per, 3.4e38));
-    r.sum = higher ? r.sum * w + q.sum : r.sum + q.sum * w;
-  }
-  if (higher) r.top = q.top, r.at = q.at;
-}
-// Of all pieces, by a lane: sixteen at a time under way.  (The order of the sum depends on the number of pieces alone.)
-template <bool EXACT>
-__device__ inline RowSum row_sum(const VerifyArgs& p, int row, double per) {
-  const PieceSum* s = p.sums + (size_t)row * p.pieces;
-  RowSum r{0.0, -INFINITY, INT32_MAX};
-  for (int c0 = 0; c0 < p.pieces; c0 += 16) {
-    PieceSum q[16];
+// Of the rows that the lanes name (-1: none), each in its lane, by a wave; exact: in fp64.  A row's sum depends on its pieces alone, bit for bit.
+__device__ inline RowSum sums_of_rows(const VerifyArgs& p, int row, double per, bool exact) {
+  RowSum mine{0.0, -INFINITY, INT32_MAX};
+  if (!exact) {   // a row a lane, sixteen pieces at a time under way
+    const float per32 = (float)fmin(per, 3.4e38);
+#pragma unroll 1
+    for (int c0 = 0; row >= 0 && c0 < p.pieces; c0 += 16) {
+      PieceSum q[16];
 #pragma unroll
-    for (int c = 0; c < 16; ++c) q[c] = s[min(c0 + c, p.pieces - 1)];
+      for (int c = 0; c < 16; ++c) q[c] = p.sums[(size_t)row * p.pieces + min(c0 + c, p.pieces - 1)];
+      float top = mine.top;
 #pragma unroll
-    for (int c = 0; c < 16; ++c)
-      if (c0 + c < p.pieces) add_piece<EXACT>(r, q[c], per);
+      for (int c = 0; c < 16; ++c) top = fmaxf(top, q[c].top);
+      if (top == -INFINITY) continue;
+      const auto scale = [&](float x) { return x == -INFINITY ? 0.0 : (double)__builtin_amdgcn_exp2f((x - top) * per32); };
+      if (mine.top != top) {
+        mine.sum *= scale(mine.top);
+#pragma unroll
+        for (int c = 15; c >= 0; --c) mine.at = q[c].top == top ? q[c].at : mine.at;
+      }
+      mine.top = top;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) mine.sum += c0 + c < p.pieces ? q[c].sum * scale(q[c].top) : 0.0;
+    }
+    if (!(per > 0.0)) mine.sum = 0.0;
+    return mine;
   }
-  return r;
+  // a piece a lane, the lanes of a row next to each other, as many rows at a time as that leaves (unrolled over sixteen pieces a lane, the exponentials are 6 KB of
+  // instructions that a launch has to fetch first: eight chains of six with distributions, 50001 tokens, 24.3 us that way, 23.3 this way)
+  const int lane = threadIdx.x & 63, wide = p.pieces >= 64 ? 64 : p.pieces > 1 ? 1 << (32 - __clz(p.pieces - 1)) : 1, at_once = 64 / wide;
+  const auto of_round = [&](int r0) { return __shfl(row, min(r0 + lane / wide, 63), 64); };
+  const auto fetch = [&](int of, int c) { return of >= 0 && c < p.pieces ? p.sums[(size_t)of * p.pieces + c] : PieceSum{0.0, -INFINITY, INT32_MAX}; };
+  const auto scale = [&](float x, float top) { return x == -INFINITY ? 0.0 : weight_of(x, top, per); };
+  const uint64_t named = __ballot(row >= 0);
+  const int end = named ? 64 - __clzll((long long)named) : 0;
+  int of = of_round(0);
+  PieceSum next = fetch(of, lane % wide);
+#pragma unroll 1
+  for (int r0 = 0; r0 < end; r0 += at_once) {
+    PieceSum q = next;
+    const int now = of;
+    of = of_round(r0 + at_once);
+    if (r0 + at_once < end) next = fetch(of, lane % wide);
+#pragma unroll 1
+    for (int c = lane % wide + 64; c < p.pieces; c += 64) {   // (more than 64 pieces: 524288 tokens)
+      const PieceSum more = fetch(now, c);
+      const float top = fmaxf(q.top, more.top);
+      q.at = more.top > q.top ? more.at : q.at;
+      if (per > 0.0) q.sum = q.sum * scale(q.top, top) + more.sum * scale(more.top, top);
+      q.top = top;
+    }
+    float top = q.top;
+#pragma unroll 1
+    for (int m = wide / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    double sum = per > 0.0 ? q.sum * scale(q.top, top) : 0.0;
+    int at = q.top == top && top != -INFINITY ? q.at : INT32_MAX;
+#pragma unroll 1
+    for (int m = wide / 2; m > 0; m >>= 1) {
+      sum += __shfl_xor(sum, m, 64);
+      at = min(at, __shfl_xor(at, m, 64));
+    }
+    const int from = (lane - r0) * wide;   // where this lane's row is, in its round
+    sum = __shfl(sum, from & 63, 64), top = __shfl(top, from & 63, 64), at = __shfl(at, from & 63, 64);
+    if (lane >= r0 && lane < r0 + at_once) mine = {sum, top, at};
+  }
+  return mine;
 }
 // Largest logit and its lowest index, by a wave
 __device__ inline RowSum row_top(const VerifyArgs& p, int row) {
@@ -393,10 +434,15 @@ __device__ inline double exact_sum(const VerifyArgs& p, int row, float top, doub
   return wave_sum(sum);
 }
 
+__device__ inline RowSum of_lane(const RowSum& r, int lane) {   // lane: the same in all lanes
+  return {lane_double(r.sum, lane), __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, r.top), lane)), __builtin_amdgcn_readlane(r.at, lane)};
+}
+
 // ---- the way through the tree ------------------------------------------------------------------------------------------------------------------
 struct Way {
   int at, kept, tried, token;   // the last node, how many are kept, how many of its children were rejected; temperature 0: the token
   double times;                 // with distributions: t
+  RowSum row;                   // of the last node (FIRST: of lanes' nodes)
 };
 // By one wave.  FIRST: one step only (at: the accepted child of node 0, or 0).  write: this workgroup writes path and emitted.  draw: where the tokens of the
 // last node's children go.
@@ -404,28 +450,38 @@ template <bool F32, bool FIRST>
 __device__ inline Way walk(const VerifyArgs& p, const Span& s, double per, bool write, Draw* draw = nullptr) {
   const int lane = threadIdx.x & 63;
   const bool probs = p.d.draft_probs != nullptr;
-  Way w{0, 1, 0, -1, 0.0};
+  Way w{0, 1, 0, -1, 0.0, {0.0, -INFINITY, INT32_MAX}};
   double taken = 0.0;   // by rejected children, of the present row
   write = write && lane == 0;
   if (write) p.d.path[s.first] = 0;
+  // Up to 64 nodes all rows' sums are on their way, a node a lane, while it is looked up whose children the nodes are
+  const bool few = s.n <= 64;
+  if (few) w.row = sums_of_rows(p, lane < (FIRST ? 1 : s.n) ? s.first + lane : -1, per, probs);
   for (int c0 = 0; c0 < s.n; c0 += 64) {
     // a node a lane: its parent's row, what the target gives its token, what the draft gave it
     const int j = c0 + lane;
     int parent = -1, token = -1;
     double u = 0.0, mine = 0.0, q = 0.0;
     RowSum r{0.0, -INFINITY, INT32_MAX};
-    if (j < s.n && j > 0) {
-      parent = p.d.parents[s.first + j], token = p.d.tokens[s.first + j];
-      if (parent >= j) parent = -1;
-    }
-    if (parent >= w.at && (!FIRST || parent == 0)) {   // (the others cannot be reached)
+    if (j < s.n && j > 0) parent = p.d.parents[s.first + j], token = p.d.tokens[s.first + j];
+    if (parent >= j) parent = -1;
+    bool there = false;
+    float x = -INFINITY;
+    if (parent >= w.at && (!FIRST || parent == 0)) {
       const int row = s.first + parent;
       u = random_of(p, s.first + j);
-      const bool there = token >= 0 && token < p.d.vocab;
-      const float x = there ? number(logit<F32>(p, row, token)) : -INFINITY;
+      there = token >= 0 && token < p.d.vocab;
+      if (there) x = logit<F32>(p, row, token);
       if (there && probs) q = draft_prob(p, row, token);
-      r = probs ? row_sum<true>(p, row, per) : row_sum<false>(p, row, per);
-      if (per > 0.0) mine = r.sum > 0.0 ? weight_of(x, r.top, per) / r.sum : 0.0;
+    }
+    if (few) {
+      const int from = parent > 0 ? parent : 0;
+      r = {__shfl(w.row.sum, from, 64), __shfl(w.row.top, from, 64), __shfl(w.row.at, from, 64)};
+    } else {
+      r = sums_of_rows(p, parent >= w.at && (!FIRST || parent == 0) ? s.first + parent : -1, per, probs);
+    }
+    if (parent >= w.at && (!FIRST || parent == 0)) {   // (the others cannot be reached)
+      if (per > 0.0) mine = r.sum > 0.0 ? weight_of(there ? number(x) : -INFINITY, r.top, per) / r.sum : 0.0;
       if (!there) token = -1;
     } else {
       parent = -1;
@@ -492,6 +548,8 @@ __device__ inline Way walk(const VerifyArgs& p, const Span& s, double per, bool 
     }
   }
   if (!FIRST && s.n > 64 && lane == 0) draw->many = -1;
+  if (!FIRST && !few) w.row = sums_of_rows(p, lane == 0 ? s.first + w.at : -1, per, probs);
+  if (!FIRST) w.row = of_lane(w.row, few ? w.at : 0);
   if (probs && per > 0.0) w.times = w.tried > 1 ? p.times[s.first + w.at] : (double)w.tried;   // (p.times is there with distributions only)
   return w;
 }
@@ -574,7 +632,7 @@ __device__ inline double wave_running(double v) {
 }
 // The next token, by a workgroup, whose threads share the kShort elements among which it lies
 template <bool F32>
-__device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw& of, double per, int b) {
+__device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw& of, double per, double random, int b) {
   __shared__ double wave_at[kThreads / 64];
   __shared__ int firsts[kThreads / 64], lasts[kThreads / 64];
   __shared__ Draw all_of_it;
@@ -582,9 +640,11 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
   bool nothing_left = false;
   const auto piece_sum = [&](int c) -> double { return c < p.shorts ? p.left[(size_t)b * p.shorts + c] : 0.0; };
   // every wave: pieces a lane, 64 at a time
+  double mine0, upto0;   // of the first 64
   const auto sum_of_all = [&] {
-    double sum = 0.0;
-    for (int c0 = 0; c0 < p.shorts; c0 += 64) sum += lane_double(wave_running(piece_sum(c0 + lane)), 63);
+    mine0 = piece_sum(lane), upto0 = wave_running(mine0);
+    double sum = lane_double(upto0, 63);
+    for (int c0 = 64; c0 < p.shorts; c0 += 64) sum += lane_double(wave_running(piece_sum(c0 + lane)), 63);
     return sum;
   };
   double all = sum_of_all();
@@ -609,11 +669,11 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
     __syncthreads();
     all = sum_of_all();
   }
-  const double want = random_of(p, s.first) * all;
+  const double want = random * all;
   int piece = 0;
   double before = 0.0, sum = 0.0;   // before: the sum of the pieces in front
   for (int c0 = 0; c0 < p.shorts; c0 += 64) {
-    const double mine = piece_sum(c0 + lane), upto = wave_running(mine);
+    const double mine = c0 == 0 ? mine0 : piece_sum(c0 + lane), upto = c0 == 0 ? upto0 : wave_running(mine);
     const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && sum + upto > want);
     if (some) {   // (the last one with anything, if rounding leaves `want` at the sum of all)
       const int k = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
@@ -661,8 +721,7 @@ template <bool F32>
 __device__ inline void find_way(const VerifyArgs& p, const Span& s, double per, int b, bool write, Draw& draw) {
   const int lane = threadIdx.x & 63;
   const Way w = walk<F32, false>(p, s, per, write, &draw);
-  RowSum r = row_top(p, s.first + w.at);
-  if (w.times > 0.0) r.sum = row_sum<true>(p, s.first + w.at, per).sum;
+  const RowSum r = w.row;
   const bool none = per == 0.0 || r.top == -INFINITY;
   const int out = s.first + w.kept - 1;
   if (lane == 0) {
@@ -681,13 +740,14 @@ __device__ inline void find_way(const VerifyArgs& p, const Span& s, double per, 
 template <bool F32, int SHORTS>
 __device__ inline void sum_shorts(const VerifyArgs& p, const Span& s, const Draw& d, double per, int b, int first) {
   __shared__ double scratch[kThreads / 64][SHORTS];
-  Source<F32> from[SHORTS];
-#pragma unroll
-  for (int k = 0; k < SHORTS; ++k) from[k] = source_of<F32>(p, d, (first + k) * kShort + (int)threadIdx.x * kOnce);
-#pragma unroll
+  Source<F32> next = source_of<F32>(p, d, first * kShort + (int)threadIdx.x * kOnce);
+#pragma unroll 1
   for (int k = 0; k < SHORTS; ++k) {
+    const Source<F32> from = next;
+    const int i = (first + k) * kShort + (int)threadIdx.x * kOnce;
+    if (k + 1 < SHORTS) next = source_of<F32>(p, d, i + kShort);
     double w[kOnce], sum = 0.0;
-    weights_of<F32>(p, s, d, per, (first + k) * kShort + (int)threadIdx.x * kOnce, from[k], w);
+    weights_of<F32>(p, s, d, per, i, from, w);
 #pragma unroll
     for (int j = 0; j < kOnce; ++j) sum += w[j];
     sum = wave_sum(sum);
@@ -715,6 +775,7 @@ __global__ __launch_bounds__(kThreads) void walk_and_draw_kernel(VerifyArgs p) {
     if (piece == 0 && threadIdx.x == 0) p.d.accepted[b] = 0;
     return;
   }
+  const double random = random_of(p, s.first);
   if (threadIdx.x < 64) find_way<F32>(p, s, per, b, piece == 0, draw);
   __syncthreads();
   if (draw.how == kNothing) return;
@@ -726,7 +787,7 @@ __global__ __launch_bounds__(kThreads) void walk_and_draw_kernel(VerifyArgs p) {
   __syncthreads();
   if (before_me != p.shorts - 1) return;
   __threadfence();   // the others' sums
-  draw_token<F32>(p, s, draw, per, b);
+  draw_token<F32>(p, s, draw, per, random, b);
 }
 
 // Many: a launch each
@@ -752,7 +813,9 @@ __global__ __launch_bounds__(kThreads) void left_sums_kernel(VerifyArgs p) {
 template <bool F32>
 __global__ __launch_bounds__(kThreads) void draw_kernel(VerifyArgs p) {
   const int b = blockIdx.x;
-  if (p.draws[b].how != kNothing) draw_token<F32>(p, span_of(p, b), p.draws[b], inverse_temperature(p, b), b);
+  if (p.draws[b].how == kNothing) return;
+  const Span s = span_of(p, b);
+  draw_token<F32>(p, s, p.draws[b], inverse_temperature(p, b), random_of(p, s.first), b);
 }
 
 // ---- children one after the other, where drafts come with distributions ----------------------------------------------------------------------------
@@ -779,21 +842,21 @@ __global__ __launch_bounds__(kThreads) void children_kernel(VerifyArgs p) {
   const int v = row - s.first;
   int child = next_child(p, s, v, v + 1);
   if (child >= s.n) return;
-  const RowSum r = row_sum<true>(p, row, per);
+  const RowSum r = of_lane(sums_of_rows(p, (threadIdx.x & 63) == 0 ? row : -1, per, true), 0);
   if (accepts<F32>(p, row, r, per, s.first + child, 0.0, 1.0)) return;
   const auto sum_of = [&](int c, double t) {   // of piece c
     double sum = 0.0;
     if (r.sum > 0.0) {
       Draw rest{};
       rest.times = t, rest.sum = r.sum, rest.top = r.top, rest.row = row, rest.how = kRest;
-      Source<F32> from[kParts];
-      const int i = c * kPiece + (int)threadIdx.x * kOnce;
-#pragma unroll
-      for (int k = 0; k < kParts; ++k) from[k] = source_of<F32>(p, rest, i + k * kShort);
-#pragma unroll
-      for (int k = 0; k < kParts; ++k) {
+      int i = c * kPiece + (int)threadIdx.x * kOnce;
+      Source<F32> next = source_of<F32>(p, rest, i);
+#pragma unroll 1
+      for (int k = 0; k < kParts; ++k, i += kShort) {
+        const Source<F32> from = next;
+        if (k + 1 < kParts) next = source_of<F32>(p, rest, i + kShort);
         double w[kOnce];
-        weights_of<F32>(p, s, rest, per, i + k * kShort, from[k], w);
+        weights_of<F32>(p, s, rest, per, i, from, w);
 #pragma unroll
         for (int j = 0; j < kOnce; ++j) sum += w[j];
       }
