@@ -366,8 +366,8 @@ __device__ inline RowSum sums_of_rows(const VerifyArgs& p, int row, double per, 
     if (!(per > 0.0)) mine.sum = 0.0;
     return mine;
   }
-  // a piece a lane, the lanes of a row next to each other, as many rows at a time as that leaves (unrolled over sixteen pieces a lane, the exponentials are 6 KB of
-  // instructions that a launch has to fetch first: eight chains of six with distributions, 50001 tokens, 24.3 us that way, 23.3 this way)
+  // a piece a lane, the lanes of a row next to each other, as many rows at a time as that leaves (with a row a lane up to sixteen exponentials of 25 dependent
+  // instructions follow each other: eight chains of six with distributions, 50001 tokens, 24.3 us that way, 23.3 this way)
   const int lane = threadIdx.x & 63, wide = p.pieces >= 64 ? 64 : p.pieces > 1 ? 1 << (32 - __clz(p.pieces - 1)) : 1, at_once = 64 / wide;
   const auto of_round = [&](int r0) { return __shfl(row, min(r0 + lane / wide, 63), 64); };
   const auto fetch = [&](int of, int c) { return of >= 0 && c < p.pieces ? p.sums[(size_t)of * p.pieces + c] : PieceSum{0.0, -INFINITY, INT32_MAX}; };
