@@ -340,6 +340,19 @@ def test_odd_logits(gpu, f32):
         _verify(gpu, d, [t if t == t else 0.0 for t in temps])
 
 
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("vocab", [140001, 600011])
+def test_many_pieces(gpu, vocab, probs):
+    """More pieces of a row than are looked at together; at temperature 0 equal largest logits far apart, the lowest of which counts; pieces without a number."""
+    d = _draft(12, [5, 1, 4], vocab, f32=True, probs=probs)
+    for row, at in ((0, (vocab - 1, vocab // 2, 8192 * 3 + 5)), (5, (vocab - 2, 8192 * 16)), (6, (7, vocab - 9))):
+        d["logits"][row, list(at)] = 30.0
+    d["logits"][2, :8192 * 16] = -np.inf
+    d["logits"][7, 8192:] = np.nan
+    for temps in ([0.0, 0.0, 0.0], [1.0, 0.6, 2.0]):
+        _verify(gpu, d, temps, extra=1)
+
+
 def test_rejected_with_nothing_left(gpu):
     """Draft distributions above the target's everywhere (no sum of 1), and all of the target's tokens among rejected children."""
     d = _draft(5, [4, 4], 50, probs=True, chain=True)
