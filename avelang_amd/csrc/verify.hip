@@ -126,9 +126,8 @@ __device__ inline double weight_of(float x, double top, double per) {
   return x == -INFINITY ? 0.0 : __builtin_bit_cast(double, bits);
 }
 
-// A NaN counts as -inf, infinity as the largest number
-// (the middle of three with a NaN is the least of the others)
-__device__ inline float number(float x) { return __builtin_amdgcn_fmed3f(x, -INFINITY, 3.402823466e38f); }
+// A NaN counts as -inf, infinity as the largest number.  (The lesser of a NaN and a number is the number: a NaN has to be told apart by itself.)
+__device__ inline float number(float x) { return x == x ? fminf(x, 3.402823466e38f) : -INFINITY; }
 template <bool F32>
 __device__ inline float logit(const VerifyArgs& p, int row, int i) {
   if constexpr (F32) return static_cast<const float*>(p.d.logits)[(int64_t)row * p.d.logits_stride + i];

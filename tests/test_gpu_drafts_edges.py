@@ -1,0 +1,69 @@
+"""Acceptance of drafted tokens where logits are no ordinary numbers, on rows that the way through the tree is shown to reach."""
+import numpy as np
+import pytest
+
+from tests import draft_helpers as D
+from tests.test_gpu_drafts import _draft, _verify
+
+pytestmark = pytest.mark.gpu
+
+
+def _visited(d, want):
+    """Rows of the nodes that are kept."""
+    return {int(d["cu"][b] + j) for b, n in enumerate(want[0]) for j in want[1][d["cu"][b]:d["cu"][b] + n]}
+
+
+def _likeliest(d, nodes):
+    """Every node is the first child of the one before and has the token that its parent's row prefers, so that small random numbers accept all of them."""
+    for b in range(len(d["cu"]) - 1):
+        for j in range(1, nodes):
+            x = d["logits"][d["cu"][b] + j - 1]
+            d["tokens"][d["cu"][b] + j] = int(np.argmax(np.where(np.isnan(x), -np.inf, x)))
+            d["parents"][d["cu"][b] + j] = j - 1
+
+
+#: what a row of at least 7 tokens holds beside ordinary logits: (where, what)
+ODD = [[(3, np.nan)], [(0, np.nan)], [(-1, np.nan)], [(5, np.inf)], [(5, np.inf), (-3, np.inf)], [(2, np.nan), (6, np.inf)], [(1, np.nan), (4, -np.inf)],
+       [(slice(0, None, 2), np.nan)], [(slice(1, None, 2), -np.inf), (0, np.nan)], [(slice(0, -2), np.nan)]]
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("vocab", [7, 700, 20011])
+@pytest.mark.parametrize("chain", [1, 4])
+def test_nan_and_infinity_among_numbers(gpu, chain, vocab, f32, probs):
+    """A NaN counts as -inf, +inf as the largest number, in rows that are only drawn from (one node) and in rows whose children are accepted (four)."""
+    seen = set()
+    for shift in range(0, len(ODD), chain):
+        d = _draft(41 + shift, [chain] * 8, vocab, chain=True, f32=f32, probs=probs)
+        for row in range(8 * chain):
+            for at, value in ODD[(row + shift) % len(ODD)]:
+                d["logits"][row, at] = value
+        _likeliest(d, chain)
+        first = np.arange(0, 8 * chain, chain)
+        numbers = d["uniform"][first].copy()
+        d["uniform"] *= np.float32(2.0 ** -14)      # accepted
+        d["uniform"][first] = numbers               # drawn
+        want = _verify(gpu, d, [1.0, 0.6, 1.4, 1.0, 0.3, 1.0, 1.0, 2.0])
+        seen |= {(row + shift) % len(ODD) for row in _visited(d, want)}
+        assert chain == 1 or (want[0] > 2).sum() >= 6
+    assert seen == set(range(len(ODD)))
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("f32", [False, True])
+def test_children_without_a_number(gpu, f32, probs):
+    """A child whose token has a NaN for a logit is never accepted, whatever its random number, and its elder or younger sibling is."""
+    d = _draft(51, [4] * 8, 900, f32=f32, probs=probs)
+    for b in range(8):
+        r = slice(4 * b, 4 * b + 4)
+        d["parents"][r] = [-1, 0, 0, 2 - b % 2]
+        order = np.argsort(-d["logits"][4 * b], kind="stable")
+        d["tokens"][r] = [0, order[0], order[1], order[2]]
+        d["logits"][4 * b, order[b % 2]] = np.nan
+        d["logits"][4 * b + 2 - b % 2, order[2]] = np.nan
+        if probs:
+            d["probs"][4 * b, order[:2]] = 2.0 ** -10
+        d["uniform"][r] = [d["uniform"][4 * b], 0.0, 0.0, 0.0] if b < 4 else [d["uniform"][4 * b], 1e-6, 1e-6, 1e-6]
+    want = _verify(gpu, d, [1.0, 0.7] * 4)
+    assert (want[0] == 2).all() and {int(want[1][4 * b + 1]) for b in range(8)} == {1, 2}
