@@ -106,11 +106,12 @@ __device__ inline double inverse_temperature(const VerifyArgs& p, int b) {
   return t > 0.0f ? 1.4426950408889634 / (double)fminf(t, 3.402823466e38f) : 0.0;
 }
 
-// exp((x - top) / temperature) for x <= top; 0 for -inf.  2^y = 2^n 2^f with n the nearest integer (out of the low bits of y + 1.5 2^52) and the Taylor
-// polynomial of 2^f, |f| <= 1/2, whose first missing term is 2^-42 of it; 2^n by adding to the exponent.  What is below 2^-1000 counts as that.
+// exp((x - top) / temperature) for x <= top.  2^y = 2^n 2^f with n the nearest integer (out of the low bits of y + 1.5 2^52) and the Taylor
+// polynomial of 2^f, |f| <= 1/2, whose first missing term is 2^-42 of it; 2^n by adding to the exponent.  0 for -inf, and for what is below 2^-1020, next to where
+// numbers of 64 bits end: a finite mask leaves nothing.
 __device__ inline double weight_of(float x, double top, double per) {
   constexpr double kRound = 6755399441055744.0;
-  const double y = fmax(((double)x - top) * per, -1000.0), up = y + kRound, f = y - (up - kRound);
+  const double y = ((double)x - top) * per, up = y + kRound, f = y - (up - kRound);
   double r = 7.0549116208011233e-9;   // (ln 2)^k / k!
   r = fma(r, f, 1.0178086009239699e-7);
   r = fma(r, f, 1.3215486790144307e-6);
@@ -123,7 +124,7 @@ __device__ inline double weight_of(float x, double top, double per) {
   r = fma(r, f, 0.69314718055994531);
   r = fma(r, f, 1.0);
   const uint64_t bits = __builtin_bit_cast(uint64_t, r) + ((uint64_t)(unsigned)__builtin_bit_cast(uint64_t, up) << 52);
-  return x == -INFINITY ? 0.0 : __builtin_bit_cast(double, bits);
+  return y >= -1020.0 ? __builtin_bit_cast(double, bits) : 0.0;
 }
 
 // A NaN counts as -inf, infinity as the largest number.  (The lesser of a NaN and a number is the number: a NaN has to be told apart by itself.)

@@ -67,3 +67,32 @@ def test_children_without_a_number(gpu, f32, probs):
         d["uniform"][r] = [d["uniform"][4 * b], 0.0, 0.0, 0.0] if b < 4 else [d["uniform"][4 * b], 1e-6, 1e-6, 1e-6]
     want = _verify(gpu, d, [1.0, 0.7] * 4)
     assert (want[0] == 2).all() and {int(want[1][4 * b + 1]) for b in range(8)} == {1, 2}
+
+
+@pytest.mark.parametrize("mask", ["lowest", -1.0e30, -4096.0])
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("vocab", [12, 3001, 20011])
+def test_finite_masks(gpu, vocab, f32, probs, mask):
+    """Logits so low that in 64 bits nothing is left of them (e^-745 and less) are neither drawn nor accepted: not by a random number of 0, and not where
+    all other tokens have been rejected, which leaves nothing, so that the token comes from the whole row."""
+    low = float(np.finfo(np.float32).min if f32 else -np.float32(2 - 2 ** -7) * 2.0 ** 127) if mask == "lowest" else mask
+    allowed = [3, vocab - 4]
+    d = _draft(61, [3] * 6, vocab, f32=f32, probs=probs)
+    d["logits"][:, :3] = d["logits"][:, -3:] = low
+    for b in range(6):
+        r = slice(3 * b, 3 * b + 3)
+        d["parents"][r] = [-1, 0, 0]
+        if b < 2:                            # children whose tokens are masked, drawn by 0
+            d["tokens"][r], d["uniform"][r] = [0, 1, vocab - 1], 0.0
+            if probs:
+                d["probs"][r, [0, 1, vocab - 1]] = 0.125
+        else:                                # two tokens of a half each, both rejected
+            d["logits"][r] = low
+            d["logits"][r, allowed] = -1.5
+            d["tokens"][r], d["uniform"][r] = [0, *allowed], [(0.0, 0.25, 0.5, 0.75)[b - 2], 1.0, 1.0]
+            if probs:
+                d["probs"][r] = 0.0
+                d["probs"][r, allowed] = 0.5
+    want = _verify(gpu, d, [1.0, 0.7, 1.0, 1.0, 0.5, 2.0])
+    assert (want[0] == 1).all() and want[2][6::3].tolist() == [3, 3, vocab - 4, vocab - 4]
