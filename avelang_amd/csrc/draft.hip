@@ -205,7 +205,7 @@ __global__ __launch_bounds__(512) void keep_many_kernel(KeepArgs p) {
 }
 
 template <int PIECES>
-void launch_keep(const KeepArgs& p, int layers, hipStream_t s) {
+void launch_keep(const KeepArgs& p, int layers, int cus, hipStream_t s) {
   for (int b = 0; b < p.k.batch; b += 65535) {
     KeepArgs part = p;
     part.k.page_table = p.k.page_table + (int64_t)b * p.k.page_table_stride;
@@ -213,7 +213,7 @@ void launch_keep(const KeepArgs& p, int layers, hipStream_t s) {
     if (part.k.kept_lens) part.k.kept_lens += b;
     const unsigned y = (unsigned)std::min(p.k.batch - b, 65535);
     if (p.k.max_q <= 256) {
-      const int each = std::max(1, std::min(layers, (int)((int64_t)layers * y / (8 * compute_units()))));
+      const int each = std::max(1, std::min(layers, (int)((int64_t)layers * y / (8 * cus))));
       hipLaunchKernelGGL((keep_few_kernel<PIECES>), dim3((unsigned)((layers + each - 1) / each), y), dim3(256), 0, s, part, layers, each);
     } else {
       hipLaunchKernelGGL((keep_many_kernel<PIECES>), dim3(2 * (unsigned)p.kv_heads, y, (unsigned)layers), dim3(512), 0, s, part);
@@ -232,6 +232,8 @@ hipError_t launch_draft_tree(const int32_t* parents, const int32_t* cu_q, const 
 
 hipError_t launch_keep_kv(const ave_fp4_kv_cache* caches, int layers, const ave_fp4_keep& k, hipStream_t s) {
   const ave_fp4_kv_cache& c0 = caches[0];
+  const int cus = compute_units();
+  if (cus <= 0) return hipErrorInvalidDevice;
   for (int from = 0; from < layers; from += kLayers) {
     const int now = std::min(layers - from, kLayers);
     KeepArgs p{};
@@ -241,9 +243,9 @@ hipError_t launch_keep_kv(const ave_fp4_kv_cache* caches, int layers, const ave_
       const ave_fp4_kv_cache& c = caches[from + i];
       p.layer[i] = {{c.k, c.k_scale, c.v, c.v_scale}, {c.k_page_stride, c.k_scale_page_stride, c.v_page_stride, c.v_scale_page_stride}};
     }
-    if (c0.head_dim == 64) launch_keep<2>(p, now, s);
-    else if (c0.head_dim == 128) launch_keep<4>(p, now, s);
-    else launch_keep<8>(p, now, s);
+    if (c0.head_dim == 64) launch_keep<2>(p, now, cus, s);
+    else if (c0.head_dim == 128) launch_keep<4>(p, now, cus, s);
+    else launch_keep<8>(p, now, cus, s);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;
