@@ -71,6 +71,25 @@ Range range(const T* p, int64_t n) {
   return {from, p ? from + (uintptr_t)n * sizeof(T) : from};
 }
 bool overlap(const Range& a, const Range& b) { return a.from < b.to && b.from < a.to; }
+// Rows of so many bytes, so many bytes apart: what is between them is nobody's
+struct Rows {
+  uintptr_t from;
+  int64_t rows, stride, bytes;
+};
+bool overlap(const Rows& r, const Range& o) {
+  if (!r.from || r.rows <= 0 || r.bytes <= 0 || o.from >= o.to) return false;
+  const __int128 stride = r.stride < 0 ? -(__int128)r.stride : r.stride, from = r.from + (r.stride < 0 ? (r.rows - 1) * (__int128)r.stride : 0);
+  // the first row that ends behind the range's start
+  const __int128 ahead = (__int128)o.from - from - r.bytes, row = ahead < 0 || stride == 0 ? 0 : ahead / stride + 1;
+  return row < r.rows && from + row * stride < (__int128)o.to && (__int128)o.from < from + row * stride + r.bytes;
+}
+template <size_t I, size_t O>
+bool overlap(const Rows (&in)[I], const Range (&out)[O]) {
+  for (const Rows& r : in)
+    for (const Range& o : out)
+      if (overlap(r, o)) return true;
+  return false;
+}
 // Does an output overlap an input or another output?
 template <size_t I, size_t O>
 bool overlap(const Range (&in)[I], const Range (&out)[O]) {
@@ -263,7 +282,10 @@ int ave_fp4_verify_draft(const ave_fp4_draft* draft, void* workspace, size_t wor
   if (!aligned(d.logits, d.logits_f32 ? 4 : 2) || !aligned(d.draft_probs, 4)) return fail_inval("logits and draft_probs must be aligned to their elements.");
   const Range in[] = {range(d.tokens, d.rows), range(d.parents, d.rows), range(d.cu_q, (int64_t)d.batch + 1), range(d.uniform, d.rows), range(d.temperature, d.batch)};
   const Range out[] = {range(d.accepted, d.batch), range(d.path, d.rows), range(d.emitted, d.rows)};
-  if (overlap(in, out)) return fail_inval("accepted, path and emitted must not overlap the inputs, nor each other.");
+  const int64_t size = d.logits_f32 ? 4 : 2;
+  const Rows read[] = {{reinterpret_cast<uintptr_t>(d.logits), d.rows, d.logits_stride * size, d.vocab * size},
+                       {reinterpret_cast<uintptr_t>(d.draft_probs), d.rows, d.draft_probs_stride * 4, d.vocab * (int64_t)4}};
+  if (overlap(in, out) || overlap(read, out)) return fail_inval("accepted, path and emitted must not overlap the inputs, nor each other.");
   const size_t need = ave::verify_draft_workspace_bytes(d);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail_inval("the workspace must have %zu bytes, got %zu.", need, workspace ? workspace_bytes : (size_t)0);
@@ -292,7 +314,17 @@ int ave_fp4_keep_kv_mxfp4(const ave_fp4_kv_cache* caches, int layers, const ave_
   if (!k.seq_lens || !k.cu_q || !k.accepted || (k.tokens > 0 && !k.path) || (k.table_pages > 0 && !k.page_table)) return fail_inval("null device pointer.");
   const Range in[] = {range(k.seq_lens, k.batch), range(k.cu_q, (int64_t)k.batch + 1), range(k.path, k.tokens), range(k.accepted, k.batch)};
   const Range out[] = {range(k.kept_lens, k.batch)};
-  if (overlap(in, out)) return fail_inval("kept_lens must not overlap an input.");
+  const Rows table[] = {{reinterpret_cast<uintptr_t>(k.page_table), k.batch, k.page_table_stride * 4, k.table_pages * (int64_t)4}};
+  bool overlaps = overlap(in, out) || overlap(table, out);
+  for (int i = 0; i < layers && !overlaps; ++i) {
+    const ave_fp4_kv_cache& c = caches[i];
+    const int64_t codes = (int64_t)c.kv_heads * c.page_size * (c.head_dim / 2);
+    const Rows pages[] = {{reinterpret_cast<uintptr_t>(c.k), c.pages, c.k_page_stride, codes}, {reinterpret_cast<uintptr_t>(c.v), c.pages, c.v_page_stride, codes},
+                          {reinterpret_cast<uintptr_t>(c.k_scale), c.pages, c.k_scale_page_stride, codes / 16},
+                          {reinterpret_cast<uintptr_t>(c.v_scale), c.pages, c.v_scale_page_stride, codes / 16}};
+    overlaps = overlap(pages, out);
+  }
+  if (overlaps) return fail_inval("kept_lens must not overlap an input, nor a cache.");
   return finish(ave::launch_keep_kv(caches, layers, k, static_cast<hipStream_t>(hip_stream)), "key/value keep kernel");
 }
 

@@ -1,7 +1,9 @@
-"""Acceptance of drafted tokens where logits are no ordinary numbers, on rows that the way through the tree is shown to reach."""
+"""Acceptance of drafted tokens where logits are no ordinary numbers, on rows that the way through the tree is shown to reach; outputs next to inputs."""
 import numpy as np
 import pytest
+import torch
 
+import avelang_amd as ave
 from tests import draft_helpers as D
 from tests.test_gpu_drafts import _draft, _verify
 
@@ -96,3 +98,19 @@ def test_finite_masks(gpu, vocab, f32, probs, mask):
                 d["probs"][r, allowed] = 0.5
     want = _verify(gpu, d, [1.0, 0.7, 1.0, 1.0, 0.5, 2.0])
     assert (want[0] == 1).all() and want[2][6::3].tolist() == [3, 3, vocab - 4, vocab - 4]
+
+
+def test_outputs_between_rows_of_logits(gpu):
+    """What lies between rows belongs to nobody: outputs may be there, in rows of an input they may not."""
+    d = _draft(71, [5, 4], 100, f32=True)
+    rest = [D.tensor(d[k], gpu) for k in ("tokens", "parents", "cu", "uniform")]
+    buffer = torch.zeros(9, 140, device=gpu)
+    logits, between = buffer[:, :100], buffer.view(torch.int32)
+    logits.copy_(D.tensor(d["logits"], gpu))
+    want = ave.verify_draft(logits.contiguous(), *rest)
+    outs = between[0, 100:102], between[3, 101:110], between[7, 131:140]
+    got = ave.verify_draft(logits, *rest, accepted=outs[0], path=outs[1], emitted=outs[2])
+    assert all(g.data_ptr() == o.data_ptr() and torch.equal(g, w) for g, o, w in zip(got, outs, want))
+    for name, out in (("path", between[8, 99:108]), ("emitted", between.view(-1)[132:141]), ("path", between[2, :9])):
+        with pytest.raises(ValueError, match="must not overlap"):
+            ave.verify_draft(logits, *rest, **{name: out})
