@@ -4,8 +4,9 @@ import pytest
 import torch
 
 import avelang_amd as ave
+from tests import attention_helpers as A
 from tests import draft_helpers as D
-from tests.test_gpu_drafts import _draft, _verify
+from tests.test_gpu_drafts import _draft, _parents, _verify
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +115,94 @@ def test_outputs_between_rows_of_logits(gpu):
     for name, out in (("path", between[8, 99:108]), ("emitted", between.view(-1)[132:141]), ("path", between[2, :9])):
         with pytest.raises(ValueError, match="must not overlap"):
             ave.verify_draft(logits, *rest, **{name: out})
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("border", [False, True])
+def test_sampled_with_much_to_read(gpu, border, f32):
+    """Rows of more than 64 MB, sampled from: sums of node 0's rows and of those behind the accepted child decide, at several temperatures, in sequences of fewer
+    and of more than 64 nodes.  `border`: numbers of children are the fp32 ones nearest to the probabilities that they are compared with."""
+    rng = np.random.default_rng(81)
+    counts, temps = [80, 9, 14, 1, 12, 20], [1.0, 0.7, 1.3, 1.0, 0.5, 0.9]
+    d = _draft(81, counts, 300007, chain=True, f32=f32)
+    assert len(d["tokens"]) * 300007 * (4 if f32 else 2) > 64 << 20 and len(d["tokens"]) >= 3 * len(counts)
+    exact = {}
+    for b, n in enumerate(counts):
+        first = d["cu"][b]
+        for j in range(1, n):
+            # nodes 1 and 2 hang at node 0, 3 and 4 at 2, 5 and 6 at 4: the first has its parent's second token, the other one the first
+            d["parents"][first + j] = j - 1 if j % 2 else j - 2
+            x = d["logits"][first + d["parents"][first + j]]
+            order = np.argpartition(-x, 3)[:4]
+            order = order[np.argsort(-x[order], kind="stable")]
+            d["tokens"][first + j] = order[j % 2]
+            if j % 2 and (not border or b % 2):
+                d["uniform"][first + j] = 0.9
+            elif not border or j > 6:
+                d["uniform"][first + j] *= np.float32(2.0 ** -10)
+            else:
+                p = D.softmax(x, temps[b])[order]
+                exact[first + j] = p[1] if j % 2 else p[0] / (1 - p[1])
+                d["uniform"][first + j] = exact[first + j]
+    assert all(abs(float(d["uniform"][i]) - e) <= 2.0 ** -24 * e for i, e in exact.items()) and len(exact) == (24 if border else 0)
+    want = _verify(gpu, d, temps, extra=2)
+    if border:
+        assert 2 in want[0] and want[0].max() > 4, want[0]
+    else:
+        assert want[0][0] > 33 and (want[0][[1, 2, 4, 5]] > 3).all(), want[0]   # (the 64 first nodes and more)
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("vocab", [140001, 600011])
+def test_pieces_without_a_number(gpu, vocab, probs):
+    """Rows most of whose vocabulary is -inf or NaN, in front, in the middle or behind, more pieces than are looked at together: drawn from, and accepted from."""
+    rng = np.random.default_rng(91)
+    seen = set()
+    for chain in (1, 3):
+        d = _draft(91 + chain, [chain] * 6, vocab, chain=True, f32=True)
+        for row, x in enumerate(d["logits"]):
+            what = np.nan if row % 2 else -np.inf
+            if row % 3 == 0:
+                x[:8192 * 16] = what
+            elif row % 3 == 1:
+                x[8192:] = what
+            else:
+                x[100:vocab - 100] = what
+        _likeliest(d, chain)
+        if probs:
+            d["probs"] = np.stack([D.softmax(x + rng.standard_normal(vocab), 1.0) for x in d["logits"]]).astype(np.float32)
+        first = np.arange(0, 6 * chain, chain)
+        numbers = d["uniform"][first].copy()
+        d["uniform"] *= np.float32(2.0 ** -14)
+        d["uniform"][first] = numbers
+        want = _verify(gpu, d, [1.0, 0.6, 2.0, 1.0, 0.8, 0.0], extra=1)
+        assert (want[0] == chain).all()
+        seen |= {row % 6 for row in _visited(d, want)}
+    assert seen == set(range(6))
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("nodes", [1, 8, 20, 70])
+@pytest.mark.parametrize("window", [0, 200])
+def test_tables_wide_enough_for_units_beyond_32_bits(gpu, d, nodes, window):
+    """The width of the page table alone decides how units are numbered, so that short sequences reach the 64-bit forms: of few rows, of blocks of 64 rows
+    and of 128.  (With a window units are few, and 32 bits do.)"""
+    hq, hkv, page = 16, 8, 4096
+    rows = [(nodes, nodes + 290 - 17 * i) for i in range(14)] + [(nodes, 1500), (0, 9), (nodes, nodes), (min(nodes, 3), 64)]
+    pages = (1 << 31) // page - 1
+    tokens = sum(n for n, _ in rows)
+    assert min(2 * tokens // 128 + len(rows), 2 * tokens) * hkv * (pages * page // 64) > 1 << 32
+    batch = A.Batch(rows, hq, hkv, d, page, seed=nodes)
+    t = batch.tensors(gpu)
+    wide = torch.full((len(rows), pages), 1 << 30, dtype=torch.int32, device=gpu)
+    wide[:, :t["page_table"].shape[1]] = t["page_table"]
+    above = [D.ancestors(p) for p in _parents(batch, 7)]
+    seen = D.tensor(np.concatenate([D.words_of(a, 2) for a in above]), gpu)
+    want, want_lse, tol, lse_tol = D.masked_reference(batch, [D.visible(a, k, window) for a, (_, k) in zip(above, batch.rows)], sinks=batch.sinks)
+    lse = torch.full(batch.q.shape[:2], float("nan"), device=gpu)
+    out = torch.full(batch.q.shape, float("nan"), dtype=torch.bfloat16, device=gpu)
+    ave.tree_attention_mxfp4(t["q"], t["cache"], wide, t["seq_lens"], t["cu_q"], seen, out, lse, max_q=nodes, window=window, sinks=D.tensor(batch.sinks, gpu))
+    err = np.abs(out.float().cpu().numpy() - want)
+    assert (err <= tol).all(), float((err / tol).max())
+    assert (np.abs(lse.cpu().numpy() - want_lse) <= lse_tol).all()
