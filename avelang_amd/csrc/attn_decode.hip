@@ -532,12 +532,21 @@ hipError_t launch_attn_decode(A p, int row_tiles, void* ws, hipStream_t s) {
     if (p.c.head_dim == 128) return launch_form<128, 2, 4, 2, Units>(p, whole, ws, s);
     return launch_form<256, 2, 4, 2, Units>(p, whole, ws, s);
   }
+  // (trees: two row tiles come with up to 1024 keys only, where items of 64 and 128 channels stay whole, and four do not come)
   switch (p.c.head_dim * 8 + row_tiles) {
     case 64 * 8 + 1: return whole ? launch_form<64, 1, 8, 4>(p, whole, ws, s) : launch_form<64, 1, 4, 4>(p, whole, ws, s);
-    case 64 * 8 + 2: return whole ? launch_form<64, 2, 8, 4>(p, whole, ws, s) : launch_form<64, 2, 4, 4>(p, whole, ws, s);
+    case 64 * 8 + 2:
+      if constexpr (!kTree<A>)
+        if (!whole) return launch_form<64, 2, 4, 4>(p, whole, ws, s);
+      return launch_form<64, 2, 8, 4>(p, whole, ws, s);
     case 128 * 8 + 1: return whole ? launch_form<128, 1, 8, 2>(p, whole, ws, s) : launch_form<128, 1, 4, 2>(p, whole, ws, s);
-    case 128 * 8 + 2: return whole ? launch_form<128, 2, 8, 2>(p, whole, ws, s) : launch_form<128, 2, 4, 2>(p, whole, ws, s);
-    case 128 * 8 + 4: return launch_form<128, 4, 4, 4>(p, whole, ws, s);
+    case 128 * 8 + 2:
+      if constexpr (!kTree<A>)
+        if (!whole) return launch_form<128, 2, 4, 2>(p, whole, ws, s);
+      return launch_form<128, 2, 8, 2>(p, whole, ws, s);
+    case 128 * 8 + 4:
+      if constexpr (!kTree<A>) return launch_form<128, 4, 4, 4>(p, whole, ws, s);
+      return hipErrorInvalidValue;
     case 256 * 8 + 1: return launch_form<256, 1, 4, 2>(p, whole, ws, s);
     default: return launch_form<256, 2, 4, 2>(p, whole, ws, s);
   }
