@@ -527,7 +527,7 @@ __device__ inline Way walk(const VerifyArgs& p, const Span& s, double per, bool 
             now = weight_of(number(logit<F32>(p, row, child_token)), of_row.top, per) / sum;
             against = u_child * (1.0 - gone);
           }
-          accepted = against < now;
+          accepted = against < now && now > 0.0 && u_child < 1.0;   // (no r is above 1; `against` may be off by the last bit of a sum of 1)
           if (!accepted) taken += p_child;
         }
       }

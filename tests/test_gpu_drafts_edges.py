@@ -101,6 +101,23 @@ def test_finite_masks(gpu, vocab, f32, probs, mask):
     assert (want[0] == 1).all() and want[2][6::3].tolist() == [3, 3, vocab - 4, vocab - 4]
 
 
+@pytest.mark.parametrize("number", [1.0, 3.0, np.inf])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("allowed", [2, 3, 9])
+def test_a_number_of_one_accepts_nothing(gpu, allowed, f32, number):
+    """No probability is above 1, not that of the last token that is left either, and a masked token behind it has none."""
+    batch, nodes, vocab = 512, allowed + 2, 40
+    d = _draft(62, [nodes] * batch, vocab, f32=f32)
+    d["logits"][:, allowed:] = -np.inf
+    d["parents"] = np.tile(np.array([-1] + [0] * (nodes - 1), np.int32), batch)
+    d["tokens"] = np.tile(np.array([0, *range(allowed), vocab - 1], np.int32), batch)
+    numbers = d["uniform"][::nodes].copy()
+    d["uniform"][:] = number
+    d["uniform"][::nodes] = numbers
+    want = _verify(gpu, d, [1.0] * batch)
+    assert (want[0] == 1).all()
+
+
 def test_outputs_between_rows_of_logits(gpu):
     """What lies between rows belongs to nobody: outputs may be there, in rows of an input they may not."""
     d = _draft(71, [5, 4], 100, f32=True)
