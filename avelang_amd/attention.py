@@ -239,6 +239,8 @@ def attention_mxfp4(q, cache, page_table, seq_lens, cu_q=None, out=None, lse=Non
     ``scale`` defaults to ``head_dim ** -0.5``.  ``causal``: a token sees itself and what is before it, with ``window`` only the last
     ``window`` of these.  ``sinks`` fp32 ``[heads]``: a logit beside the keys' in the softmax's denominator.  ``lse`` (fp32 ``[T, heads]``,
     optional) is filled with the log of the denominator.  A row that sees no key gives zeros (lse -inf, or its sink).
+    Scores, softmax and sums are fp32, queries count to 2^-19 of their row's largest; probabilities enter the product with the values as bf16, each off by up to 2^-8 of
+    itself, as the result is (measured against fp64: 0.0023 of the output's norm, where the result's rounding alone gives 0.0017).
     Partial results of sequences that several workgroups share go through a workspace from torch's allocator (stream-ordered)."""
     if max_q is None:
         max_q = 1 if cu_q is None else q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0

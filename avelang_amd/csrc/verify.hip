@@ -10,9 +10,10 @@
 // With little to read the last three are one launch, whose workgroups find the way each by itself.  With much, the children of node 0 are decided on first,
 // from its row alone, and then only rows that descend from the accepted one are read.
 //
-// Bound by HBM where there is much to read: 64 trees of 16 nodes, 131072 tokens in bf16, 65 us of which 23 are the wanted 377 of 1024 rows at 4.2 TB/s
+// Bound by HBM where there is much to read: 64 trees of 16 nodes, 131072 tokens in bf16, 63 us of which 23 are the wanted 377 of 1024 rows at 4.2 TB/s
 // (all rows at 4.9 TB/s would be 55); else by the way from one launch to the next and by chains of loads: six nodes of 32768 tokens 9 us; eight chains of six
-// with distributions, 50001 tokens, 23.  Beside that, fp64: the sums over 64 rows of 131072 take 14 us, about 25 instructions an element.
+// with distributions, 50001 tokens, 23.  The fp64 sums over 64 rows of 131072 take 14 us, of which vector instructions are 8 (38 an element, 17 of them in fp64, at
+// four cycles a wave); the rest are the launch's start and end and waits for the row.
 //
 // Rejections with distributions: r_0 = p, r_(k+1) = max(r_k - q, 0) / sum is max(p - t_k q, 0) / s_k with t_0 = 0, s_0 = 1, t_(k+1) = t_k + s_k and
 // s_k = sum max(p - t_k q, 0), so that a row needs its logits, q and two numbers.

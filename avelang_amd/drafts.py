@@ -93,7 +93,8 @@ def verify_draft(logits, tokens, parents, cu_q, uniform, temperature=None, draft
     first index where the running sum of ``r`` is above ``uniform[node 0]`` of the whole (temperature 0: the largest logit's, the lowest of equal ones).
     ``accepted`` counts the kept nodes, node 0 among them; ``path[cu_q[b]:][:accepted[b]]`` are their indices in the sequence, and ``emitted`` as many
     tokens: the kept nodes' from the second on, then the new one; the rest of a sequence's rows is -1, and rows of no sequence are left alone.
-    Sums are formed in fp64; a NaN logit counts as -inf."""
+    What is chosen is what softmax and sums in fp64 choose (fp32 sums decide an acceptance only where they are exact enough to say).  A NaN logit counts as -inf; a
+    logit 708 temperatures and more below the row's largest hides its token, too."""
     done = _native.verify_draft(logits, tokens, parents, cu_q, uniform, temperature, draft_probs, accepted, path, emitted)
     if done is not None:
         return done
