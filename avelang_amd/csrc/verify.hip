@@ -670,7 +670,7 @@ __device__ inline void draw_token(const VerifyArgs& p, const Span& s, const Draw
     __syncthreads();
     all = sum_of_all();
   }
-  const double want = random * all;
+  const double want = random < 1.0 ? random * all : INFINITY;   // (no sum is above the whole, nor does rounding make one)
   int piece = 0;
   double before = 0.0, sum = 0.0;   // before: the sum of the pieces in front
   for (int c0 = 0; c0 < p.shorts; c0 += 64) {

@@ -118,6 +118,20 @@ def test_a_number_of_one_accepts_nothing(gpu, allowed, f32, number):
     assert (want[0] == 1).all()
 
 
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("vocab", [101, 2047, 9001, 140001])
+def test_numbers_from_one_on_draw_the_last_token(gpu, vocab, probs):
+    """No running sum is above the whole, however the two are rounded: the last token that has a weight."""
+    batch = 64 if vocab > 1 << 16 else 512
+    d = _draft(63, [1] * batch, vocab, f32=True, probs=probs, sharp=1.0)
+    d["logits"][:, vocab - 7:] = -np.inf
+    d["logits"][:, vocab - 8] = -60.0
+    call = lambda uniform: ave.verify_draft(*(D.tensor(d[k], gpu) for k in ("logits", "tokens", "parents", "cu")), D.tensor(uniform, gpu), None,   # noqa: E731
+                                            D.tensor(d["probs"], gpu) if probs else None)[2]
+    for number in (1.0, 7.0, np.inf):
+        assert call(np.full(batch, number, np.float32)).eq(vocab - 8).all()
+
+
 def test_outputs_between_rows_of_logits(gpu):
     """What lies between rows belongs to nobody: outputs may be there, in rows of an input they may not."""
     d = _draft(71, [5, 4], 100, f32=True)
