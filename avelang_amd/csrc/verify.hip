@@ -21,7 +21,8 @@
 // Precision.  A token is drawn by where a number lies among the running sums of 10^5 probabilities; in fp32 one draw in some hundred to
 // thousand would go to a neighbour by rounding, so what is drawn from is summed in fp64, and with distributions the row sums are, too.  Without, a node's
 // acceptance is one comparison: the row sums behind it are formed in fp32 (kSumError), and where the comparison comes out nearer than that, the row
-// is summed again in fp64.
+// is summed again in fp64.  Probabilities are exact to 2^-42 of themselves, so a remainder that rejections leave is exact to 2^-42 of p: one to which they come with a
+// probability of 2^-40 is not told from rounding.
 #include <algorithm>
 
 #include "fp4_common.hpp"

@@ -510,11 +510,12 @@ int ave_fp4_tree_attention_mxfp4(const ave_fp4_attention* a, const ave_fp4_tree*
  * the token of the largest logit).  If rejections leave nothing of r, it is p (draft_probs: c is then rejected; tokens: r(token) is 0).
  * accepted[b]: nodes kept, node 0 among them (0 for a sequence without nodes); path[cu_q[b] + i], i < accepted[b]: their indices, rising; emitted: as many
  * tokens, those of the kept nodes from the second on, then the drawn one.  Both are -1 for the other nodes of the sequence.
- * Choices are those of softmax, sums and products in 64 bits (a choice lies between sums of very many probabilities); without draft_probs a node's acceptance is
- * decided by a row sum in fp32 where that is exact enough to say, else in 64, and a random number of 1 accepts none.  A probability below 2^-1020 of the row's largest
- * is none: a logit 708 temperatures and more below the largest one hides its token as -inf does.  A NaN among the logits counts as -inf, +inf as the largest
- * finite number; a row without any number accepts no child and draws -1.  uniform is taken into [0, 1], NaN as 0 (1 draws the last index that r has);
- * a token that is no index of the vocabulary is never accepted; NaN and negative numbers in draft_probs count as 0, as they are otherwise (no sum of 1 is asked for).
+ * Choices are those of softmax, sums and products in 64 bits (a choice lies between sums of very many probabilities), exponentials to 2^-42: what rejections leave of
+ * draft_probs with a probability near that is not told from rounding.  Without draft_probs a node's acceptance is decided by a row sum in fp32 where that is exact enough
+ * to say, else in 64, and a random number of 1 accepts none.  A probability below 2^-1020 of the row's largest is none: a logit 708 temperatures and more below the
+ * largest one hides its token as -inf does.  A NaN among the logits counts as -inf, +inf as the largest finite number; a row without any number accepts no child and
+ * draws -1.  uniform is taken into [0, 1], NaN as 0 (1 draws the last index that r has); a token that is no index of the vocabulary is never accepted; NaN and negative
+ * numbers in draft_probs count as 0, as they are otherwise (no sum of 1 is asked for).
  * Rows behind cu_q[batch] are not written, and what they hold does not matter.  No output may overlap another output or an input.  Offsets are cut to the
  * rows; nothing in device memory leads out of the arrays.
  * The workspace (16-byte aligned, no initialisation) belongs to one call at a time.  Equal inputs give equal outputs.
